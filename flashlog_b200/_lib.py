@@ -12,9 +12,10 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libflashlog_b200.so")
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["api.cu", "scan.cu", "topc.cu", "hop.cu", "rules.cu", "csr.cu", "readout.cu", "masks.cu"]
+SOURCES = ["api.cu", "scan.cu", "topc.cu", "hop.cu", "rules.cu", "csr.cu", "readout.cu", "masks.cu",
+           "gemm.cu", "linear.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-              "-fmad=false", "-Xcompiler", "-fPIC", "-shared"]
+              "-fmad=false", "-Xcompiler", "-fPIC", "-shared", "-t", "0"]
 
 FL_SKIP_NONPOS_W = 1
 FL_DROP_MASKED = 2
@@ -33,6 +34,14 @@ FL_MASK_F32 = 1
 FL_ENTRY_INFO_INTS = 5  # int32 values per entry in fl_hop_params.entry_info
 NO_BUDGET = 1 << 62
 FL_STATUS_SLOT_OVERFLOW = 1
+FL_F32 = 0
+FL_F16 = 1
+FL_BF16 = 2
+FL_ACT_NONE = 0
+FL_ACT_RELU = 1
+FL_ACT_TANH = 2
+FL_ACT_SILU = 3
+FL_ACT_GELU = 4
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -84,6 +93,16 @@ class fl_dropout(ctypes.Structure):
 
 
 _DROP = ctypes.POINTER(fl_dropout)
+
+
+class fl_linear(ctypes.Structure):
+    """Mirror of fl_linear (include/flashlog_b200.h): the operands of the relation head."""
+    _fields_ = [("x", _P), ("w", _P), ("bias", _P), ("residual", _P), ("ld_x", _I64), ("ld_w", _I64),
+                ("ld_res", _I64), ("rows", _I64), ("n", _I64), ("k", _I64), ("dtype", ctypes.c_int),
+                ("act", ctypes.c_int)]
+
+
+_LINEAR = ctypes.POINTER(fl_linear)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -146,6 +165,11 @@ SIGNATURES = {
     "fl_filtered_ranks": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, ctypes.c_int, _P, _P, _SZ,
                                          _P]),
     "fl_filtered_ranks_noalloc": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, ctypes.c_int, _P, _P]),
+    "fl_linear_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int]),
+    "fl_linear_forward": (ctypes.c_int, [_LINEAR, _P, _I64, _P, _P, _SZ, _P]),
+    "fl_linear_backward_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int, ctypes.c_int]),
+    "fl_linear_backward": (ctypes.c_int, [_LINEAR, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "fl_gemm_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
 }
 
 _lib = None

@@ -1,0 +1,116 @@
+// gemm.cuh -- the tcgen05 matrix product behind the linear head and the
+// Newton-Schulz products: D[i, j] = sum_k A(i, k) B(j, k), batched.
+//
+// Operands are 16-bit arrays in global memory, each as 1 or 2 planes.  Two
+// fp16 planes hold one fp32 matrix as hi + lo (22 bits); the product is then
+// hi*hi + hi*lo + lo*hi into one fp32 accumulator (the dropped lo*lo is below
+// 2^-22 of each term), three matrix instructions per step on operands that
+// were loaded once.  An operand is K-major (its contraction index is
+// contiguous) or MN-major (its output index is), so products with a transposed
+// operand need no transposing pass.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace fl {
+
+enum { kF16 = 0, kBF16 = 1 };                 // operand type
+enum { kOutF32 = 0, kOutF16 = 1, kOutBF16 = 2 };  // fl_dtype values (FL_F32, FL_F16, FL_BF16)
+
+struct GemmOperand {
+    const void *ptr;         // 16-byte aligned
+    int64_t ld;              // elements between lines, a multiple of 8
+    int64_t plane;           // elements between the planes (multiple of 8)
+    int64_t batch;           // elements between the batch's matrices (multiple of 8)
+    int planes;              // 1 or 2
+    int mn_major;            // 0: lines are output indices, k contiguous; 1: lines are k
+};
+
+// Epilogue of the linear head: z = acc * 2^(ea[i] + eb[j]) + bias[j],
+// y = act(z) + residual[i, j].
+struct LinearEpilogue {
+    const int *row_exp, *col_exp;  // NULL: 0
+    const void *bias;
+    const void *residual;
+    int64_t ld_res;
+    void *out;
+    int64_t ld_out;
+    float *z;                // pre-activation for the backward, or NULL
+    int64_t ld_z;
+    int dtype, act;
+};
+
+// Epilogue of a Newton-Schulz product: v = alpha * acc + beta * C[i, j], where
+// C is a 2-plane array, written as planes (mirrored when symmetric), or as the
+// last product's result: out = v * out_scale + keep * base.
+struct PlanesEpilogue {
+    float alpha, beta;       // on the accumulator and on the planes' sum
+    const __half *c;         // NULL: no C
+    int64_t c_ld, c_plane, c_batch;
+    __half *out;             // planes out, or NULL
+    int64_t ld, plane, batch;
+    __half *out2;            // second planes output v * alpha2 + diag on the diagonal, or NULL
+    float alpha2, diag;
+    int64_t ld2, plane2, batch2;
+    void *fin;               // final output, or NULL; element (b, i, j) at b * fin_b + i * fin_i + j * fin_j
+    int64_t fin_b, fin_i, fin_j;
+    const float *base;       // fin = v + keep * base[...] (fp32 only), or NULL
+    int64_t base_b, base_i, base_j;
+    float keep;
+    int dtype;
+};
+
+struct GemmShape {
+    int64_t m, n, k, batch;
+    int symmetric;           // D is symmetric: elements i >= j are computed and mirrored
+    int kind;                // kF16 or kBF16
+};
+
+int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
+                cudaStream_t st);
+int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
+                cudaStream_t st);
+
+// ---- activations -------------------------------------------------------------
+enum { kActNone = 0, kActRelu = 1, kActTanh = 2, kActSilu = 3, kActGelu = 4 };
+
+__device__ __forceinline__ float act_value(float z, int act) {
+    switch (act) {
+        case kActRelu: return z > 0.0f ? z : (z <= 0.0f ? 0.0f : z);  // NaN stays NaN
+        case kActTanh: return tanhf(z);
+        case kActSilu: return z / (1.0f + expf(-z));
+        case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+    switch (act) {
+        case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+        case kActTanh: { const float t = tanhf(z); return (1.0f - t) * (1.0f + t); }
+        case kActSilu: { const float t = 1.0f / (1.0f + expf(-z)); return t * (1.0f + z * (1.0f - t)); }
+        case kActGelu:
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+        default: return 1.0f;
+    }
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// v * 2^e without an overflow or underflow on the way: the power is applied in
+// two halves of one sign (|e| <= 252 as each side's exponent is within 126)
+__device__ __forceinline__ float scale_pow2(float v, int e) {
+    const int h = e / 2;
+    return v * __int_as_float((h + 127) << 23) * __int_as_float((e - h + 127) << 23);
+}
+
+}  // namespace fl

@@ -1,0 +1,411 @@
+// linear.cu -- the relation head: y = act(x W^T + bias) + residual and its
+// gradients, on the tcgen05 product of gemm.cu.
+//
+// fp32 operands are split into two fp16 planes, hi + lo, after scaling each
+// line of the uncontracted index by a power of two that brings its largest
+// value to [2^14, 2^15): a value keeps 22 bits down to 2^-18 of its line's
+// largest, and no line can lose bits to another line's size.  The exponents
+// are undone in the product's epilogue.
+#include "gemm.cuh"
+
+namespace fl {
+
+namespace {
+
+constexpr int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
+constexpr int kSumRows = 128;  // rows per partial column sum
+
+int elem_size(int dtype) { return dtype == FL_F32 ? 4 : 2; }
+
+// exponent e with max * 2^-e in [2^14, 2^15); 0 for a zero or non-finite line
+__device__ __forceinline__ int line_exponent(float absmax) {
+    if (!(absmax > 0.0f) || !(absmax <= 3.402823466e38f)) return 0;
+    int e = ((__float_as_int(absmax) >> 23) & 255) - 127;
+    if (e < -100) e = -100;  // subnormal or tiny lines: 2^-e stays representable
+    return e - 14;
+}
+
+__device__ __forceinline__ void split_scaled(float v, int e, __half &hi, __half &lo) {
+    const float s = scale_pow2(v, -e);
+    hi = __float2half_rn(s);
+    lo = __float2half_rn(s - __half2float(hi));
+}
+
+__device__ __forceinline__ float block_max(float v, float *scratch) {
+    v = warp_max(v);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float r = scratch[0];
+    for (int i = 1; i < static_cast<int>(blockDim.x >> 5); ++i) r = fmaxf(r, scratch[i]);
+    __syncthreads();
+    return r;
+}
+
+// One block per row: the row's exponent, then its planes (second read from L1/L2).
+__global__ void pack_rows_kernel(const float *src, int64_t ld, int64_t cols, __half *out, int64_t ldp, int64_t plane,
+                                 int *exps) {
+    __shared__ float scratch[32];
+    const int64_t r = blockIdx.x;
+    const float *row = src + r * ld;
+    const bool vec = ((reinterpret_cast<uintptr_t>(src) & 15) == 0) && (ld & 3) == 0;
+    const int64_t quads = vec ? cols >> 2 : 0;
+    float mx = 0.0f;
+    for (int64_t q = threadIdx.x; q < quads; q += blockDim.x) {
+        const float4 v = reinterpret_cast<const float4 *>(row)[q];
+        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x)), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    }
+    for (int64_t c = quads * 4 + threadIdx.x; c < cols; c += blockDim.x) mx = fmaxf(mx, fabsf(row[c]));
+    const int e = line_exponent(block_max(mx, scratch));
+    if (threadIdx.x == 0) exps[r] = e;
+    __half *hi = out + r * ldp, *lo = hi + plane;
+    for (int64_t q = threadIdx.x; q < quads; q += blockDim.x) {
+        const float4 v = reinterpret_cast<const float4 *>(row)[q];
+        union { __half h[4]; uint2 u; } a, b;
+        split_scaled(v.x, e, a.h[0], b.h[0]);
+        split_scaled(v.y, e, a.h[1], b.h[1]);
+        split_scaled(v.z, e, a.h[2], b.h[2]);
+        split_scaled(v.w, e, a.h[3], b.h[3]);
+        reinterpret_cast<uint2 *>(hi)[q] = a.u;
+        reinterpret_cast<uint2 *>(lo)[q] = b.u;
+    }
+    for (int64_t c = quads * 4 + threadIdx.x; c < cols; c += blockDim.x) {
+        __half x, y;
+        split_scaled(row[c], e, x, y);
+        hi[c] = x;
+        lo[c] = y;
+    }
+}
+
+// Largest |value| of each column, as fp32 bits (order-independent): a block
+// takes 32 columns x a range of rows.
+__global__ void col_absmax_kernel(const float *src, int64_t ld, int64_t rows, int64_t cols, int64_t chunk,
+                                  unsigned *out) {
+    __shared__ float part[8][33];
+    const int64_t c = blockIdx.x * int64_t(32) + threadIdx.x;
+    const int64_t r0 = blockIdx.y * chunk, r1 = min(rows, r0 + chunk);
+    float mx = 0.0f;
+    if (c < cols)
+        for (int64_t r = r0 + threadIdx.y; r < r1; r += 8) mx = fmaxf(mx, fabsf(src[r * ld + c]));
+    part[threadIdx.y][threadIdx.x] = mx;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < cols) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, part[i][threadIdx.x]);
+        atomicMax(out + c, __float_as_uint(mx));
+    }
+}
+
+__global__ void col_exponent_kernel(const unsigned *bits, int *exps, int64_t n) {
+    const int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
+    if (i < n) exps[i] = line_exponent(__uint_as_float(bits[i]));
+}
+
+// Planes of a matrix scaled per column; 64 columns x 32 rows per block.
+__global__ void pack_cols_kernel(const float *src, int64_t ld, int64_t rows, int64_t cols, const int *exps,
+                                 __half *out, int64_t ldp, int64_t plane) {
+    const int64_t c = blockIdx.x * int64_t(64) + 2 * threadIdx.x;
+    if (c >= cols) return;
+    const int e0 = exps[c], e1 = c + 1 < cols ? exps[c + 1] : 0;
+    const bool vec = ((reinterpret_cast<uintptr_t>(src) & 7) == 0) && (ld & 1) == 0 && c + 1 < cols;
+    const int64_t r1 = min(rows, (blockIdx.y + int64_t(1)) * 32);
+    for (int64_t r = blockIdx.y * int64_t(32) + threadIdx.y; r < r1; r += 8) {
+        const float *p = src + r * ld + c;
+        float2 v;
+        if (vec) v = *reinterpret_cast<const float2 *>(p);
+        else v = make_float2(p[0], c + 1 < cols ? p[1] : 0.0f);
+        union { __half h[2]; unsigned u; } a, b;
+        split_scaled(v.x, e0, a.h[0], b.h[0]);
+        split_scaled(v.y, e1, a.h[1], b.h[1]);
+        // the pitch is a multiple of 8 and at least cols: the pair fits in the row
+        *reinterpret_cast<unsigned *>(out + r * ldp + c) = a.u;
+        *reinterpret_cast<unsigned *>(out + plane + r * ldp + c) = b.u;
+    }
+}
+
+// 16-bit rows copied to an aligned pitch (rows whose pitch or base TMA cannot take).
+__global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uint16_t *out, int64_t ldp) {
+    const int64_t r = blockIdx.y;
+    const int64_t c = (blockIdx.x * int64_t(blockDim.x) + threadIdx.x) * 2;
+    if (c >= cols) return;
+    const uint16_t *p = src + r * ld + c;
+    const unsigned a = p[0], b = c + 1 < cols ? p[1] : 0;
+    *reinterpret_cast<unsigned *>(out + r * ldp + c) = a | (b << 16);
+}
+
+// dz = gy * act'(z), written as T with pitch ldo (or not at all), and its
+// column sums over kSumRows rows at a time, taken before the rounding.
+template <typename T>
+__global__ void dz_kernel(const T *gy, int64_t ld_gy, const float *z, int64_t rows, int64_t n, int act, T *out,
+                          int64_t ldo, float *partial) {
+    __shared__ float part[8][33];
+    const int64_t c = blockIdx.x * int64_t(32) + threadIdx.x;
+    const int64_t r0 = blockIdx.y * int64_t(kSumRows), r1 = min(rows, r0 + kSumRows);
+    float sum = 0.0f;
+    if (c < n)
+        for (int64_t r = r0 + threadIdx.y; r < r1; r += 8) {
+            float d = to_f32<T>(gy[r * ld_gy + c]);
+            if (act != kActNone) d *= act_slope(z[r * n + c], act);
+            if (out != nullptr) out[r * ldo + c] = from_f32<T>(d);
+            sum += d;
+        }
+    part[threadIdx.y][threadIdx.x] = sum;
+    __syncthreads();
+    if (partial != nullptr && threadIdx.y == 0 && c < n) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) sum += part[i][threadIdx.x];
+        partial[blockIdx.y * n + c] = sum;
+    }
+}
+
+template <typename T>
+__global__ void sum_partials_kernel(const float *partial, int64_t parts, int64_t n, T *out) {
+    const int64_t c = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
+    if (c >= n) return;
+    float s = 0.0f;
+    for (int64_t p = 0; p < parts; ++p) s += partial[p * n + c];
+    out[c] = from_f32<T>(s);
+}
+
+// ---- host side -------------------------------------------------------------
+bool tma_ready(const void *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+
+size_t operand_bytes(int64_t lines, int64_t inner, int64_t exps, int dtype) {
+    const int planes = dtype == FL_F32 ? 2 : 1;
+    return carve_bytes<__half>(planes * lines * round8(inner)) + carve_bytes<int>(exps) + carve_bytes<unsigned>(exps);
+}
+
+// Readies the matrix src [lines, inner] as a product operand.  by_line: the
+// uncontracted index is the line (K-major), else the inner index (MN-major).
+int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool by_line, int dtype, Carve &ws,
+                 GemmOperand *op, const int **exps, cudaStream_t st) {
+    op->batch = 0;
+    op->mn_major = by_line ? 0 : 1;
+    *exps = nullptr;
+    if (dtype != FL_F32) {
+        op->planes = 1;
+        op->plane = 0;
+        if (tma_ready(src, ld)) {
+            op->ptr = src;
+            op->ld = ld;
+            return FL_OK;
+        }
+        const int64_t ldp = round8(inner);
+        uint16_t *out = ws.take<uint16_t>(lines * ldp);
+        FL_REQUIRE(out != nullptr, "linear: workspace too small");
+        // grid.y is limited to 65535 rows: the rows go in slices
+        for (int64_t r = 0; r < lines; r += 65535) {
+            const int64_t cnt = lines - r < 65535 ? lines - r : 65535;
+            launch(pack16_kernel, dim3(static_cast<unsigned>((inner + 511) / 512), static_cast<unsigned>(cnt)), 256, 0, st,
+                   static_cast<const uint16_t *>(src) + r * ld, ld, inner, out + r * ldp, ldp);
+        }
+        op->ptr = out;
+        op->ld = ldp;
+        return check_launch("linear pack");
+    }
+    const int64_t ldp = round8(inner), plane = lines * ldp;
+    __half *out = ws.take<__half>(2 * plane);
+    int *ex = ws.take<int>(by_line ? lines : inner);
+    FL_REQUIRE(out != nullptr && ex != nullptr, "linear: workspace too small");
+    const float *x = static_cast<const float *>(src);
+    if (by_line) {
+        launch(pack_rows_kernel, static_cast<unsigned>(lines), inner > 2048 ? 512 : 128, 0, st, x, ld, inner, out, ldp,
+               plane, ex);
+    } else {
+        unsigned *bits = ws.take<unsigned>(inner);
+        FL_REQUIRE(bits != nullptr, "linear: workspace too small");
+        FL_CUDA(cudaMemsetAsync(bits, 0, inner * sizeof(unsigned), st));
+        int64_t chunk = 256;
+        while ((lines + chunk - 1) / chunk > 65535) chunk *= 2;
+        launch(col_absmax_kernel, dim3(static_cast<unsigned>((inner + 31) / 32),
+                                       static_cast<unsigned>((lines + chunk - 1) / chunk)),
+               dim3(32, 8), 0, st, x, ld, lines, inner, chunk, bits);
+        launch(col_exponent_kernel, static_cast<unsigned>((inner + 255) / 256), 256, 0, st, bits, ex, inner);
+        for (int64_t r = 0; r < lines; r += 65535 * 32) {
+            const int64_t cnt = lines - r < 65535 * 32 ? lines - r : 65535 * 32;
+            launch(pack_cols_kernel, dim3(static_cast<unsigned>((inner + 63) / 64), static_cast<unsigned>((cnt + 31) / 32)),
+                   dim3(32, 8), 0, st, x + r * ld, ld, cnt, inner, ex, out + r * ldp, ldp, plane);
+        }
+    }
+    op->ptr = out;
+    op->ld = ldp;
+    op->plane = plane;
+    op->planes = 2;
+    *exps = ex;
+    return check_launch("linear pack");
+}
+
+int check_linear(const fl_linear *p) {
+    FL_REQUIRE(p != nullptr, "linear: null parameters");
+    FL_REQUIRE(p->dtype == FL_F32 || p->dtype == FL_F16 || p->dtype == FL_BF16, "linear: bad dtype %d", p->dtype);
+    FL_REQUIRE(p->act >= FL_ACT_NONE && p->act <= FL_ACT_GELU, "linear: bad activation %d", p->act);
+    FL_REQUIRE(p->rows >= 0 && p->n > 0 && p->k > 0 && p->rows < (1ll << 30) && p->n < (1ll << 30) && p->k < (1ll << 30),
+               "linear: bad shape");
+    FL_REQUIRE(p->x != nullptr && p->w != nullptr && p->ld_x >= p->k && p->ld_w >= p->k &&
+                   (p->residual == nullptr || p->ld_res >= p->n),
+               "linear: bad operand");
+    return FL_OK;
+}
+
+GemmShape shape(int64_t m, int64_t n, int64_t k, int dtype) {
+    GemmShape s;
+    s.m = m;
+    s.n = n;
+    s.k = k;
+    s.batch = 1;
+    s.symmetric = 0;
+    s.kind = dtype == FL_BF16 ? kBF16 : kF16;
+    return s;
+}
+
+LinearEpilogue plain_epilogue(void *out, int64_t ld, int dtype, const int *re, const int *ce) {
+    LinearEpilogue e{};
+    e.row_exp = re;
+    e.col_exp = ce;
+    e.out = out;
+    e.ld_out = ld;
+    e.dtype = dtype;
+    e.act = kActNone;
+    return e;
+}
+
+template <typename T>
+int linear_dz(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, T *out, int64_t ldo, float *partial,
+              cudaStream_t st) {
+    // grid.y (row groups) is limited to 65535: 8 million rows
+    const int64_t parts = (p->rows + kSumRows - 1) / kSumRows;
+    FL_REQUIRE(parts <= 65535, "linear: more than %d rows in a backward pass", 65535 * kSumRows);
+    launch(dz_kernel<T>, dim3(static_cast<unsigned>((p->n + 31) / 32), static_cast<unsigned>(parts)), dim3(32, 8), 0, st,
+           static_cast<const T *>(gy), ld_gy, z, p->rows, p->n, p->act, out, ldo, partial);
+    return check_launch("linear dz");
+}
+
+}  // namespace
+
+size_t linear_workspace(int64_t rows, int64_t n, int64_t k, int dtype) {
+    return operand_bytes(rows, k, rows, dtype) + operand_bytes(n, k, n, dtype);
+}
+
+int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *wsp, size_t ws_bytes, cudaStream_t st) {
+    int rc = check_linear(p);
+    if (rc) return rc;
+    FL_REQUIRE(y != nullptr && ld_y >= p->n, "linear: bad output");
+    if (p->rows == 0) return FL_OK;
+    Carve ws(wsp, ws_bytes);
+    GemmOperand a, b;
+    const int *ea, *eb;
+    rc = make_operand(p->x, p->ld_x, p->rows, p->k, true, p->dtype, ws, &a, &ea, st);
+    if (!rc) rc = make_operand(p->w, p->ld_w, p->n, p->k, true, p->dtype, ws, &b, &eb, st);
+    if (rc) return rc;
+    LinearEpilogue e = plain_epilogue(y, ld_y, p->dtype, ea, eb);
+    e.bias = p->bias;
+    e.residual = p->residual;
+    e.ld_res = p->ld_res;
+    e.z = z;
+    e.ld_z = p->n;
+    e.act = p->act;
+    return gemm_linear(shape(p->rows, p->n, p->k, p->dtype), a, b, e, st);
+}
+
+size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act) {
+    size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
+    if (act != FL_ACT_NONE) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
+    const size_t ops = operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
+    return dz + ops + carve_bytes<float>(((rows + kSumRows - 1) / kSumRows) * n);
+}
+
+int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw, void *dbias,
+                    void *wsp, size_t ws_bytes, cudaStream_t st) {
+    int rc = check_linear(p);
+    if (rc) return rc;
+    FL_REQUIRE(gy != nullptr && ld_gy >= p->n, "linear backward: bad gradient");
+    FL_REQUIRE(p->act == FL_ACT_NONE || z != nullptr, "linear backward: an activation needs the pre-activation");
+    const int es = elem_size(p->dtype);
+    if (p->rows == 0) {
+        if (dw != nullptr) FL_CUDA(cudaMemsetAsync(dw, 0, p->n * p->k * es, st));
+        if (dbias != nullptr) FL_CUDA(cudaMemsetAsync(dbias, 0, p->n * es, st));
+        return FL_OK;
+    }
+    Carve ws(wsp, ws_bytes);
+    const void *dz = gy;
+    int64_t ld_dz = ld_gy;
+    if (p->act != FL_ACT_NONE || dbias != nullptr) {
+        void *out = nullptr;
+        const int64_t ldo = round8(p->n);
+        if (p->act != FL_ACT_NONE) {
+            out = ws.take<char>(p->rows * ldo * es);
+            FL_REQUIRE(out != nullptr, "linear backward: workspace too small");
+            dz = out;
+            ld_dz = ldo;
+        }
+        const int64_t parts = (p->rows + kSumRows - 1) / kSumRows;
+        float *partial = nullptr;
+        if (dbias != nullptr) {
+            partial = ws.take<float>(parts * p->n);
+            FL_REQUIRE(partial != nullptr, "linear backward: workspace too small");
+        }
+        const unsigned grid = static_cast<unsigned>((p->n + 127) / 128);
+        if (p->dtype == FL_F32) {
+            rc = linear_dz<float>(p, z, gy, ld_gy, static_cast<float *>(out), ldo, partial, st);
+            if (!rc && dbias) launch(sum_partials_kernel<float>, grid, 128, 0, st, partial, parts, p->n, static_cast<float *>(dbias));
+        } else if (p->dtype == FL_F16) {
+            rc = linear_dz<__half>(p, z, gy, ld_gy, static_cast<__half *>(out), ldo, partial, st);
+            if (!rc && dbias) launch(sum_partials_kernel<__half>, grid, 128, 0, st, partial, parts, p->n, static_cast<__half *>(dbias));
+        } else {
+            rc = linear_dz<__nv_bfloat16>(p, z, gy, ld_gy, static_cast<__nv_bfloat16 *>(out), ldo, partial, st);
+            if (!rc && dbias)
+                launch(sum_partials_kernel<__nv_bfloat16>, grid, 128, 0, st, partial, parts, p->n,
+                       static_cast<__nv_bfloat16 *>(dbias));
+        }
+        if (rc) return rc;
+    }
+    GemmOperand a, b;
+    const int *ea, *eb;
+    if (dx != nullptr) {  // dz [rows, n] contracted over n with W [n, k]
+        rc = make_operand(dz, ld_dz, p->rows, p->n, true, p->dtype, ws, &a, &ea, st);
+        if (!rc) rc = make_operand(p->w, p->ld_w, p->n, p->k, false, p->dtype, ws, &b, &eb, st);
+        if (!rc)
+            rc = gemm_linear(shape(p->rows, p->k, p->n, p->dtype), a, b, plain_epilogue(dx, p->k, p->dtype, ea, eb), st);
+        if (rc) return rc;
+    }
+    if (dw != nullptr) {  // dz [rows, n] and x [rows, k] contracted over the rows
+        if (dx == nullptr || p->dtype == FL_F32) {
+            rc = make_operand(dz, ld_dz, p->rows, p->n, false, p->dtype, ws, &a, &ea, st);
+            if (rc) return rc;
+        } else {
+            a.mn_major = 1;  // 16-bit types: the operand that dx used, read along its other index
+        }
+        rc = make_operand(p->x, p->ld_x, p->rows, p->k, false, p->dtype, ws, &b, &eb, st);
+        if (!rc)
+            rc = gemm_linear(shape(p->n, p->k, p->rows, p->dtype), a, b, plain_epilogue(dw, p->k, p->dtype, ea, eb), st);
+        if (rc) return rc;
+    }
+    return check_launch("linear backward");
+}
+
+int gemm_fault(int *fault);
+
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" {
+
+size_t fl_linear_workspace(int64_t rows, int64_t n, int64_t k, int dtype) { return linear_workspace(rows, n, k, dtype); }
+
+int fl_linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws, size_t ws_bytes,
+                      fl_stream_t stream) {
+    return linear_forward(p, y, ld_y, z, ws, ws_bytes, as_stream(stream));
+}
+
+size_t fl_linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act) {
+    return linear_backward_workspace(rows, n, k, dtype, act);
+}
+
+int fl_linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw,
+                       void *dbias, void *ws, size_t ws_bytes, fl_stream_t stream) {
+    return linear_backward(p, z, gy, ld_gy, dx, dw, dbias, ws, ws_bytes, as_stream(stream));
+}
+
+int fl_gemm_fault(int *fault) { return gemm_fault(fault); }
+
+}  // extern "C"

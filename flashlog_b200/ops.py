@@ -660,3 +660,110 @@ def readout_backward(row_ptr, ent, N: int, targets, g_scores, n_val: int, val_li
                                     None, _stream()),
           "readout_backward")
     return grad[:n_val]
+
+
+# --------------------------------------------------------------------------
+# relation attention: head, weights, update
+# --------------------------------------------------------------------------
+FL_DTYPE = {torch.float32: L.FL_F32, torch.float16: L.FL_F16, torch.bfloat16: L.FL_BF16}
+
+
+def _one_device(what, *ts):
+    """The tensors' common CUDA device; raises unless there is exactly one."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+class _on:
+    """Makes `device` current for a launch (a no-op when it already is) and gives its current stream."""
+    __slots__ = ("index", "old")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.old = torch.cuda.current_device()
+        if self.old != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.old != self.index:
+            torch.cuda.set_device(self.old)
+
+
+def _lines(t):
+    """t as [rows, cols] lines the library can address: unit inner stride, rows at least a row apart."""
+    if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+        return t
+    return t.contiguous()
+
+
+def _ld(t):
+    return max(t.stride(0), t.shape[1])
+
+
+def _linear_params(x, weight, bias, residual, act):
+    return L.fl_linear(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                       None if residual is None else residual.data_ptr(), _ld(x), _ld(weight),
+                       0 if residual is None else _ld(residual), x.shape[0], weight.shape[0], weight.shape[1],
+                       FL_DTYPE[x.dtype], act)
+
+
+def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE, want_z: bool = False):
+    """y = act(x W^T + bias) + residual of [rows, k] and [n, k] matrices of one
+    dtype; with want_z also the fp32 pre-activation (None without an
+    activation).  Returns (y, z)."""
+    dev = _one_device("linear", x, weight, bias, residual)
+    x, weight = _lines(x), _lines(weight)
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else _lines(residual)
+    rows, (n, k) = x.shape[0], weight.shape
+    y = torch.empty((rows, n), dtype=x.dtype, device=dev)
+    z = torch.empty((rows, n), dtype=torch.float32, device=dev) if want_z and act != L.FL_ACT_NONE else None
+    if rows == 0:
+        return y, z
+    p = _linear_params(x, weight, bias, residual, act)
+    nbytes = lib().fl_linear_workspace(rows, n, k, p.dtype)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as st:
+        rc = lib().fl_linear_forward(ctypes.byref(p), y.data_ptr(), n, None if z is None else z.data_ptr(),
+                                     None if ws is None else ws.data_ptr(), nbytes, st)
+    check(rc, "linear")
+    return y, z
+
+
+def linear_backward(x, weight, z, gy, act: int = L.FL_ACT_NONE, want=(True, True, True)):
+    """(dx, dweight, dbias) of linear_forward for the gradient gy [rows, n];
+    want says which (None in the place of the others)."""
+    dev = _one_device("linear backward", x, weight, z, gy)
+    x, weight, gy = _lines(x), _lines(weight), _lines(gy)
+    rows, (n, k) = x.shape[0], weight.shape
+    dx = torch.empty((rows, k), dtype=x.dtype, device=dev) if want[0] else None
+    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if want[1] else None
+    db = torch.empty(n, dtype=x.dtype, device=dev) if want[2] else None
+    p = _linear_params(x, weight, None, None, act)
+    nbytes = lib().fl_linear_backward_workspace(rows, n, k, p.dtype, act)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as st:
+        rc = lib().fl_linear_backward(ctypes.byref(p), None if z is None else z.data_ptr(), gy.data_ptr(), _ld(gy),
+                                      *(None if t is None else t.data_ptr() for t in (dx, dw, db)),
+                                      None if ws is None else ws.data_ptr(), nbytes, st)
+    check(rc, "linear backward")
+    return dx, dw, db
+
+
+def gemm_fault() -> bool:
+    """Whether a bounded wait of a matrix product ran out since the last call (synchronizes)."""
+    f = ctypes.c_int(0)
+    check(lib().fl_gemm_fault(ctypes.byref(f)), "gemm_fault")
+    return bool(f.value)

@@ -462,6 +462,42 @@ int fl_filtered_ranks_noalloc(const int64_t *idx_b, const int64_t *idx_e, const 
                               const int64_t *targets, const int64_t *filter_keys, int64_t n_filter, int64_t B,
                               int64_t E, int use_eql, float *ranks, fl_stream_t stream);
 
+/* ---- the relation attention: head, weights, update -------------------------
+ * Element types of the head, the logits and the updates. */
+enum { FL_F32 = 0, FL_F16 = 1, FL_BF16 = 2 };
+/* Activations of the head. gelu is 0.5 z (1 + erf(z / sqrt 2)). */
+enum { FL_ACT_NONE = 0, FL_ACT_RELU = 1, FL_ACT_TANH = 2, FL_ACT_SILU = 3, FL_ACT_GELU = 4 };
+
+/* y = act(x W^T + bias) + residual: x [rows, k], W [n, k], bias [n] or NULL,
+ * residual [rows, n] or NULL, all of one dtype; ld_* are elements between
+ * rows (at least the row's length).  fp32 is computed to fp32 accuracy
+ * (operands as two fp16 planes scaled per line, or fp32 multiply-adds for few
+ * rows), 16-bit types with fp32 sums and one rounding at the end. */
+typedef struct fl_linear {
+    const void *x, *w, *bias, *residual;
+    int64_t ld_x, ld_w, ld_res;
+    int64_t rows, n, k;
+    int dtype, act;
+} fl_linear;
+
+/* z (f32 [rows, n], contiguous) or NULL receives the pre-activation, which
+ * fl_linear_backward of an activation needs. */
+size_t fl_linear_workspace(int64_t rows, int64_t n, int64_t k, int dtype);
+int fl_linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws, size_t ws_bytes,
+                      fl_stream_t stream);
+
+/* Gradients for gy [rows, n]: dz = gy * act'(z), dx [rows, k] = dz W,
+ * dw [n, k] = dz^T x, dbias [n] = sum over rows of dz (each contiguous, of
+ * p's dtype, or NULL: not wanted).  The residual's gradient is gy itself.
+ * Sums run in a fixed order: results do not change from run to run. */
+size_t fl_linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act);
+int fl_linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw,
+                       void *dbias, void *ws, size_t ws_bytes, fl_stream_t stream);
+
+/* 1 if a bounded wait of a matrix-product kernel ran out since the last call
+ * (its outputs hold NaN), else 0, in *fault; clears it.  Synchronizes. */
+int fl_gemm_fault(int *fault);
+
 #ifdef __cplusplus
 }
 #endif
