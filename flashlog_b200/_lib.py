@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libflashlog_b200.so")
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["api.cu", "scan.cu", "topc.cu", "hop.cu", "rules.cu", "csr.cu", "readout.cu", "masks.cu",
-           "gemm.cu", "linear.cu"]
+           "gemm.cu", "linear.cu", "weights.cu", "muon.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "-fmad=false", "-Xcompiler", "-fPIC", "-shared", "-t", "0"]
 
@@ -104,6 +104,26 @@ class fl_linear(ctypes.Structure):
 
 _LINEAR = ctypes.POINTER(fl_linear)
 
+
+class fl_weights(ctypes.Structure):
+    """Mirror of fl_weights (include/flashlog_b200.h): logits and the rules applied to them."""
+    _fields_ = [("logits", _P), ("bias", _P), ("mask", _P), ("states", _P), ("history", _P), ("ld", _I64),
+                ("bias_ld", _I64), ("mask_ld", _I64), ("n_states", _I64), ("hist_ld", _I64), ("hist", _I64),
+                ("rows", _I64), ("n", _I64), ("tau", ctypes.c_double), ("repetition", ctypes.c_double),
+                ("frequency", ctypes.c_double), ("presence", ctypes.c_double), ("dtype", ctypes.c_int)]
+
+
+_WEIGHTS = ctypes.POINTER(fl_weights)
+
+
+class fl_matrices(ctypes.Structure):
+    """Mirror of fl_matrices (include/flashlog_b200.h): a strided batch of matrices."""
+    _fields_ = [("ptr", _P), ("stride_b1", _I64), ("stride_b2", _I64), ("stride_i", _I64), ("stride_j", _I64)]
+
+
+_MATRICES = ctypes.POINTER(fl_matrices)
+_D = ctypes.c_double
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "fl_last_error": (ctypes.c_char_p, []),
@@ -169,6 +189,14 @@ SIGNATURES = {
     "fl_linear_forward": (ctypes.c_int, [_LINEAR, _P, _I64, _P, _P, _SZ, _P]),
     "fl_linear_backward_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int, ctypes.c_int]),
     "fl_linear_backward": (ctypes.c_int, [_LINEAR, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "fl_relation_weights": (ctypes.c_int, [_WEIGHTS, _P, _P]),
+    "fl_relation_weights_workspace": (_SZ, [_I64, _I64]),
+    "fl_relation_weights_backward": (ctypes.c_int, [_WEIGHTS, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
+    "fl_newton_schulz_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int]),
+    "fl_orthogonalize": (ctypes.c_int, [_MATRICES, _MATRICES, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int,
+                                        _D, _D, _D, _D, _P, _SZ, _P]),
+    "fl_muon_update": (ctypes.c_int, [_MATRICES, _MATRICES, _MATRICES, _MATRICES, _MATRICES, _I64, _I64, _I64, _I64,
+                                      _D, _D, ctypes.c_int, _D, _D, ctypes.c_int, _D, _D, _D, _D, _P, _SZ, _P]),
     "fl_gemm_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
 }
 

@@ -1,10 +1,14 @@
-"""The attention over relation operators: the head that makes its logits.
+"""The attention over relation operators: the head that makes its logits, and the weights made of them.
 
 The models turn a hidden state into a logit for each of the n = 2R + 1
 relation operators with a linear layer (src/model_DRUM_kernel_sp.py:99-110),
 and the hops propagate by the softmax of those logits:
 
-* linear: y = act(x W^T + bias) + residual, in one product with its epilogue.
+* linear: y = act(x W^T + bias) + residual, in one product with its epilogue;
+* relation_weights: the softmax, with what a rule's body may contain built in:
+  penalties for operators that the body has already, a bias per operator, and
+  a mask of the operators that may follow the body's state (such as
+  rules.first_operator_mask).
 
 Everything runs in the library's kernels on the current stream, forward and
 backward, and can be captured in a CUDA graph.
@@ -77,3 +81,86 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none"):
     else:
         y, _ = ops.linear_forward(x, weight, bias, residual, act)
     return y if len(shape) == 2 else y.view(shape)
+
+
+class _RelationWeights(autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, mask, states, history, tau, repetition, frequency, presence):
+        w = ops.relation_weights(logits, bias, mask, states, history, tau, repetition, frequency, presence)
+        ctx.tau, ctx.repetition = tau, repetition
+        # the history matters to the gradient through the sign of penalised logits only
+        ctx.save_for_backward(w, logits, bias, history if repetition != 1.0 else None)
+        return w
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        w, logits, bias, history = ctx.saved_tensors
+        dz = db = None
+        if w.numel() == 0:
+            dz, db = torch.zeros_like(logits), None if bias is None else torch.zeros_like(bias)
+        elif ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            dz, db = ops.relation_weights_backward(w, g, logits, bias, history, ctx.tau, ctx.repetition,
+                                                   ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return dz, db, None, None, None, None, None, None, None
+
+
+def relation_weights(logits, *, tau: float = 1.0, mask=None, states=None, bias=None, history=None,
+                     repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0):
+    """The hops' weights, fp32 [..., n], from logits [..., n] (fp32, fp16 or bf16; 1 <= n <= 65536):
+
+        u = z / repetition (z > 0) or z * repetition (z <= 0) for operators in the row's history, z otherwise
+        u = u - frequency * count - presence * [count > 0] + bias
+        w = softmax(u / tau) over the operators that the mask allows, 0 elsewhere
+
+    history: int64 [..., H], the operators used so far (entries outside [0, n), such as a padding of -1, do not
+    count).  bias: [n] or the logits' shape, of their dtype.  mask: bool or uint8; with states (int64 [...]) a
+    table [S, n] of what may follow each state, and a state outside [0, S) allows nothing; without states [n],
+    or the logits' shape.  A row with nothing left gets weights 0 (it propagates nothing) and gradient 0.  Masked
+    logits may hold anything, NaN included; a NaN or +inf that is not masked makes its row NaN.  Differentiable
+    once, in logits and bias."""
+    if logits.dim() < 1 or logits.dtype not in ops.FL_DTYPE:
+        raise ValueError(f"relation_weights takes float32, float16 or bfloat16 logits [..., n], got {logits.dtype}")
+    lead, n = logits.shape[:-1], logits.shape[-1]
+    if not 1 <= n <= ops.MAX_WEIGHT_COLUMNS:
+        raise ValueError(f"relation_weights: need 1 to {ops.MAX_WEIGHT_COLUMNS} operators, got {n}")
+    tau, repetition, frequency, presence = float(tau), float(repetition), float(frequency), float(presence)
+    # compared as the fp32 values that the kernels use
+    if not (1e-30 < tau < 1e30 and 1e-30 < repetition < 1e30):
+        raise ValueError(f"relation_weights: tau and repetition must be positive, got {tau} and {repetition}")
+    if not (abs(frequency) < 1e30 and abs(presence) < 1e30):
+        raise ValueError(f"relation_weights: penalties must be finite, got {frequency} and {presence}")
+    if bias is not None:
+        if bias.dtype != logits.dtype or bias.shape not in ((n,), logits.shape):
+            raise ValueError(f"relation_weights: bias must be [{n}] or the logits' shape, of their dtype")
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"relation_weights: mask must be bool or uint8, got {mask.dtype}")
+        if states is not None:
+            ok = mask.dim() == 2 and mask.shape[1] == n and mask.shape[0] > 0
+        else:
+            ok = mask.shape in ((n,), logits.shape)
+        if not ok:
+            raise ValueError(f"relation_weights: mask must be [states, {n}] with states, else [{n}] or the logits' "
+                             f"shape, got {tuple(mask.shape)}")
+    if states is not None and (mask is None or states.dtype != torch.int64 or states.shape != lead):
+        raise ValueError(f"relation_weights: states must be int64 {tuple(lead)}, next to a mask")
+    if history is not None and (history.dtype != torch.int64 or history.dim() < 1 or history.shape[:-1] != lead):
+        raise ValueError(f"relation_weights: history must be int64 {tuple(lead)} + [H]")
+    ops._one_device("relation_weights", logits, bias, mask, states, history)
+    z = logits if logits.dim() == 2 else logits.reshape(-1, n)
+    if not (z.stride(1) == 1 and (z.stride(0) >= n or z.shape[0] <= 1)):
+        z = z.contiguous()
+    if bias is not None:
+        bias = bias.contiguous() if bias.dim() == 1 else bias.reshape(-1, n).contiguous()
+    if mask is not None:
+        mask = ops._lines(mask.reshape(-1, n))
+    if states is not None:
+        states = states.reshape(-1).contiguous()
+    if history is not None:
+        history = None if history.shape[-1] == 0 else ops._lines(history.reshape(-1, history.shape[-1]))
+    if torch.is_grad_enabled() and (z.requires_grad or (bias is not None and bias.requires_grad)):
+        w = _RelationWeights.apply(z, bias, mask, states, history, tau, repetition, frequency, presence)
+    else:
+        w = ops.relation_weights(z, bias, mask, states, history, tau, repetition, frequency, presence)
+    return w if logits.dim() == 2 else w.view(logits.shape)

@@ -208,9 +208,9 @@ __device__ __forceinline__ void planes_row(__half *hi, int64_t plane, const floa
 template <typename T>
 __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float (&v)[32], float *stage, int b,
                                             int64_t row0, int64_t col0, int64_t m, int64_t n, int lane) {
-    T *out = static_cast<T *>(e.fin) + b * e.fin_b;
-    const float *base = e.base != nullptr ? e.base + b * e.base_b : nullptr;
-    if (e.fin_i == 1) {  // lane = row is the contiguous direction
+    T *out = static_cast<T *>(e.fin.ptr) + e.fin.at(b, e.nb2);
+    const float *base = e.base.ptr != nullptr ? static_cast<const float *>(e.base.ptr) + e.base.at(b, e.nb2) : nullptr;
+    if (e.fin.i == 1) {  // lane = row is the contiguous direction
         const int64_t row = row0 + lane;
         if (row < m) {
 #pragma unroll
@@ -218,8 +218,8 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
                 const int64_t col = col0 + c;
                 if (col < n) {
                     float x = v[c];
-                    if (base != nullptr) x += e.keep * base[row * e.base_i + col * e.base_j];
-                    out[row + col * e.fin_j] = from_f32<T>(x);
+                    if (base != nullptr) x = fmaf(e.keep, base[row * e.base.i + col * e.base.j], x);
+                    out[row + col * e.fin.j] = from_f32<T>(x);
                 }
             }
         }
@@ -234,8 +234,8 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
         for (int r = 0; r < rows; ++r) {
             const int64_t row = row0 + r;
             float x = stage[r * kStagePad + lane];
-            if (base != nullptr) x += e.keep * base[row * e.base_i + col * e.base_j];
-            out[row * e.fin_i + col * e.fin_j] = from_f32<T>(x);
+            if (base != nullptr) x = fmaf(e.keep, base[row * e.base.i + col * e.base.j], x);
+            out[row * e.fin.i + col * e.fin.j] = from_f32<T>(x);
         }
     }
     __syncwarp();
@@ -270,7 +270,7 @@ struct EpiPlanes {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
         }
-        if (p.fin != nullptr) {
+        if (p.fin.ptr != nullptr) {
             if (p.dtype == kOutF32) final_store<float>(p, v, stage, b, row0, col0, m, n, lane);
             else if (p.dtype == kOutF16) final_store<__half>(p, v, stage, b, row0, col0, m, n, lane);
             else final_store<__nv_bfloat16>(p, v, stage, b, row0, col0, m, n, lane);
@@ -603,7 +603,7 @@ int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, 
 
 int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
                 cudaStream_t st) {
-    FL_REQUIRE(a.planes == 2 && b.planes == 2 && (!s.symmetric || (s.m == s.n && e.fin == nullptr)), "gemm: planes");
+    FL_REQUIRE(a.planes == 2 && b.planes == 2 && (!s.symmetric || (s.m == s.n && e.fin.ptr == nullptr)), "gemm: planes");
     if (s.symmetric) return run_any<2>(s, a, b, EpiPlanes<true>{e}, st);
     return run_any<2>(s, a, b, EpiPlanes<false>{e}, st);
 }

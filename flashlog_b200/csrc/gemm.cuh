@@ -43,9 +43,17 @@ struct LinearEpilogue {
     int dtype, act;
 };
 
+// A batch of matrices in a caller's memory: element (b, i, j) lies at
+// (b / nb2) * .b1 + (b % nb2) * .b2 + i * .i + j * .j (nb2 is shared by the tensors of a call).
+struct Strided {
+    void *ptr;
+    int64_t b1, b2, i, j;
+    __host__ __device__ int64_t at(int64_t b, int64_t nb2) const { return (b / nb2) * b1 + (b % nb2) * b2; }
+};
+
 // Epilogue of a Newton-Schulz product: v = alpha * acc + beta * C[i, j], where
 // C is a 2-plane array, written as planes (mirrored when symmetric), or as the
-// last product's result: out = v * out_scale + keep * base.
+// last product's result: fin = v + keep * base.
 struct PlanesEpilogue {
     float alpha, beta;       // on the accumulator and on the planes' sum
     const __half *c;         // NULL: no C
@@ -55,11 +63,10 @@ struct PlanesEpilogue {
     __half *out2;            // second planes output v * alpha2 + diag on the diagonal, or NULL
     float alpha2, diag;
     int64_t ld2, plane2, batch2;
-    void *fin;               // final output, or NULL; element (b, i, j) at b * fin_b + i * fin_i + j * fin_j
-    int64_t fin_b, fin_i, fin_j;
-    const float *base;       // fin = v + keep * base[...] (fp32 only), or NULL
-    int64_t base_b, base_i, base_j;
+    Strided fin;             // final output (dtype), or no pointer
+    Strided base;            // fin = v + keep * base (fp32 only), or no pointer
     float keep;
+    int64_t nb2;
     int dtype;
 };
 

@@ -1,0 +1,522 @@
+// muon.cu -- orthogonalised updates by Newton-Schulz products.
+//
+// X = U / (|U|_F + eps), then `steps` times X <- a X + (b A + c A^2) X with
+// A = X X^T (the shorter side first): every singular value goes through the odd
+// polynomial a s + b s^3 + c s^5.  The Muon step applies it to
+// U = g + beta m' (or m'), m' = beta m + g:  p <- p (1 - lr wd) - lr scale O.
+//
+// All products run on the tensor cores with both operands as two fp16 planes
+// (22 bits): what a product rounds off is amplified by up to a^steps in the
+// directions of small singular values, so single 16-bit planes would lose two
+// to three digits of the result on matrices whose spectrum decays (7% error
+// measured on a rank-3 matrix with 0.1% noise, 2e-5 with two planes).  The
+// planes are scaled by powers of two: |X| <= 1.3 entries by 2^13, A and
+// b A + c A^2 by 2^12.
+//
+// Two forms, by the sides' ratio r = long / short, in units of 2 short^3
+// operations with symmetric products at half:
+//   direct: X is multiplied in every step:    steps (1.5 r + 0.5)
+//   Gram:   everything but the first and last product is short x short: with
+//           P = a I + b A + c A^2, A <- P A P and Q <- P Q, at the end O = Q X:
+//           1.5 r + 2 steps - 1.5
+// All the short matrices are polynomials of the first A: symmetric, so only
+// their lower triangles are computed.  For five steps the Gram form does less
+// from r = 1.02 on; it is taken from r = 1.5: it works with squared singular
+// values, and nearly square matrices have ones so small that this costs it a
+// digit against the direct form (2e-5 instead of 1e-6 at 75 x 74; at 1.5 the
+// smallest singular value of noise is 0.1 of the largest, and both are alike).
+//
+// Matrices too small to fill a tile run whole in one block, in fp32
+// multiply-adds from shared memory: one launch instead of about fifteen.
+#include <math.h>
+
+#include "gemm.cuh"
+
+namespace fl {
+
+namespace {
+
+constexpr int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
+constexpr float kScaleX = 8192.0f, kScaleA = 4096.0f;
+constexpr int kMaxParts = 1024;
+
+// What the update is made of, in the caller's orientation [m, n].
+struct Source {
+    Strided u;          // the update itself (dtype), or the gradient of a Muon step (fp32)
+    Strided mom;        // momentum in (no pointer: a plain update)
+    Strided mom_out;
+    float beta;
+    int nesterov, dtype;
+    int64_t batch, nb2, m, n;
+};
+
+template <typename T>
+__device__ __forceinline__ float load_as(const void *p, int64_t at) {
+    return to_f32<T>(static_cast<const T *>(p)[at]);
+}
+__device__ __forceinline__ float load_any(const void *p, int64_t at, int dtype) {
+    if (dtype == kOutF32) return load_as<float>(p, at);
+    if (dtype == kOutF16) return load_as<__half>(p, at);
+    return load_as<__nv_bfloat16>(p, at);
+}
+
+// The update's element (i, j); FIRST: also writes the new momentum, which the
+// later passes then read.
+template <bool FIRST>
+__device__ __forceinline__ float update_at(const Source &s, int64_t ub, int64_t mb, int64_t ob, int64_t i, int64_t j) {
+    const float g = load_any(s.u.ptr, ub + i * s.u.i + j * s.u.j, s.dtype);
+    if (s.mom_out.ptr == nullptr) return g;
+    float *out = static_cast<float *>(s.mom_out.ptr) + ob + i * s.mom_out.i + j * s.mom_out.j;
+    float v;
+    if (FIRST) {
+        v = fmaf(s.beta, static_cast<const float *>(s.mom.ptr)[mb + i * s.mom.i + j * s.mom.j], g);
+        *out = v;
+    } else {
+        v = *out;
+    }
+    return s.nesterov ? fmaf(s.beta, v, g) : v;
+}
+
+// Sum of squares over the block in 64 bits, the same on every run.
+__device__ __forceinline__ double block_sum(double v, double *scratch) {
+    v = warp_sum(v);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double r = 0.0;
+    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) r += scratch[i];
+    __syncthreads();
+    return r;
+}
+
+// Pass 1: new momentum, and partial sums of squares of the update: grid (parts, batch).
+__global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double *partial) {
+    __shared__ double scratch[8];
+    const int64_t b = blockIdx.y;
+    const int64_t ub = s.u.at(b, s.nb2), mb = s.mom.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
+    double sum = 0.0;
+    for (int64_t i = blockIdx.x; i < s.m; i += gridDim.x)
+        for (int64_t j = threadIdx.x; j < s.n; j += blockDim.x) {
+            const double v = update_at<true>(s, ub, mb, ob, i, j);
+            sum += v * v;
+        }
+    sum = block_sum(sum, scratch);
+    if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = sum;
+}
+
+// Pass 2: planes of X * 2^13, turned to [short, long]: 32 x 32 tiles, grid (tiles of j, tiles of i, batch).
+__global__ void __launch_bounds__(256) normalize_kernel(const Source s, const double *partial, int parts, double eps,
+                                                        int turned, __half *out, int64_t ld, int64_t plane) {
+    __shared__ double scratch[8];
+    __shared__ float tile[32][33];
+    const int64_t b = blockIdx.z;
+    double sum = 0.0;
+    for (int p = threadIdx.y * 32 + threadIdx.x; p < parts; p += 256) sum += partial[b * parts + p];
+    sum = warp_sum(sum);
+    if (threadIdx.x == 0) scratch[threadIdx.y] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int i = 0; i < 8; ++i) sum += scratch[i];
+    const double scale = static_cast<double>(kScaleX) / (sqrt(sum) + eps);
+    const int64_t ub = s.u.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
+    const int64_t i0 = blockIdx.y * int64_t(32), j0 = blockIdx.x * int64_t(32);
+    __half *hi = out + b * 2 * plane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + threadIdx.x;
+        float v = 0.0f;
+        if (i < s.m && j < s.n) v = static_cast<float>(update_at<false>(s, ub, 0, ob, i, j) * scale);
+        if (turned) {
+            tile[threadIdx.y + 8 * k][threadIdx.x] = v;
+        } else if (i < s.m && j < s.n) {
+            const __half h = __float2half_rn(v);
+            hi[i * ld + j] = h;
+            hi[plane + i * ld + j] = __float2half_rn(v - __half2float(h));
+        }
+    }
+    if (!turned) return;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t j = j0 + threadIdx.y + 8 * k, i = i0 + threadIdx.x;
+        if (i < s.m && j < s.n) {
+            const float v = tile[threadIdx.x][threadIdx.y + 8 * k];
+            const __half h = __float2half_rn(v);
+            hi[j * ld + i] = h;
+            hi[plane + j * ld + i] = __float2half_rn(v - __half2float(h));
+        }
+    }
+}
+
+struct Finish {
+    Strided out, base;  // out = factor * O + keep * base
+    float factor, keep;
+    int dtype;
+};
+
+__device__ __forceinline__ void store_any(void *p, int64_t at, float v, int dtype) {
+    if (dtype == kOutF32) static_cast<float *>(p)[at] = v;
+    else if (dtype == kOutF16) static_cast<__half *>(p)[at] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
+}
+
+// C[i, j] = sum_k A[i, k] * (B_T ? B[j, k] : B[k, j]) from shared memory: 2 x 2
+// outputs a thread, rows and columns strided so that neighbours read neighbours.
+template <bool B_T, typename F>
+__device__ __forceinline__ void small_product(const float *A, int lda, const float *B, int ldb, int rows, int cols,
+                                              int depth, F store) {
+    const int rh = (rows + 1) / 2, ch = (cols + 1) / 2;
+    for (int t = threadIdx.x; t < rh * ch; t += blockDim.x) {
+        const int i0 = t / ch, j0 = t - i0 * ch, i1 = i0 + rh, j1 = j0 + ch;
+        const int i1c = i1 < rows ? i1 : i0, j1c = j1 < cols ? j1 : j0;
+        float s00 = 0.0f, s01 = 0.0f, s10 = 0.0f, s11 = 0.0f;
+        for (int k = 0; k < depth; ++k) {
+            const float a0 = A[i0 * lda + k], a1 = A[i1c * lda + k];
+            const float b0 = B_T ? B[j0 * ldb + k] : B[k * ldb + j0], b1 = B_T ? B[j1c * ldb + k] : B[k * ldb + j1c];
+            s00 = fmaf(a0, b0, s00);
+            s01 = fmaf(a0, b1, s01);
+            s10 = fmaf(a1, b0, s10);
+            s11 = fmaf(a1, b1, s11);
+        }
+        store(i0, j0, s00);
+        if (j1 < cols) store(i0, j1, s01);
+        if (i1 < rows) store(i1, j0, s10);
+        if (i1 < rows && j1 < cols) store(i1, j1, s11);
+    }
+}
+
+// The whole step of one small matrix in one block.
+__global__ void __launch_bounds__(512) small_kernel(const Source s, const Finish f, int turned, int lo, int hi,
+                                                    int steps, float ca, float cb, float cc, double eps) {
+    extern __shared__ float sm[];
+    __shared__ double scratch[16];
+    const int ldx = hi | 1, lda = lo | 1;  // odd pitches: columns fall into different banks
+    float *X = sm, *Y = X + lo * ldx, *A = Y + lo * ldx, *B = A + lo * lda;
+    const int64_t b = blockIdx.x;
+    const int64_t ub = s.u.at(b, s.nb2), mb = s.mom.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
+    const int m = static_cast<int>(s.m), n = static_cast<int>(s.n);
+    double sum = 0.0;
+    for (int t = threadIdx.x; t < m * n; t += blockDim.x) {
+        const int i = t / n, j = t - i * n;
+        const float v = update_at<true>(s, ub, mb, ob, i, j);
+        sum += static_cast<double>(v) * v;
+        X[turned ? j * ldx + i : i * ldx + j] = v;
+    }
+    sum = block_sum(sum, scratch);
+    const double scale = 1.0 / (sqrt(sum) + eps);
+    for (int t = threadIdx.x; t < lo * hi; t += blockDim.x) {
+        const int i = t / hi, j = t - i * hi;
+        X[i * ldx + j] = static_cast<float>(X[i * ldx + j] * scale);
+    }
+    __syncthreads();
+    for (int k = 0; k < steps; ++k) {
+        small_product<true>(X, ldx, X, ldx, lo, lo, hi, [&](int i, int j, float v) { A[i * lda + j] = v; });
+        __syncthreads();
+        small_product<true>(A, lda, A, lda, lo, lo, lo,
+                            [&](int i, int j, float v) { B[i * lda + j] = fmaf(cc, v, cb * A[i * lda + j]); });
+        __syncthreads();
+        small_product<false>(B, lda, X, ldx, lo, hi, lo,
+                             [&](int i, int j, float v) { Y[i * ldx + j] = fmaf(ca, X[i * ldx + j], v); });
+        __syncthreads();
+        float *t = X;
+        X = Y;
+        Y = t;
+    }
+    const int64_t fb = f.out.at(b, s.nb2), bb = f.base.at(b, s.nb2);
+    for (int t = threadIdx.x; t < m * n; t += blockDim.x) {
+        const int i = t / n, j = t - i * n;
+        float v = f.factor * X[turned ? j * ldx + i : i * ldx + j];
+        if (f.base.ptr != nullptr)
+            v = fmaf(f.keep, static_cast<const float *>(f.base.ptr)[bb + i * f.base.i + j * f.base.j], v);
+        store_any(f.out.ptr, fb + i * f.out.i + j * f.out.j, v, f.dtype);
+    }
+}
+
+size_t small_smem(int64_t lo, int64_t hi) { return (2 * lo * (hi | 1) + 2 * lo * (lo | 1)) * sizeof(float); }
+
+// One block holds the matrix, and its products (fp32 multiply-adds on one SM)
+// take no longer than the tensor path's launches.
+bool is_small(int64_t lo, int64_t hi, int steps) {
+    return small_smem(lo, hi) <= 200 * 1024 && steps * lo * lo * (2 * hi + lo) <= 2500000;
+}
+
+bool use_gram(int64_t lo, int64_t hi, int steps) {
+    const double r = static_cast<double>(hi) / static_cast<double>(lo);
+    return r >= 1.5 && 1.5 * r + 2.0 * steps - 1.5 < steps * (1.5 * r + 0.5);
+}
+
+int parts_of(int64_t batch, int64_t m) {
+    int64_t p = (148 * 8 + batch - 1) / batch;
+    if (p > m) p = m;
+    if (p > kMaxParts) p = kMaxParts;
+    return static_cast<int>(p);
+}
+
+// Largest |x|, |A|, |b A + c A^2|, |A P| and |Q| (the factor O / X) over
+// singular values in [0, 1]: what the fp16 planes have to hold.
+struct Range {
+    double x, a, b, ap, q;
+};
+Range polynomial_range(double ca, double cb, double cc, int steps) {
+    // a function of four numbers that a program hardly ever changes: the last answer is kept
+    thread_local double key[4] = {0, 0, 0, -1};
+    thread_local Range r;
+    if (key[0] == ca && key[1] == cb && key[2] == cc && key[3] == steps) return r;
+    key[0] = ca;
+    key[1] = cb;
+    key[2] = cc;
+    key[3] = steps;
+    r = Range{0, 0, 0, 0, 0};
+    for (int i = 0; i <= 4096; ++i) {
+        double x = i / 4096.0, q = 1.0;
+        for (int k = 0; k < steps; ++k) {
+            const double t = x * x, bt = cb * t + cc * t * t, p = ca + bt;
+            r.x = fmax(r.x, fabs(x));
+            r.a = fmax(r.a, t);
+            r.b = fmax(r.b, fabs(bt));
+            r.ap = fmax(r.ap, fabs(t * p));
+            x *= p;
+            q *= p;
+            r.q = fmax(r.q, fabs(q));
+            if (!(fabs(x) < 1e6)) { r.x = 1e6; return r; }
+        }
+        r.x = fmax(r.x, fabs(x));
+    }
+    return r;
+}
+
+struct Planes {
+    __half *p;
+    int64_t ld, plane;
+    GemmOperand operand(int mn_major) const { return GemmOperand{p, ld, plane, 2 * plane, 2, mn_major}; }
+};
+Planes take_planes(Carve &ws, int64_t batch, int64_t rows, int64_t cols) {
+    Planes p;
+    p.ld = round8(cols);
+    p.plane = rows * p.ld;
+    p.p = ws.take<__half>(batch * 2 * p.plane);
+    return p;
+}
+size_t planes_bytes(int64_t batch, int64_t rows, int64_t cols) {
+    return carve_bytes<__half>(batch * 2 * rows * round8(cols));
+}
+
+GemmShape shape(int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric) {
+    GemmShape s;
+    s.m = m;
+    s.n = n;
+    s.k = k;
+    s.batch = batch;
+    s.symmetric = symmetric;
+    s.kind = kF16;
+    return s;
+}
+
+PlanesEpilogue epilogue(float alpha, const Planes *c, float beta, const Planes *out) {
+    PlanesEpilogue e{};
+    e.alpha = alpha;
+    if (c != nullptr) {
+        e.beta = beta;
+        e.c = c->p;
+        e.c_ld = c->ld;
+        e.c_plane = c->plane;
+        e.c_batch = 2 * c->plane;
+    }
+    if (out != nullptr) {
+        e.out = out->p;
+        e.ld = out->ld;
+        e.plane = out->plane;
+        e.batch = 2 * out->plane;
+    }
+    e.nb2 = 1;
+    return e;
+}
+
+Strided turn(Strided s, bool turned) {
+    if (turned) { const int64_t t = s.i; s.i = s.j; s.j = t; }
+    return s;
+}
+
+int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double cb, double cc, double eps, void *wsp,
+                  size_t ws_bytes, cudaStream_t st) {
+    const bool turned = s.m > s.n;
+    const int64_t lo = turned ? s.n : s.m, hi = turned ? s.m : s.n;
+    const Range r = polynomial_range(ca, cb, cc, steps);
+    FL_REQUIRE(r.x <= 3.0 && r.b <= 12.0 && r.ap <= 12.0 && r.q < 1e9,
+               "newton-schulz: these coefficients do not keep singular values of [0, 1] within 3");
+    const float fa = static_cast<float>(ca), fb = static_cast<float>(cb), fc = static_cast<float>(cc);
+    if (is_small(lo, hi, steps)) {
+        const size_t smem = small_smem(lo, hi);
+        FL_CUDA(cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        launch(small_kernel, static_cast<unsigned>(s.batch), lo * hi >= 2048 ? 512 : 256, smem, st, s, f, turned,
+               static_cast<int>(lo), static_cast<int>(hi), steps, fa, fb, fc, eps);
+        return check_launch("newton-schulz");
+    }
+    FL_REQUIRE(s.batch <= 65535 && (s.m + 31) / 32 <= 65535, "newton-schulz: too large a batch or matrix");
+    Carve ws(wsp, ws_bytes);
+    const int parts = parts_of(s.batch, s.m);
+    double *partial = ws.take<double>(s.batch * parts);
+    const bool gram = use_gram(lo, hi, steps);
+    Planes x = take_planes(ws, s.batch, lo, hi), a = take_planes(ws, s.batch, lo, lo), b = take_planes(ws, s.batch, lo, lo);
+    Planes x2{}, q{}, q2{}, t{};
+    if (gram) {
+        q = take_planes(ws, s.batch, lo, lo);
+        q2 = take_planes(ws, s.batch, lo, lo);
+        t = take_planes(ws, s.batch, lo, lo);
+    } else {
+        x2 = take_planes(ws, s.batch, lo, hi);
+    }
+    FL_REQUIRE(partial && x.p && a.p && b.p && (gram ? t.p != nullptr : x2.p != nullptr), "newton-schulz: workspace too small");
+
+    launch(square_sum_kernel, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial);
+    launch(normalize_kernel, dim3(static_cast<unsigned>((s.n + 31) / 32), static_cast<unsigned>((s.m + 31) / 32),
+                                  static_cast<unsigned>(s.batch)),
+           dim3(32, 8), 0, st, s, partial, parts, eps, static_cast<int>(turned), x.p, x.ld, x.plane);
+    int rc = check_launch("newton-schulz normalize");
+    if (rc) return rc;
+
+    PlanesEpilogue last = epilogue(0.0f, nullptr, 0.0f, nullptr);
+    last.fin = turn(f.out, turned);
+    last.base = turn(f.base, turned);
+    last.keep = f.keep;
+    last.dtype = f.dtype;
+    last.nb2 = s.nb2;
+    const GemmShape square = shape(lo, lo, lo, s.batch, true);
+    // A = X X^T
+    const PlanesEpilogue to_a = epilogue(kScaleA / (kScaleX * kScaleX), nullptr, 0.0f, &a);
+    const GemmShape outer = shape(lo, lo, hi, s.batch, true);
+    if (!gram) {
+        for (int k = 0; k < steps && !rc; ++k) {
+            rc = gemm_planes(outer, x.operand(0), x.operand(0), to_a, st);
+            // B = b A + c A^2
+            if (!rc) rc = gemm_planes(square, a.operand(0), a.operand(0), epilogue(fc / kScaleA, &a, fb, &b), st);
+            if (rc) break;
+            // X <- a X + B X
+            if (k + 1 < steps) {
+                rc = gemm_planes(shape(lo, hi, lo, s.batch, false), b.operand(0), x.operand(1),
+                                 epilogue(1.0f / kScaleA, &x, fa, &x2), st);
+                const Planes u = x;
+                x = x2;
+                x2 = u;
+            } else {
+                PlanesEpilogue e = last;
+                const PlanesEpilogue c = epilogue(0.0f, &x, f.factor * fa / kScaleX, nullptr);
+                e.alpha = f.factor / (kScaleA * kScaleX);
+                e.beta = c.beta;
+                e.c = c.c;
+                e.c_ld = c.c_ld;
+                e.c_plane = c.c_plane;
+                e.c_batch = c.c_batch;
+                rc = gemm_planes(shape(lo, hi, lo, s.batch, false), b.operand(0), x.operand(1), e, st);
+            }
+        }
+        return rc;
+    }
+    // Gram form.  Q's scale leaves room for its largest factor (a^steps in the null space).
+    const float scale_q = exp2f(floorf(log2f(32768.0f / static_cast<float>(r.q))));
+    rc = gemm_planes(outer, x.operand(0), x.operand(0), to_a, st);
+    for (int k = 0; k < steps && !rc; ++k) {
+        PlanesEpilogue e = epilogue(fc / kScaleA, &a, fb, &b);  // B = b A + c A^2
+        if (k == 0) {                                           // and Q = a I + B
+            e.out2 = q.p;
+            e.ld2 = q.ld;
+            e.plane2 = q.plane;
+            e.batch2 = 2 * q.plane;
+            e.alpha2 = scale_q / kScaleA;
+            e.diag = fa * scale_q;
+        }
+        rc = gemm_planes(square, a.operand(0), a.operand(0), e, st);
+        if (!rc && k > 0) {  // Q <- a Q + B Q
+            rc = gemm_planes(square, b.operand(0), q.operand(0), epilogue(1.0f / kScaleA, &q, fa, &q2), st);
+            const Planes u = q;
+            q = q2;
+            q2 = u;
+        }
+        if (!rc && k + 1 < steps) {  // A <- P A P: T = a A + B A, A = a T + T B
+            rc = gemm_planes(square, b.operand(0), a.operand(0), epilogue(1.0f / kScaleA, &a, fa, &t), st);
+            if (!rc) rc = gemm_planes(square, t.operand(0), b.operand(0), epilogue(1.0f / kScaleA, &t, fa, &a), st);
+        }
+    }
+    if (rc) return rc;
+    last.alpha = f.factor / (scale_q * kScaleX);
+    return gemm_planes(shape(lo, hi, lo, s.batch, false), q.operand(0), x.operand(1), last, st);
+}
+
+Strided strided(const fl_matrices *t) {
+    if (t == nullptr) return Strided{nullptr, 0, 0, 0, 0};
+    return Strided{t->ptr, t->stride_b1, t->stride_b2, t->stride_i, t->stride_j};
+}
+
+int check_batch(int64_t b1, int64_t b2, int64_t m, int64_t n, int steps) {
+    FL_REQUIRE(b1 >= 0 && b2 >= 0 && m > 0 && n > 0 && m < (1 << 24) && n < (1 << 24), "newton-schulz: bad shape");
+    FL_REQUIRE(steps >= 1 && steps <= 64, "newton-schulz: 1 to 64 steps");
+    return FL_OK;
+}
+
+}  // namespace
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" {
+
+size_t fl_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n, int steps) {
+    if (batch <= 0 || m <= 0 || n <= 0) return 0;
+    const int64_t lo = m < n ? m : n, hi = m < n ? n : m;
+    if (is_small(lo, hi, steps)) return 0;
+    size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + planes_bytes(batch, lo, hi) + 2 * planes_bytes(batch, lo, lo);
+    return b + (use_gram(lo, hi, steps) ? 3 * planes_bytes(batch, lo, lo) : planes_bytes(batch, lo, hi));
+}
+
+int fl_orthogonalize(const fl_matrices *in, const fl_matrices *out, int64_t b1, int64_t b2, int64_t m, int64_t n,
+                     int dtype, int steps, double a, double b, double c, double eps, void *ws, size_t ws_bytes,
+                     fl_stream_t stream) {
+    int rc = check_batch(b1, b2, m, n, steps);
+    if (rc) return rc;
+    FL_REQUIRE(dtype == FL_F32 || dtype == FL_F16 || dtype == FL_BF16, "orthogonalize: bad dtype %d", dtype);
+    if (b1 * b2 == 0) return FL_OK;
+    FL_REQUIRE(in != nullptr && out != nullptr && in->ptr != nullptr && out->ptr != nullptr, "orthogonalize: null matrix");
+    Source s{};
+    s.u = strided(in);
+    s.dtype = dtype;
+    s.batch = b1 * b2;
+    s.nb2 = b2;
+    s.m = m;
+    s.n = n;
+    Finish f{};
+    f.out = strided(out);
+    f.factor = 1.0f;
+    f.dtype = dtype;
+    return newton_schulz(s, f, steps, a, b, c, eps, ws, ws_bytes, as_stream(stream));
+}
+
+int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_matrices *momentum,
+                   const fl_matrices *param_out, const fl_matrices *momentum_out, int64_t b1, int64_t b2, int64_t m,
+                   int64_t n, double lr, double beta, int nesterov, double weight_decay, double scale, int steps,
+                   double a, double b, double c, double eps, void *ws, size_t ws_bytes, fl_stream_t stream) {
+    int rc = check_batch(b1, b2, m, n, steps);
+    if (rc) return rc;
+    if (b1 * b2 == 0) return FL_OK;
+    FL_REQUIRE(param && grad && momentum && param_out && momentum_out && param->ptr && grad->ptr && momentum->ptr &&
+                   param_out->ptr && momentum_out->ptr,
+               "muon_update: null matrix");
+    Source s{};
+    s.u = strided(grad);
+    s.mom = strided(momentum);
+    s.mom_out = strided(momentum_out);
+    s.beta = static_cast<float>(beta);
+    s.nesterov = nesterov;
+    s.dtype = FL_F32;
+    s.batch = b1 * b2;
+    s.nb2 = b2;
+    s.m = m;
+    s.n = n;
+    Finish f{};
+    f.out = strided(param_out);
+    f.base = strided(param);
+    f.factor = static_cast<float>(-lr * scale);
+    f.keep = static_cast<float>(1.0 - lr * weight_decay);
+    f.dtype = FL_F32;
+    return newton_schulz(s, f, steps, a, b, c, eps, ws, ws_bytes, as_stream(stream));
+}
+
+}  // extern "C"

@@ -762,6 +762,146 @@ def linear_backward(x, weight, z, gy, act: int = L.FL_ACT_NONE, want=(True, True
     return dx, dw, db
 
 
+MAX_WEIGHT_COLUMNS = 65536
+
+
+def _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence):
+    rows, n = logits.shape
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    return L.fl_weights(logits.data_ptr(), ptr(bias), ptr(mask), ptr(states), ptr(history), _ld(logits),
+                        0 if bias is None or bias.dim() == 1 else n, 0 if mask is None else _ld(mask),
+                        0 if mask is None else mask.shape[0], 0 if history is None else _ld(history),
+                        0 if history is None else history.shape[1], rows, n, tau, repetition, frequency, presence,
+                        FL_DTYPE[logits.dtype])
+
+
+def relation_weights(logits, bias=None, mask=None, states=None, history=None, tau=1.0, repetition=1.0, frequency=0.0,
+                     presence=0.0):
+    """fl_relation_weights on 2-D tensors: logits [rows, n] (unit inner
+    stride), bias [n] or [rows, n], mask bool or uint8 [states, n], states
+    int64 [rows], history int64 [rows, H].  Returns f32 [rows, n]."""
+    dev = _one_device("relation weights", logits, bias, mask, states, history)
+    w = torch.empty(logits.shape, dtype=torch.float32, device=dev)
+    if w.numel() == 0:
+        return w
+    p = _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence)
+    with _on(dev) as st:
+        rc = lib().fl_relation_weights(ctypes.byref(p), w.data_ptr(), st)
+    check(rc, "relation weights")
+    return w
+
+
+def relation_weights_backward(w, g, logits, bias=None, history=None, tau=1.0, repetition=1.0, want_logits=True,
+                              want_bias=False):
+    """(dlogits, dbias) of relation_weights for the gradient g f32 [rows, n]
+    (rows may share one line: stride 0)."""
+    dev = _one_device("relation weights backward", w, g, logits, bias, history)
+    rows, n = w.shape
+    dz = torch.empty((rows, n), dtype=logits.dtype, device=dev) if want_logits else None
+    db = torch.empty_like(bias) if want_bias else None
+    if g.stride(1) != 1:
+        g = g.contiguous()
+    p = _weights_params(logits, bias, None, None, history, tau, repetition, 0.0, 0.0)
+    nbytes = lib().fl_relation_weights_workspace(rows, n) if want_bias and bias.dim() == 1 else 0
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as st:
+        rc = lib().fl_relation_weights_backward(ctypes.byref(p), w.data_ptr(), g.data_ptr(), g.stride(0),
+                                                None if dz is None else dz.data_ptr(),
+                                                None if db is None else db.data_ptr(),
+                                                None if ws is None else ws.data_ptr(), nbytes, st)
+    check(rc, "relation weights backward")
+    return dz, db
+
+
+def _batch_dims(t):
+    """[..., m, n] as (b1, b2, strides) with at most two strided batch dimensions, or None when its leading
+    dimensions need more."""
+    dims = [(n, s) for n, s in zip(t.shape[:-2], t.stride()[:-2]) if n != 1]
+    merged = []
+    for n, s in dims:
+        if merged and merged[-1][1] == n * s:
+            merged[-1] = (merged[-1][0] * n, s)
+        else:
+            merged.append((n, s))
+    return merged if len(merged) <= 2 else None
+
+
+def _as_batch(ts):
+    """A common (b1, b2) of tensors [..., m, n] of one shape, with each one's fl_matrices; None when the strides
+    of some cannot be expressed."""
+    lead = ts[0].shape[:-2]
+    total = 1
+    for n in lead:
+        total *= n
+    split = 1  # b2: the innermost batch dimensions that every tensor holds at one stride
+    for t in ts:
+        dims = _batch_dims(t)
+        if dims is None:
+            return None
+        if len(dims) == 2:
+            if split not in (1, dims[1][0]):
+                return None
+            split = dims[1][0]
+    out = []
+    for t in ts:
+        dims = _batch_dims(t)
+        if len(dims) == 2:
+            s1, s2 = dims[0][1], dims[1][1]
+        else:
+            s2 = dims[0][1] if dims else 0
+            s1 = s2 * split
+        out.append(L.fl_matrices(t.data_ptr(), s1, s2, t.stride(-2), t.stride(-1)))
+    return (total // split if split else 0), split, out
+
+
+def orthogonalize(update, steps: int, coefficients, eps: float):
+    """fl_orthogonalize of update [..., m, n]: a new contiguous tensor of its dtype."""
+    dev = _one_device("orthogonalize", update)
+    out = torch.empty(update.shape, dtype=update.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    got = _as_batch((update, out))
+    if got is None:  # strides that two batch dimensions cannot express
+        update = update.contiguous()
+        got = _as_batch((update, out))
+    b1, b2, (src, dst) = got
+    m, n = update.shape[-2:]
+    a, b, c = coefficients
+    nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as st:
+        rc = lib().fl_orthogonalize(ctypes.byref(src), ctypes.byref(dst), b1, b2, m, n, FL_DTYPE[update.dtype], steps,
+                                    a, b, c, eps, None if ws is None else ws.data_ptr(), nbytes, st)
+    check(rc, "orthogonalize")
+    return out
+
+
+def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nesterov, weight_decay, scale, steps,
+                coefficients, eps):
+    """fl_muon_update of fp32 tensors [..., m, n] of one shape, into the two outputs."""
+    dev = _one_device("muon_update", param, grad, momentum, param_out, momentum_out)
+    if param.numel() == 0:
+        return
+    got = _as_batch((param, grad, momentum, param_out, momentum_out))
+    if got is None:  # strides that two batch dimensions cannot express: through plain copies
+        p2, m2 = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (param_out, momentum_out))
+        muon_update(param.contiguous(), grad.contiguous(), momentum.contiguous(), p2, m2, lr=lr, beta=beta,
+                    nesterov=nesterov, weight_decay=weight_decay, scale=scale, steps=steps,
+                    coefficients=coefficients, eps=eps)
+        param_out.copy_(p2)
+        momentum_out.copy_(m2)
+        return
+    b1, b2, ts = got
+    m, n = param.shape[-2:]
+    a, b, c = coefficients
+    nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on(dev) as st:
+        rc = lib().fl_muon_update(*(ctypes.byref(t) for t in ts), b1, b2, m, n, lr, beta, int(nesterov), weight_decay,
+                                  scale, steps, a, b, c, eps, None if ws is None else ws.data_ptr(), nbytes, st)
+    check(rc, "muon_update")
+
+
 def gemm_fault() -> bool:
     """Whether a bounded wait of a matrix product ran out since the last call (synchronizes)."""
     f = ctypes.c_int(0)

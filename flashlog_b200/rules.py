@@ -66,6 +66,28 @@ def available_first_operators(sources, csr_struct, relations: int):
     return avail
 
 
+def first_operator_mask(sources, csr_struct, relations: int):
+    """bool [len(sources), 2R + 1]: available_first_operators of each source by
+    itself, as a mask for attention.relation_weights (a first hop along any
+    other operator reaches nothing).  No host synchronization."""
+    c = tuple(csr_struct)
+    s = sources.to(torch.int64)
+    n = 2 * relations + 1
+    avail = torch.zeros((s.numel(), n), dtype=torch.bool, device=s.device)
+    for gptr, grel, off in ((c[8], c[9], 0), (c[12], c[13], relations)):
+        groups = grel.numel()
+        if groups == 0:
+            continue
+        a, b = gptr[s].to(torch.int64), gptr[s + 1].to(torch.int64)
+        # a source has at most one group per relation
+        idx = a[:, None] + torch.arange(min(relations, groups), device=s.device)
+        cols = grel[idx.clamp_max(groups - 1)].to(torch.int64) + off
+        # absent groups write the identity's column, which is set anyway
+        avail.scatter_(1, torch.where(idx < b[:, None], cols, torch.full_like(cols, n - 1)), True)
+    avail[:, n - 1] = True
+    return avail
+
+
 def _weights_and_ops(rules, relations, dev):
     ranks = len(rules[0]["rank_weights"])
     weights = torch.tensor([list(r["rank_weights"]) for r in rules], dtype=torch.float32, device=dev)

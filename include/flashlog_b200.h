@@ -494,6 +494,65 @@ size_t fl_linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtyp
 int fl_linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw,
                        void *dbias, void *ws, size_t ws_bytes, fl_stream_t stream);
 
+/* The hops' weights from relation logits [rows, n] (n <= 65536, the int16
+ * relation limit of the CSR): with z a logit, count its operator's occurrences
+ * in the row's history,
+ *   u = z > 0 ? z / repetition : z * repetition   where count > 0, z elsewhere
+ *   u = u - frequency * count - presence * [count > 0] + bias
+ *   w = softmax(u / tau) over the operators that the mask allows, 0 elsewhere;
+ * a row that the mask (or -inf logits) leaves empty is all 0.  Masked logits
+ * and biases are not read into the result, whatever they hold. */
+typedef struct fl_weights {
+    const void *logits;      /* dtype, ld elements between rows                  */
+    const void *bias;        /* dtype: [n] (bias_ld 0), [rows, n], or NULL       */
+    const void *mask;        /* u8 [n_states, n], nonzero: allowed; or NULL      */
+    const int64_t *states;   /* [rows]: each row's mask row (one out of range
+                                allows nothing); NULL: row r has mask row
+                                min(r, n_states - 1)                             */
+    const int64_t *history;  /* [rows, hist] operators used so far; entries
+                                outside [0, n) (padding) do not count; or NULL   */
+    int64_t ld, bias_ld, mask_ld, n_states, hist_ld, hist, rows, n;
+    double tau, repetition, frequency, presence;
+    int dtype;
+} fl_weights;
+
+/* w f32 [rows, n], contiguous. */
+int fl_relation_weights(const fl_weights *p, float *w, fl_stream_t stream);
+
+/* Gradients for g f32 [rows, n] (ld_g elements between rows; 0: one row for
+ * all): dlogits [rows, n] or NULL, dbias of the bias' shape or NULL, in dtype.
+ * An operator of weight 0 gets and passes nothing.  Sums over rows run in a
+ * fixed order.  The workspace serves a bias of shape [n]. */
+size_t fl_relation_weights_workspace(int64_t rows, int64_t n);
+int fl_relation_weights_backward(const fl_weights *p, const float *w, const float *g, int64_t ld_g, void *dlogits,
+                                 void *dbias, void *ws, size_t ws_bytes, fl_stream_t stream);
+
+/* A batch of b1 * b2 matrices: element (p, q, i, j) lies at
+ * p * stride_b1 + q * stride_b2 + i * stride_i + j * stride_j (in elements). */
+typedef struct fl_matrices {
+    void *ptr;
+    int64_t stride_b1, stride_b2, stride_i, stride_j;
+} fl_matrices;
+
+/* Newton-Schulz orthogonalisation of each [m, n] matrix U of the batch:
+ * X = U / (|U|_F + eps), then `steps` times X = a X + (b A + c A^2) X with
+ * A = X X^T (of the shorter side), to fp32 accuracy for every dtype, rounded
+ * once into `out`.  The coefficients must keep singular values of [0, 1]
+ * within 3. */
+size_t fl_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n, int steps);
+int fl_orthogonalize(const fl_matrices *in, const fl_matrices *out, int64_t b1, int64_t b2, int64_t m, int64_t n,
+                     int dtype, int steps, double a, double b, double c, double eps, void *ws, size_t ws_bytes,
+                     fl_stream_t stream);
+
+/* One Muon step, all f32: momentum_out = beta * momentum + grad; U =
+ * grad + beta * momentum_out (nesterov) or momentum_out; param_out = param *
+ * (1 - lr * weight_decay) - lr * scale * orthogonalised(U).  The outputs may
+ * be the inputs (element for element). */
+int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_matrices *momentum,
+                   const fl_matrices *param_out, const fl_matrices *momentum_out, int64_t b1, int64_t b2, int64_t m,
+                   int64_t n, double lr, double beta, int nesterov, double weight_decay, double scale, int steps,
+                   double a, double b, double c, double eps, void *ws, size_t ws_bytes, fl_stream_t stream);
+
 /* 1 if a bounded wait of a matrix-product kernel ran out since the last call
  * (its outputs hold NaN), else 0, in *fault; clears it.  Synchronizes. */
 int fl_gemm_fault(int *fault);
