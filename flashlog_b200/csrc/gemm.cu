@@ -6,7 +6,7 @@
 // (128 + BN/2) lines for 128 x BN outputs; with one CTA per tile the L2 -> SM
 // traffic would be 1.5 times that, above what the L2 delivers at the full
 // matrix rate.  Roles per CTA: one warp loads by TMA (128-byte swizzle), one
-// warp (of the pair's first CTA) issues the matrix instructions, four warps
+// warp (of the pair's first CTA) issues the matrix instructions, eight warps
 // read the accumulators back (two TMEM buffers, so a tile's epilogue runs
 // under the next tile's products).  Waits are bounded: one that runs out marks
 // the device fault word, and the tiles left get NaN.
@@ -20,8 +20,10 @@ namespace {
 
 constexpr int kBM = 128;        // rows of A per CTA
 constexpr int kBK = 64;         // contraction per stage: one 128-byte swizzle line
-constexpr int kThreads = 192;   // warps 0-3: epilogue, 4: loads, 5: products
-constexpr int kStageBudget = 200 * 1024;
+constexpr int kEpiWarps = 8;    // warp w reads TMEM lanes 32 (w % 4).., columns of half w / 4
+constexpr int kLoadWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
+constexpr int kThreads = 32 * (kEpiWarps + 2);
+constexpr int kStageBudget = 196 * 1024;
 constexpr int kStagePad = 33;   // row pitch (words) of the epilogue's transposing tile
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // four seconds: far above any wait between healthy roles
 
@@ -139,39 +141,142 @@ __device__ __forceinline__ void tile_of(const TileGrid &g, int t, int &b, int &t
 }
 
 // ---- epilogues: 32 rows x 32 columns per call, lane = row, v[c] = column c -----
-template <typename T>
-__device__ __forceinline__ void linear_store(const LinearEpilogue &e, const float (&v)[32], float *stage, int64_t row0,
-                                             int64_t col0, int64_t m, int64_t n, int lane) {
+template <int N>
+__device__ __forceinline__ void apply_act(float (&z)[N], int act) {
+    if (act == kActNone) return;
+    if (act == kActRelu) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c) stage[lane * kStagePad + c] = v[c];
-    __syncwarp();
-    const int64_t col = col0 + lane;
-    const bool in = col < n;
-    const float bias = in && e.bias != nullptr ? to_f32(static_cast<const T *>(e.bias)[col]) : 0.0f;
-    const int eb = in && e.col_exp != nullptr ? e.col_exp[col] : 0;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
-    if (in) {
-        for (int r = 0; r < rows; ++r) {
-            const int64_t row = row0 + r;
-            float z = stage[r * kStagePad + lane];
-            if (e.row_exp != nullptr) z = scale_pow2(z, e.row_exp[row] + eb);
-            z += bias;
-            if (e.z != nullptr) e.z[row * e.ld_z + col] = z;
-            float y = act_value(z, e.act);
-            if (e.residual != nullptr) y += to_f32(static_cast<const T *>(e.residual)[row * e.ld_res + col]);
-            static_cast<T *>(e.out)[row * e.ld_out + col] = from_f32<T>(y);
+        for (int i = 0; i < N; ++i) z[i] = act_value(z[i], kActRelu);
+    } else if (act == kActTanh) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = act_value(z[i], kActTanh);
+    } else if (act == kActSilu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = act_value(z[i], kActSilu);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = act_value(z[i], kActGelu);
+    }
+}
+
+// Lane = column (or a pair of columns, two rows at a time, for 16-bit types
+// whose rows are 4-byte aligned): the warp's stores are whole 64- or 128-byte
+// pieces of a row at any alignment.  Eight rows are in flight at once.
+template <typename T, bool PAIR>
+__device__ __forceinline__ void linear_rows(const LinearEpilogue &e, const float *stage, int64_t row0, int64_t col0,
+                                            int rows, int64_t n, int lane, bool exact_scale, int row_exp) {
+    constexpr int kW = PAIR ? 2 : 1;              // columns per lane
+    const int sub = PAIR ? lane >> 4 : 0;         // which of the two rows
+    const int lc = PAIR ? (lane & 15) * 2 : lane;
+    const int64_t col = col0 + lc;
+    float bias[kW], factor[kW];
+    int ce[kW];
+    bool in[kW];
+#pragma unroll
+    for (int w = 0; w < kW; ++w) {
+        in[w] = col + w < n;
+        bias[w] = in[w] && e.bias != nullptr ? to_f32(static_cast<const T *>(e.bias)[col + w]) : 0.0f;
+        ce[w] = in[w] && e.col_exp != nullptr ? e.col_exp[col + w] : 0;
+        factor[w] = exact_scale ? 1.0f : __int_as_float((ce[w] + 127) << 23);
+    }
+    constexpr int kRows = 8;                      // rows per batch (per half warp: 2 kRows in all)
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += kRows * kW) {
+        float z[kRows * kW], res[kRows * kW];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int r = r0 + k * kW + sub;
+#pragma unroll
+            for (int w = 0; w < kW; ++w) {
+                z[k * kW + w] = stage[r * kStagePad + lc + w];
+                res[k * kW + w] = 0.0f;
+            }
+        }
+        if (e.residual != nullptr) {
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                const int r = r0 + k * kW + sub;
+                const T *p = static_cast<const T *>(e.residual) + (row0 + r) * e.ld_res + col;
+                if (PAIR) {
+                    if (r < rows && in[kW - 1]) {
+                        union { unsigned u; T t[2]; } x;
+                        x.u = *reinterpret_cast<const unsigned *>(p);
+                        res[k * kW] = to_f32(x.t[0]);
+                        res[k * kW + kW - 1] = to_f32(x.t[1]);
+                    } else if (r < rows && in[0]) {
+                        res[k * kW] = to_f32(p[0]);
+                    }
+                } else if (r < rows && in[0]) {
+                    res[k] = to_f32(p[0]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kRows; ++k)
+#pragma unroll
+            for (int w = 0; w < kW; ++w) {
+                float x = z[k * kW + w];
+                if (exact_scale) {
+                    const int re = __shfl_sync(kFull, row_exp, r0 + k * kW + sub);
+                    x = scale_pow2(x, re + ce[w]);
+                } else {
+                    x *= factor[w];
+                }
+                z[k * kW + w] = x + bias[w];
+            }
+        if (e.z != nullptr) {
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                const int r = r0 + k * kW + sub;
+                float *p = e.z + (row0 + r) * e.ld_z + col;
+#pragma unroll
+                for (int w = 0; w < kW; ++w)
+                    if (r < rows && in[w]) p[w] = z[k * kW + w];
+            }
+        }
+        apply_act(z, e.act);
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const int r = r0 + k * kW + sub;
+            T *p = static_cast<T *>(e.out) + (row0 + r) * e.ld_out + col;
+            if (PAIR && r < rows && in[kW - 1]) {
+                union { unsigned u; T t[2]; } x;
+                x.t[0] = from_f32<T>(z[k * kW] + res[k * kW]);
+                x.t[PAIR ? 1 : 0] = from_f32<T>(z[k * kW + kW - 1] + res[k * kW + kW - 1]);
+                *reinterpret_cast<unsigned *>(p) = x.u;
+            } else if (r < rows && in[0]) {
+                p[0] = from_f32<T>(z[k * kW] + res[k * kW]);
+            }
         }
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)[32], float *stage, int64_t row0,
+                                             int64_t col0, int64_t m, int64_t n, int lane) {
+    // exponents within +-60 multiply in two exact steps; larger ones take the slow exact form
+    int re = 0, ce = 0;
+    if (e.row_exp != nullptr) {
+        if (row0 + lane < m) re = e.row_exp[row0 + lane];
+        if (col0 + lane < n) ce = e.col_exp[col0 + lane];
+    }
+    const bool exact_scale = __any_sync(kFull, re > 60 || re < -60 || ce > 60 || ce < -60);
+    const float rf = exact_scale ? 1.0f : __int_as_float((re + 127) << 23);
+#pragma unroll
+    for (int c = 0; c < 32; ++c) stage[lane * kStagePad + c] = v[c] * rf;
+    __syncwarp();
+    const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
+    if (sizeof(T) == 2 && e.pair) linear_rows<T, sizeof(T) == 2>(e, stage, row0, col0, rows, n, lane, exact_scale, re);
+    else linear_rows<T, false>(e, stage, row0, col0, rows, n, lane, exact_scale, re);
     __syncwarp();
 }
 
+template <typename T>
 struct EpiLinear {
     LinearEpilogue p;
-    __device__ __forceinline__ void operator()(const float (&v)[32], float *stage, int, int64_t row0, int64_t col0,
+    __device__ __forceinline__ void operator()(float (&v)[32], float *stage, int, int64_t row0, int64_t col0,
                                                int64_t m, int64_t n, int lane) const {
-        if (p.dtype == kOutF32) linear_store<float>(p, v, stage, row0, col0, m, n, lane);
-        else if (p.dtype == kOutF16) linear_store<__half>(p, v, stage, row0, col0, m, n, lane);
-        else linear_store<__nv_bfloat16>(p, v, stage, row0, col0, m, n, lane);
+        linear_store<T>(p, v, stage, row0, col0, m, n, lane);
     }
 };
 
@@ -323,7 +428,7 @@ struct Config {
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
     static constexpr int kStage = PLANES * (kA + kB);
     static constexpr int kStages = kStageBudget / kStage > 8 ? 8 : kStageBudget / kStage;
-    static constexpr int kSmem = kStages * kStage + 4 * 32 * kStagePad * 4 + 1024;
+    static constexpr int kSmem = kStages * kStage + kEpiWarps * 32 * kStagePad * 4 + 1024;
 };
 
 template <int BN, int PLANES, typename Epi>
@@ -353,11 +458,11 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         for (int s = 0; s < 2; ++s) {
             bar_init(acc_full + 8 * s, 1);
-            bar_init(acc_empty + 8 * s, 8);  // four warps of each CTA
+            bar_init(acc_empty + 8 * s, 2 * kEpiWarps);  // of both CTAs
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 5) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
                      "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -369,7 +474,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const uint32_t tmem = tmem_slot;
     const int kblocks = static_cast<int>((k + kBK - 1) / kBK);
 
-    if (warp == 4 && lane == 0) {
+    if (warp == kLoadWarp && lane == 0) {
         // ---- loads ----
         int s = 0;
         uint32_t phase = 0;
@@ -414,7 +519,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             ok = bar_wait(empty + 8 * s, phase ^ 1, &failed);
             if (++s == C::kStages) { s = 0; phase ^= 1; }
         }
-    } else if (warp == 5 && cta == 0 && lane == 0) {
+    } else if (warp == kMmaWarp && cta == 0 && lane == 0) {
         // ---- products (for the pair) ----
         const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;  // 16 of k, in 16-byte units
         const uint32_t a_lbo = a_mn ? 8192u : 16u, b_lbo = b_mn ? 8192u : 16u;
@@ -453,7 +558,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             mma_commit(acc_full + 8 * buf);
             if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
-    } else if (warp < 4) {
+    } else if (warp < kEpiWarps) {
         // ---- epilogue ----
         float *stage = stage_epi + warp * 32 * kStagePad;
         int buf = 0;
@@ -462,13 +567,14 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         for (int t = pair; t < grid.total; t += pairs) {
             int b, ti, tj;
             tile_of<BN>(grid, t, b, ti, tj);
-            const int64_t row0 = static_cast<int64_t>(ti) * 2 * kBM + cta * kBM + warp * 32;
+            const int64_t row0 = static_cast<int64_t>(ti) * 2 * kBM + cta * kBM + (warp & 3) * 32;
             const int64_t col0 = static_cast<int64_t>(tj) * BN;
             if (ok) ok = bar_wait(acc_full + 8 * buf, acc_phase, &failed);
             ok = __all_sync(kFull, ok);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>(warp * 32) << 16);
-            for (int c = 0; c < BN; c += 32) {
+            const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const int half = (warp >> 2) * (BN / 2);
+            for (int c = half; c < half + BN / 2; c += 32) {
                 float v[32];
                 if (ok) {
                     tmem_read32(v, src + c);
@@ -489,7 +595,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     cluster_sync();
-    if (warp == 5) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
     }
@@ -542,6 +648,15 @@ int operand_map(CUtensorMap *map, const GemmOperand &o, int64_t lines_mn, int64_
     return FL_OK;
 }
 
+// Tiles of one matrix of the batch.
+int64_t tile_count(const GemmShape &s, int bn) {
+    const int64_t tm = (s.m + 2 * kBM - 1) / (2 * kBM), tn = (s.n + bn - 1) / bn;
+    if (!s.symmetric) return tm * tn;
+    int64_t per = 0;
+    for (int64_t i = 0; i < tm; ++i) per += (i + 1) * (2 * kBM / bn) < tn ? (i + 1) * (2 * kBM / bn) : tn;
+    return per;
+}
+
 template <int BN, int PLANES, typename Epi>
 int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, cudaStream_t st) {
     using C = Config<BN, PLANES>;
@@ -556,11 +671,7 @@ int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Ep
     g.symmetric = s.symmetric;
     g.batch = static_cast<int>(s.batch);
     g.n_fast = g.tiles_n <= g.tiles_m;  // the operand with fewer tiles is the one read again and again, from L2
-    int64_t per = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-    if (s.symmetric) {
-        per = 0;
-        for (int i = 0; i < g.tiles_m; ++i) per += (i + 1) * (2 * kBM / BN) < g.tiles_n ? (i + 1) * (2 * kBM / BN) : g.tiles_n;
-    }
+    const int64_t per = tile_count(s, BN);
     FL_REQUIRE(per * s.batch < (1 << 30), "gemm: too many tiles");
     g.per_batch = static_cast<int>(per);
     g.total = static_cast<int>(per * s.batch);
@@ -579,26 +690,39 @@ int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Ep
     return check_launch("gemm");
 }
 
-// 256-wide tiles when they fill the pairs of SMs at least twice over (or the
-// matrix is that wide only), else 128-wide ones.
+// 256-wide or 128-wide tiles: whichever needs less time on the slowest pair of
+// SMs, 256 when equal (half the loads of A per product).
 template <int PLANES, typename Epi>
 int run_any(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, cudaStream_t st) {
     FL_REQUIRE(s.m > 0 && s.n > 0 && s.k > 0 && s.batch > 0 && s.m < (1ll << 31) - 512 && s.n < (1ll << 31) - 512 &&
                    s.k < (1ll << 31) - 512 && s.batch < (1ll << 31),
                "gemm: bad shape");
-    const int64_t tm = (s.m + 255) / 256, tn = (s.n + 255) / 256;
-    const int64_t tiles = (s.symmetric ? (tm * (tm + 1)) / 2 : tm * tn) * s.batch;
-    if (tiles >= 74) return run<256, PLANES, Epi>(s, a, b, epi, st);
+    const int sms = fl_device_sm_count();
+    const int64_t pairs = (sms > 1 ? sms : 148) / 2;
+    const int64_t wide = (tile_count(s, 256) * s.batch + pairs - 1) / pairs;
+    const int64_t narrow = (tile_count(s, 128) * s.batch + pairs - 1) / pairs;
+    if (2 * wide <= narrow) return run<256, PLANES, Epi>(s, a, b, epi, st);
     return run<128, PLANES, Epi>(s, a, b, epi, st);
+}
+
+template <typename T>
+int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
+                 cudaStream_t st) {
+    EpiLinear<T> epi{e};
+    epi.p.pair = (reinterpret_cast<uintptr_t>(e.out) & 3) == 0 && (e.ld_out & 1) == 0 &&
+                 (e.residual == nullptr || ((reinterpret_cast<uintptr_t>(e.residual) & 3) == 0 && (e.ld_res & 1) == 0));
+    return run_any<sizeof(T) == 4 ? 2 : 1>(s, a, b, epi, st);
 }
 
 }  // namespace
 
 int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
                 cudaStream_t st) {
-    FL_REQUIRE(a.planes == b.planes && !s.symmetric, "gemm: planes");
-    EpiLinear epi{e};
-    return a.planes == 2 ? run_any<2>(s, a, b, epi, st) : run_any<1>(s, a, b, epi, st);
+    const int planes = e.dtype == kOutF32 ? 2 : 1;
+    FL_REQUIRE(a.planes == planes && b.planes == planes && !s.symmetric, "gemm: planes");
+    if (e.dtype == kOutF32) return linear_typed<float>(s, a, b, e, st);
+    if (e.dtype == kOutF16) return linear_typed<__half>(s, a, b, e, st);
+    return linear_typed<__nv_bfloat16>(s, a, b, e, st);
 }
 
 int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,

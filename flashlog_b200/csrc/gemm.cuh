@@ -41,6 +41,7 @@ struct LinearEpilogue {
     float *z;                // pre-activation for the backward, or NULL
     int64_t ld_z;
     int dtype, act;
+    int pair;                // set by gemm_linear: 16-bit rows may be stored two columns at a time
 };
 
 // A batch of matrices in a caller's memory: element (b, i, j) lies at

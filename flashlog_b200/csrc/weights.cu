@@ -83,8 +83,10 @@ __device__ __forceinline__ float rescale(float m, float to, float inv_tau) {
     return m == to ? 1.0f : expf((m - to) * inv_tau);  // equal (both -inf too): nothing to do
 }
 
+// 1024 threads per SM with up to 64 registers each: enough rows in flight to
+// cover the loads' latency while other rows are in their reductions.
 template <typename T, int THREADS, int VPT, bool CL>
-__global__ __launch_bounds__(THREADS) void weights_forward_kernel(const WeightsArgs a, float *out) {
+__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_forward_kernel(const WeightsArgs a, float *out) {
     extern __shared__ unsigned dyn[];
     constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
     unsigned *seen = dyn, *count = dyn + kChunk / 32;
@@ -107,22 +109,49 @@ __global__ __launch_bounds__(THREADS) void weights_forward_kernel(const WeightsA
         const int64_t state = a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
         const bool legal = state >= 0 && state < a.n_states;
         const uint8_t *mask = a.mask + (legal ? state * a.mask_ld : 0);
+        // all of the row's loads first: they are in flight together
         float u[VPT], m = -INFINITY;
+        T raw[VPT];
+        unsigned allowed = 0u;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t col = c0 + i * THREADS + tid;
+            raw[i] = col < a.n ? z[col] : from_f32<T>(0.0f);
+        }
+        if (a.mask == nullptr) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) allowed |= (c0 + i * THREADS + tid < a.n ? 1u : 0u) << i;
+        } else if (legal) {
+            uint8_t ok[VPT];
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int64_t col = c0 + i * THREADS + tid;
+                ok[i] = col < a.n ? mask[col] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) allowed |= (ok[i] != 0 ? 1u : 0u) << i;
+        }
+        if (a.bias != nullptr) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                const int64_t col = c0 + i * THREADS + tid;
+                u[i] = col < a.n ? to_f32<T>(bias[col]) : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) u[i] = 0.0f;
+        }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = i * THREADS + tid;
-            const int64_t col = c0 + c;
-            u[i] = -INFINITY;
-            if (col < a.n && (a.mask == nullptr || (legal && mask[col] != 0))) {
-                float v = to_f32<T>(z[col]);
-                if (a.hist > 0 && (seen[c >> 5] >> (c & 31)) & 1u) {
-                    v = v > 0.0f ? v / a.theta : v * a.theta;
-                    v = v - a.frequency * static_cast<float>(count[c]) - a.presence;
-                }
-                if (a.bias != nullptr) v += to_f32<T>(bias[col]);
-                u[i] = v;
+            float v = to_f32<T>(raw[i]);
+            if (a.hist > 0 && (seen[c >> 5] >> (c & 31)) & 1u) {
+                v = v > 0.0f ? v / a.theta : v * a.theta;
+                v = v - a.frequency * static_cast<float>(count[c]) - a.presence;
             }
-            m = fmaxf(m, u[i]);
+            v = (allowed >> i) & 1u ? v + u[i] : -INFINITY;
+            u[i] = v;
+            m = fmaxf(m, v);
         }
         float s = 0.0f;
 #pragma unroll
@@ -172,7 +201,7 @@ __global__ __launch_bounds__(THREADS) void weights_forward_kernel(const WeightsA
 // dbias_partial: [blocks / ranks, n] sums of du over the rows each cluster took (a fixed set), or NULL;
 // du: [rows, n] for a bias of the logits' shape, or NULL.
 template <typename T, int THREADS, int VPT, bool CL>
-__global__ __launch_bounds__(THREADS) void weights_backward_kernel(const WeightsArgs a, const float *w, const float *g,
+__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_backward_kernel(const WeightsArgs a, const float *w, const float *g,
                                                                    int64_t ld_g, T *dz, T *du, float *dbias_partial) {
     extern __shared__ unsigned dyn[];
     constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
