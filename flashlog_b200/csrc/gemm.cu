@@ -5,11 +5,13 @@
 // shared memory, and the pair's tensor cores read both halves, so an SM loads
 // (128 + BN/2) lines for 128 x BN outputs; with one CTA per tile the L2 -> SM
 // traffic would be 1.5 times that, above what the L2 delivers at the full
-// matrix rate.  Roles per CTA: one warp loads by TMA (128-byte swizzle), one
-// warp (of the pair's first CTA) issues the matrix instructions, eight warps
-// read the accumulators back (two TMEM buffers, so a tile's epilogue runs
-// under the next tile's products).  Waits are bounded: one that runs out marks
-// the device fault word, and the tiles left get NaN.
+// matrix rate.  Roles per CTA: two warps load by TMA (128-byte swizzle), one A
+// and one B, both planes of an operand at once (issuing a load takes about 130
+// cycles: one warp for both would hold up 128-wide tiles); one warp (of the
+// pair's first CTA) issues the matrix instructions; eight warps read the
+// accumulators back (two TMEM buffers, so a tile's epilogue runs under the next
+// tile's products).  Waits are bounded: one that runs out marks the device
+// fault word, and the tiles left get NaN.
 #include <cuda.h>
 
 #include "gemm.cuh"
@@ -21,10 +23,9 @@ namespace {
 constexpr int kBM = 128;        // rows of A per CTA
 constexpr int kBK = 64;         // contraction per stage: one 128-byte swizzle line
 constexpr int kEpiWarps = 8;    // warp w reads TMEM lanes 32 (w % 4).., columns of half w / 4
-constexpr int kLoadWarp = kEpiWarps, kMmaWarp = kEpiWarps + 1;
-constexpr int kThreads = 32 * (kEpiWarps + 2);
-constexpr int kStageBudget = 196 * 1024;
-constexpr int kStagePad = 33;   // row pitch (words) of the epilogue's transposing tile
+constexpr int kLoadA = kEpiWarps, kLoadB = kEpiWarps + 1, kMmaWarp = kEpiWarps + 2;
+constexpr int kThreads = 32 * (kEpiWarps + 3);
+constexpr int kStageBudget = 192 * 1024;
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // four seconds: far above any wait between healthy roles
 
 __device__ int g_gemm_fault;    // set when a bounded wait ran out
@@ -46,7 +47,7 @@ __device__ __forceinline__ void bar_arrive_cta0(uint32_t bar) {
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
@@ -64,6 +65,19 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     *failed = 1;
     atomicExch(&g_gemm_fault, 1);
     return false;
+}
+
+// bar_wait by a whole warp, with one answer
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *failed) {
+    return __all_sync(kFull, bar_wait(bar, parity, failed));
+}
+
+// One lane of a converged warp, in a form the compiler knows to be one: the
+// load and product instructions take their operands from uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
 }
 
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2,
@@ -100,8 +114,10 @@ __device__ __forceinline__ void tmem_read32(float (&v)[32], uint32_t addr) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Execution only: the barriers' initialisation has its own fence, and nothing
+// else passes from one CTA's threads to the other's.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle (8 lines of 128 bytes per
@@ -141,6 +157,8 @@ __device__ __forceinline__ void tile_of(const TileGrid &g, int t, int &b, int &t
 }
 
 // ---- epilogues: 32 rows x 32 columns per call, lane = row, v[c] = column c -----
+// A tile's epilogue runs once or a few times per block: its code comes from
+// memory, so loops that need no unrolling for their registers stay rolled.
 template <int N>
 __device__ __forceinline__ void apply_act(float (&z)[N], int act) {
     if (act == kActNone) return;
@@ -159,95 +177,113 @@ __device__ __forceinline__ void apply_act(float (&z)[N], int act) {
     }
 }
 
-// Lane = column (or a pair of columns, two rows at a time, for 16-bit types
-// whose rows are 4-byte aligned): the warp's stores are whole 64- or 128-byte
-// pieces of a row at any alignment.  Eight rows are in flight at once.
-template <typename T, bool PAIR>
-__device__ __forceinline__ void linear_rows(const LinearEpilogue &e, const float *stage, int64_t row0, int64_t col0,
-                                            int rows, int64_t n, int lane, bool exact_scale, int row_exp) {
-    constexpr int kW = PAIR ? 2 : 1;              // columns per lane
-    const int sub = PAIR ? lane >> 4 : 0;         // which of the two rows
-    const int lc = PAIR ? (lane & 15) * 2 : lane;
-    const int64_t col = col0 + lc;
-    float bias[kW], factor[kW];
-    int ce[kW];
-    bool in[kW];
+// The epilogue's transposing tile, 32 x 32 words: the 16-byte pieces of row r
+// are permuted by r % 8, so neither row writes nor column reads meet in a bank.
+__device__ __forceinline__ int stage_at(int r, int c) { return r * 32 + ((((c >> 2) ^ r) & 7) << 2) + (c & 3); }
+
+__device__ __forceinline__ void stage_rows(float *stage, const float (&v)[32], int lane) {
 #pragma unroll
-    for (int w = 0; w < kW; ++w) {
-        in[w] = col + w < n;
-        bias[w] = in[w] && e.bias != nullptr ? to_f32(static_cast<const T *>(e.bias)[col + w]) : 0.0f;
-        ce[w] = in[w] && e.col_exp != nullptr ? e.col_exp[col + w] : 0;
-        factor[w] = exact_scale ? 1.0f : __int_as_float((ce[w] + 127) << 23);
+    for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<float4 *>(stage + stage_at(lane, 4 * q)) =
+            make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+
+// 32 consecutive values of a row as 16-byte pieces
+template <typename T>
+__device__ __forceinline__ void load_row(const T *p, float (&v)[32]) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < 32 / kPer; ++q) {
+        union { uint4 u; T t[kPer]; } x;
+        x.u = reinterpret_cast<const uint4 *>(p)[q];
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) v[q * kPer + c] = to_f32<T>(x.t[c]);
     }
-    constexpr int kRows = 8;                      // rows per batch (per half warp: 2 kRows in all)
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T *p, const float (&v)[32]) {
+    constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += kRows * kW) {
-        float z[kRows * kW], res[kRows * kW];
+    for (int q = 0; q < 32 / kPer; ++q) {
+        union { uint4 u; T t[kPer]; } x;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-            const int r = r0 + k * kW + sub;
+        for (int c = 0; c < kPer; ++c) x.t[c] = from_f32<T>(v[q * kPer + c]);
+        reinterpret_cast<uint4 *>(p)[q] = x.u;
+    }
+}
+
+// Rows that start on 16 bytes: lane = row, whole 16-byte pieces.
+template <typename T>
+__device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[32], int64_t row, int64_t col0, bool in,
+                                            float row_factor) {
+    if (e.row_exp != nullptr) {
 #pragma unroll
-            for (int w = 0; w < kW; ++w) {
-                z[k * kW + w] = stage[r * kStagePad + lc + w];
-                res[k * kW + w] = 0.0f;
-            }
+        for (int q = 0; q < 8; ++q) {
+            const int4 x = *reinterpret_cast<const int4 *>(e.col_exp + col0 + 4 * q);
+            const int ex[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[4 * q + c] *= row_factor * __int_as_float((ex[c] + 127) << 23);
         }
-        if (e.residual != nullptr) {
+    }
+    float t[32];
+    if (e.bias != nullptr) {
+        load_row<T>(static_cast<const T *>(e.bias) + col0, t);
 #pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                const int r = r0 + k * kW + sub;
-                const T *p = static_cast<const T *>(e.residual) + (row0 + r) * e.ld_res + col;
-                if (PAIR) {
-                    if (r < rows && in[kW - 1]) {
-                        union { unsigned u; T t[2]; } x;
-                        x.u = *reinterpret_cast<const unsigned *>(p);
-                        res[k * kW] = to_f32(x.t[0]);
-                        res[k * kW + kW - 1] = to_f32(x.t[1]);
-                    } else if (r < rows && in[0]) {
-                        res[k * kW] = to_f32(p[0]);
-                    }
-                } else if (r < rows && in[0]) {
-                    res[k] = to_f32(p[0]);
-                }
-            }
+        for (int c = 0; c < 32; ++c) v[c] += t[c];
+    }
+    if (!in) return;
+    if (e.z != nullptr) store_row<float>(e.z + row * e.ld_z + col0, v);
+    if (e.residual != nullptr) load_row<T>(static_cast<const T *>(e.residual) + row * e.ld_res + col0, t);
+    apply_act(v, e.act);
+    if (e.residual != nullptr) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] += t[c];
+    }
+    store_row<T>(static_cast<T *>(e.out) + row * e.ld_out + col0, v);
+}
+
+// Any alignment: lane = column, the rows one after another from the staging
+// tile, so that a warp's store is a whole 64- or 128-byte piece of a row.
+template <typename T>
+__device__ __forceinline__ void linear_columns(const LinearEpilogue &e, const float *stage, int64_t row0, int64_t col0,
+                                               int rows, int64_t n, int lane, bool exact_scale, int row_exp,
+                                               int col_exp) {
+    const int64_t col = col0 + lane;
+    const bool in = col < n;
+    const float bias = in && e.bias != nullptr ? to_f32(static_cast<const T *>(e.bias)[col]) : 0.0f;
+    const float factor = exact_scale ? 1.0f : __int_as_float((col_exp + 127) << 23);
+    T *out = static_cast<T *>(e.out) + row0 * e.ld_out + col;
+    const T *res = static_cast<const T *>(e.residual) + row0 * e.ld_res + col;
+    float *pz = e.z + row0 * e.ld_z + col;
+    const bool plain = !exact_scale && e.z == nullptr && e.act == kActNone && e.residual == nullptr && rows == 32;
+    if (plain) {
+#pragma unroll
+        for (int r = 0; r < 32; ++r) {
+            const T y = from_f32<T>(fmaf(stage[stage_at(r, lane)], factor, bias));
+            if (in) *out = y;
+            out += e.ld_out;
         }
+        return;
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < rows; r0 += 8) {
+        float z[8], y[8];
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
-#pragma unroll
-            for (int w = 0; w < kW; ++w) {
-                float x = z[k * kW + w];
-                if (exact_scale) {
-                    const int re = __shfl_sync(kFull, row_exp, r0 + k * kW + sub);
-                    x = scale_pow2(x, re + ce[w]);
-                } else {
-                    x *= factor[w];
-                }
-                z[k * kW + w] = x + bias[w];
-            }
-        if (e.z != nullptr) {
-#pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                const int r = r0 + k * kW + sub;
-                float *p = e.z + (row0 + r) * e.ld_z + col;
-#pragma unroll
-                for (int w = 0; w < kW; ++w)
-                    if (r < rows && in[w]) p[w] = z[k * kW + w];
-            }
+        for (int k = 0; k < 8; ++k) {
+            const bool on = in && r0 + k < rows;
+            y[k] = e.residual != nullptr && on ? to_f32(res[k * e.ld_res]) : 0.0f;
+            z[k] = stage[stage_at(r0 + k, lane)];
+            if (exact_scale) z[k] = scale_pow2(z[k], __shfl_sync(kFull, row_exp, r0 + k) + col_exp);
+            z[k] = fmaf(z[k], factor, bias);
+            if (e.z != nullptr && on) pz[k * e.ld_z] = z[k];
         }
         apply_act(z, e.act);
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
-            const int r = r0 + k * kW + sub;
-            T *p = static_cast<T *>(e.out) + (row0 + r) * e.ld_out + col;
-            if (PAIR && r < rows && in[kW - 1]) {
-                union { unsigned u; T t[2]; } x;
-                x.t[0] = from_f32<T>(z[k * kW] + res[k * kW]);
-                x.t[PAIR ? 1 : 0] = from_f32<T>(z[k * kW + kW - 1] + res[k * kW + kW - 1]);
-                *reinterpret_cast<unsigned *>(p) = x.u;
-            } else if (r < rows && in[0]) {
-                p[0] = from_f32<T>(z[k * kW] + res[k * kW]);
-            }
-        }
+        for (int k = 0; k < 8; ++k)
+            if (in && r0 + k < rows) out[k * e.ld_out] = from_f32<T>(z[k] + y[k]);
+        out += 8 * e.ld_out;
+        res += 8 * e.ld_res;
+        pz += 8 * e.ld_z;
     }
 }
 
@@ -262,12 +298,18 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
     }
     const bool exact_scale = __any_sync(kFull, re > 60 || re < -60 || ce > 60 || ce < -60);
     const float rf = exact_scale ? 1.0f : __int_as_float((re + 127) << 23);
+    if (e.aligned && !exact_scale && col0 + 32 <= n) {
+        linear_rows<T>(e, v, row0 + lane, col0, row0 + lane < m, rf);
+        return;
+    }
+    if (e.row_exp != nullptr) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c) stage[lane * kStagePad + c] = v[c] * rf;
+        for (int c = 0; c < 32; ++c) v[c] *= rf;
+    }
+    stage_rows(stage, v, lane);
     __syncwarp();
     const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
-    if (sizeof(T) == 2 && e.pair) linear_rows<T, sizeof(T) == 2>(e, stage, row0, col0, rows, n, lane, exact_scale, re);
-    else linear_rows<T, false>(e, stage, row0, col0, rows, n, lane, exact_scale, re);
+    linear_columns<T>(e, stage, row0, col0, rows, n, lane, exact_scale, re, ce);
     __syncwarp();
 }
 
@@ -285,28 +327,18 @@ __device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// 32 consecutive columns of one row as two planes; the row's padding (up to ld)
-// may be written, it is never read (the tensor maps end at n).
-__device__ __forceinline__ void planes_row(__half *hi, int64_t plane, const float (&v)[32], int cols) {
+// 32 consecutive columns of one row as two planes.  Pitches and line counts of
+// the planes are multiples of 32, so whole pieces fit; what lies past the
+// matrix is never read (the tensor maps end with it).
+__device__ __forceinline__ void planes_row(__half *hi, int64_t plane, const float (&v)[32]) {
     __half *lo = hi + plane;
-    if (cols >= 32) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            union { __half h[8]; uint4 u; } a, b;
+    for (int q = 0; q < 4; ++q) {
+        union { __half h[8]; uint4 u; } a, b;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) split_half(v[q * 8 + c], a.h[c], b.h[c]);
-            reinterpret_cast<uint4 *>(hi)[q] = a.u;
-            reinterpret_cast<uint4 *>(lo)[q] = b.u;
-        }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 32; ++c)
-            if (c < cols) {
-                __half a, b;
-                split_half(v[c], a, b);
-                hi[c] = a;
-                lo[c] = b;
-            }
+        for (int c = 0; c < 8; ++c) split_half(v[q * 8 + c], a.h[c], b.h[c]);
+        reinterpret_cast<uint4 *>(hi)[q] = a.u;
+        reinterpret_cast<uint4 *>(lo)[q] = b.u;
     }
 }
 
@@ -330,15 +362,15 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
         }
         return;
     }
-#pragma unroll
-    for (int c = 0; c < 32; ++c) stage[lane * kStagePad + c] = v[c];
+    stage_rows(stage, v, lane);
     __syncwarp();
     const int64_t col = col0 + lane;
     const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
     if (col < n) {
+#pragma unroll 8
         for (int r = 0; r < rows; ++r) {
             const int64_t row = row0 + r;
-            float x = stage[r * kStagePad + lane];
+            float x = stage[stage_at(r, lane)];
             if (base != nullptr) x = fmaf(e.keep, base[row * e.base.i + col * e.base.j], x);
             out[row * e.fin.i + col * e.fin.j] = from_f32<T>(x);
         }
@@ -351,74 +383,59 @@ struct EpiPlanes {
     PlanesEpilogue p;
     __device__ __forceinline__ void operator()(float (&v)[32], float *stage, int b, int64_t row0, int64_t col0,
                                                int64_t m, int64_t n, int lane) const {
-        if (SYM && col0 > row0 + 31) return;  // all of it above the diagonal: its mirror image writes it
+        if (SYM && col0 > row0) return;  // all of it above the diagonal: its mirror image writes it
         const int64_t row = row0 + lane;
-        const int cols = static_cast<int>(min(static_cast<int64_t>(32), n - col0));
-        const bool in = row < m;
-        if (p.c != nullptr && in) {
-            const __half *hi = p.c + b * p.c_batch + row * p.c_ld + col0;
-            const __half *lo = hi + p.c_plane;
-            // ld is a multiple of 8 and at least n: whole vectors stay within the row
+        if (p.c != nullptr) {
+            const uint4 *hi = reinterpret_cast<const uint4 *>(p.c + b * p.c_batch + row * p.c_ld + col0);
+            const uint4 *lo = reinterpret_cast<const uint4 *>(p.c + b * p.c_batch + p.c_plane + row * p.c_ld + col0);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                if (q * 8 < cols) {
-                    union { uint4 u; __half h[8]; } a, z;
-                    a.u = reinterpret_cast<const uint4 *>(hi)[q];
-                    z.u = reinterpret_cast<const uint4 *>(lo)[q];
+                union { uint4 u; __half h[8]; } a, z;
+                a.u = hi[q];
+                z.u = lo[q];
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        v[q * 8 + c] = fmaf(p.alpha, v[q * 8 + c],
-                                            p.beta * (__half2float(a.h[c]) + __half2float(z.h[c])));
-                }
+                for (int c = 0; c < 8; ++c)
+                    v[q * 8 + c] =
+                        fmaf(p.alpha, v[q * 8 + c], p.beta * (__half2float(a.h[c]) + __half2float(z.h[c])));
             }
         } else {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
         }
-        if (p.fin.ptr != nullptr) {
+        if (!SYM && p.fin.ptr != nullptr) {
             if (p.dtype == kOutF32) final_store<float>(p, v, stage, b, row0, col0, m, n, lane);
             else if (p.dtype == kOutF16) final_store<__half>(p, v, stage, b, row0, col0, m, n, lane);
             else final_store<__nv_bfloat16>(p, v, stage, b, row0, col0, m, n, lane);
-        }
-        if (p.out != nullptr && in) write<0>(v, b, row, row0, col0, cols);
-        if (p.out2 != nullptr && in) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col0 + c == row ? p.diag : 0.0f);
-            write<1>(v, b, row, row0, col0, cols);
-        }
-    }
-    template <int WHICH>
-    __device__ __forceinline__ void write(const float (&v)[32], int b, int64_t row, int64_t row0, int64_t col0,
-                                          int cols) const {
-        __half *base = WHICH == 0 ? p.out + b * p.batch : p.out2 + b * p.batch2;
-        const int64_t ld = WHICH == 0 ? p.ld : p.ld2, plane = WHICH == 0 ? p.plane : p.plane2;
-        __half *hi = base + row * ld + col0;
-        if (!SYM) {
-            planes_row(hi, plane, v, cols);
             return;
         }
-        if (col0 + 31 <= row0) {  // below the diagonal for every lane
-            planes_row(hi, plane, v, cols);
-        } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-                if (c < cols && col0 + c <= row) {
-                    __half x, y;
-                    split_half(v[c], x, y);
-                    hi[c] = x;
-                    hi[plane + c] = y;
-                }
+        if (!SYM) {
+            planes_row(p.out + b * p.batch + row * p.ld + col0, p.plane, v);
+            return;
         }
-        // the mirror image: lane = row is the contiguous direction
+#pragma unroll 1
+        for (int o = 0; o < (p.out2 != nullptr ? 2 : 1); ++o) {
+            __half *base = o == 0 ? p.out + b * p.batch : p.out2 + b * p.batch2;
+            const int64_t ld = o == 0 ? p.ld : p.ld2, plane = o == 0 ? p.plane : p.plane2;
+            if (o == 1) {
 #pragma unroll
-        for (int c = 0; c < 32; ++c)
-            if (c < cols && col0 + c < row) {
-                __half x, y;
-                split_half(v[c], x, y);
-                __half *t = base + (col0 + c) * ld + row;
-                t[0] = x;
-                t[plane] = y;
+                for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col0 + c == row ? p.diag : 0.0f);
             }
+            stage_rows(stage, v, lane);
+            __syncwarp();
+            float t[32];
+            if (col0 == row0) {
+                // the block on the diagonal: its upper half from the lower
+#pragma unroll
+                for (int c = 0; c < 32; ++c) t[c] = stage[stage_at(max(c, lane), min(c, lane))];
+                planes_row(base + row * ld + col0, plane, t);
+            } else {
+                planes_row(base + row * ld + col0, plane, v);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) t[c] = stage[stage_at(c, lane)];
+                planes_row(base + (col0 + lane) * ld + row0, plane, t);
+            }
+            __syncwarp();
+        }
     }
 };
 
@@ -428,7 +445,7 @@ struct Config {
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
     static constexpr int kStage = PLANES * (kA + kB);
     static constexpr int kStages = kStageBudget / kStage > 8 ? 8 : kStageBudget / kStage;
-    static constexpr int kSmem = kStages * kStage + kEpiWarps * 32 * kStagePad * 4 + 1024;
+    static constexpr int kSmem = kStages * kStage + kEpiWarps * 32 * 32 * 4 + 1024;
 };
 
 template <int BN, int PLANES, typename Epi>
@@ -437,29 +454,25 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                  int64_t n, int64_t k, TileGrid grid, int a_mn, int b_mn, uint32_t idesc, const Epi epi) {
     using C = Config<BN, PLANES>;
     extern __shared__ unsigned char raw[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
+    unsigned char *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float *stage_epi = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
     __shared__ uint64_t bars[2 * C::kStages + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint32_t cta;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::kStages, acc_full = empty + 8 * C::kStages,
                    acc_empty = acc_full + 16;
 
-    if (threadIdx.x == 0) {
-        failed = 0;
-        for (int s = 0; s < C::kStages; ++s) {
-            bar_init(full + 8 * s, 1);
-            bar_init(empty + 8 * s, 1);
-        }
-        for (int s = 0; s < 2; ++s) {
-            bar_init(acc_full + 8 * s, 1);
-            bar_init(acc_empty + 8 * s, 2 * kEpiWarps);  // of both CTAs
-        }
+    if (threadIdx.x < 2 * C::kStages + 4) {
+        const int i = threadIdx.x;
+        // the last two, accumulator buffers free: every epilogue warp of both CTAs arrives
+        bar_init(full + 8 * i, i < 2 * C::kStages + 2 ? 1 : 2 * kEpiWarps);
+        if (i == 0) failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -467,6 +480,8 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                      "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
+    if (warp == kLoadA && lane < 2)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_a : &map_b)));
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     cluster_sync();
@@ -474,37 +489,38 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const uint32_t tmem = tmem_slot;
     const int kblocks = static_cast<int>((k + kBK - 1) / kBK);
 
-    if (warp == kLoadWarp && lane == 0) {
+    if (warp == kLoadA || warp == kLoadB) {
         // ---- loads ----
+        const bool is_a = warp == kLoadA;
+        const CUtensorMap *map = is_a ? &map_a : &map_b;
+        const bool mn = is_a ? a_mn != 0 : b_mn != 0;
+        const int pieces = mn ? (is_a ? kBM / 64 : BN / 128) : 1;  // 64 lines of an MN-major operand per load
+        const uint32_t offset = is_a ? 0 : PLANES * C::kA, plane = is_a ? C::kA : C::kB;
+        const bool expects = is_a && cta == 0;
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int t = pair; ok && t < grid.total; t += pairs) {
             int b, ti, tj;
             tile_of<BN>(grid, t, b, ti, tj);
-            const int row = ti * 2 * kBM + static_cast<int>(cta) * kBM, col = tj * BN + static_cast<int>(cta) * (BN / 2);
+            const int line = is_a ? ti * 2 * kBM + static_cast<int>(cta) * kBM : tj * BN + static_cast<int>(cta) * (BN / 2);
             for (int kb = 0; kb < kblocks; ++kb) {
-                ok = bar_wait(empty + 8 * s, phase ^ 1, &failed);
+                ok = warp_wait(empty + 8 * s, phase ^ 1, &failed);
                 if (!ok) break;
-                if (cta == 0) bar_expect(full + 8 * s, 2 * C::kStage);
-                const uint32_t sa = smem_u32(smem) + s * C::kStage, sb = sa + PLANES * C::kA;
+                const uint32_t dst = smem_u32(smem) + s * C::kStage + offset;
+                if (elect_one()) {
+                    // the other CTA's and the other warp's bytes may arrive before they are expected
+                    if (expects) bar_expect(full + 8 * s, 2 * C::kStage);
+                    if (mn) {
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    if (a_mn) {
-#pragma unroll
-                        for (int h = 0; h < kBM / 64; ++h)
-                            tma_load(sa + p * C::kA + h * 8192, &map_a, full + 8 * s, row + 64 * h, kb * kBK, p, b);
+                        for (int p = 0; p < PLANES; ++p)
+                            for (int h = 0; h < pieces; ++h)
+                                tma_load(dst + p * plane + h * 8192, map, full + 8 * s, line + 64 * h, kb * kBK, p, b);
                     } else {
-                        tma_load(sa + p * C::kA, &map_a, full + 8 * s, kb * kBK, row, p, b);
-                    }
-                    if (b_mn) {
-#pragma unroll
-                        for (int h = 0; h < BN / 128; ++h)
-                            tma_load(sb + p * C::kB + h * 8192, &map_b, full + 8 * s, col + 64 * h, kb * kBK, p, b);
-                    } else {
-                        tma_load(sb + p * C::kB, &map_b, full + 8 * s, kb * kBK, col, p, b);
+                        tma_load(dst, map, full + 8 * s, kb * kBK, line, 0, b);  // all planes
                     }
                 }
+                __syncwarp();
                 if (++s == C::kStages) { s = 0; phase ^= 1; }
             }
         }
@@ -516,10 +532,10 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 for (int w = 0; w < 4096; ++w) __nanosleep(256);
                 break;
             }
-            ok = bar_wait(empty + 8 * s, phase ^ 1, &failed);
+            ok = warp_wait(empty + 8 * s, phase ^ 1, &failed);
             if (++s == C::kStages) { s = 0; phase ^= 1; }
         }
-    } else if (warp == kMmaWarp && cta == 0 && lane == 0) {
+    } else if (warp == kMmaWarp && cta == 0) {
         // ---- products (for the pair) ----
         const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;  // 16 of k, in 16-byte units
         const uint32_t a_lbo = a_mn ? 8192u : 16u, b_lbo = b_mn ? 8192u : 16u;
@@ -527,40 +543,42 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (int t = pair; ok && t < grid.total; t += pairs) {
-            ok = bar_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
+            ok = warp_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t d = tmem + buf * BN;
-            uint32_t accumulate = 0;
             for (int kb = 0; kb < kblocks; ++kb) {
-                ok = bar_wait(full + 8 * s, phase, &failed);
+                ok = warp_wait(full + 8 * s, phase, &failed);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t sa = smem_u32(smem) + s * C::kStage, sb = sa + PLANES * C::kA;
-                uint64_t da[PLANES], db[PLANES];
+                if (elect_one()) {
+                    uint64_t da[PLANES], db[PLANES];
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    da[p] = smem_desc(sa + p * C::kA, a_lbo, 1024);
-                    db[p] = smem_desc(sb + p * C::kB, b_lbo, 1024);
-                }
-#pragma unroll
-                for (int j = 0; j < kBK / 16; ++j) {
-                    mma_f16(d, da[0] + j * a_step, db[0] + j * b_step, idesc, accumulate);
-                    accumulate = 1;
-                    if (PLANES == 2) {
-                        mma_f16(d, da[0] + j * a_step, db[PLANES - 1] + j * b_step, idesc, 1);
-                        mma_f16(d, da[PLANES - 1] + j * a_step, db[0] + j * b_step, idesc, 1);
+                    for (int p = 0; p < PLANES; ++p) {
+                        da[p] = smem_desc(sa + p * C::kA, a_lbo, 1024);
+                        db[p] = smem_desc(sb + p * C::kB, b_lbo, 1024);
                     }
+#pragma unroll
+                    for (int j = 0; j < kBK / 16; ++j) {
+                        mma_f16(d, da[0] + j * a_step, db[0] + j * b_step, idesc, (kb | j) != 0);
+                        if (PLANES == 2) {
+                            mma_f16(d, da[0] + j * a_step, db[PLANES - 1] + j * b_step, idesc, 1);
+                            mma_f16(d, da[PLANES - 1] + j * a_step, db[0] + j * b_step, idesc, 1);
+                        }
+                    }
+                    mma_commit(empty + 8 * s);
                 }
-                mma_commit(empty + 8 * s);
+                __syncwarp();
                 if (++s == C::kStages) { s = 0; phase ^= 1; }
             }
-            mma_commit(acc_full + 8 * buf);
+            if (elect_one()) mma_commit(acc_full + 8 * buf);
+            __syncwarp();
             if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        float *stage = stage_epi + warp * 32 * kStagePad;
+        float *stage = stage_epi + warp * 32 * 32;
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -569,11 +587,11 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             tile_of<BN>(grid, t, b, ti, tj);
             const int64_t row0 = static_cast<int64_t>(ti) * 2 * kBM + cta * kBM + (warp & 3) * 32;
             const int64_t col0 = static_cast<int64_t>(tj) * BN;
-            if (ok) ok = bar_wait(acc_full + 8 * buf, acc_phase, &failed);
-            ok = __all_sync(kFull, ok);
+            if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>((warp & 3) * 32) << 16);
             const int half = (warp >> 2) * (BN / 2);
+#pragma unroll 1
             for (int c = half; c < half + BN / 2; c += 32) {
                 float v[32];
                 if (ok) {
@@ -635,7 +653,8 @@ int operand_map(CUtensorMap *map, const GemmOperand &o, int64_t lines_mn, int64_
     // unused strides still have to be multiples of 16 that are not 0
     cuuint64_t strides[3] = {ld, o.planes > 1 ? static_cast<cuuint64_t>(o.plane) * 2 : ld,
                              batch > 1 ? static_cast<cuuint64_t>(o.batch) * 2 : ld};
-    cuuint32_t box[4] = {64, static_cast<cuuint32_t>(o.mn_major ? kBK : box_rows), 1, 1};
+    cuuint32_t box[4] = {64, static_cast<cuuint32_t>(o.mn_major ? kBK : box_rows),
+                         static_cast<cuuint32_t>(o.mn_major ? 1 : o.planes), 1};
     cuuint32_t unit[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, kind == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                           const_cast<void *>(o.ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -709,8 +728,12 @@ template <typename T>
 int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
                  cudaStream_t st) {
     EpiLinear<T> epi{e};
-    epi.p.pair = (reinterpret_cast<uintptr_t>(e.out) & 3) == 0 && (e.ld_out & 1) == 0 &&
-                 (e.residual == nullptr || ((reinterpret_cast<uintptr_t>(e.residual) & 3) == 0 && (e.ld_res & 1) == 0));
+    const int per = 16 / static_cast<int>(sizeof(T));
+    auto rows_ready = [&](const void *p, int64_t ld, int64_t unit) {
+        return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % unit == 0);
+    };
+    epi.p.aligned = rows_ready(e.out, e.ld_out, per) && rows_ready(e.residual, e.ld_res, per) && rows_ready(e.bias, 0, 1) &&
+                    rows_ready(e.z, e.ld_z, 4);
     return run_any<sizeof(T) == 4 ? 2 : 1>(s, a, b, epi, st);
 }
 

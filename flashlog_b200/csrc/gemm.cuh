@@ -41,7 +41,7 @@ struct LinearEpilogue {
     float *z;                // pre-activation for the backward, or NULL
     int64_t ld_z;
     int dtype, act;
-    int pair;                // set by gemm_linear: 16-bit rows may be stored two columns at a time
+    int aligned;             // set by gemm_linear: rows of all arrays start on 16 bytes
 };
 
 // A batch of matrices in a caller's memory: element (b, i, j) lies at
@@ -54,7 +54,8 @@ struct Strided {
 
 // Epilogue of a Newton-Schulz product: v = alpha * acc + beta * C[i, j], where
 // C is a 2-plane array, written as planes (mirrored when symmetric), or as the
-// last product's result: fin = v + keep * base.
+// last product's result: fin = v + keep * base.  Pitches and line counts of C
+// and the outputs are multiples of 32.
 struct PlanesEpilogue {
     float alpha, beta;       // on the accumulator and on the planes' sum
     const __half *c;         // NULL: no C
