@@ -188,34 +188,61 @@ __device__ __forceinline__ void stage_rows(float *stage, const float (&v)[32], i
             make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
 
-// 32 consecutive values of a row as 16-byte pieces
+// A 32 x 32 tile of 16-bit values in 64-byte rows, as TMA's 64-byte swizzle
+// lays it out: the same freedom from bank conflicts, and loads, stores and
+// ldmatrix address whole 16-byte pieces.
+__device__ __forceinline__ int piece_at(int r, int q) { return r * 64 + (((q ^ (r >> 1)) & 3) << 4); }
+
+// Global memory takes 16-byte accesses at one cache line per cycle: a lane per
+// row would touch 32 lines at a time, so rows are moved with the lanes side by
+// side (four or eight to a row), through the staging tile.
 template <typename T>
-__device__ __forceinline__ void load_row(const T *p, float (&v)[32]) {
+__device__ __forceinline__ void rows_to_stage(unsigned char *stage, const float (&v)[32], int lane) {
+    if (sizeof(T) == 4) {
+        stage_rows(reinterpret_cast<float *>(stage), v, lane);
+        return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        union { uint4 u; T t[16 / sizeof(T)]; } x;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) x.t[c % (16 / sizeof(T))] = from_f32<T>(v[q * 8 + c]);
+        *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = x.u;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void rows_from_stage(const unsigned char *stage, float (&v)[32], int lane) {
     constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
     for (int q = 0; q < 32 / kPer; ++q) {
         union { uint4 u; T t[kPer]; } x;
-        x.u = reinterpret_cast<const uint4 *>(p)[q];
+        x.u = *reinterpret_cast<const uint4 *>(
+            stage + (sizeof(T) == 4 ? 4 * stage_at(lane, 4 * q) : piece_at(lane, q)));
 #pragma unroll
         for (int c = 0; c < kPer; ++c) v[q * kPer + c] = to_f32<T>(x.t[c]);
     }
 }
-template <typename T>
-__device__ __forceinline__ void store_row(T *p, const float (&v)[32]) {
-    constexpr int kPer = 16 / sizeof(T);
+template <typename T, bool STORE>
+__device__ __forceinline__ void stage_global(unsigned char *stage, T *p, int64_t ld, int rows, int lane) {
+    constexpr int kLanes = 2 * sizeof(T);  // per row of 32 values
+    constexpr int kRows = 32 / kLanes;
+    const int q = lane % kLanes;
 #pragma unroll
-    for (int q = 0; q < 32 / kPer; ++q) {
-        union { uint4 u; T t[kPer]; } x;
-#pragma unroll
-        for (int c = 0; c < kPer; ++c) x.t[c] = from_f32<T>(v[q * kPer + c]);
-        reinterpret_cast<uint4 *>(p)[q] = x.u;
+    for (int it = 0; it < 32 / kRows; ++it) {
+        const int r = it * kRows + lane / kLanes;
+        uint4 *s = reinterpret_cast<uint4 *>(stage + (sizeof(T) == 4 ? 4 * stage_at(r, 4 * q) : piece_at(r, q)));
+        if (r < rows) {
+            uint4 *g = reinterpret_cast<uint4 *>(p + r * ld) + q;
+            if (STORE) *g = *s;
+            else *s = *g;
+        }
     }
 }
 
-// Rows that start on 16 bytes: lane = row, whole 16-byte pieces.
+// Rows that start on 16 bytes: lane = row for the arithmetic.
 template <typename T>
-__device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[32], int64_t row, int64_t col0, bool in,
-                                            float row_factor) {
+__device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[32], unsigned char *stage, int64_t row0,
+                                            int64_t col0, int rows, int lane, float row_factor) {
     if (e.row_exp != nullptr) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
@@ -225,21 +252,38 @@ __device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[
             for (int c = 0; c < 4; ++c) v[4 * q + c] *= row_factor * __int_as_float((ex[c] + 127) << 23);
         }
     }
-    float t[32];
     if (e.bias != nullptr) {
-        load_row<T>(static_cast<const T *>(e.bias) + col0, t);
+        constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] += t[c];
+        for (int q = 0; q < 32 / kPer; ++q) {
+            union { uint4 u; T t[kPer]; } x;
+            x.u = reinterpret_cast<const uint4 *>(static_cast<const T *>(e.bias) + col0)[q];
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) v[q * kPer + c] += to_f32<T>(x.t[c]);
+        }
     }
-    if (!in) return;
-    if (e.z != nullptr) store_row<float>(e.z + row * e.ld_z + col0, v);
-    if (e.residual != nullptr) load_row<T>(static_cast<const T *>(e.residual) + row * e.ld_res + col0, t);
+    if (e.z != nullptr) {
+        rows_to_stage<float>(stage, v, lane);
+        __syncwarp();
+        stage_global<float, true>(stage, e.z + row0 * e.ld_z + col0, e.ld_z, rows, lane);
+        __syncwarp();
+    }
     apply_act(v, e.act);
     if (e.residual != nullptr) {
+        // (a residual array may be read-only: the template's pointer type is shared with the stores)
+        stage_global<T, false>(stage, const_cast<T *>(static_cast<const T *>(e.residual)) + row0 * e.ld_res + col0,
+                               e.ld_res, rows, lane);
+        __syncwarp();
+        float t[32];
+        rows_from_stage<T>(stage, t, lane);
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < 32; ++c) v[c] += t[c];
     }
-    store_row<T>(static_cast<T *>(e.out) + row * e.ld_out + col0, v);
+    rows_to_stage<T>(stage, v, lane);
+    __syncwarp();
+    stage_global<T, true>(stage, static_cast<T *>(e.out) + row0 * e.ld_out + col0, e.ld_out, rows, lane);
+    __syncwarp();
 }
 
 // Any alignment: lane = column, the rows one after another from the staging
@@ -298,8 +342,9 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
     }
     const bool exact_scale = __any_sync(kFull, re > 60 || re < -60 || ce > 60 || ce < -60);
     const float rf = exact_scale ? 1.0f : __int_as_float((re + 127) << 23);
+    const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
     if (e.aligned && !exact_scale && col0 + 32 <= n) {
-        linear_rows<T>(e, v, row0 + lane, col0, row0 + lane < m, rf);
+        linear_rows<T>(e, v, reinterpret_cast<unsigned char *>(stage), row0, col0, rows, lane, rf);
         return;
     }
     if (e.row_exp != nullptr) {
@@ -308,18 +353,27 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
     }
     stage_rows(stage, v, lane);
     __syncwarp();
-    const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
     linear_columns<T>(e, stage, row0, col0, rows, n, lane, exact_scale, re, ce);
     __syncwarp();
 }
 
+// What an epilogue warp keeps from chunk to chunk.
+struct EpiWarp {
+    float *stage;          // its staging tile (4 KB)
+    uint32_t bar, phase;   // its barrier for loads into the tile
+    volatile int *failed;
+    int lane;
+};
+
 template <typename T>
 struct EpiLinear {
     LinearEpilogue p;
-    __device__ __forceinline__ void operator()(float (&v)[32], float *stage, int, int64_t row0, int64_t col0,
-                                               int64_t m, int64_t n, int lane) const {
-        linear_store<T>(p, v, stage, row0, col0, m, n, lane);
+    __device__ __forceinline__ void prepare(EpiWarp &, int, int64_t, int64_t) const {}
+    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0, int64_t m,
+                                               int64_t n, bool) const {
+        linear_store<T>(p, v, w.stage, row0, col0, m, n, w.lane);
     }
+    __device__ __forceinline__ void finish(EpiWarp &) const {}
 };
 
 __device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
@@ -327,19 +381,31 @@ __device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// 32 consecutive columns of one row as two planes.  Pitches and line counts of
-// the planes are multiples of 32, so whole pieces fit; what lies past the
-// matrix is never read (the tensor maps end with it).
-__device__ __forceinline__ void planes_row(__half *hi, int64_t plane, const float (&v)[32]) {
-    __half *lo = hi + plane;
+// ---- 32 x 32 tiles of two planes: hi at the staging tile's start, lo 2 KB on ----
+__device__ __forceinline__ void planes_to_stage(unsigned char *stage, const float (&v)[32], int lane) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         union { __half h[8]; uint4 u; } a, b;
 #pragma unroll
         for (int c = 0; c < 8; ++c) split_half(v[q * 8 + c], a.h[c], b.h[c]);
-        reinterpret_cast<uint4 *>(hi)[q] = a.u;
-        reinterpret_cast<uint4 *>(lo)[q] = b.u;
+        *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = a.u;
+        *reinterpret_cast<uint4 *>(stage + 2048 + piece_at(lane, q)) = b.u;
     }
+}
+// Stores the staged tile (all lanes have written it); lane 0 owns the copy.
+__device__ __forceinline__ void stage_store(const CUtensorMap *map, uint32_t stage, int col, int row, int b, int lane) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                         reinterpret_cast<uint64_t>(map)), "r"(stage), "r"(col), "r"(row), "r"(0), "r"(b) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+}
+// The staging tile may be written again.
+__device__ __forceinline__ void stage_free(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
 }
 
 template <typename T>
@@ -378,63 +444,110 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
     __syncwarp();
 }
 
+// Planes go to and come from memory by TMA: whole tiles through the warp's
+// staging tile, C for a tile's first chunk already under the products.
 template <bool SYM>
 struct EpiPlanes {
     PlanesEpilogue p;
-    __device__ __forceinline__ void operator()(float (&v)[32], float *stage, int b, int64_t row0, int64_t col0,
-                                               int64_t m, int64_t n, int lane) const {
-        if (SYM && col0 > row0) return;  // all of it above the diagonal: its mirror image writes it
-        const int64_t row = row0 + lane;
+    CUtensorMap map_c, map_out, map_out2;
+
+    __device__ __forceinline__ void load_c(EpiWarp &w, int b, int64_t row0, int64_t col0) const {
+        if (w.lane == 0) {
+            bar_expect(w.bar, 4096);
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(w.stage)),
+                "l"(reinterpret_cast<uint64_t>(&map_c)), "r"(w.bar), "r"(static_cast<int>(col0)),
+                "r"(static_cast<int>(row0)), "r"(0), "r"(b) : "memory");
+        }
+    }
+    __device__ __forceinline__ bool wanted(int64_t row0, int64_t col0) const {
+        return !SYM || col0 <= row0;  // the rest is written as a mirror image
+    }
+    // The first chunk's C, before the products are waited for.
+    __device__ __forceinline__ void prepare(EpiWarp &w, int b, int64_t row0, int64_t col0) const {
+        if (p.c != nullptr && wanted(row0, col0)) load_c(w, b, row0, col0);
+    }
+    __device__ __forceinline__ void finish(EpiWarp &w) const {
+        if (w.lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
+    }
+    // first: whether prepare has loaded C
+    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int b, int64_t row0, int64_t col0, int64_t m,
+                                               int64_t n, bool first) const {
+        if (!wanted(row0, col0)) return;
+        const int lane = w.lane;
+        unsigned char *stage = reinterpret_cast<unsigned char *>(w.stage);
+        const uint32_t s32 = smem_u32(stage);
         if (p.c != nullptr) {
-            const uint4 *hi = reinterpret_cast<const uint4 *>(p.c + b * p.c_batch + row * p.c_ld + col0);
-            const uint4 *lo = reinterpret_cast<const uint4 *>(p.c + b * p.c_batch + p.c_plane + row * p.c_ld + col0);
+            if (!first) load_c(w, b, row0, col0);
+            const bool ok = warp_wait(w.bar, w.phase, w.failed);
+            w.phase ^= 1;
+            if (!ok) return;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 union { uint4 u; __half h[8]; } a, z;
-                a.u = hi[q];
-                z.u = lo[q];
+                a.u = *reinterpret_cast<const uint4 *>(stage + piece_at(lane, q));
+                z.u = *reinterpret_cast<const uint4 *>(stage + 2048 + piece_at(lane, q));
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     v[q * 8 + c] =
                         fmaf(p.alpha, v[q * 8 + c], p.beta * (__half2float(a.h[c]) + __half2float(z.h[c])));
             }
+            __syncwarp();
         } else {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
         }
         if (!SYM && p.fin.ptr != nullptr) {
-            if (p.dtype == kOutF32) final_store<float>(p, v, stage, b, row0, col0, m, n, lane);
-            else if (p.dtype == kOutF16) final_store<__half>(p, v, stage, b, row0, col0, m, n, lane);
-            else final_store<__nv_bfloat16>(p, v, stage, b, row0, col0, m, n, lane);
+            if (p.dtype == kOutF32) final_store<float>(p, v, w.stage, b, row0, col0, m, n, lane);
+            else if (p.dtype == kOutF16) final_store<__half>(p, v, w.stage, b, row0, col0, m, n, lane);
+            else final_store<__nv_bfloat16>(p, v, w.stage, b, row0, col0, m, n, lane);
+            // the staging tile is next written by a TMA load: order it behind these accesses
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
             return;
         }
-        if (!SYM) {
-            planes_row(p.out + b * p.batch + row * p.ld + col0, p.plane, v);
-            return;
+        const int row = static_cast<int>(row0), col = static_cast<int>(col0);
+        if (SYM && col == row) {
+            // the tile on the diagonal: its upper half from the lower
+            stage_rows(w.stage, v, lane);
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = w.stage[stage_at(max(c, lane), min(c, lane))];
+            __syncwarp();
         }
 #pragma unroll 1
-        for (int o = 0; o < (p.out2 != nullptr ? 2 : 1); ++o) {
-            __half *base = o == 0 ? p.out + b * p.batch : p.out2 + b * p.batch2;
-            const int64_t ld = o == 0 ? p.ld : p.ld2, plane = o == 0 ? p.plane : p.plane2;
+        for (int o = 0; o < (SYM && p.out2 != nullptr ? 2 : 1); ++o) {
+            const CUtensorMap *map = o == 0 ? &map_out : &map_out2;
             if (o == 1) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col0 + c == row ? p.diag : 0.0f);
+                for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col + c == row + lane ? p.diag : 0.0f);
             }
-            stage_rows(stage, v, lane);
-            __syncwarp();
-            float t[32];
-            if (col0 == row0) {
-                // the block on the diagonal: its upper half from the lower
+            planes_to_stage(stage, v, lane);
+            stage_store(map, s32, col, row, b, lane);
+            if (SYM && col != row) {
+                // the mirror image: 8 x 8 blocks turned on their way through registers
+                uint32_t r[2][4][4];
+                const int j = lane >> 3, k = lane & 7;
 #pragma unroll
-                for (int c = 0; c < 32; ++c) t[c] = stage[stage_at(max(c, lane), min(c, lane))];
-                planes_row(base + row * ld + col0, plane, t);
-            } else {
-                planes_row(base + row * ld + col0, plane, v);
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int c = 0; c < 32; ++c) t[c] = stage[stage_at(c, lane)];
-                planes_row(base + (col0 + lane) * ld + row0, plane, t);
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(r[q][i][0]), "=r"(r[q][i][1]), "=r"(r[q][i][2]), "=r"(r[q][i][3])
+                                     : "r"(s32 + 2048 * q + piece_at(8 * i + k, j)) : "memory");
+                stage_free(lane);
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                                         s32 + 2048 * q + piece_at(8 * j + k, i)),
+                                     "r"(r[q][i][0]), "r"(r[q][i][1]), "r"(r[q][i][2]), "r"(r[q][i][3]) : "memory");
+                stage_store(map, s32, row, col, b, lane);
             }
-            __syncwarp();
+            stage_free(lane);
         }
     }
 };
@@ -451,13 +564,13 @@ struct Config {
 template <int BN, int PLANES, typename Epi>
 __global__ __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, int64_t m,
-                 int64_t n, int64_t k, TileGrid grid, int a_mn, int b_mn, uint32_t idesc, const Epi epi) {
+                 int64_t n, int64_t k, TileGrid grid, int a_mn, int b_mn, uint32_t idesc, const __grid_constant__ Epi epi) {
     using C = Config<BN, PLANES>;
     extern __shared__ unsigned char raw[];
     // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
     unsigned char *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float *stage_epi = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
-    __shared__ uint64_t bars[2 * C::kStages + 4];
+    __shared__ uint64_t bars[2 * C::kStages + 4 + kEpiWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
@@ -468,10 +581,10 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::kStages, acc_full = empty + 8 * C::kStages,
                    acc_empty = acc_full + 16;
 
-    if (threadIdx.x < 2 * C::kStages + 4) {
-        const int i = threadIdx.x;
-        // the last two, accumulator buffers free: every epilogue warp of both CTAs arrives
-        bar_init(full + 8 * i, i < 2 * C::kStages + 2 ? 1 : 2 * kEpiWarps);
+    if (threadIdx.x < 2 * C::kStages + 4 + kEpiWarps) {
+        const int i = threadIdx.x, k = i - (2 * C::kStages + 2);
+        // accumulator buffers free: every epilogue warp of both CTAs arrives
+        bar_init(full + 8 * i, k == 0 || k == 1 ? 2 * kEpiWarps : 1);
         if (i == 0) failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -578,7 +691,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        float *stage = stage_epi + warp * 32 * 32;
+        EpiWarp w{stage_epi + warp * 32 * 32, acc_empty + 16 + 8 * warp, 0, &failed, lane};
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -587,10 +700,11 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             tile_of<BN>(grid, t, b, ti, tj);
             const int64_t row0 = static_cast<int64_t>(ti) * 2 * kBM + cta * kBM + (warp & 3) * 32;
             const int64_t col0 = static_cast<int64_t>(tj) * BN;
+            const int half = (warp >> 2) * (BN / 2);
+            if (ok && row0 < m && col0 + half < n) epi.prepare(w, b, row0, col0 + half);
             if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-            const int half = (warp >> 2) * (BN / 2);
 #pragma unroll 1
             for (int c = half; c < half + BN / 2; c += 32) {
                 float v[32];
@@ -600,7 +714,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
                 }
-                if (row0 < m && col0 + c < n) epi(v, stage, b, row0, col0 + c, m, n, lane);
+                if (row0 < m && col0 + c < n) epi(v, w, b, row0, col0 + c, m, n, c == half);
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -608,6 +722,7 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (lane == 0) bar_arrive_cta0(acc_empty + 8 * buf);
             if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
+        epi.finish(w);
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -659,6 +774,30 @@ int operand_map(CUtensorMap *map, const GemmOperand &o, int64_t lines_mn, int64_
     const CUresult r = fn(map, kind == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                           const_cast<void *>(o.ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("gemm: tensor map rejected (%d)", static_cast<int>(r));
+        return FL_EINVAL;
+    }
+    return FL_OK;
+}
+
+// Tensor map of 32 x 32 tiles of a two-plane array [rows, cols].
+int planes_map(CUtensorMap *map, const __half *ptr, int64_t ld, int64_t plane, int64_t batch_stride, int64_t rows,
+               int64_t cols, int64_t batch) {
+    FL_REQUIRE((reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % 8 == 0 && plane % 8 == 0 && batch_stride % 8 == 0,
+               "gemm: planes alignment");
+    EncodeFn fn = encode_fn();
+    if (fn == nullptr) {
+        set_error("gemm: cuTensorMapEncodeTiled is not available");
+        return FL_ECUDA;
+    }
+    cuuint64_t dims[4] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), 2, static_cast<cuuint64_t>(batch)};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(plane) * 2,
+                             static_cast<cuuint64_t>(batch_stride) * 2};
+    cuuint32_t box[4] = {32, 32, 2, 1}, unit[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half *>(ptr), dims, strides, box, unit,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         set_error("gemm: tensor map rejected (%d)", static_cast<int>(r));
@@ -737,6 +876,18 @@ int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b,
     return run_any<sizeof(T) == 4 ? 2 : 1>(s, a, b, epi, st);
 }
 
+template <bool SYM>
+int planes_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
+                 cudaStream_t st) {
+    EpiPlanes<SYM> epi{};
+    epi.p = e;
+    int rc = FL_OK;
+    if (e.c != nullptr) rc = planes_map(&epi.map_c, e.c, e.c_ld, e.c_plane, e.c_batch, s.m, s.n, s.batch);
+    if (!rc && e.out != nullptr) rc = planes_map(&epi.map_out, e.out, e.ld, e.plane, e.batch, s.m, s.n, s.batch);
+    if (!rc && e.out2 != nullptr) rc = planes_map(&epi.map_out2, e.out2, e.ld2, e.plane2, e.batch2, s.m, s.n, s.batch);
+    return rc ? rc : run_any<2>(s, a, b, epi, st);
+}
+
 }  // namespace
 
 int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
@@ -751,8 +902,8 @@ int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, 
 int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
                 cudaStream_t st) {
     FL_REQUIRE(a.planes == 2 && b.planes == 2 && (!s.symmetric || (s.m == s.n && e.fin.ptr == nullptr)), "gemm: planes");
-    if (s.symmetric) return run_any<2>(s, a, b, EpiPlanes<true>{e}, st);
-    return run_any<2>(s, a, b, EpiPlanes<false>{e}, st);
+    FL_REQUIRE(e.out != nullptr || e.fin.ptr != nullptr, "gemm: no output");
+    return s.symmetric ? planes_typed<true>(s, a, b, e, st) : planes_typed<false>(s, a, b, e, st);
 }
 
 // Reads and clears the device fault word (synchronizes the device).

@@ -54,8 +54,7 @@ struct Strided {
 
 // Epilogue of a Newton-Schulz product: v = alpha * acc + beta * C[i, j], where
 // C is a 2-plane array, written as planes (mirrored when symmetric), or as the
-// last product's result: fin = v + keep * base.  Pitches and line counts of C
-// and the outputs are multiples of 32.
+// last product's result: fin = v + keep * base.  Pitches are multiples of 8.
 struct PlanesEpilogue {
     float alpha, beta;       // on the accumulator and on the planes' sum
     const __half *c;         // NULL: no C

@@ -36,7 +36,7 @@ namespace fl {
 
 namespace {
 
-constexpr int64_t round32(int64_t v) { return (v + 31) & ~int64_t(31); }
+constexpr int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
 constexpr float kScaleX = 8192.0f, kScaleA = 4096.0f;
 constexpr int kMaxParts = 1024;
 
@@ -291,13 +291,13 @@ struct Planes {
 };
 Planes take_planes(Carve &ws, int64_t batch, int64_t rows, int64_t cols) {
     Planes p;
-    p.ld = round32(cols);
-    p.plane = round32(rows) * p.ld;
+    p.ld = round8(cols);
+    p.plane = rows * p.ld;
     p.p = ws.take<__half>(batch * 2 * p.plane);
     return p;
 }
 size_t planes_bytes(int64_t batch, int64_t rows, int64_t cols) {
-    return carve_bytes<__half>(batch * 2 * round32(rows) * round32(cols));
+    return carve_bytes<__half>(batch * 2 * rows * round8(cols));
 }
 
 GemmShape shape(int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric) {
