@@ -204,9 +204,9 @@ __device__ __forceinline__ void rows_to_stage(unsigned char *stage, const float 
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        union { uint4 u; T t[16 / sizeof(T)]; } x;
+        union { uint4 u; unsigned w[4]; } x;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) x.t[c % (16 / sizeof(T))] = from_f32<T>(v[q * 8 + c]);
+        for (int c = 0; c < 4; ++c) x.w[c] = pack_pair<T>(v[q * 8 + 2 * c], v[q * 8 + 2 * c + 1]);
         *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = x.u;
     }
 }
@@ -376,18 +376,13 @@ struct EpiLinear {
     __device__ __forceinline__ void finish(EpiWarp &) const {}
 };
 
-__device__ __forceinline__ void split_half(float v, __half &hi, __half &lo) {
-    hi = __float2half_rn(v);
-    lo = __float2half_rn(v - __half2float(hi));
-}
-
 // ---- 32 x 32 tiles of two planes: hi at the staging tile's start, lo 2 KB on ----
 __device__ __forceinline__ void planes_to_stage(unsigned char *stage, const float (&v)[32], int lane) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        union { __half h[8]; uint4 u; } a, b;
+        union { __half2 h[4]; uint4 u; } a, b;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) split_half(v[q * 8 + c], a.h[c], b.h[c]);
+        for (int c = 0; c < 4; ++c) split_pair(v[q * 8 + 2 * c], v[q * 8 + 2 * c + 1], a.h[c], b.h[c]);
         *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = a.u;
         *reinterpret_cast<uint4 *>(stage + 2048 + piece_at(lane, q)) = b.u;
     }
@@ -413,33 +408,36 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
                                             int64_t row0, int64_t col0, int64_t m, int64_t n, int lane) {
     T *out = static_cast<T *>(e.fin.ptr) + e.fin.at(b, e.nb2);
     const float *base = e.base.ptr != nullptr ? static_cast<const float *>(e.base.ptr) + e.base.at(b, e.nb2) : nullptr;
-    if (e.fin.i == 1) {  // lane = row is the contiguous direction
-        const int64_t row = row0 + lane;
-        if (row < m) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                const int64_t col = col0 + c;
-                if (col < n) {
-                    float x = v[c];
-                    if (base != nullptr) x = fmaf(e.keep, base[row * e.base.i + col * e.base.j], x);
-                    out[row + col * e.fin.j] = from_f32<T>(x);
-                }
-            }
-        }
-        return;
+    const bool by_row = e.fin.i == 1;  // lane = row is the contiguous direction
+    if (!by_row) {
+        stage_rows(stage, v, lane);
+        __syncwarp();
     }
-    stage_rows(stage, v, lane);
-    __syncwarp();
-    const int64_t col = col0 + lane;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(32), m - row0));
-    if (col < n) {
-#pragma unroll 8
-        for (int r = 0; r < rows; ++r) {
-            const int64_t row = row0 + r;
-            float x = stage[stage_at(r, lane)];
-            if (base != nullptr) x = fmaf(e.keep, base[row * e.base.i + col * e.base.j], x);
-            out[row * e.fin.i + col * e.fin.j] = from_f32<T>(x);
+    const int64_t row = by_row ? row0 + lane : row0, col = by_row ? col0 : col0 + lane;
+    const int lines = static_cast<int>(min(static_cast<int64_t>(32), by_row ? n - col0 : m - row0));
+    const bool in = row < m && col < n;
+    T *po = out + row * e.fin.i + col * e.fin.j;
+    const float *pb = base != nullptr ? base + row * e.base.i + col * e.base.j : nullptr;
+    const int64_t so = by_row ? e.fin.j : e.fin.i, sb = by_row ? e.base.j : e.base.i;
+    // eight lines at a time: the base's loads are in flight together, ahead of the stores that may alias it
+#pragma unroll
+    for (int l0 = 0; l0 < 32; l0 += 8) {
+        if (l0 >= lines) break;
+        float x[8], b0[8];
+        if (base != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) b0[k] = in && l0 + k < lines ? pb[k * sb] : 0.0f;
         }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            x[k] = by_row ? v[l0 + k] : stage[stage_at(l0 + k, lane)];
+            if (base != nullptr) x[k] = fmaf(e.keep, b0[k], x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (in && l0 + k < lines) po[k * so] = from_f32<T>(x[k]);
+        po += 8 * so;
+        pb += 8 * sb;
     }
     __syncwarp();
 }
@@ -486,13 +484,15 @@ struct EpiPlanes {
             if (!ok) return;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                union { uint4 u; __half h[8]; } a, z;
+                union { uint4 u; __half2 h[4]; } a, z;
                 a.u = *reinterpret_cast<const uint4 *>(stage + piece_at(lane, q));
                 z.u = *reinterpret_cast<const uint4 *>(stage + 2048 + piece_at(lane, q));
 #pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    v[q * 8 + c] =
-                        fmaf(p.alpha, v[q * 8 + c], p.beta * (__half2float(a.h[c]) + __half2float(z.h[c])));
+                for (int c = 0; c < 4; ++c) {
+                    const float2 x = __half22float2(a.h[c]), y = __half22float2(z.h[c]);
+                    v[q * 8 + 2 * c] = fmaf(p.alpha, v[q * 8 + 2 * c], p.beta * (x.x + y.x));
+                    v[q * 8 + 2 * c + 1] = fmaf(p.alpha, v[q * 8 + 2 * c + 1], p.beta * (x.y + y.y));
+                }
             }
             __syncwarp();
         } else {

@@ -114,6 +114,26 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// two values at a time: one conversion instruction packs both
+template <typename T> __device__ __forceinline__ unsigned pack_pair(float a, float b);
+template <> __device__ __forceinline__ unsigned pack_pair<float>(float, float) { return 0; }  // not a 16-bit type
+template <> __device__ __forceinline__ unsigned pack_pair<__half>(float a, float b) {
+    union { __half2 h; unsigned u; } x;
+    x.h = __floats2half2_rn(a, b);
+    return x.u;
+}
+template <> __device__ __forceinline__ unsigned pack_pair<__nv_bfloat16>(float a, float b) {
+    union { __nv_bfloat162 h; unsigned u; } x;
+    x.h = __floats2bfloat162_rn(a, b);
+    return x.u;
+}
+// v = hi + lo to 22 bits
+__device__ __forceinline__ void split_pair(float a, float b, __half2 &hi, __half2 &lo) {
+    hi = __floats2half2_rn(a, b);
+    const float2 h = __half22float2(hi);
+    lo = __floats2half2_rn(a - h.x, b - h.y);
+}
+
 // v * 2^e without an overflow or underflow on the way: the power is applied in
 // two halves of one sign (|e| <= 252 as each side's exponent is within 126)
 __device__ __forceinline__ float scale_pow2(float v, int e) {

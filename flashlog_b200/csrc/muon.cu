@@ -50,22 +50,12 @@ struct Source {
     int64_t batch, nb2, m, n;
 };
 
-template <typename T>
-__device__ __forceinline__ float load_as(const void *p, int64_t at) {
-    return to_f32<T>(static_cast<const T *>(p)[at]);
-}
-__device__ __forceinline__ float load_any(const void *p, int64_t at, int dtype) {
-    if (dtype == kOutF32) return load_as<float>(p, at);
-    if (dtype == kOutF16) return load_as<__half>(p, at);
-    return load_as<__nv_bfloat16>(p, at);
-}
-
 // The update's element (i, j); FIRST: also writes the new momentum, which the
 // later passes then read.
-template <bool FIRST>
+template <typename T, bool MUON, bool FIRST>
 __device__ __forceinline__ float update_at(const Source &s, int64_t ub, int64_t mb, int64_t ob, int64_t i, int64_t j) {
-    const float g = load_any(s.u.ptr, ub + i * s.u.i + j * s.u.j, s.dtype);
-    if (s.mom_out.ptr == nullptr) return g;
+    const float g = to_f32(static_cast<const T *>(s.u.ptr)[ub + i * s.u.i + j * s.u.j]);
+    if (!MUON) return g;
     float *out = static_cast<float *>(s.mom_out.ptr) + ob + i * s.mom_out.i + j * s.mom_out.j;
     float v;
     if (FIRST) {
@@ -88,27 +78,65 @@ __device__ __forceinline__ double block_sum(double v, double *scratch) {
     return r;
 }
 
-// Pass 1: new momentum, and partial sums of squares of the update: grid (parts, batch).
+// Pass 1: new momentum, and partial sums of squares of the update: grid (parts,
+// batch).  Four columns a thread are in flight; the sums run in 64 bits, where
+// no square of an fp32 value overflows.
+template <typename T, bool MUON>
 __global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double *partial) {
     __shared__ double scratch[8];
     const int64_t b = blockIdx.y;
     const int64_t ub = s.u.at(b, s.nb2), mb = s.mom.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
-    double sum = 0.0;
-    for (int64_t i = blockIdx.x; i < s.m; i += gridDim.x)
-        for (int64_t j = threadIdx.x; j < s.n; j += blockDim.x) {
-            const double v = update_at<true>(s, ub, mb, ob, i, j);
-            sum += v * v;
+    double sum[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int64_t i = blockIdx.x; i < s.m; i += gridDim.x) {
+        const T *pu = static_cast<const T *>(s.u.ptr) + ub + i * s.u.i;
+        const float *pm = MUON ? static_cast<const float *>(s.mom.ptr) + mb + i * s.mom.i : nullptr;
+        float *po = MUON ? static_cast<float *>(s.mom_out.ptr) + ob + i * s.mom_out.i : nullptr;
+        for (int64_t j0 = threadIdx.x; j0 < s.n; j0 += 1024) {
+            float g[4], v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t j = j0 + 256 * q;
+                const bool in = j < s.n;
+                g[q] = in ? to_f32(pu[j * s.u.j]) : 0.0f;
+                v[q] = MUON && in ? pm[j * s.mom.j] : 0.0f;
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t j = j0 + 256 * q;
+                float u = g[q];
+                if (MUON) {
+                    v[q] = fmaf(s.beta, v[q], g[q]);
+                    if (j < s.n) po[j * s.mom_out.j] = v[q];
+                    u = s.nesterov ? fmaf(s.beta, v[q], g[q]) : v[q];
+                }
+                sum[q] = fma(static_cast<double>(u), static_cast<double>(u), sum[q]);
+            }
         }
-    sum = block_sum(sum, scratch);
-    if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = sum;
+    }
+    const double total = block_sum((sum[0] + sum[1]) + (sum[2] + sum[3]), scratch);
+    if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = total;
 }
 
-// Pass 2: planes of X * 2^13, turned to [short, long]: 32 x 32 tiles, grid (tiles of j, tiles of i, batch).
+// Pass 2: planes of X * 2^13, turned to [short, long]: 64 x 64 tiles, grid
+// (tiles of j, tiles of i, batch); a lane holds two neighbours, so rows are
+// written in whole cache lines.
+template <typename T, bool MUON, bool TURNED>
 __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const double *partial, int parts, double eps,
-                                                        int turned, __half *out, int64_t ld, int64_t plane) {
+                                                        __half *out, int64_t ld, int64_t plane) {
     __shared__ double scratch[8];
-    __shared__ float tile[32][33];
+    __shared__ float tile[TURNED ? 64 : 1][65];
     const int64_t b = blockIdx.z;
+    const int64_t ub = s.u.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
+    const int64_t i0 = blockIdx.y * int64_t(64), j0 = blockIdx.x * int64_t(64);
+    float v[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            // turned tiles are read a lane per element (they turn in shared memory), others two neighbours a lane
+            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (TURNED ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
+            v[k][w] = i < s.m && j < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i, j) : 0.0f;
+        }
     double sum = 0.0;
     for (int p = threadIdx.y * 32 + threadIdx.x; p < parts; p += 256) sum += partial[b * parts + p];
     sum = warp_sum(sum);
@@ -117,34 +145,38 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     sum = 0.0;
     for (int i = 0; i < 8; ++i) sum += scratch[i];
     const double scale = static_cast<double>(kScaleX) / (sqrt(sum) + eps);
-    const int64_t ub = s.u.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
-    const int64_t i0 = blockIdx.y * int64_t(32), j0 = blockIdx.x * int64_t(32);
     __half *hi = out + b * 2 * plane;
+    if (TURNED) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + threadIdx.x;
-        float v = 0.0f;
-        if (i < s.m && j < s.n) v = static_cast<float>(update_at<false>(s, ub, 0, ob, i, j) * scale);
-        if (turned) {
-            tile[threadIdx.y + 8 * k][threadIdx.x] = v;
-        } else if (i < s.m && j < s.n) {
-            const __half h = __float2half_rn(v);
-            hi[i * ld + j] = h;
-            hi[plane + i * ld + j] = __float2half_rn(v - __half2float(h));
-        }
-    }
-    if (!turned) return;
-    __syncthreads();
+        for (int k = 0; k < 8; ++k)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t j = j0 + threadIdx.y + 8 * k, i = i0 + threadIdx.x;
-        if (i < s.m && j < s.n) {
-            const float v = tile[threadIdx.x][threadIdx.y + 8 * k];
-            const __half h = __float2half_rn(v);
-            hi[j * ld + i] = h;
-            hi[plane + j * ld + i] = __float2half_rn(v - __half2float(h));
-        }
+            for (int w = 0; w < 2; ++w) tile[threadIdx.y + 8 * k][threadIdx.x + 32 * w] = static_cast<float>(v[k][w] * scale);
+        __syncthreads();
     }
+    const int64_t rows = TURNED ? s.n : s.m, cols = TURNED ? s.m : s.n, r0 = TURNED ? j0 : i0, c0 = TURNED ? i0 : j0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int64_t r = r0 + threadIdx.y + 8 * k, c = c0 + 2 * threadIdx.x;
+        if (r >= rows || c >= cols) continue;
+        const float a = TURNED ? tile[2 * threadIdx.x][threadIdx.y + 8 * k] : static_cast<float>(v[k][0] * scale);
+        const float z = TURNED ? tile[2 * threadIdx.x + 1][threadIdx.y + 8 * k] : static_cast<float>(v[k][1] * scale);
+        __half2 h, l;
+        split_pair(a, z, h, l);
+        // the pitch is a multiple of 8 and at least cols: the pair fits in the row
+        *reinterpret_cast<__half2 *>(hi + r * ld + c) = h;
+        *reinterpret_cast<__half2 *>(hi + plane + r * ld + c) = l;
+    }
+}
+
+template <typename T, bool MUON>
+int normalize(const Source &s, bool turned, double eps, double *partial, int parts, __half *x, int64_t ld,
+              int64_t plane, cudaStream_t st) {
+    launch(square_sum_kernel<T, MUON>, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial);
+    const dim3 grid(static_cast<unsigned>((s.n + 63) / 64), static_cast<unsigned>((s.m + 63) / 64),
+                    static_cast<unsigned>(s.batch));
+    if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
+    else launch(normalize_kernel<T, MUON, false>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
+    return check_launch("newton-schulz normalize");
 }
 
 struct Finish {
@@ -185,6 +217,7 @@ __device__ __forceinline__ void small_product(const float *A, int lda, const flo
 }
 
 // The whole step of one small matrix in one block.
+template <typename T, bool MUON>
 __global__ void __launch_bounds__(512) small_kernel(const Source s, const Finish f, int turned, int lo, int hi,
                                                     int steps, float ca, float cb, float cc, double eps) {
     extern __shared__ float sm[];
@@ -197,8 +230,8 @@ __global__ void __launch_bounds__(512) small_kernel(const Source s, const Finish
     double sum = 0.0;
     for (int t = threadIdx.x; t < m * n; t += blockDim.x) {
         const int i = t / n, j = t - i * n;
-        const float v = update_at<true>(s, ub, mb, ob, i, j);
-        sum += static_cast<double>(v) * v;
+        const float v = update_at<T, MUON, true>(s, ub, mb, ob, i, j);
+        sum = fma(static_cast<double>(v), static_cast<double>(v), sum);
         X[turned ? j * ldx + i : i * ldx + j] = v;
     }
     sum = block_sum(sum, scratch);
@@ -336,6 +369,16 @@ Strided turn(Strided s, bool turned) {
     return s;
 }
 
+template <typename T, bool MUON>
+int run_small(const Source &s, const Finish &f, bool turned, int64_t lo, int64_t hi, int steps, float a, float b, float c,
+              double eps, cudaStream_t st) {
+    auto kernel = small_kernel<T, MUON>;
+    FL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    launch(kernel, static_cast<unsigned>(s.batch), lo * hi >= 2048 ? 512 : 256, small_smem(lo, hi), st, s, f,
+           static_cast<int>(turned), static_cast<int>(lo), static_cast<int>(hi), steps, a, b, c, eps);
+    return check_launch("newton-schulz");
+}
+
 int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double cb, double cc, double eps, void *wsp,
                   size_t ws_bytes, cudaStream_t st) {
     const bool turned = s.m > s.n;
@@ -345,13 +388,12 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
                "newton-schulz: these coefficients do not keep singular values of [0, 1] within 3");
     const float fa = static_cast<float>(ca), fb = static_cast<float>(cb), fc = static_cast<float>(cc);
     if (is_small(lo, hi, steps)) {
-        const size_t smem = small_smem(lo, hi);
-        FL_CUDA(cudaFuncSetAttribute(small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-        launch(small_kernel, static_cast<unsigned>(s.batch), lo * hi >= 2048 ? 512 : 256, smem, st, s, f, turned,
-               static_cast<int>(lo), static_cast<int>(hi), steps, fa, fb, fc, eps);
-        return check_launch("newton-schulz");
+        if (s.mom_out.ptr != nullptr) return run_small<float, true>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
+        if (s.dtype == FL_F32) return run_small<float, false>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
+        if (s.dtype == FL_F16) return run_small<__half, false>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
+        return run_small<__nv_bfloat16, false>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
     }
-    FL_REQUIRE(s.batch <= 65535 && (s.m + 31) / 32 <= 65535, "newton-schulz: too large a batch or matrix");
+    FL_REQUIRE(s.batch <= 65535 && (s.m + 63) / 64 <= 65535, "newton-schulz: too large a batch or matrix");
     Carve ws(wsp, ws_bytes);
     const int parts = parts_of(s.batch, s.m);
     double *partial = ws.take<double>(s.batch * parts);
@@ -367,11 +409,11 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     }
     FL_REQUIRE(partial && x.p && a.p && b.p && (gram ? t.p != nullptr : x2.p != nullptr), "newton-schulz: workspace too small");
 
-    launch(square_sum_kernel, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial);
-    launch(normalize_kernel, dim3(static_cast<unsigned>((s.n + 31) / 32), static_cast<unsigned>((s.m + 31) / 32),
-                                  static_cast<unsigned>(s.batch)),
-           dim3(32, 8), 0, st, s, partial, parts, eps, static_cast<int>(turned), x.p, x.ld, x.plane);
-    int rc = check_launch("newton-schulz normalize");
+    int rc;
+    if (s.mom_out.ptr != nullptr) rc = normalize<float, true>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
+    else if (s.dtype == FL_F32) rc = normalize<float, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
+    else if (s.dtype == FL_F16) rc = normalize<__half, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
+    else rc = normalize<__nv_bfloat16, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
     if (rc) return rc;
 
     PlanesEpilogue last = epilogue(0.0f, nullptr, 0.0f, nullptr);
