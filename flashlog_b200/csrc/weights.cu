@@ -10,12 +10,11 @@
 // One pass over the row: its values stay in registers, and one joint reduction
 // gives the maximum and the sum, each thread having summed relative to its own
 // maximum.  A row wider than one block's registers is spread over a cluster of
-// up to eight blocks, which exchange their (maximum, sum) pairs through shared
-// memory.  The operation is bound by HBM: a value is read once and written once.
+// up to eight blocks, which send each other their (maximum, sum) pairs.  The operation is bound by HBM: a value is read once and written once.
 //
 // The history's counts live in shared memory next to one "seen" bit per
 // column; a warp's 32 columns share one word of bits, so columns without
-// history cost one broadcast read per warp.  Counts are cleared by walking the
+// history cost nothing per column.  Counts are cleared by walking the
 // history again, not by clearing the row.
 #include "gemm.cuh"
 
@@ -50,37 +49,101 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float peer_float(const float *p, uint32_t rank) {
-    float v;
-    asm volatile(
-        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
-        : "=f"(v) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank) : "memory");
-    return v;
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
-// History counts of one row for the columns [c0, c0 + chunk): add (or clear).
-template <int THREADS, bool ADD>
-__device__ __forceinline__ void history_pass(const WeightsArgs &a, int64_t row, int64_t c0, int chunk, unsigned *seen,
+// The blocks of a cluster exchange one 8-byte value each per row: every block
+// sends its own to all (itself too) with a store that counts on the receiver's
+// barrier, so no fence has to wait for the rows written to global memory.  Two
+// slots alternate: a block can only send for row r + 2 after it has received
+// everything for row r + 1, which the others send after reading row r.
+struct Exchange {
+    uint64_t bar[2];
+    float2 slot[2][8];
+};
+constexpr uint64_t kWaitLimitNs = 4000000000ull;
+
+__device__ __forceinline__ void exchange_init(Exchange &x) {
+    if (threadIdx.x < 2)
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n fence.mbarrier_init.release.cluster;" ::"r"(
+                         smem_u32(&x.bar[threadIdx.x])) : "memory");
+    __syncthreads();
+    cluster_barrier();
+}
+// Called by warp 0 after the block's value is known; `round` counts rows.
+__device__ __forceinline__ void exchange_send(Exchange &x, int flip, uint32_t rank, uint32_t ranks, float a, float b) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&x.bar[flip])),
+                     "r"(ranks * 8) : "memory");
+    __syncwarp();
+    if (lane < static_cast<int>(ranks)) {
+        const uint64_t v = static_cast<uint64_t>(__float_as_uint(a)) | (static_cast<uint64_t>(__float_as_uint(b)) << 32);
+        asm volatile(
+            "{\n .reg .b32 d, m;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 m, %1, %2;\n"
+            " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [d], %3, [m];\n}" ::"r"(
+                smem_u32(&x.slot[flip][rank])), "r"(smem_u32(&x.bar[flip])), "r"(lane), "l"(v) : "memory");
+    }
+}
+// All blocks' values, lane r holding block r's.  A wait that runs out (which no
+// healthy run does) gives NaN.
+__device__ __forceinline__ float2 exchange_receive(Exchange &x, int flip, uint32_t parity, uint32_t ranks) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t bar = smem_u32(&x.bar[flip]);
+    uint64_t start = 0, now = 0;
+    for (int i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+            " selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) break;
+        if ((i & 63) == 63) {
+            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+            if (start == 0) start = now;
+            if (now - start > kWaitLimitNs) {
+                const float nan = __int_as_float(0x7fc00000);
+                return make_float2(nan, nan);
+            }
+        }
+    }
+    return lane < static_cast<int>(ranks) ? x.slot[flip][lane] : make_float2(-INFINITY, 0.0f);
+}
+
+// A thread's columns of its block are i * THREADS + threadIdx.x.  The seen bits
+// of a warp's 32 columns form one word; the words of a warp lie together, so
+// one load and a ballot tell a warp which of its VPT words are not empty.
+template <int THREADS, int VPT>
+__device__ __forceinline__ int word_of(int c) {  // column of the block -> word
+    const int i = c / THREADS, w = (c % THREADS) >> 5;
+    return w * VPT + i;
+}
+
+// History counts of one row for the block's columns: add (or clear).
+template <int THREADS, int VPT, bool ADD>
+__device__ __forceinline__ void history_pass(const WeightsArgs &a, int64_t row, int c0, unsigned *seen,
                                              unsigned *count) {
     const int64_t *h = a.history + row * a.hist_ld;
-    for (int64_t j = threadIdx.x; j < a.hist; j += THREADS) {
+    const int hist = static_cast<int>(a.hist);
+    for (int j = threadIdx.x; j < hist; j += THREADS) {
         const int64_t v = h[j];
-        if (v < 0 || v >= a.n) continue;
         const int64_t c = v - c0;
-        if (c < 0 || c >= chunk) continue;
+        if (v < 0 || v >= a.n || c < 0 || c >= THREADS * VPT) continue;
+        const int k = static_cast<int>(c);
         if (ADD) {
-            atomicAdd(count + c, 1u);
-            atomicOr(seen + (c >> 5), 1u << (c & 31));
+            atomicAdd(count + k, 1u);
+            atomicOr(seen + word_of<THREADS, VPT>(k), 1u << (k & 31));
         } else {
-            count[c] = 0u;
-            seen[c >> 5] = 0u;
+            count[k] = 0u;
+            seen[word_of<THREADS, VPT>(k)] = 0u;
         }
     }
 }
 
-// (max, sum relative to it) of two parts
-__device__ __forceinline__ float rescale(float m, float to, float inv_tau) {
-    return m == to ? 1.0f : expf((m - to) * inv_tau);  // equal (both -inf too): nothing to do
+// exp((from - to) * k / log2 e): the rescaling of a part summed relative to
+// `from`.  Equal (both -inf too): nothing to do.
+__device__ __forceinline__ float rescale(float from, float to, float k) {
+    return from == to ? 1.0f : exp2f((from - to) * k);
 }
 
 // 1024 threads per SM with up to 64 registers each: enough rows in flight to
@@ -90,188 +153,205 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_forward_kerne
     extern __shared__ unsigned dyn[];
     constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
     unsigned *seen = dyn, *count = dyn + kChunk / 32;
-    __shared__ float warp_m[2][kWarps], warp_s[2][kWarps], block_m[2], block_s[2];
+    __shared__ float warp_m[2][kWarps], warp_s[2][kWarps];
+    __shared__ Exchange ex;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CL ? cluster_rank() : 0, ranks = CL ? cluster_size() : 1;
-    const int64_t c0 = static_cast<int64_t>(rank) * kChunk;
-    if (a.hist > 0) {
+    const int c0 = static_cast<int>(rank) * kChunk;
+    const int left = static_cast<int>(a.n) - c0 - tid;  // the thread's column i exists iff i * THREADS < left
+    const bool hist = a.hist > 0;
+    const float k = a.inv_tau * 1.4426950408889634f;
+    if (hist)
         for (int i = tid; i < kChunk / 32 + kChunk; i += THREADS) dyn[i] = 0u;
-        __syncthreads();
-    }
+    if (CL) exchange_init(ex);
+    __syncthreads();
     int flip = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks, flip ^= 1) {
-        if (a.hist > 0) {
-            history_pass<THREADS, true>(a, row, c0, kChunk, seen, count);
-            __syncthreads();
-        }
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
-        const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld;
-        const int64_t state = a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
-        const bool legal = state >= 0 && state < a.n_states;
-        const uint8_t *mask = a.mask + (legal ? state * a.mask_ld : 0);
+    uint32_t parity = 0;
+    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
         // all of the row's loads first: they are in flight together
-        float u[VPT], m = -INFINITY;
+        const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
         T raw[VPT];
-        unsigned allowed = 0u;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t col = c0 + i * THREADS + tid;
-            raw[i] = col < a.n ? z[col] : from_f32<T>(0.0f);
-        }
+        for (int i = 0; i < VPT; ++i) raw[i] = i * THREADS < left ? z[i * THREADS] : from_f32<T>(0.0f);
+        unsigned allowed = 0u;
         if (a.mask == nullptr) {
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) allowed |= (c0 + i * THREADS + tid < a.n ? 1u : 0u) << i;
-        } else if (legal) {
-            uint8_t ok[VPT];
+            for (int i = 0; i < VPT; ++i) allowed |= (i * THREADS < left ? 1u : 0u) << i;
+        } else {
+            const int64_t state = a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
+            if (state >= 0 && state < a.n_states) {
+                const uint8_t *mask = a.mask + state * a.mask_ld + c0 + tid;
+                uint8_t ok[VPT];
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int64_t col = c0 + i * THREADS + tid;
-                ok[i] = col < a.n ? mask[col] : 0;
+                for (int i = 0; i < VPT; ++i) ok[i] = i * THREADS < left ? mask[i * THREADS] : 0;
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) allowed |= (ok[i] != 0 ? 1u : 0u) << i;
             }
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) allowed |= (ok[i] != 0 ? 1u : 0u) << i;
         }
+        float u[VPT], m = -INFINITY;
         if (a.bias != nullptr) {
+            const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld + c0 + tid;
 #pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                const int64_t col = c0 + i * THREADS + tid;
-                u[i] = col < a.n ? to_f32<T>(bias[col]) : 0.0f;
-            }
+            for (int i = 0; i < VPT; ++i) u[i] = i * THREADS < left ? to_f32<T>(bias[i * THREADS]) : 0.0f;
         } else {
 #pragma unroll
             for (int i = 0; i < VPT; ++i) u[i] = 0.0f;
         }
+        unsigned word = 0u, any = 0u;
+        if (hist) {
+            history_pass<THREADS, VPT, true>(a, row, c0, seen, count);
+            __syncthreads();
+            word = lane < VPT ? seen[warp * VPT + lane] : 0u;
+            any = __ballot_sync(kFull, word != 0u);
+        }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int c = i * THREADS + tid;
             float v = to_f32<T>(raw[i]);
-            if (a.hist > 0 && (seen[c >> 5] >> (c & 31)) & 1u) {
-                v = v > 0.0f ? v / a.theta : v * a.theta;
-                v = v - a.frequency * static_cast<float>(count[c]) - a.presence;
+            if ((any >> i) & 1u) {  // the same for the whole warp
+                if ((__shfl_sync(kFull, word, i) >> lane) & 1u) {
+                    v = v > 0.0f ? v / a.theta : v * a.theta;
+                    v = v - a.frequency * static_cast<float>(count[i * THREADS + tid]) - a.presence;
+                }
             }
-            v = (allowed >> i) & 1u ? v + u[i] : -INFINITY;
-            u[i] = v;
-            m = fmaxf(m, v);
+            u[i] = (allowed >> i) & 1u ? v + u[i] : -INFINITY;
+            m = fmaxf(m, u[i]);
         }
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             // -inf contributes nothing even where it is also the maximum; a NaN stays one
-            u[i] = u[i] == -INFINITY ? 0.0f : expf((u[i] - m) * a.inv_tau);
+            u[i] = u[i] == -INFINITY ? 0.0f : exp2f((u[i] - m) * k);
             s += u[i];
         }
         const float wm = warp_max(m);
-        const float ws = warp_sum(s * rescale(m, wm, a.inv_tau));
-        if (lane == 0) {
-            warp_m[flip][warp] = wm;
-            warp_s[flip][warp] = ws;
-        }
-        __syncthreads();
-        float bm = lane < kWarps ? warp_m[flip][lane] : -INFINITY;
-        float bs = lane < kWarps ? warp_s[flip][lane] : 0.0f;
-        float top = warp_max(bm);
-        float total = warp_sum(bs * rescale(bm, top, a.inv_tau));
-        if (CL) {
-            if (tid == 0) {
-                block_m[flip] = top;
-                block_s[flip] = total;
+        const float ws = warp_sum(s * rescale(m, wm, k));
+        float top = wm, total = ws;
+        if (kWarps > 1) {
+            if (lane == 0) {
+                warp_m[flip][warp] = wm;
+                warp_s[flip][warp] = ws;
             }
-            cluster_barrier();
-            bm = lane < static_cast<int>(ranks) ? peer_float(&block_m[flip], lane) : -INFINITY;
-            bs = lane < static_cast<int>(ranks) ? peer_float(&block_s[flip], lane) : 0.0f;
+            __syncthreads();
+            const float bm = lane < kWarps ? warp_m[flip][lane] : -INFINITY;
+            const float bs = lane < kWarps ? warp_s[flip][lane] : 0.0f;
             top = warp_max(bm);
-            total = warp_sum(bs * rescale(bm, top, a.inv_tau));
+            total = warp_sum(bs * rescale(bm, top, k));
         }
-        const float f = total == 0.0f ? 0.0f : rescale(m, top, a.inv_tau) / total;
-        float *w = out + row * a.n;
+        if (CL) {
+            if (warp == 0) exchange_send(ex, flip, rank, ranks, top, total);
+            const float2 b = exchange_receive(ex, flip, parity, ranks);
+            top = warp_max(b.x);
+            total = warp_sum(b.y * rescale(b.x, top, k));
+        }
+        const float f = total == 0.0f ? 0.0f : rescale(m, top, k) / total;
+        float *w = out + row * a.n + c0 + tid;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t col = c0 + i * THREADS + tid;
-            if (col < a.n) w[col] = u[i] * f;
-        }
-        if (a.hist > 0) {
-            // every thread read its counts before the reduction's barrier
-            history_pass<THREADS, false>(a, row, c0, kChunk, seen, count);
+        for (int i = 0; i < VPT; ++i)
+            if (i * THREADS < left) w[i * THREADS] = u[i] * f;
+        if (hist) {
+            if (kWarps == 1) __syncwarp();  // otherwise the reduction's barrier lies behind every read of the counts
+            history_pass<THREADS, VPT, false>(a, row, c0, seen, count);
             __syncthreads();
         }
+        flip ^= 1;
+        if (flip == 0) parity ^= 1;
     }
-    if (CL) cluster_barrier();  // no block leaves while another may read its pair
+    if (CL) cluster_barrier();  // no block leaves while another may write to its slots
 }
 
 // dbias_partial: [blocks / ranks, n] sums of du over the rows each cluster took (a fixed set), or NULL;
 // du: [rows, n] for a bias of the logits' shape, or NULL.
 template <typename T, int THREADS, int VPT, bool CL>
-__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_backward_kernel(const WeightsArgs a, const float *w, const float *g,
-                                                                   int64_t ld_g, T *dz, T *du, float *dbias_partial) {
+__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_backward_kernel(const WeightsArgs a, const float *w,
+                                                                                   const float *g, int64_t ld_g, T *dz,
+                                                                                   T *du, float *dbias_partial) {
     extern __shared__ unsigned dyn[];
     constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
     unsigned *seen = dyn, *count = dyn + kChunk / 32;
-    __shared__ float warp_s[2][kWarps], block_s[2];
+    __shared__ float warp_s[2][kWarps];
+    __shared__ Exchange ex;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t rank = CL ? cluster_rank() : 0, ranks = CL ? cluster_size() : 1;
-    const int64_t c0 = static_cast<int64_t>(rank) * kChunk;
+    const int c0 = static_cast<int>(rank) * kChunk;
+    const int left = static_cast<int>(a.n) - c0 - tid;
     const bool hist = a.hist > 0 && a.theta != 1.0f && dz != nullptr;  // only the repetition penalty has a slope
-    if (hist) {
+    if (hist)
         for (int i = tid; i < kChunk / 32 + kChunk; i += THREADS) dyn[i] = 0u;
-        __syncthreads();
-    }
+    if (CL) exchange_init(ex);
+    __syncthreads();
     float acc[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) acc[i] = 0.0f;
     int flip = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks, flip ^= 1) {
-        if (hist) {
-            history_pass<THREADS, true>(a, row, c0, kChunk, seen, count);
-            __syncthreads();
-        }
+    uint32_t parity = 0;
+    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
+        const float *pw = w + row * a.n + c0 + tid, *pg = g + row * ld_g + c0 + tid;
         float p[VPT], q[VPT], s = 0.0f;
 #pragma unroll
+        for (int i = 0; i < VPT; ++i) p[i] = i * THREADS < left ? pw[i * THREADS] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) q[i] = i * THREADS < left ? pg[i * THREADS] : 0.0f;
+        unsigned word = 0u, any = 0u;
+        if (hist) {
+            history_pass<THREADS, VPT, true>(a, row, c0, seen, count);
+            __syncthreads();
+            word = lane < VPT ? seen[warp * VPT + lane] : 0u;
+            any = __ballot_sync(kFull, word != 0u);
+        }
+#pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int64_t col = c0 + i * THREADS + tid;
-            p[i] = col < a.n ? w[row * a.n + col] : 0.0f;
-            q[i] = col < a.n ? g[row * ld_g + col] : 0.0f;
             if (p[i] == 0.0f) q[i] = 0.0f;  // a weight of 0 passes nothing on, whatever the gradient there
             s = fmaf(p[i], q[i], s);
         }
-        s = warp_sum(s);
-        if (lane == 0) warp_s[flip][warp] = s;
-        __syncthreads();
-        float dot = warp_sum(lane < kWarps ? warp_s[flip][lane] : 0.0f);
-        if (CL) {
-            if (tid == 0) block_s[flip] = dot;
-            cluster_barrier();
-            dot = warp_sum(lane < static_cast<int>(ranks) ? peer_float(&block_s[flip], lane) : 0.0f);
+        float dot = warp_sum(s);
+        if (kWarps > 1) {
+            if (lane == 0) warp_s[flip][warp] = dot;
+            __syncthreads();
+            dot = warp_sum(lane < kWarps ? warp_s[flip][lane] : 0.0f);
         }
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+        if (CL) {
+            if (warp == 0) exchange_send(ex, flip, rank, ranks, dot, 0.0f);
+            const float2 b = exchange_receive(ex, flip, parity, ranks);
+            dot = warp_sum(lane < static_cast<int>(ranks) ? b.x : 0.0f);
+        }
+        const int64_t at = row * a.n + c0 + tid;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int c = i * THREADS + tid;
-            const int64_t col = c0 + c;
-            if (col < a.n) {
-                const float d = p[i] == 0.0f ? 0.0f : p[i] * (q[i] - dot) * a.inv_tau;
-                acc[i] += d;
-                if (du != nullptr) du[row * a.n + col] = from_f32<T>(d);
-                if (dz != nullptr) {
-                    float x = d;
-                    if (hist && (seen[c >> 5] >> (c & 31)) & 1u)
-                        x = to_f32<T>(z[col]) > 0.0f ? d / a.theta : d * a.theta;
-                    dz[row * a.n + col] = from_f32<T>(x);
+            const float d = p[i] == 0.0f ? 0.0f : p[i] * (q[i] - dot) * a.inv_tau;
+            p[i] = d;
+            acc[i] += d;
+        }
+        if (du != nullptr) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+                if (i * THREADS < left) du[at + i * THREADS] = from_f32<T>(p[i]);
+        }
+        if (dz != nullptr) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                if ((any >> i) & 1u) {
+                    if (((__shfl_sync(kFull, word, i) >> lane) & 1u) && i * THREADS < left) {
+                        const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
+                        p[i] = to_f32<T>(z[i * THREADS]) > 0.0f ? p[i] / a.theta : p[i] * a.theta;
+                    }
                 }
+                if (i * THREADS < left) dz[at + i * THREADS] = from_f32<T>(p[i]);
             }
         }
         if (hist) {
-            __syncthreads();  // the seen bits were read after the reduction's barrier
-            history_pass<THREADS, false>(a, row, c0, kChunk, seen, count);
+            // the seen words were read before the reduction's barrier
+            if (kWarps == 1) __syncwarp();
+            history_pass<THREADS, VPT, false>(a, row, c0, seen, count);
             __syncthreads();
         }
+        flip ^= 1;
+        if (flip == 0) parity ^= 1;
     }
     if (dbias_partial != nullptr) {
-        float *out = dbias_partial + (blockIdx.x / ranks) * a.n;
+        float *po = dbias_partial + (blockIdx.x / ranks) * a.n + c0 + tid;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t col = c0 + i * THREADS + tid;
-            if (col < a.n) out[col] = acc[i];
-        }
+        for (int i = 0; i < VPT; ++i)
+            if (i * THREADS < left) po[i * THREADS] = acc[i];
     }
     if (CL) cluster_barrier();
 }
@@ -316,9 +396,7 @@ Layout layout(int64_t rows, int64_t n) {
         while (l.ranks < 8 && static_cast<int64_t>(l.ranks) * 512 * vpt < n) l.ranks *= 2;
         l.vpt = static_cast<int64_t>(l.ranks) * 512 * vpt >= n ? vpt : 16;
     }
-    // 2048 threads per SM bound the rows in flight
-    int64_t fit = static_cast<int64_t>(sms) * (2048 / l.threads < 32 ? 2048 / l.threads : 32) / l.ranks;
-    if (l.vpt == 16) fit = fit / 2 > 0 ? fit / 2 : 1;
+    const int64_t fit = static_cast<int64_t>(sms) * (1024 / l.threads) / l.ranks;  // rows in flight
     l.clusters = rows < fit ? rows : fit;
     return l;
 }
