@@ -113,7 +113,7 @@ def relation_weights(logits, *, tau: float = 1.0, mask=None, states=None, bias=N
         u = u - frequency * count - presence * [count > 0] + bias
         w = softmax(u / tau) over the operators that the mask allows, 0 elsewhere
 
-    history: int64 [..., H], the operators used so far (entries outside [0, n), such as a padding of -1, do not
+    history: int64 [..., H], H <= 65535, the operators used so far (entries outside [0, n), such as a padding of -1, do not
     count).  bias: [n] or the logits' shape, of their dtype.  mask: bool or uint8; with states (int64 [...]) a
     table [S, n] of what may follow each state, and a state outside [0, S) allows nothing; without states [n],
     or the logits' shape.  A row with nothing left gets weights 0 (it propagates nothing) and gradient 0.  Masked
@@ -147,6 +147,8 @@ def relation_weights(logits, *, tau: float = 1.0, mask=None, states=None, bias=N
         raise ValueError(f"relation_weights: states must be int64 {tuple(lead)}, next to a mask")
     if history is not None and (history.dtype != torch.int64 or history.dim() < 1 or history.shape[:-1] != lead):
         raise ValueError(f"relation_weights: history must be int64 {tuple(lead)} + [H]")
+    if history is not None and history.shape[-1] > ops.MAX_HISTORY:
+        raise ValueError(f"relation_weights: at most {ops.MAX_HISTORY} history entries, got {history.shape[-1]}")
     ops._one_device("relation_weights", logits, bias, mask, states, history)
     z = logits if logits.dim() == 2 else logits.reshape(-1, n)
     if not (z.stride(1) == 1 and (z.stride(0) >= n or z.shape[0] <= 1)):

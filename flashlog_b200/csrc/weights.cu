@@ -36,80 +36,6 @@ struct WeightsArgs {
     float theta, frequency, presence, inv_tau;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// The blocks of a cluster exchange one 8-byte value each per row: every block
-// sends its own to all (itself too) with a store that counts on the receiver's
-// barrier, so no fence has to wait for the rows written to global memory.  Two
-// slots alternate: a block can only send for row r + 2 after it has received
-// everything for row r + 1, which the others send after reading row r.
-struct Exchange {
-    uint64_t bar[2];
-    float2 slot[2][8];
-};
-constexpr uint64_t kWaitLimitNs = 4000000000ull;
-
-__device__ __forceinline__ void exchange_init(Exchange &x) {
-    if (threadIdx.x < 2)
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;\n fence.mbarrier_init.release.cluster;" ::"r"(
-                         smem_u32(&x.bar[threadIdx.x])) : "memory");
-    __syncthreads();
-    cluster_barrier();
-}
-// Called by warp 0 after the block's value is known; `round` counts rows.
-__device__ __forceinline__ void exchange_send(Exchange &x, int flip, uint32_t rank, uint32_t ranks, float a, float b) {
-    const int lane = threadIdx.x & 31;
-    if (lane == 0)
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&x.bar[flip])),
-                     "r"(ranks * 8) : "memory");
-    __syncwarp();
-    if (lane < static_cast<int>(ranks)) {
-        const uint64_t v = static_cast<uint64_t>(__float_as_uint(a)) | (static_cast<uint64_t>(__float_as_uint(b)) << 32);
-        asm volatile(
-            "{\n .reg .b32 d, m;\n mapa.shared::cluster.u32 d, %0, %2;\n mapa.shared::cluster.u32 m, %1, %2;\n"
-            " st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [d], %3, [m];\n}" ::"r"(
-                smem_u32(&x.slot[flip][rank])), "r"(smem_u32(&x.bar[flip])), "r"(lane), "l"(v) : "memory");
-    }
-}
-// All blocks' values, lane r holding block r's.  A wait that runs out (which no
-// healthy run does) gives NaN.
-__device__ __forceinline__ float2 exchange_receive(Exchange &x, int flip, uint32_t parity, uint32_t ranks) {
-    const int lane = threadIdx.x & 31;
-    const uint32_t bar = smem_u32(&x.bar[flip]);
-    uint64_t start = 0, now = 0;
-    for (int i = 0;; ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-            " selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) break;
-        if ((i & 63) == 63) {
-            asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-            if (start == 0) start = now;
-            if (now - start > kWaitLimitNs) {
-                const float nan = __int_as_float(0x7fc00000);
-                return make_float2(nan, nan);
-            }
-        }
-    }
-    return lane < static_cast<int>(ranks) ? x.slot[flip][lane] : make_float2(-INFINITY, 0.0f);
-}
-
 // A thread's columns of its block are i * THREADS + threadIdx.x.  The seen bits
 // of a warp's 32 columns form one word; the words of a warp lie together, so
 // one load and a ballot tell a warp which of its VPT words are not empty.
@@ -119,202 +45,237 @@ __device__ __forceinline__ int word_of(int c) {  // column of the block -> word
     return w * VPT + i;
 }
 
-// History counts of one row for the block's columns: add (or clear).
+// History counts of a row for the block's columns.  `token` is the thread's
+// first entry, loaded a row ahead; longer histories are read here.  Three
+// buffers rotate: between two of the row loop's barriers the counts of the next
+// row are added while those of the row before are cleared, by walking its
+// history again.
 template <int THREADS, int VPT, bool ADD>
-__device__ __forceinline__ void history_pass(const WeightsArgs &a, int64_t row, int c0, unsigned *seen,
-                                             unsigned *count) {
-    const int64_t *h = a.history + row * a.hist_ld;
-    const int hist = static_cast<int>(a.hist);
-    for (int j = threadIdx.x; j < hist; j += THREADS) {
-        const int64_t v = h[j];
-        const int64_t c = v - c0;
-        if (v < 0 || v >= a.n || c < 0 || c >= THREADS * VPT) continue;
-        const int k = static_cast<int>(c);
-        if (ADD) {
-            atomicAdd(count + k, 1u);
-            atomicOr(seen + word_of<THREADS, VPT>(k), 1u << (k & 31));
-        } else {
-            count[k] = 0u;
-            seen[word_of<THREADS, VPT>(k)] = 0u;
-        }
+__device__ __forceinline__ void history_entry(const WeightsArgs &a, int64_t v, unsigned *buf) {
+    if (v < 0 || v >= a.n) return;
+    const int k = static_cast<int>(v);
+    unsigned *seen = buf + word_of<THREADS, VPT>(k), *count = buf + THREADS * VPT / 32 + k;
+    if (ADD) {
+        atomicAdd(count, 1u);
+        atomicOr(seen, 1u << (k & 31));
+    } else {
+        *count = 0u;
+        *seen = 0u;
     }
 }
+template <int THREADS, int VPT, bool ADD>
+__device__ __forceinline__ void history_pass(const WeightsArgs &a, int64_t row, int64_t token, unsigned *buf) {
+    history_entry<THREADS, VPT, ADD>(a, token, buf);
+    const int64_t *h = a.history + row * a.hist_ld;
+    for (int64_t j0 = threadIdx.x + THREADS; j0 < a.hist; j0 += 8 * THREADS) {
+        int64_t v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = j0 + q * THREADS < a.hist ? h[j0 + q * THREADS] : -1;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) history_entry<THREADS, VPT, ADD>(a, v[q], buf);
+    }
+}
+__device__ __forceinline__ int64_t first_token(const WeightsArgs &a, int64_t row) {
+    return static_cast<int64_t>(threadIdx.x) < a.hist ? a.history[row * a.hist_ld + threadIdx.x] : -1;
+}
+__device__ __forceinline__ int64_t state_of(const WeightsArgs &a, int64_t row) {
+    return a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
+}
 
+// 2^x, to 2^-22; results below 2^-126 are 0
+__device__ __forceinline__ float power2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // exp((from - to) * k / log2 e): the rescaling of a part summed relative to
 // `from`.  Equal (both -inf too): nothing to do.
 __device__ __forceinline__ float rescale(float from, float to, float k) {
-    return from == to ? 1.0f : exp2f((from - to) * k);
+    return from == to ? 1.0f : power2((from - to) * k);
+}
+// Blocks per SM to compile for: 16 values a thread with their prefetched
+// successors want about 80 registers.
+constexpr int min_blocks(int threads, int vpt) {
+    const int b = (vpt > 8 ? 768 : 1024) / threads;
+    return b > 24 ? 24 : b;
 }
 
-// 1024 threads per SM with up to 64 registers each: enough rows in flight to
-// cover the loads' latency while other rows are in their reductions.
-template <typename T, int THREADS, int VPT, bool CL>
-__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_forward_kernel(const WeightsArgs a, float *out) {
+// What a thread holds of a row before its turn.
+template <typename T, int VPT>
+struct RowInputs {
+    T logit[VPT];
+    uint8_t ok[VPT];
+    int64_t token;
+};
+template <typename T, int THREADS, int VPT>
+__device__ __forceinline__ void load_inputs(const WeightsArgs &a, int64_t row, int64_t state, int left,
+                                            RowInputs<T, VPT> &in) {
+    const T *z = static_cast<const T *>(a.logits) + row * a.ld + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) in.logit[i] = i * THREADS < left ? z[i * THREADS] : from_f32<T>(0.0f);
+    const bool legal = state >= 0 && state < a.n_states;
+    if (a.mask != nullptr && legal) {
+        const uint8_t *mask = a.mask + state * a.mask_ld + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) in.ok[i] = i * THREADS < left ? mask[i * THREADS] : 0;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) in.ok[i] = a.mask == nullptr && i * THREADS < left ? 1 : 0;
+    }
+    in.token = first_token(a, row);
+}
+
+// A row's loads are issued while the row before it is reduced and written (and
+// its state a row earlier still): one barrier per row, and the block never
+// waits for memory that it has only just asked for.
+template <typename T, int THREADS, int VPT>
+__global__ __launch_bounds__(THREADS, min_blocks(THREADS, VPT)) void weights_forward_kernel(const WeightsArgs a, float *out) {
     extern __shared__ unsigned dyn[];
-    constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
-    unsigned *seen = dyn, *count = dyn + kChunk / 32;
+    constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32, kCounts = kChunk / 32 + kChunk;
     __shared__ float warp_m[2][kWarps], warp_s[2][kWarps];
-    __shared__ Exchange ex;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t rank = CL ? cluster_rank() : 0, ranks = CL ? cluster_size() : 1;
-    const int c0 = static_cast<int>(rank) * kChunk;
-    const int left = static_cast<int>(a.n) - c0 - tid;  // the thread's column i exists iff i * THREADS < left
+    const int left = static_cast<int>(a.n) - tid;  // the thread's column i exists iff i * THREADS < left
     const bool hist = a.hist > 0;
     const float k = a.inv_tau * 1.4426950408889634f;
-    if (hist)
-        for (int i = tid; i < kChunk / 32 + kChunk; i += THREADS) dyn[i] = 0u;
-    if (CL) exchange_init(ex);
+    const int64_t step = gridDim.x;
+    int64_t row = blockIdx.x;
+    RowInputs<T, VPT> in;
+    int64_t state = 0;
+    if (row < a.rows) {
+        load_inputs<T, THREADS, VPT>(a, row, state_of(a, row), left, in);
+        if (row + step < a.rows) state = state_of(a, row + step);
+    }
+    if (hist) {
+        for (int i = tid; i < 3 * kCounts; i += THREADS) dyn[i] = 0u;
+        __syncthreads();
+        if (row < a.rows) history_pass<THREADS, VPT, true>(a, row, in.token, dyn);
+    }
     __syncthreads();
-    int flip = 0;
-    uint32_t parity = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
-        // all of the row's loads first: they are in flight together
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
-        T raw[VPT];
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) raw[i] = i * THREADS < left ? z[i * THREADS] : from_f32<T>(0.0f);
-        unsigned allowed = 0u;
-        if (a.mask == nullptr) {
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) allowed |= (i * THREADS < left ? 1u : 0u) << i;
-        } else {
-            const int64_t state = a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
-            if (state >= 0 && state < a.n_states) {
-                const uint8_t *mask = a.mask + state * a.mask_ld + c0 + tid;
-                uint8_t ok[VPT];
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) ok[i] = i * THREADS < left ? mask[i * THREADS] : 0;
-#pragma unroll
-                for (int i = 0; i < VPT; ++i) allowed |= (ok[i] != 0 ? 1u : 0u) << i;
-            }
+    int flip = 0, buf = 0;
+    for (; row < a.rows; row += step) {
+        const unsigned *seen = dyn + buf * kCounts, *count = seen + kChunk / 32;
+        unsigned word = 0u, any = 0u;
+        if (hist) {
+            word = lane < VPT ? seen[warp * VPT + lane] : 0u;
+            any = __ballot_sync(kFull, word != 0u);
         }
         float u[VPT], m = -INFINITY;
         if (a.bias != nullptr) {
-            const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld + c0 + tid;
+            const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld + tid;
 #pragma unroll
             for (int i = 0; i < VPT; ++i) u[i] = i * THREADS < left ? to_f32<T>(bias[i * THREADS]) : 0.0f;
         } else {
 #pragma unroll
             for (int i = 0; i < VPT; ++i) u[i] = 0.0f;
         }
-        unsigned word = 0u, any = 0u;
-        if (hist) {
-            history_pass<THREADS, VPT, true>(a, row, c0, seen, count);
-            __syncthreads();
-            word = lane < VPT ? seen[warp * VPT + lane] : 0u;
-            any = __ballot_sync(kFull, word != 0u);
-        }
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            float v = to_f32<T>(raw[i]);
+            float v = to_f32<T>(in.logit[i]);
             if ((any >> i) & 1u) {  // the same for the whole warp
                 if ((__shfl_sync(kFull, word, i) >> lane) & 1u) {
                     v = v > 0.0f ? v / a.theta : v * a.theta;
                     v = v - a.frequency * static_cast<float>(count[i * THREADS + tid]) - a.presence;
                 }
             }
-            u[i] = (allowed >> i) & 1u ? v + u[i] : -INFINITY;
+            u[i] = in.ok[i] != 0 ? v + u[i] : -INFINITY;
             m = fmaxf(m, u[i]);
         }
+        // the next row's inputs, and the state after it
+        const int64_t token = in.token;
+        if (row + step < a.rows) {
+            load_inputs<T, THREADS, VPT>(a, row + step, state, left, in);
+            if (row + 2 * step < a.rows) state = state_of(a, row + 2 * step);
+        }
+        // -inf contributes nothing even where it is also the maximum; a NaN stays one
+        const float from = m == -INFINITY ? 0.0f : m;
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            // -inf contributes nothing even where it is also the maximum; a NaN stays one
-            u[i] = u[i] == -INFINITY ? 0.0f : exp2f((u[i] - m) * k);
+            u[i] = power2((u[i] - from) * k);
             s += u[i];
         }
         const float wm = warp_max(m);
         const float ws = warp_sum(s * rescale(m, wm, k));
-        float top = wm, total = ws;
-        if (kWarps > 1) {
-            if (lane == 0) {
-                warp_m[flip][warp] = wm;
-                warp_s[flip][warp] = ws;
-            }
-            __syncthreads();
-            const float bm = lane < kWarps ? warp_m[flip][lane] : -INFINITY;
-            const float bs = lane < kWarps ? warp_s[flip][lane] : 0.0f;
-            top = warp_max(bm);
-            total = warp_sum(bs * rescale(bm, top, k));
+        if (lane == 0) {
+            warp_m[flip][warp] = wm;
+            warp_s[flip][warp] = ws;
         }
-        if (CL) {
-            if (warp == 0) exchange_send(ex, flip, rank, ranks, top, total);
-            const float2 b = exchange_receive(ex, flip, parity, ranks);
-            top = warp_max(b.x);
-            total = warp_sum(b.y * rescale(b.x, top, k));
-        }
+        const int next = buf == 2 ? 0 : buf + 1;
+        if (hist && row + step < a.rows)
+            history_pass<THREADS, VPT, true>(a, row + step, in.token, dyn + next * kCounts);
+        __syncthreads();
+        const float bm = lane < kWarps ? warp_m[flip][lane] : -INFINITY;
+        const float bs = lane < kWarps ? warp_s[flip][lane] : 0.0f;
+        const float top = warp_max(bm);
+        const float total = warp_sum(bs * rescale(bm, top, k));
+        if (hist) history_pass<THREADS, VPT, false>(a, row, token, dyn + buf * kCounts);
         const float f = total == 0.0f ? 0.0f : rescale(m, top, k) / total;
-        float *w = out + row * a.n + c0 + tid;
+        float *w = out + row * a.n + tid;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
             if (i * THREADS < left) w[i * THREADS] = u[i] * f;
-        if (hist) {
-            if (kWarps == 1) __syncwarp();  // otherwise the reduction's barrier lies behind every read of the counts
-            history_pass<THREADS, VPT, false>(a, row, c0, seen, count);
-            __syncthreads();
-        }
         flip ^= 1;
-        if (flip == 0) parity ^= 1;
+        buf = next;
     }
-    if (CL) cluster_barrier();  // no block leaves while another may write to its slots
 }
 
-// dbias_partial: [blocks / ranks, n] sums of du over the rows each cluster took (a fixed set), or NULL;
+// dbias_partial: [blocks, n] sums of du over the rows each block took (a fixed set), or NULL;
 // du: [rows, n] for a bias of the logits' shape, or NULL.
-template <typename T, int THREADS, int VPT, bool CL>
-__global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_backward_kernel(const WeightsArgs a, const float *w,
+template <typename T, int THREADS, int VPT>
+__global__ __launch_bounds__(THREADS, min_blocks(THREADS, VPT)) void weights_backward_kernel(const WeightsArgs a, const float *w,
                                                                                    const float *g, int64_t ld_g, T *dz,
                                                                                    T *du, float *dbias_partial) {
     extern __shared__ unsigned dyn[];
-    constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32;
-    unsigned *seen = dyn, *count = dyn + kChunk / 32;
+    constexpr int kChunk = THREADS * VPT, kWarps = THREADS / 32, kCounts = kChunk / 32 + kChunk;
     __shared__ float warp_s[2][kWarps];
-    __shared__ Exchange ex;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t rank = CL ? cluster_rank() : 0, ranks = CL ? cluster_size() : 1;
-    const int c0 = static_cast<int>(rank) * kChunk;
-    const int left = static_cast<int>(a.n) - c0 - tid;
+    const int left = static_cast<int>(a.n) - tid;
     const bool hist = a.hist > 0 && a.theta != 1.0f && dz != nullptr;  // only the repetition penalty has a slope
-    if (hist)
-        for (int i = tid; i < kChunk / 32 + kChunk; i += THREADS) dyn[i] = 0u;
-    if (CL) exchange_init(ex);
-    __syncthreads();
-    float acc[VPT];
+    const int64_t step = gridDim.x;
+    int64_t row = blockIdx.x, token = -1;
+    float acc[VPT], p_next[VPT], q_next[VPT];
+    auto load = [&](int64_t r) {
+        const float *pw = w + r * a.n + tid, *pg = g + r * ld_g + tid;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) p_next[i] = i * THREADS < left ? pw[i * THREADS] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) q_next[i] = i * THREADS < left ? pg[i * THREADS] : 0.0f;
+        if (hist) token = first_token(a, r);
+    };
+    if (row < a.rows) load(row);
 #pragma unroll
     for (int i = 0; i < VPT; ++i) acc[i] = 0.0f;
-    int flip = 0;
-    uint32_t parity = 0;
-    for (int64_t row = blockIdx.x / ranks; row < a.rows; row += gridDim.x / ranks) {
-        const float *pw = w + row * a.n + c0 + tid, *pg = g + row * ld_g + c0 + tid;
-        float p[VPT], q[VPT], s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) p[i] = i * THREADS < left ? pw[i * THREADS] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) q[i] = i * THREADS < left ? pg[i * THREADS] : 0.0f;
+    if (hist) {
+        for (int i = tid; i < 3 * kCounts; i += THREADS) dyn[i] = 0u;
+        __syncthreads();
+        if (row < a.rows) history_pass<THREADS, VPT, true>(a, row, token, dyn);
+    }
+    __syncthreads();
+    int flip = 0, buf = 0;
+    for (; row < a.rows; row += step) {
         unsigned word = 0u, any = 0u;
         if (hist) {
-            history_pass<THREADS, VPT, true>(a, row, c0, seen, count);
-            __syncthreads();
-            word = lane < VPT ? seen[warp * VPT + lane] : 0u;
+            word = lane < VPT ? dyn[buf * kCounts + warp * VPT + lane] : 0u;
             any = __ballot_sync(kFull, word != 0u);
         }
+        float p[VPT], q[VPT], s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            if (p[i] == 0.0f) q[i] = 0.0f;  // a weight of 0 passes nothing on, whatever the gradient there
+            p[i] = p_next[i];
+            q[i] = p[i] == 0.0f ? 0.0f : q_next[i];  // a weight of 0 passes nothing on, whatever the gradient there
             s = fmaf(p[i], q[i], s);
         }
-        float dot = warp_sum(s);
-        if (kWarps > 1) {
-            if (lane == 0) warp_s[flip][warp] = dot;
-            __syncthreads();
-            dot = warp_sum(lane < kWarps ? warp_s[flip][lane] : 0.0f);
-        }
-        if (CL) {
-            if (warp == 0) exchange_send(ex, flip, rank, ranks, dot, 0.0f);
-            const float2 b = exchange_receive(ex, flip, parity, ranks);
-            dot = warp_sum(lane < static_cast<int>(ranks) ? b.x : 0.0f);
-        }
-        const int64_t at = row * a.n + c0 + tid;
+        const int64_t old_token = token;
+        const int next = buf == 2 ? 0 : buf + 1;
+        if (row + step < a.rows) load(row + step);
+        const float ws = warp_sum(s);
+        if (lane == 0) warp_s[flip][warp] = ws;
+        if (hist && row + step < a.rows)
+            history_pass<THREADS, VPT, true>(a, row + step, token, dyn + next * kCounts);
+        __syncthreads();
+        const float dot = warp_sum(lane < kWarps ? warp_s[flip][lane] : 0.0f);
+        if (hist) history_pass<THREADS, VPT, false>(a, row, old_token, dyn + buf * kCounts);
+        const int64_t at = row * a.n + tid;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const float d = p[i] == 0.0f ? 0.0f : p[i] * (q[i] - dot) * a.inv_tau;
@@ -331,29 +292,383 @@ __global__ __launch_bounds__(THREADS, 1024 / THREADS) void weights_backward_kern
             for (int i = 0; i < VPT; ++i) {
                 if ((any >> i) & 1u) {
                     if (((__shfl_sync(kFull, word, i) >> lane) & 1u) && i * THREADS < left) {
-                        const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
+                        const T *z = static_cast<const T *>(a.logits) + row * a.ld + tid;
                         p[i] = to_f32<T>(z[i * THREADS]) > 0.0f ? p[i] / a.theta : p[i] * a.theta;
                     }
                 }
                 if (i * THREADS < left) dz[at + i * THREADS] = from_f32<T>(p[i]);
             }
         }
-        if (hist) {
-            // the seen words were read before the reduction's barrier
-            if (kWarps == 1) __syncwarp();
-            history_pass<THREADS, VPT, false>(a, row, c0, seen, count);
-            __syncthreads();
-        }
         flip ^= 1;
-        if (flip == 0) parity ^= 1;
+        buf = next;
     }
     if (dbias_partial != nullptr) {
-        float *po = dbias_partial + (blockIdx.x / ranks) * a.n + c0 + tid;
+        float *po = dbias_partial + blockIdx.x * a.n + tid;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
             if (i * THREADS < left) po[i * THREADS] = acc[i];
     }
-    if (CL) cluster_barrier();
+}
+
+// ---- rows of more than 4096 columns ------------------------------------------
+// Two passes by one block: the first stores u where w will lie and keeps the
+// running maximum and the sum relative to it, the second reads u back (from L2:
+// the rows in flight fit) and writes w.  A cluster per row with the values in
+// registers measured 184 us for 1536 x 29649 with masks and histories, half of
+// it in the exchange between its blocks.
+constexpr int kStreamThreads = 512, kStreamUnroll = 8;
+
+// Counts of a long row: 16 bits each, two to a word (no history has more than
+// 65535 entries), behind one seen bit per column.
+template <bool ADD>
+__device__ __forceinline__ void stream_history(const WeightsArgs &a, int64_t row, unsigned *seen, unsigned *count) {
+    const int64_t *h = a.history + row * a.hist_ld;
+    for (int64_t j = threadIdx.x; j < a.hist; j += kStreamThreads) {
+        const int64_t v = h[j];
+        if (v < 0 || v >= a.n) continue;
+        const int c = static_cast<int>(v);
+        if (ADD) {
+            atomicAdd(count + (c >> 1), 1u << (16 * (c & 1)));
+            atomicOr(seen + (c >> 5), 1u << (c & 31));
+        } else {
+            count[c >> 1] = 0u;
+            seen[c >> 5] = 0u;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStreamThreads) weights_stream_kernel(const WeightsArgs a, float *out) {
+    extern __shared__ unsigned dyn[];
+    constexpr int kWarps = kStreamThreads / 32, U = kStreamUnroll;
+    __shared__ float warp_m[2][kWarps], warp_s[2][kWarps];
+    const int n = static_cast<int>(a.n), words = (n + 31) / 32;
+    unsigned *seen = dyn, *count = dyn + words;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool hist = a.hist > 0;
+    const float k = a.inv_tau * 1.4426950408889634f;
+    if (hist)
+        for (int i = tid; i < words + (n + 1) / 2; i += kStreamThreads) dyn[i] = 0u;
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+        if (hist) {
+            __syncthreads();  // the counts are clear
+            stream_history<true>(a, row, seen, count);
+            __syncthreads();
+        }
+        const int64_t state = state_of(a, row);
+        const bool legal = state >= 0 && state < a.n_states;
+        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+        const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld;
+        const uint8_t *mask = a.mask + (legal ? state * a.mask_ld : 0);
+        float *w = out + row * a.n;
+        float m = -INFINITY, s = 0.0f;
+        for (int base = tid; base < n; base += U * kStreamThreads) {
+            T raw[U], extra[U];
+            uint8_t ok[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int c = base + i * kStreamThreads;
+                raw[i] = c < n ? z[c] : from_f32<T>(0.0f);
+                ok[i] = c < n ? 1 : 0;
+            }
+            if (a.mask != nullptr) {
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int c = base + i * kStreamThreads;
+                    ok[i] = legal && c < n ? mask[c] : 0;
+                }
+            }
+            if (a.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const int c = base + i * kStreamThreads;
+                    extra[i] = c < n ? bias[c] : from_f32<T>(0.0f);
+                }
+            }
+            float u[U], top = m;
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int c = base + i * kStreamThreads;
+                float v = to_f32<T>(raw[i]);
+                if (hist && c < n) {
+                    const unsigned word = seen[c >> 5];
+                    if ((word >> (c & 31)) & 1u) {
+                        v = v > 0.0f ? v / a.theta : v * a.theta;
+                        const unsigned cnt = (count[c >> 1] >> (16 * (c & 1))) & 65535u;
+                        v = v - a.frequency * static_cast<float>(cnt) - a.presence;
+                    }
+                }
+                if (a.bias != nullptr) v += to_f32<T>(extra[i]);
+                u[i] = ok[i] != 0 ? v : -INFINITY;
+                top = fmaxf(top, u[i]);
+                if (c < n) w[c] = u[i];
+            }
+            const float from = top == -INFINITY ? 0.0f : top;
+            s *= rescale(m, top, k);
+            m = top;
+#pragma unroll
+            for (int i = 0; i < U; ++i) s += power2((u[i] - from) * k);
+        }
+        const float wm = warp_max(m);
+        const float ws = warp_sum(s * rescale(m, wm, k));
+        if (lane == 0) {
+            warp_m[flip][warp] = wm;
+            warp_s[flip][warp] = ws;
+        }
+        __syncthreads();
+        const float bm = lane < kWarps ? warp_m[flip][lane] : -INFINITY;
+        const float bs = lane < kWarps ? warp_s[flip][lane] : 0.0f;
+        const float top = warp_max(bm);
+        const float total = warp_sum(bs * rescale(bm, top, k));
+        if (hist) stream_history<false>(a, row, seen, count);
+        const float from = top == -INFINITY ? 0.0f : top;
+        const float f = total == 0.0f ? 0.0f : 1.0f / total;
+        for (int base = tid; base < n; base += U * kStreamThreads) {
+            float u[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) u[i] = base + i * kStreamThreads < n ? w[base + i * kStreamThreads] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (base + i * kStreamThreads < n) w[base + i * kStreamThreads] = power2((u[i] - from) * k) * f;
+        }
+    }
+}
+
+// The gradient of long rows: the sum w g first, then both are read again.
+// dbias_partial [blocks, n] holds zeros, or is NULL.
+template <typename T>
+__global__ void __launch_bounds__(kStreamThreads) weights_stream_backward_kernel(const WeightsArgs a, const float *w,
+                                                                                 const float *g, int64_t ld_g, T *dz,
+                                                                                 T *du, float *dbias_partial) {
+    extern __shared__ unsigned dyn[];
+    constexpr int kWarps = kStreamThreads / 32, U = kStreamUnroll;
+    __shared__ float warp_s[2][kWarps];
+    const int n = static_cast<int>(a.n), words = (n + 31) / 32;
+    unsigned *seen = dyn;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool hist = a.hist > 0 && a.theta != 1.0f && dz != nullptr;  // only the repetition penalty has a slope
+    float *partial = dbias_partial != nullptr ? dbias_partial + blockIdx.x * a.n : nullptr;
+    int flip = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+        if (hist) {
+            __syncthreads();
+            for (int i = tid; i < words; i += kStreamThreads) seen[i] = 0u;
+            __syncthreads();
+            const int64_t *h = a.history + row * a.hist_ld;
+            for (int64_t j = tid; j < a.hist; j += kStreamThreads) {
+                const int64_t v = h[j];
+                if (v >= 0 && v < a.n) atomicOr(seen + (v >> 5), 1u << (v & 31));
+            }
+        }
+        const float *pw = w + row * a.n, *pg = g + row * ld_g;
+        float s = 0.0f;
+        for (int base = tid; base < n; base += U * kStreamThreads) {
+            float p[U], q[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int c = base + i * kStreamThreads;
+                p[i] = c < n ? pw[c] : 0.0f;
+                q[i] = c < n ? pg[c] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) s = fmaf(p[i], p[i] == 0.0f ? 0.0f : q[i], s);
+        }
+        const float ws = warp_sum(s);
+        if (lane == 0) warp_s[flip][warp] = ws;
+        __syncthreads();
+        const float dot = warp_sum(lane < kWarps ? warp_s[flip][lane] : 0.0f);
+        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+        const int64_t at = row * a.n;
+        for (int base = tid; base < n; base += U * kStreamThreads) {
+            float p[U], q[U], r[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int c = base + i * kStreamThreads;
+                p[i] = c < n ? pw[c] : 0.0f;
+                q[i] = c < n ? pg[c] : 0.0f;
+                r[i] = partial != nullptr && c < n ? partial[c] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int c = base + i * kStreamThreads;
+                if (c >= n) continue;
+                // a weight of 0 gets and passes nothing
+                float d = p[i] == 0.0f ? 0.0f : p[i] * (q[i] - dot) * a.inv_tau;
+                if (partial != nullptr) partial[c] = r[i] + d;
+                if (du != nullptr) du[at + c] = from_f32<T>(d);
+                if (dz != nullptr) {
+                    if (hist && (seen[c >> 5] >> (c & 31)) & 1u) d = to_f32<T>(z[c]) > 0.0f ? d / a.theta : d * a.theta;
+                    dz[at + c] = from_f32<T>(d);
+                }
+            }
+        }
+    }
+}
+
+// ---- a few long rows: eight blocks to a row ----------------------------------
+// One row would leave all SMs but one idle: a cluster of eight blocks holds it
+// in registers (19 us -> 7 us for one row of 29649).  The blocks read each
+// other's sums from shared memory, once.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_float(const float *p, uint32_t rank) {
+    float v;
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.f32 %0, [a];\n}"
+        : "=f"(v) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank) : "memory");
+    return v;
+}
+constexpr int kWideBlocks = 8;
+
+// Which of a block's columns are in the row's history, and how often.
+template <int VPT>
+__device__ __forceinline__ void wide_history(const WeightsArgs &a, int64_t row, int c0, unsigned *seen,
+                                             unsigned *count) {
+    constexpr int kChunk = kStreamThreads * VPT;
+    for (int i = threadIdx.x; i < kChunk / 32 + kChunk; i += kStreamThreads) seen[i] = 0u;
+    __syncthreads();
+    const int64_t *h = a.history + row * a.hist_ld;
+    for (int64_t j = threadIdx.x; j < a.hist; j += kStreamThreads) {
+        const int64_t v = h[j];
+        const int64_t c = v - c0;
+        if (v < 0 || v >= a.n || c < 0 || c >= kChunk) continue;
+        atomicAdd(count + c, 1u);
+        atomicOr(seen + (c >> 5), 1u << (c & 31));
+    }
+    __syncthreads();
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kStreamThreads) __cluster_dims__(kWideBlocks, 1, 1)
+    weights_wide_kernel(const WeightsArgs a, float *out) {
+    extern __shared__ unsigned dyn[];
+    constexpr int kChunk = kStreamThreads * VPT, kWarps = kStreamThreads / 32;
+    __shared__ float warp_m[kWarps], warp_s[kWarps], block_m, block_s;
+    unsigned *seen = dyn, *count = dyn + kChunk / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int c0 = static_cast<int>(cluster_rank()) * kChunk, left = static_cast<int>(a.n) - c0 - tid;
+    const int64_t row = blockIdx.x / kWideBlocks;
+    const bool hist = a.hist > 0;
+    const float k = a.inv_tau * 1.4426950408889634f;
+    const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
+    const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld + c0 + tid;
+    T raw[VPT], extra[VPT];
+    uint8_t ok[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) raw[i] = i * kStreamThreads < left ? z[i * kStreamThreads] : from_f32<T>(0.0f);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+        extra[i] = a.bias != nullptr && i * kStreamThreads < left ? bias[i * kStreamThreads] : from_f32<T>(0.0f);
+    const int64_t state = state_of(a, row);
+    const bool legal = state >= 0 && state < a.n_states;
+    const uint8_t *mask = a.mask + (legal ? state * a.mask_ld : 0) + c0 + tid;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        ok[i] = i * kStreamThreads < left ? 1 : 0;
+        if (a.mask != nullptr) ok[i] = legal && ok[i] ? mask[i * kStreamThreads] : 0;
+    }
+    if (hist) wide_history<VPT>(a, row, c0, seen, count);
+    float u[VPT], m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int c = i * kStreamThreads + tid;
+        float v = to_f32<T>(raw[i]);
+        if (hist && (seen[c >> 5] >> (c & 31)) & 1u) {
+            v = v > 0.0f ? v / a.theta : v * a.theta;
+            v = v - a.frequency * static_cast<float>(count[c]) - a.presence;
+        }
+        if (a.bias != nullptr) v += to_f32<T>(extra[i]);
+        u[i] = ok[i] != 0 ? v : -INFINITY;
+        m = fmaxf(m, u[i]);
+    }
+    const float from = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        u[i] = power2((u[i] - from) * k);
+        s += u[i];
+    }
+    const float wm = warp_max(m);
+    const float ws = warp_sum(s * rescale(m, wm, k));
+    if (lane == 0) {
+        warp_m[warp] = wm;
+        warp_s[warp] = ws;
+    }
+    __syncthreads();
+    float bm = lane < kWarps ? warp_m[lane] : -INFINITY;
+    float bs = lane < kWarps ? warp_s[lane] : 0.0f;
+    float top = warp_max(bm);
+    float total = warp_sum(bs * rescale(bm, top, k));
+    if (tid == 0) {
+        block_m = top;
+        block_s = total;
+    }
+    cluster_barrier();
+    bm = lane < kWideBlocks ? peer_float(&block_m, lane) : -INFINITY;
+    bs = lane < kWideBlocks ? peer_float(&block_s, lane) : 0.0f;
+    top = warp_max(bm);
+    total = warp_sum(bs * rescale(bm, top, k));
+    const float f = total == 0.0f ? 0.0f : rescale(m, top, k) / total;
+    float *w = out + row * a.n + c0 + tid;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+        if (i * kStreamThreads < left) w[i * kStreamThreads] = u[i] * f;
+    cluster_barrier();  // no block leaves while another may read its sums
+}
+
+// dbias_partial: [rows, n], or NULL.
+template <typename T, int VPT>
+__global__ void __launch_bounds__(kStreamThreads) __cluster_dims__(kWideBlocks, 1, 1)
+    weights_wide_backward_kernel(const WeightsArgs a, const float *w, const float *g, int64_t ld_g, T *dz, T *du,
+                                 float *dbias_partial) {
+    extern __shared__ unsigned dyn[];
+    constexpr int kChunk = kStreamThreads * VPT, kWarps = kStreamThreads / 32;
+    __shared__ float warp_s[kWarps], block_s;
+    unsigned *seen = dyn, *count = dyn + kChunk / 32;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int c0 = static_cast<int>(cluster_rank()) * kChunk, left = static_cast<int>(a.n) - c0 - tid;
+    const int64_t row = blockIdx.x / kWideBlocks, at = row * a.n + c0 + tid;
+    const bool hist = a.hist > 0 && a.theta != 1.0f && dz != nullptr;  // only the repetition penalty has a slope
+    float p[VPT], q[VPT], s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) p[i] = i * kStreamThreads < left ? w[at + i * kStreamThreads] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) q[i] = i * kStreamThreads < left ? g[row * ld_g + c0 + tid + i * kStreamThreads] : 0.0f;
+    if (hist) wide_history<VPT>(a, row, c0, seen, count);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if (p[i] == 0.0f) q[i] = 0.0f;  // a weight of 0 passes nothing on, whatever the gradient there
+        s = fmaf(p[i], q[i], s);
+    }
+    const float ws = warp_sum(s);
+    if (lane == 0) warp_s[warp] = ws;
+    __syncthreads();
+    float dot = warp_sum(lane < kWarps ? warp_s[lane] : 0.0f);
+    if (tid == 0) block_s = dot;
+    cluster_barrier();
+    dot = warp_sum(lane < kWideBlocks ? peer_float(&block_s, lane) : 0.0f);
+    const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if (i * kStreamThreads >= left) continue;
+        const int c = i * kStreamThreads + tid;
+        float d = p[i] == 0.0f ? 0.0f : p[i] * (q[i] - dot) * a.inv_tau;
+        if (dbias_partial != nullptr) dbias_partial[at + i * kStreamThreads] = d;
+        if (du != nullptr) du[at + i * kStreamThreads] = from_f32<T>(d);
+        if (dz != nullptr) {
+            if (hist && (seen[c >> 5] >> (c & 31)) & 1u)
+                d = to_f32<T>(z[i * kStreamThreads]) > 0.0f ? d / a.theta : d * a.theta;
+            dz[at + i * kStreamThreads] = from_f32<T>(d);
+        }
+    }
+    cluster_barrier();
 }
 
 // Column sums of [parts, n] in a fixed order: 32 columns x 32 groups of parts per block.
@@ -362,8 +677,14 @@ __global__ void column_sum_kernel(const float *partial, int64_t parts, int64_t n
     __shared__ float part[32][33];
     const int64_t c = blockIdx.x * int64_t(32) + threadIdx.x;
     float s = 0.0f;
-    if (c < n)
-        for (int64_t p = threadIdx.y; p < parts; p += 32) s += partial[p * n + c];
+    if (c < n) {
+        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t p0 = threadIdx.y; p0 < parts; p0 += 128)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (p0 + 32 * q < parts) t[q] += partial[(p0 + 32 * q) * n + c];
+        s = (t[0] + t[1]) + (t[2] + t[3]);
+    }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < n) {
@@ -373,73 +694,67 @@ __global__ void column_sum_kernel(const float *partial, int64_t parts, int64_t n
     }
 }
 
-// How a row is laid over threads: the narrowest form that holds it.  The
-// counts of the widest (8192 columns) take 33 KB of shared memory.
+// How a row is laid over threads: the narrowest form that holds it.  The counts
+// of 4096 columns (three rows) take 51 KB of shared memory.
 struct Layout {
-    int threads, vpt, ranks;
-    int64_t clusters;  // rows in flight
+    int threads, vpt;  // vpt 0: the two-pass form
+    int wide;          // values a thread of the cluster form, or 0
+    int64_t blocks;    // rows in flight
 };
 
-constexpr int64_t kMaxColumns = 65536;
+constexpr int64_t kMaxColumns = 65536, kMaxHistory = 65535;
 
 Layout layout(int64_t rows, int64_t n) {
     const int sms = fl_device_sm_count() > 0 ? fl_device_sm_count() : 148;
-    Layout l{512, 16, 1, 0};
-    if (n <= 128) l = {32, 4, 1, 0};
-    else if (n <= 512) l = {64, 8, 1, 0};
-    else if (n <= 1024) l = {128, 8, 1, 0};
-    else if (n <= 2048) l = {256, 8, 1, 0};
-    else if (n <= 4096) l = {512, 8, 1, 0};
-    else {
-        // few rows: eight narrow blocks per row put more SMs to work on each
-        const int vpt = rows * 4 < sms ? 8 : 16;
-        while (l.ranks < 8 && static_cast<int64_t>(l.ranks) * 512 * vpt < n) l.ranks *= 2;
-        l.vpt = static_cast<int64_t>(l.ranks) * 512 * vpt >= n ? vpt : 16;
-    }
-    const int64_t fit = static_cast<int64_t>(sms) * (1024 / l.threads) / l.ranks;  // rows in flight
-    l.clusters = rows < fit ? rows : fit;
+    Layout l{256, 16, 0, 0};
+    // Sixteen values a thread: what a row costs each thread besides (the
+    // reductions, the history) is then spread far enough (12288 x 4096: 113 us
+    // with eight, 80 us with sixteen).
+    if (n <= 128) l = {32, 4, 0, 0};
+    else if (n <= 512) l = {32, 16, 0, 0};
+    else if (n <= 1024) l = {64, 16, 0, 0};
+    else if (n <= 2048) l = {128, 16, 0, 0};
+    else if (n > 4096) l = {kStreamThreads, 0, 0, 0};
+    if (l.vpt == 0 && rows * kWideBlocks <= 2 * sms) l.wide = n <= 8 * kWideBlocks * kStreamThreads ? 8 : 16;
+    const int64_t fit = static_cast<int64_t>(sms) * (l.vpt ? min_blocks(l.threads, l.vpt) : 3);
+    l.blocks = rows < fit ? rows : fit;
     return l;
 }
 
 template <typename K, typename... Args>
 int launch_rows(K kernel, const Layout &l, size_t smem, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(l.clusters * l.ranks));
-    cfg.blockDim = dim3(l.threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = l.ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = l.ranks > 1 ? 1 : 0;
-    note_launch();
-    FL_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    if (smem > 48 * 1024)
+        FL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    const int64_t grid = l.wide ? l.blocks * kWideBlocks : l.blocks;
+    launch(kernel, static_cast<unsigned>(grid), l.threads, smem, st, args...);
     return check_launch("relation weights");
 }
 
-size_t history_smem(const Layout &l, bool hist) {
+size_t history_smem(const Layout &l, int64_t n, bool hist, bool counts) {
+    if (!hist) return 0;
+    if (l.wide) return (l.threads * l.wide / 32 + l.threads * l.wide) * sizeof(unsigned);
+    if (l.vpt == 0) return ((n + 31) / 32 + (counts ? (n + 1) / 2 : 0)) * sizeof(unsigned);
     const size_t chunk = static_cast<size_t>(l.threads) * l.vpt;
-    return hist ? (chunk / 32 + chunk) * sizeof(unsigned) : 0;
+    return 3 * (chunk / 32 + chunk) * sizeof(unsigned);
 }
 
-#define FL_LAYOUTS(F)                                                             \
-    if (l.threads == 32) F(32, 4, false);                                         \
-    else if (l.threads == 64) F(64, 8, false);                                    \
-    else if (l.threads == 128) F(128, 8, false);                                  \
-    else if (l.threads == 256) F(256, 8, false);                                  \
-    else if (l.ranks == 1 && l.vpt == 8) F(512, 8, false);                        \
-    else if (l.ranks == 1) F(512, 16, false);                                     \
-    else if (l.vpt == 8) F(512, 8, true);                                         \
-    else F(512, 16, true);
+#define FL_LAYOUTS(F)                            \
+    if (l.vpt == 4) F(32, 4);                    \
+    else if (l.threads == 32) F(32, 16);         \
+    else if (l.threads == 64) F(64, 16);         \
+    else if (l.threads == 128) F(128, 16);       \
+    else F(256, 16);
 
 template <typename T>
 int forward_t(const WeightsArgs &a, float *w, cudaStream_t st) {
-    const Layout l = layout(a.rows, a.n);
-    const size_t smem = history_smem(l, a.hist > 0);
+    Layout l = layout(a.rows, a.n);
+    const size_t smem = history_smem(l, a.n, a.hist > 0, true);
+    if (l.wide == 8) return launch_rows(weights_wide_kernel<T, 8>, l, smem, st, a, w);
+    if (l.wide == 16) return launch_rows(weights_wide_kernel<T, 16>, l, smem, st, a, w);
+    if (l.vpt == 0 && a.rows < (1ll << 31)) l.blocks = a.rows;  // a block per row: the hardware balances them
+    if (l.vpt == 0) return launch_rows(weights_stream_kernel<T>, l, smem, st, a, w);
     int rc = FL_OK;
-#define F(TH, V, C) rc = launch_rows(weights_forward_kernel<T, TH, V, C>, l, smem, st, a, w)
+#define F(TH, V) rc = launch_rows(weights_forward_kernel<T, TH, V>, l, smem, st, a, w)
     FL_LAYOUTS(F)
 #undef F
     return rc;
@@ -451,17 +766,25 @@ int backward_t(const WeightsArgs &a, const float *w, const float *g, int64_t ld_
     const Layout l = layout(a.rows, a.n);
     float *partial = nullptr;
     if (dbias != nullptr) {
-        partial = ws.take<float>(l.clusters * a.n);
+        partial = ws.take<float>(l.blocks * a.n);
         FL_REQUIRE(partial != nullptr, "relation weights: workspace too small");
     }
-    const size_t smem = history_smem(l, a.hist > 0 && a.theta != 1.0f && dz != nullptr);
+    const size_t smem = history_smem(l, a.n, a.hist > 0 && a.theta != 1.0f && dz != nullptr, false);
     int rc = FL_OK;
-#define F(TH, V, C) \
-    rc = launch_rows(weights_backward_kernel<T, TH, V, C>, l, smem, st, a, w, g, ld_g, dz, du, partial)
-    FL_LAYOUTS(F)
+    if (l.wide == 8) {
+        rc = launch_rows(weights_wide_backward_kernel<T, 8>, l, smem, st, a, w, g, ld_g, dz, du, partial);
+    } else if (l.wide == 16) {
+        rc = launch_rows(weights_wide_backward_kernel<T, 16>, l, smem, st, a, w, g, ld_g, dz, du, partial);
+    } else if (l.vpt == 0) {
+        if (partial != nullptr) FL_CUDA(cudaMemsetAsync(partial, 0, l.blocks * a.n * sizeof(float), st));
+        rc = launch_rows(weights_stream_backward_kernel<T>, l, smem, st, a, w, g, ld_g, dz, du, partial);
+    } else {
+#define F(TH, V) rc = launch_rows(weights_backward_kernel<T, TH, V>, l, smem, st, a, w, g, ld_g, dz, du, partial)
+        FL_LAYOUTS(F)
 #undef F
+    }
     if (rc || dbias == nullptr) return rc;
-    launch(column_sum_kernel<T>, static_cast<unsigned>((a.n + 31) / 32), dim3(32, 32), 0, st, partial, l.clusters, a.n,
+    launch(column_sum_kernel<T>, static_cast<unsigned>((a.n + 31) / 32), dim3(32, 32), 0, st, partial, l.blocks, a.n,
            dbias);
     return check_launch("relation weights bias");
 }
@@ -475,7 +798,8 @@ int weights_args(const fl_weights *p, WeightsArgs *a) {
     FL_REQUIRE(p->tau > 0.0 && p->repetition > 0.0, "relation weights: tau and repetition must be positive");
     FL_REQUIRE(p->mask == nullptr || (p->n_states > 0 && (p->n_states == 1 || p->mask_ld >= p->n)),
                "relation weights: bad mask");
-    FL_REQUIRE(p->hist >= 0 && (p->hist == 0 || p->history != nullptr), "relation weights: bad history");
+    FL_REQUIRE(p->hist >= 0 && p->hist <= kMaxHistory && (p->hist == 0 || p->history != nullptr),
+               "relation weights: bad history (at most %lld entries)", static_cast<long long>(kMaxHistory));
     *a = WeightsArgs{p->logits, p->ld, p->bias, p->bias_ld, static_cast<const uint8_t *>(p->mask), p->mask_ld,
                      p->mask != nullptr ? p->n_states : 0, p->states, p->history, p->hist_ld, p->hist, p->rows, p->n,
                      static_cast<float>(p->repetition), static_cast<float>(p->frequency),
@@ -504,7 +828,7 @@ int fl_relation_weights(const fl_weights *p, float *w, fl_stream_t stream) {
 
 size_t fl_relation_weights_workspace(int64_t rows, int64_t n) {
     if (rows <= 0 || n <= 0 || n > kMaxColumns) return 0;
-    return carve_bytes<float>(layout(rows, n).clusters * n);
+    return carve_bytes<float>(layout(rows, n).blocks * n);
 }
 
 int fl_relation_weights_backward(const fl_weights *p, const float *w, const float *g, int64_t ld_g, void *dlogits,

@@ -763,6 +763,7 @@ def linear_backward(x, weight, z, gy, act: int = L.FL_ACT_NONE, want=(True, True
 
 
 MAX_WEIGHT_COLUMNS = 65536
+MAX_HISTORY = 65535
 
 
 def _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence):

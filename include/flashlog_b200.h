@@ -510,7 +510,8 @@ typedef struct fl_weights {
                                 allows nothing); NULL: row r has mask row
                                 min(r, n_states - 1)                             */
     const int64_t *history;  /* [rows, hist] operators used so far; entries
-                                outside [0, n) (padding) do not count; or NULL   */
+                                outside [0, n) (padding) do not count; at most
+                                65535 per row; or NULL                           */
     int64_t ld, bias_ld, mask_ld, n_states, hist_ld, hist, rows, n;
     double tau, repetition, frequency, presence;
     int dtype;
