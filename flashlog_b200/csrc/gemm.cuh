@@ -89,7 +89,7 @@ __device__ __forceinline__ float act_value(float z, int act) {
     switch (act) {
         case kActRelu: return z > 0.0f ? z : (z <= 0.0f ? 0.0f : z);  // NaN stays NaN
         case kActTanh: return tanhf(z);
-        case kActSilu: return z / (1.0f + expf(-z));
+        case kActSilu: return __fdividef(z, 1.0f + expf(-z));
         case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
         default: return z;
     }
@@ -98,7 +98,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     switch (act) {
         case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
         case kActTanh: { const float t = tanhf(z); return (1.0f - t) * (1.0f + t); }
-        case kActSilu: { const float t = 1.0f / (1.0f + expf(-z)); return t * (1.0f + z * (1.0f - t)); }
+        case kActSilu: { const float t = __fdividef(1.0f, 1.0f + expf(-z)); return t * (1.0f + z * (1.0f - t)); }
         case kActGelu:
             return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
         default: return 1.0f;

@@ -166,7 +166,248 @@ __global__ void sum_partials_kernel(const float *partial, int64_t parts, int64_t
     out[c] = from_f32<T>(s);
 }
 
+// ---- small products in fp32 multiply-adds ------------------------------------
+// Up to a few hundred million operations the tensor path's launches (two packs
+// and a product, about 12 us for fp32) cost more than the arithmetic: these
+// kernels read the operands as they are and take one launch.
+
+// Few rows: a warp takes four columns of W for all R rows, its lanes along k.
+// Every element of W is read once and used R times from registers; the rows of
+// x come from L1.
+template <typename T, int R, int V>
+__global__ void __launch_bounds__(256) few_rows_kernel(const fl_linear p, void *y, int64_t ld_y, float *z) {
+    const int lane = threadIdx.x & 31;
+    const int64_t j0 = (blockIdx.x * int64_t(8) + (threadIdx.x >> 5)) * 4;
+    if (j0 >= p.n) return;
+    const int64_t r0 = blockIdx.y * int64_t(R);
+    const T *x = static_cast<const T *>(p.x), *w = static_cast<const T *>(p.w);
+    const T *wj[4], *xr[R];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) wj[c] = w + (j0 + c < p.n ? j0 + c : p.n - 1) * p.ld_w;  // columns past n repeat the last
+#pragma unroll
+    for (int r = 0; r < R; ++r) xr[r] = x + (r0 + r < p.rows ? r0 + r : p.rows - 1) * p.ld_x;
+    float acc[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = 0.0f;
+    struct alignas(V * sizeof(T)) Vec { T t[V]; };
+    for (int64_t k = lane * V; k < p.k; k += 32 * V) {
+        float b[4][V];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const Vec v = *reinterpret_cast<const Vec *>(wj[c] + k);
+#pragma unroll
+            for (int e = 0; e < V; ++e) b[c][e] = to_f32(v.t[e]);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const Vec v = *reinterpret_cast<const Vec *>(xr[r] + k);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float a = to_f32(v.t[e]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[r][c] = fmaf(a, b[c][e], acc[r][c]);
+            }
+        }
+    }
+    float mine[(R * 4 + 31) / 32];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float v = warp_sum(acc[r][c]);
+            if (lane == ((r * 4 + c) & 31)) mine[(r * 4 + c) >> 5] = v;
+        }
+#pragma unroll
+    for (int q = 0; q < (R * 4 + 31) / 32; ++q) {
+        const int o = q * 32 + lane;
+        const int64_t row = r0 + (o >> 2), col = j0 + (o & 3);
+        if (o >= R * 4 || row >= p.rows || col >= p.n) continue;
+        float v = mine[q];
+        if (p.bias != nullptr) v += to_f32(static_cast<const T *>(p.bias)[col]);
+        if (z != nullptr) z[row * p.n + col] = v;
+        v = act_value(v, p.act);
+        if (p.residual != nullptr) v += to_f32(static_cast<const T *>(p.residual)[row * p.ld_res + col]);
+        static_cast<T *>(y)[row * ld_y + col] = from_f32<T>(v);
+    }
+}
+
+// D[i, j] = sum_k A(i, k) B(j, k) in 32 x 32 tiles; 128 threads of 2 x 4
+// outputs, the next tile's loads in registers under the products of this one.
+//   kForward:  A = x, B = W                      D = z -> y
+//   kGradX:    A = dz, B = W^T (k runs over n)   D = dx
+//   kGradW:    A = dz^T, B = x^T (k over rows)   D = dw, and the sums of A over k are dbias
+// dz = gy * act'(z) is formed as it is loaded and not rounded.  With more than
+// one split of k the sums go to `partial` [splits, m, n + 1] (the last column:
+// dbias) and reduce_kernel adds them in order.
+enum { kForward = 0, kGradX = 1, kGradW = 2 };
+struct SmallArgs {
+    const void *a, *b;
+    int64_t ld_a, ld_b;
+    const float *z;         // of dz (pitch ld_z), or NULL
+    int64_t ld_z, m, n, k, chunk;
+    const void *bias, *residual;
+    int64_t ld_res;
+    void *out;
+    int64_t ld_out;
+    float *z_out;
+    void *sum_out;
+    float *partial;
+    int act;
+};
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(128) small_gemm_kernel(const SmallArgs p) {
+    constexpr int kT = 32, kPitch = 36;
+    __shared__ __align__(16) float As[kT][kPitch], Bs[kT][kPitch];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t i0 = blockIdx.y * int64_t(kT), j0 = blockIdx.x * int64_t(kT);
+    const int64_t k0 = blockIdx.z * p.chunk, k1 = min(p.k, k0 + p.chunk);
+    constexpr bool kAT = MODE == kGradW, kBT = MODE != kForward;  // the output index is contiguous
+    constexpr bool kDz = MODE != kForward;
+    // line e of the thread's eight is 4 e lines on; a tile further in k is one step
+    const int64_t step_a = kAT ? kT * p.ld_a : kT, step_b = kBT ? kT * p.ld_b : kT, step_z = kAT ? kT * p.ld_z : kT;
+    const int64_t la = kAT ? k0 + warp : i0 + warp, ca = kAT ? i0 + lane : k0 + lane;
+    const T *pa = static_cast<const T *>(p.a) + la * p.ld_a + ca;
+    const float *pz = p.z != nullptr ? p.z + la * p.ld_z + ca : nullptr;
+    const T *pb = static_cast<const T *>(p.b) + (kBT ? k0 + warp : j0 + warp) * p.ld_b + (kBT ? j0 : k0) + lane;
+    unsigned ok_a = 0u, ok_b = 0u;  // which of the eight lie inside as to the output index
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        ok_a |= (i0 + (kAT ? lane : warp + 4 * e) < p.m ? 1u : 0u) << e;
+        ok_b |= (j0 + (kBT ? lane : warp + 4 * e) < p.n ? 1u : 0u) << e;
+    }
+    const bool slope = kDz && p.act != kActNone;
+    T ra[8], rb[8];
+    float rz[8];
+    auto load = [&](int left) {  // left: how much of k is left at this tile
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int s = warp + 4 * e;
+            ra[e] = ((ok_a >> e) & 1u) && (kAT ? s : lane) < left ? pa[e * 4 * p.ld_a] : from_f32<T>(0.0f);
+            rb[e] = ((ok_b >> e) & 1u) && (kBT ? s : lane) < left ? pb[e * 4 * p.ld_b] : from_f32<T>(0.0f);
+            if (slope) rz[e] = ((ok_a >> e) & 1u) && (kAT ? s : lane) < left ? pz[e * 4 * p.ld_z] : 0.0f;
+        }
+        pa += step_a;
+        pb += step_b;
+        if (slope) pz += step_z;
+    };
+    const int ti = (tid >> 3) * 2, tj = (tid & 7) * 4;
+    float acc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, sums[2] = {0, 0};
+    int left = static_cast<int>(k1 - k0);
+    load(left);
+    for (; left > 0; left -= kT) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int s = warp + 4 * e;
+            float v = to_f32(ra[e]);
+            if (slope) v *= act_slope(rz[e], p.act);
+            As[kAT ? s : lane][kAT ? lane : s] = v;
+            Bs[kBT ? s : lane][kBT ? lane : s] = to_f32(rb[e]);
+        }
+        __syncthreads();
+        if (left > kT) load(left - kT);
+#pragma unroll
+        for (int k = 0; k < kT; ++k) {
+            const float2 a = *reinterpret_cast<const float2 *>(&As[k][ti]);
+            const float4 b = *reinterpret_cast<const float4 *>(&Bs[k][tj]);
+            const float av[2] = {a.x, a.y}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (MODE == kGradW) sums[u] += av[u];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(av[u], bv[v], acc[u][v]);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int64_t i = i0 + ti + u;
+        if (i >= p.m) continue;
+        const bool owns_sum = MODE == kGradW && blockIdx.x == 0 && tj == 0;
+        if (p.partial != nullptr) {
+            float *q = p.partial + (blockIdx.z * p.m + i) * (p.n + 1);
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+                if (j0 + tj + v < p.n) q[j0 + tj + v] = acc[u][v];
+            if (owns_sum) q[p.n] = sums[u];
+            continue;
+        }
+        if (owns_sum && p.sum_out != nullptr) static_cast<T *>(p.sum_out)[i] = from_f32<T>(sums[u]);
+        if (p.out == nullptr) continue;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int64_t j = j0 + tj + v;
+            if (j >= p.n) continue;
+            float x = acc[u][v];
+            if (MODE == kForward) {
+                if (p.bias != nullptr) x += to_f32(static_cast<const T *>(p.bias)[j]);
+                if (p.z_out != nullptr) p.z_out[i * p.n + j] = x;
+                x = act_value(x, p.act);
+                if (p.residual != nullptr) x += to_f32(static_cast<const T *>(p.residual)[i * p.ld_res + j]);
+            }
+            static_cast<T *>(p.out)[i * p.ld_out + j] = from_f32<T>(x);
+        }
+    }
+}
+
+template <typename T>
+__global__ void reduce_kernel(const float *partial, int64_t splits, int64_t m, int64_t n, T *out, T *sum_out) {
+    const int64_t t = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
+    if (t >= m * (n + 1)) return;
+    const int64_t i = t / (n + 1), j = t - i * (n + 1);
+    float s = 0.0f;
+    for (int64_t q = 0; q < splits; ++q) s += partial[q * m * (n + 1) + t];
+    if (j < n) {
+        if (out != nullptr) out[i * n + j] = from_f32<T>(s);
+    } else if (sum_out != nullptr) {
+        sum_out[i] = from_f32<T>(s);
+    }
+}
+
 // ---- host side -------------------------------------------------------------
+struct Split {
+    int64_t splits, chunk;
+};
+// Splits of the contraction: enough blocks for four per SM, at least 64 long.
+Split split_of(int64_t m, int64_t n, int64_t k) {
+    const int64_t tiles = ((m + 31) / 32) * ((n + 31) / 32);
+    int64_t s = (4 * 148 + tiles - 1) / tiles;
+    const int64_t most = k / 64 > 1 ? k / 64 : 1;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    Split r;
+    r.chunk = ((k + s - 1) / s + 31) / 32 * 32;
+    r.splits = (k + r.chunk - 1) / r.chunk;
+    return r;
+}
+size_t split_bytes(int64_t m, int64_t n, int64_t k) {
+    const Split s = split_of(m, n, k);
+    return s.splits > 1 ? carve_bytes<float>(s.splits * m * (n + 1)) : 0;
+}
+
+// Which path: microseconds as measured.  A small product takes 2.5 and, for
+// every 32 of k, 0.8, or its operations at 12 TFLOP/s where there are many; the
+// tensor path 11.5 in fp32 (two packs and the product), 5.5 in 16 bits when TMA
+// takes the operands as they are and 9 when it does not, and for the gradients
+// 55 and 22 in all.
+bool is_few_rows(int64_t rows, int dtype) { return rows <= (dtype == FL_F32 ? 16 : 8); }
+double small_us(int64_t m, int64_t n, int64_t k, int64_t chunk, bool reduced) {
+    const double steps = 0.8 * static_cast<double>((chunk + 31) / 32);
+    const double ops = 2.0 * static_cast<double>(m) * static_cast<double>(n) * static_cast<double>(k) / 12e6;
+    return 2.5 + (steps > ops ? steps : ops) + (reduced ? 3.0 : 0.0);
+}
+bool is_small(int64_t rows, int64_t n, int64_t k, int dtype) {
+    return small_us(rows, n, k, k, false) <= (dtype == FL_F32 ? 11.5 : k % 8 == 0 ? 5.5 : 9.0);
+}
+bool is_small_backward(int64_t rows, int64_t n, int64_t k, int dtype) {
+    const Split x = split_of(rows, k, n), w = split_of(n, k, rows);
+    return small_us(rows, k, n, x.chunk, x.splits > 1) + small_us(n, k, rows, w.chunk, w.splits > 1) <=
+           (dtype == FL_F32 ? 55.0 : 22.0);
+}
+
 bool tma_ready(const void *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
 size_t operand_bytes(int64_t lines, int64_t inner, int64_t exps, int dtype) {
@@ -279,9 +520,102 @@ int linear_dz(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy,
     return check_launch("linear dz");
 }
 
+template <typename T, int R>
+void few_rows(const fl_linear *p, void *y, int64_t ld_y, float *z, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>((p->n + 31) / 32), static_cast<unsigned>((p->rows + R - 1) / R));
+    auto ready = [](const void *q, int64_t ld) {
+        return (reinterpret_cast<uintptr_t>(q) % (4 * sizeof(T))) == 0 && ld % 4 == 0;
+    };
+    if (p->k % 4 == 0 && ready(p->x, p->ld_x) && ready(p->w, p->ld_w))
+        launch(few_rows_kernel<T, R, 4>, grid, 256, 0, st, *p, y, ld_y, z);
+    else
+        launch(few_rows_kernel<T, R, 1>, grid, 256, 0, st, *p, y, ld_y, z);
+}
+
+template <typename T>
+int small_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, cudaStream_t st) {
+    if (is_few_rows(p->rows, p->dtype)) {
+        if (p->rows == 1) few_rows<T, 1>(p, y, ld_y, z, st);
+        else if (p->rows <= 4) few_rows<T, 4>(p, y, ld_y, z, st);
+        else few_rows<T, 8>(p, y, ld_y, z, st);
+        return check_launch("linear");
+    }
+    SmallArgs a{};
+    a.a = p->x;
+    a.ld_a = p->ld_x;
+    a.b = p->w;
+    a.ld_b = p->ld_w;
+    a.m = p->rows;
+    a.n = p->n;
+    a.k = a.chunk = p->k;
+    a.bias = p->bias;
+    a.residual = p->residual;
+    a.ld_res = p->ld_res;
+    a.out = y;
+    a.ld_out = ld_y;
+    a.z_out = z;
+    a.act = p->act;
+    FL_REQUIRE((a.m + 31) / 32 <= 65535, "linear: too many rows");
+    launch(small_gemm_kernel<T, kForward>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32)),
+           128, 0, st, a);
+    return check_launch("linear");
+}
+
+template <typename T, int MODE>
+int small_grad(SmallArgs a, Carve &ws, cudaStream_t st) {
+    const Split s = split_of(a.m, a.n, a.k);
+    a.chunk = s.chunk;
+    if (s.splits > 1) {
+        a.partial = ws.take<float>(s.splits * a.m * (a.n + 1));
+        FL_REQUIRE(a.partial != nullptr, "linear backward: workspace too small");
+    }
+    FL_REQUIRE((a.m + 31) / 32 <= 65535, "linear backward: too many rows");
+    launch(small_gemm_kernel<T, MODE>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32),
+                                            static_cast<unsigned>(s.splits)), 128, 0, st, a);
+    if (s.splits > 1)
+        launch(reduce_kernel<T>, static_cast<unsigned>((a.m * (a.n + 1) + 255) / 256), 256, 0, st, a.partial, s.splits, a.m,
+               a.n, static_cast<T *>(a.out), static_cast<T *>(MODE == kGradW ? a.sum_out : nullptr));
+    return check_launch("linear backward");
+}
+
+template <typename T>
+int small_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw, void *dbias,
+                   Carve &ws, cudaStream_t st) {
+    SmallArgs a{};
+    a.a = gy;
+    a.ld_a = ld_gy;
+    a.z = z;
+    a.ld_z = p->n;
+    a.act = p->act;
+    int rc = FL_OK;
+    if (dx != nullptr) {
+        a.b = p->w;
+        a.ld_b = p->ld_w;
+        a.m = p->rows;
+        a.n = p->k;
+        a.k = p->n;
+        a.out = dx;
+        a.ld_out = p->k;
+        rc = small_grad<T, kGradX>(a, ws, st);
+    }
+    if (!rc && (dw != nullptr || dbias != nullptr)) {
+        a.b = p->x;
+        a.ld_b = p->ld_x;
+        a.m = p->n;
+        a.n = p->k;
+        a.k = p->rows;
+        a.out = dw;
+        a.ld_out = p->k;
+        a.sum_out = dbias;
+        rc = small_grad<T, kGradW>(a, ws, st);
+    }
+    return rc;
+}
+
 }  // namespace
 
 size_t linear_workspace(int64_t rows, int64_t n, int64_t k, int dtype) {
+    if (is_small(rows, n, k, dtype) || is_few_rows(rows, dtype)) return 0;
     return operand_bytes(rows, k, rows, dtype) + operand_bytes(n, k, n, dtype);
 }
 
@@ -290,6 +624,11 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
     if (rc) return rc;
     FL_REQUIRE(y != nullptr && ld_y >= p->n, "linear: bad output");
     if (p->rows == 0) return FL_OK;
+    if (is_small(p->rows, p->n, p->k, p->dtype) || is_few_rows(p->rows, p->dtype)) {
+        if (p->dtype == FL_F32) return small_forward<float>(p, y, ld_y, z, st);
+        if (p->dtype == FL_F16) return small_forward<__half>(p, y, ld_y, z, st);
+        return small_forward<__nv_bfloat16>(p, y, ld_y, z, st);
+    }
     Carve ws(wsp, ws_bytes);
     GemmOperand a, b;
     const int *ea, *eb;
@@ -307,6 +646,7 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
 }
 
 size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act) {
+    if (is_small_backward(rows, n, k, dtype)) return split_bytes(rows, k, n) + split_bytes(n, k, rows) + 256;
     size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
     if (act != FL_ACT_NONE) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
     const size_t ops = operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
@@ -326,6 +666,11 @@ int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t 
         return FL_OK;
     }
     Carve ws(wsp, ws_bytes);
+    if (is_small_backward(p->rows, p->n, p->k, p->dtype)) {
+        if (p->dtype == FL_F32) return small_backward<float>(p, z, gy, ld_gy, dx, dw, dbias, ws, st);
+        if (p->dtype == FL_F16) return small_backward<__half>(p, z, gy, ld_gy, dx, dw, dbias, ws, st);
+        return small_backward<__nv_bfloat16>(p, z, gy, ld_gy, dx, dw, dbias, ws, st);
+    }
     const void *dz = gy;
     int64_t ld_dz = ld_gy;
     if (p->act != FL_ACT_NONE || dbias != nullptr) {
