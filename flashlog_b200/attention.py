@@ -56,31 +56,32 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none"):
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    dt = x.dtype
+    dt, shape = x.dtype, x.shape
     if dt not in ops.FL_DTYPE:
         raise ValueError(f"linear takes float32, float16 or bfloat16 tensors, got {dt}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear: x [..., k] and weight [n, k], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.dim() != 2 or not shape or shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear: x [..., k] and weight [n, k], got {tuple(shape)} and {tuple(weight.shape)}")
     n, k = weight.shape
     if n == 0 or k == 0:
         raise ValueError("linear: weight must not be empty")
-    shape = x.shape[:-1] + (n,)
-    if bias is not None and bias.shape != (n,):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n):
         raise ValueError(f"linear: bias must be [{n}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"linear: residual must be {tuple(shape)}, got {tuple(residual.shape)}")
+    if residual is not None and residual.shape != shape[:-1] + (n,):
+        raise ValueError(f"linear: residual must be {tuple(shape[:-1] + (n,))}, got {tuple(residual.shape)}")
     for t in (weight, bias, residual):
         if t is not None and t.dtype != dt:
             raise ValueError(f"linear: tensors of one dtype, got {dt} and {t.dtype}")
-    ops._one_device("linear", x, weight, bias, residual)
-    if x.dim() != 2:
+    flat = len(shape) == 2
+    if not flat:
         x = x.reshape(-1, k)
         residual = None if residual is None else residual.reshape(-1, n)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         y = _Linear.apply(x, weight, bias, residual, act)
     else:
         y, _ = ops.linear_forward(x, weight, bias, residual, act)
-    return y if len(shape) == 2 else y.view(shape)
+    return y if flat else y.view(shape[:-1] + (n,))
 
 
 class _RelationWeights(autograd.Function):
@@ -149,18 +150,16 @@ def relation_weights(logits, *, tau: float = 1.0, mask=None, states=None, bias=N
         raise ValueError(f"relation_weights: history must be int64 {tuple(lead)} + [H]")
     if history is not None and history.shape[-1] > ops.MAX_HISTORY:
         raise ValueError(f"relation_weights: at most {ops.MAX_HISTORY} history entries, got {history.shape[-1]}")
-    ops._one_device("relation_weights", logits, bias, mask, states, history)
-    z = logits if logits.dim() == 2 else logits.reshape(-1, n)
-    if not (z.stride(1) == 1 and (z.stride(0) >= n or z.shape[0] <= 1)):
-        z = z.contiguous()
+    z = ops._lines(logits if logits.dim() == 2 else logits.reshape(-1, n))
     if bias is not None:
         bias = bias.contiguous() if bias.dim() == 1 else bias.reshape(-1, n).contiguous()
     if mask is not None:
-        mask = ops._lines(mask.reshape(-1, n))
+        mask = ops._lines(mask if mask.dim() == 2 else mask.reshape(-1, n))
     if states is not None:
-        states = states.reshape(-1).contiguous()
+        states = (states if states.dim() == 1 else states.reshape(-1)).contiguous()
     if history is not None:
-        history = None if history.shape[-1] == 0 else ops._lines(history.reshape(-1, history.shape[-1]))
+        width = history.shape[-1]
+        history = None if width == 0 else ops._lines(history if history.dim() == 2 else history.reshape(-1, width))
     if torch.is_grad_enabled() and (z.requires_grad or (bias is not None and bias.requires_grad)):
         w = _RelationWeights.apply(z, bias, mask, states, history, tau, repetition, frequency, presence)
     else:

@@ -668,41 +668,43 @@ def readout_backward(row_ptr, ent, N: int, targets, g_scores, n_val: int, val_li
 FL_DTYPE = {torch.float32: L.FL_F32, torch.float16: L.FL_F16, torch.bfloat16: L.FL_BF16}
 
 
-def _one_device(what, *ts):
-    """The tensors' common CUDA device; raises unless there is exactly one."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+def _one_device(what, first, *others):
+    """The index of the tensors' common CUDA device; raises unless there is exactly one (None: no tensor)."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            if not t.is_cuda or dev < 0:
+                raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
+            raise ValueError(f"{what}: tensors on cuda:{dev} and {t.device}")
+    if dev < 0:
+        raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
     return dev
 
 
-class _on:
-    """Makes `device` current for a launch (a no-op when it already is) and gives its current stream."""
-    __slots__ = ("index", "old")
+def _call(dev, what, fn, *args):
+    """fn(*args, the current stream of device `dev`), with that device current."""
+    now = torch._C._cuda_getDevice()
+    if now == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        check(rc, what)
 
-    def __init__(self, device):
-        self.index = device.index
 
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
-    def __exit__(self, *exc):
-        if self.old != self.index:
-            torch.cuda.set_device(self.old)
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _lines(t):
     """t as [rows, cols] lines the library can address: unit inner stride, rows at least a row apart."""
+    if t.is_contiguous():
+        return t
     if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
         return t
     return t.contiguous()
@@ -713,10 +715,9 @@ def _ld(t):
 
 
 def _linear_params(x, weight, bias, residual, act):
-    return L.fl_linear(x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-                       None if residual is None else residual.data_ptr(), _ld(x), _ld(weight),
-                       0 if residual is None else _ld(residual), x.shape[0], weight.shape[0], weight.shape[1],
-                       FL_DTYPE[x.dtype], act)
+    n, k = weight.shape
+    return L.fl_linear(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), _ld(x), _ld(weight),
+                       0 if residual is None else _ld(residual), x.shape[0], n, k, FL_DTYPE[x.dtype], act)
 
 
 def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE, want_z: bool = False):
@@ -725,20 +726,19 @@ def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE
     activation).  Returns (y, z)."""
     dev = _one_device("linear", x, weight, bias, residual)
     x, weight = _lines(x), _lines(weight)
-    bias = None if bias is None else bias.contiguous()
-    residual = None if residual is None else _lines(residual)
-    rows, (n, k) = x.shape[0], weight.shape
-    y = torch.empty((rows, n), dtype=x.dtype, device=dev)
-    z = torch.empty((rows, n), dtype=torch.float32, device=dev) if want_z and act != L.FL_ACT_NONE else None
+    if bias is not None:
+        bias = bias.contiguous()
+    if residual is not None:
+        residual = _lines(residual)
+    rows, n = x.shape[0], weight.shape[0]
+    y = x.new_empty((rows, n))
+    z = x.new_empty((rows, n), dtype=torch.float32) if want_z and act != L.FL_ACT_NONE else None
     if rows == 0:
         return y, z
     p = _linear_params(x, weight, bias, residual, act)
-    nbytes = lib().fl_linear_workspace(rows, n, k, p.dtype)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as st:
-        rc = lib().fl_linear_forward(ctypes.byref(p), y.data_ptr(), n, None if z is None else z.data_ptr(),
-                                     None if ws is None else ws.data_ptr(), nbytes, st)
-    check(rc, "linear")
+    nbytes = lib().fl_linear_workspace(rows, n, p.k, p.dtype)
+    ws = _workspace(nbytes, x)
+    _call(dev, "linear", lib().fl_linear_forward, ctypes.byref(p), y.data_ptr(), n, _ptr(z), _ptr(ws), nbytes)
     return y, z
 
 
@@ -748,17 +748,14 @@ def linear_backward(x, weight, z, gy, act: int = L.FL_ACT_NONE, want=(True, True
     dev = _one_device("linear backward", x, weight, z, gy)
     x, weight, gy = _lines(x), _lines(weight), _lines(gy)
     rows, (n, k) = x.shape[0], weight.shape
-    dx = torch.empty((rows, k), dtype=x.dtype, device=dev) if want[0] else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if want[1] else None
-    db = torch.empty(n, dtype=x.dtype, device=dev) if want[2] else None
+    dx = x.new_empty((rows, k)) if want[0] else None
+    dw = x.new_empty((n, k)) if want[1] else None
+    db = x.new_empty(n) if want[2] else None
     p = _linear_params(x, weight, None, None, act)
     nbytes = lib().fl_linear_backward_workspace(rows, n, k, p.dtype, act)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as st:
-        rc = lib().fl_linear_backward(ctypes.byref(p), None if z is None else z.data_ptr(), gy.data_ptr(), _ld(gy),
-                                      *(None if t is None else t.data_ptr() for t in (dx, dw, db)),
-                                      None if ws is None else ws.data_ptr(), nbytes, st)
-    check(rc, "linear backward")
+    ws = _workspace(nbytes, x)
+    _call(dev, "linear backward", lib().fl_linear_backward, ctypes.byref(p), _ptr(z), gy.data_ptr(), _ld(gy), _ptr(dx),
+          _ptr(dw), _ptr(db), _ptr(ws), nbytes)
     return dx, dw, db
 
 
@@ -768,8 +765,7 @@ MAX_HISTORY = 65535
 
 def _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence):
     rows, n = logits.shape
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    return L.fl_weights(logits.data_ptr(), ptr(bias), ptr(mask), ptr(states), ptr(history), _ld(logits),
+    return L.fl_weights(logits.data_ptr(), _ptr(bias), _ptr(mask), _ptr(states), _ptr(history), _ld(logits),
                         0 if bias is None or bias.dim() == 1 else n, 0 if mask is None else _ld(mask),
                         0 if mask is None else mask.shape[0], 0 if history is None else _ld(history),
                         0 if history is None else history.shape[1], rows, n, tau, repetition, frequency, presence,
@@ -782,13 +778,11 @@ def relation_weights(logits, bias=None, mask=None, states=None, history=None, ta
     stride), bias [n] or [rows, n], mask bool or uint8 [states, n], states
     int64 [rows], history int64 [rows, H].  Returns f32 [rows, n]."""
     dev = _one_device("relation weights", logits, bias, mask, states, history)
-    w = torch.empty(logits.shape, dtype=torch.float32, device=dev)
+    w = logits.new_empty(logits.shape, dtype=torch.float32)
     if w.numel() == 0:
         return w
     p = _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence)
-    with _on(dev) as st:
-        rc = lib().fl_relation_weights(ctypes.byref(p), w.data_ptr(), st)
-    check(rc, "relation weights")
+    _call(dev, "relation weights", lib().fl_relation_weights, ctypes.byref(p), w.data_ptr())
     return w
 
 
@@ -798,67 +792,51 @@ def relation_weights_backward(w, g, logits, bias=None, history=None, tau=1.0, re
     (rows may share one line: stride 0)."""
     dev = _one_device("relation weights backward", w, g, logits, bias, history)
     rows, n = w.shape
-    dz = torch.empty((rows, n), dtype=logits.dtype, device=dev) if want_logits else None
+    dz = logits.new_empty((rows, n)) if want_logits else None
     db = torch.empty_like(bias) if want_bias else None
     if g.stride(1) != 1:
         g = g.contiguous()
     p = _weights_params(logits, bias, None, None, history, tau, repetition, 0.0, 0.0)
     nbytes = lib().fl_relation_weights_workspace(rows, n) if want_bias and bias.dim() == 1 else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as st:
-        rc = lib().fl_relation_weights_backward(ctypes.byref(p), w.data_ptr(), g.data_ptr(), g.stride(0),
-                                                None if dz is None else dz.data_ptr(),
-                                                None if db is None else db.data_ptr(),
-                                                None if ws is None else ws.data_ptr(), nbytes, st)
-    check(rc, "relation weights backward")
+    ws = _workspace(nbytes, w)
+    _call(dev, "relation weights backward", lib().fl_relation_weights_backward, ctypes.byref(p), w.data_ptr(),
+          g.data_ptr(), g.stride(0), _ptr(dz), _ptr(db), _ptr(ws), nbytes)
     return dz, db
 
 
-def _batch_dims(t):
-    """[..., m, n] as (b1, b2, strides) with at most two strided batch dimensions, or None when its leading
-    dimensions need more."""
-    dims = [(n, s) for n, s in zip(t.shape[:-2], t.stride()[:-2]) if n != 1]
-    merged = []
-    for n, s in dims:
-        if merged and merged[-1][1] == n * s:
-            merged[-1] = (merged[-1][0] * n, s)
-        else:
-            merged.append((n, s))
-    return merged if len(merged) <= 2 else None
-
-
 def _as_batch(ts):
-    """A common (b1, b2) of tensors [..., m, n] of one shape, with each one's fl_matrices; None when the strides
-    of some cannot be expressed."""
-    lead = ts[0].shape[:-2]
+    """A common (b1, b2) of tensors [..., m, n] of one shape, with each one's fl_matrices; None when the leading
+    dimensions of some need more than two strides."""
+    merged, split = [], 1  # split: b2, the innermost batch dimensions that every tensor holds at one stride
     total = 1
-    for n in lead:
+    for n in ts[0].shape[:-2]:
         total *= n
-    split = 1  # b2: the innermost batch dimensions that every tensor holds at one stride
     for t in ts:
-        dims = _batch_dims(t)
-        if dims is None:
+        dims = []
+        for n, s in zip(t.shape[:-2], t.stride()):
+            if n == 1:
+                continue
+            if dims and dims[-1][1] == n * s:
+                dims[-1] = (dims[-1][0] * n, s)
+            else:
+                dims.append((n, s))
+        if len(dims) > 2 or (len(dims) == 2 and split not in (1, dims[1][0])):
             return None
         if len(dims) == 2:
-            if split not in (1, dims[1][0]):
-                return None
             split = dims[1][0]
+        merged.append(dims)
     out = []
-    for t in ts:
-        dims = _batch_dims(t)
-        if len(dims) == 2:
-            s1, s2 = dims[0][1], dims[1][1]
-        else:
-            s2 = dims[0][1] if dims else 0
-            s1 = s2 * split
+    for t, dims in zip(ts, merged):
+        s2 = dims[-1][1] if dims else 0
+        s1 = dims[0][1] if len(dims) == 2 else s2 * split
         out.append(L.fl_matrices(t.data_ptr(), s1, s2, t.stride(-2), t.stride(-1)))
-    return (total // split if split else 0), split, out
+    return total // split, split, out
 
 
 def orthogonalize(update, steps: int, coefficients, eps: float):
     """fl_orthogonalize of update [..., m, n]: a new contiguous tensor of its dtype."""
     dev = _one_device("orthogonalize", update)
-    out = torch.empty(update.shape, dtype=update.dtype, device=dev)
+    out = update.new_empty(update.shape)
     if out.numel() == 0:
         return out
     got = _as_batch((update, out))
@@ -867,13 +845,10 @@ def orthogonalize(update, steps: int, coefficients, eps: float):
         got = _as_batch((update, out))
     b1, b2, (src, dst) = got
     m, n = update.shape[-2:]
-    a, b, c = coefficients
     nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as st:
-        rc = lib().fl_orthogonalize(ctypes.byref(src), ctypes.byref(dst), b1, b2, m, n, FL_DTYPE[update.dtype], steps,
-                                    a, b, c, eps, None if ws is None else ws.data_ptr(), nbytes, st)
-    check(rc, "orthogonalize")
+    ws = _workspace(nbytes, update)
+    _call(dev, "orthogonalize", lib().fl_orthogonalize, ctypes.byref(src), ctypes.byref(dst), b1, b2, m, n,
+          FL_DTYPE[update.dtype], steps, *coefficients, eps, _ptr(ws), nbytes)
     return out
 
 
@@ -885,7 +860,7 @@ def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nes
         return
     got = _as_batch((param, grad, momentum, param_out, momentum_out))
     if got is None:  # strides that two batch dimensions cannot express: through plain copies
-        p2, m2 = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (param_out, momentum_out))
+        p2, m2 = (t.new_empty(t.shape) for t in (param_out, momentum_out))
         muon_update(param.contiguous(), grad.contiguous(), momentum.contiguous(), p2, m2, lr=lr, beta=beta,
                     nesterov=nesterov, weight_decay=weight_decay, scale=scale, steps=steps,
                     coefficients=coefficients, eps=eps)
@@ -894,13 +869,10 @@ def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nes
         return
     b1, b2, ts = got
     m, n = param.shape[-2:]
-    a, b, c = coefficients
     nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on(dev) as st:
-        rc = lib().fl_muon_update(*(ctypes.byref(t) for t in ts), b1, b2, m, n, lr, beta, int(nesterov), weight_decay,
-                                  scale, steps, a, b, c, eps, None if ws is None else ws.data_ptr(), nbytes, st)
-    check(rc, "muon_update")
+    ws = _workspace(nbytes, param)
+    _call(dev, "muon_update", lib().fl_muon_update, *(ctypes.byref(t) for t in ts), b1, b2, m, n, lr, beta,
+          int(nesterov), weight_decay, scale, steps, *coefficients, eps, _ptr(ws), nbytes)
 
 
 def gemm_fault() -> bool:
