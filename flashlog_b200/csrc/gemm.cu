@@ -368,12 +368,16 @@ struct EpiWarp {
 template <typename T>
 struct EpiLinear {
     LinearEpilogue p;
-    __device__ __forceinline__ void prepare(EpiWarp &, int, int64_t, int64_t) const {}
-    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0, int64_t m,
-                                               int64_t n, bool) const {
-        linear_store<T>(p, v, w.stage, row0, col0, m, n, w.lane);
+    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int b, int64_t row0, int64_t col0, int64_t m,
+                                               int64_t n) const {
+        if (p.out_batch == 0) {
+            linear_store<T>(p, v, w.stage, row0, col0, m, n, w.lane);
+        } else {
+            LinearEpilogue q = p;
+            q.out = static_cast<T *>(p.out) + b * p.out_batch;
+            linear_store<T>(q, v, w.stage, row0, col0, m, n, w.lane);
+        }
     }
-    __device__ __forceinline__ void finish(EpiWarp &) const {}
 };
 
 // ---- 32 x 32 tiles of two planes: hi at the staging tile's start, lo 2 KB on ----
@@ -404,11 +408,11 @@ __device__ __forceinline__ void stage_free(int lane) {
 }
 
 template <typename T>
-__device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float (&v)[32], float *stage, int b,
+__device__ __forceinline__ void final_store(const FinalOutput &e, const float (&v)[32], float *stage, int b,
                                             int64_t row0, int64_t col0, int64_t m, int64_t n, int lane) {
-    T *out = static_cast<T *>(e.fin.ptr) + e.fin.at(b, e.nb2);
+    T *out = static_cast<T *>(e.out.ptr) + e.out.at(b, e.nb2);
     const float *base = e.base.ptr != nullptr ? static_cast<const float *>(e.base.ptr) + e.base.at(b, e.nb2) : nullptr;
-    const bool by_row = e.fin.i == 1;  // lane = row is the contiguous direction
+    const bool by_row = e.out.i == 1;  // lane = row is the contiguous direction
     if (!by_row) {
         stage_rows(stage, v, lane);
         __syncwarp();
@@ -416,9 +420,9 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
     const int64_t row = by_row ? row0 + lane : row0, col = by_row ? col0 : col0 + lane;
     const int lines = static_cast<int>(min(static_cast<int64_t>(32), by_row ? n - col0 : m - row0));
     const bool in = row < m && col < n;
-    T *po = out + row * e.fin.i + col * e.fin.j;
+    T *po = out + row * e.out.i + col * e.out.j;
     const float *pb = base != nullptr ? base + row * e.base.i + col * e.base.j : nullptr;
-    const int64_t so = by_row ? e.fin.j : e.fin.i, sb = by_row ? e.base.j : e.base.i;
+    const int64_t so = by_row ? e.out.j : e.out.i, sb = by_row ? e.base.j : e.base.i;
     // eight lines at a time: the base's loads are in flight together, ahead of the stores that may alias it
 #pragma unroll
     for (int l0 = 0; l0 < 32; l0 += 8) {
@@ -442,115 +446,382 @@ __device__ __forceinline__ void final_store(const PlanesEpilogue &e, const float
     __syncwarp();
 }
 
-// Planes go to and come from memory by TMA: whole tiles through the warp's
-// staging tile, C for a tile's first chunk already under the products.
-template <bool SYM>
-struct EpiPlanes {
-    PlanesEpilogue p;
-    CUtensorMap map_c, map_out, map_out2;
+// The epilogue of a Newton-Schulz product, v = alpha * acc + beta * C.  Planes
+// go to and come from memory by TMA, whole 32 x 32 tiles through the warp's
+// staging tile; C for a tile's first chunk is loaded under the products.
+struct PlanesJob {
+    float alpha, beta;
+    const CUtensorMap *c, *out, *out2;  // C and out2 may be absent; out is, where the result is final
+    float alpha2, diag;                 // out2 = alpha2 * v + diag on the diagonal
+    bool symmetric;                     // elements on and below the diagonal, the others as their mirror image
+};
 
-    __device__ __forceinline__ void load_c(EpiWarp &w, int b, int64_t row0, int64_t col0) const {
-        if (w.lane == 0) {
-            bar_expect(w.bar, 4096);
-            asm volatile(
-                "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-                " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(w.stage)),
-                "l"(reinterpret_cast<uint64_t>(&map_c)), "r"(w.bar), "r"(static_cast<int>(col0)),
-                "r"(static_cast<int>(row0)), "r"(0), "r"(b) : "memory");
+__device__ __forceinline__ bool planes_wanted(const PlanesJob &p, int64_t row0, int64_t col0) {
+    return !p.symmetric || col0 <= row0;
+}
+__device__ __forceinline__ void planes_load_c(const PlanesJob &p, EpiWarp &w, int b, int64_t row0, int64_t col0) {
+    if (w.lane == 0) {
+        bar_expect(w.bar, 4096);
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(w.stage)),
+            "l"(reinterpret_cast<uint64_t>(p.c)), "r"(w.bar), "r"(static_cast<int>(col0)),
+            "r"(static_cast<int>(row0)), "r"(0), "r"(b) : "memory");
+    }
+}
+// loaded: whether C of this chunk is on its way already
+__device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutput &f, float (&v)[32], EpiWarp &w, int b,
+                                             int64_t row0, int64_t col0, int64_t m, int64_t n, bool loaded) {
+    if (!planes_wanted(p, row0, col0)) return;
+    const int lane = w.lane;
+    unsigned char *stage = reinterpret_cast<unsigned char *>(w.stage);
+    const uint32_t s32 = smem_u32(stage);
+    if (p.c != nullptr) {
+        if (!loaded) planes_load_c(p, w, b, row0, col0);
+        const bool ok = warp_wait(w.bar, w.phase, w.failed);
+        w.phase ^= 1;
+        if (!ok) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            union { uint4 u; __half2 h[4]; } a, z;
+            a.u = *reinterpret_cast<const uint4 *>(stage + piece_at(lane, q));
+            z.u = *reinterpret_cast<const uint4 *>(stage + 2048 + piece_at(lane, q));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float2 x = __half22float2(a.h[c]), y = __half22float2(z.h[c]);
+                v[q * 8 + 2 * c] = fmaf(p.alpha, v[q * 8 + 2 * c], p.beta * (x.x + y.x));
+                v[q * 8 + 2 * c + 1] = fmaf(p.alpha, v[q * 8 + 2 * c + 1], p.beta * (x.y + y.y));
+            }
         }
+        __syncwarp();
+    } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
     }
-    __device__ __forceinline__ bool wanted(int64_t row0, int64_t col0) const {
-        return !SYM || col0 <= row0;  // the rest is written as a mirror image
+    if (p.out == nullptr) {
+        if (f.dtype == kOutF32) final_store<float>(f, v, w.stage, b, row0, col0, m, n, lane);
+        else if (f.dtype == kOutF16) final_store<__half>(f, v, w.stage, b, row0, col0, m, n, lane);
+        else final_store<__nv_bfloat16>(f, v, w.stage, b, row0, col0, m, n, lane);
+        // the staging tile is next written by a TMA load: order it behind these accesses
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        return;
     }
-    // The first chunk's C, before the products are waited for.
-    __device__ __forceinline__ void prepare(EpiWarp &w, int b, int64_t row0, int64_t col0) const {
-        if (p.c != nullptr && wanted(row0, col0)) load_c(w, b, row0, col0);
-    }
-    __device__ __forceinline__ void finish(EpiWarp &w) const {
-        if (w.lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    const int row = static_cast<int>(row0), col = static_cast<int>(col0);
+    if (p.symmetric && col == row) {
+        // the tile on the diagonal: its upper half from the lower
+        stage_rows(w.stage, v, lane);
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = w.stage[stage_at(max(c, lane), min(c, lane))];
         __syncwarp();
     }
-    // first: whether prepare has loaded C
-    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int b, int64_t row0, int64_t col0, int64_t m,
-                                               int64_t n, bool first) const {
-        if (!wanted(row0, col0)) return;
-        const int lane = w.lane;
-        unsigned char *stage = reinterpret_cast<unsigned char *>(w.stage);
-        const uint32_t s32 = smem_u32(stage);
-        if (p.c != nullptr) {
-            if (!first) load_c(w, b, row0, col0);
-            const bool ok = warp_wait(w.bar, w.phase, w.failed);
-            w.phase ^= 1;
-            if (!ok) return;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                union { uint4 u; __half2 h[4]; } a, z;
-                a.u = *reinterpret_cast<const uint4 *>(stage + piece_at(lane, q));
-                z.u = *reinterpret_cast<const uint4 *>(stage + 2048 + piece_at(lane, q));
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float2 x = __half22float2(a.h[c]), y = __half22float2(z.h[c]);
-                    v[q * 8 + 2 * c] = fmaf(p.alpha, v[q * 8 + 2 * c], p.beta * (x.x + y.x));
-                    v[q * 8 + 2 * c + 1] = fmaf(p.alpha, v[q * 8 + 2 * c + 1], p.beta * (x.y + y.y));
-                }
-            }
-            __syncwarp();
-        } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
-        }
-        if (!SYM && p.fin.ptr != nullptr) {
-            if (p.dtype == kOutF32) final_store<float>(p, v, w.stage, b, row0, col0, m, n, lane);
-            else if (p.dtype == kOutF16) final_store<__half>(p, v, w.stage, b, row0, col0, m, n, lane);
-            else final_store<__nv_bfloat16>(p, v, w.stage, b, row0, col0, m, n, lane);
-            // the staging tile is next written by a TMA load: order it behind these accesses
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            return;
-        }
-        const int row = static_cast<int>(row0), col = static_cast<int>(col0);
-        if (SYM && col == row) {
-            // the tile on the diagonal: its upper half from the lower
-            stage_rows(w.stage, v, lane);
-            __syncwarp();
-#pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = w.stage[stage_at(max(c, lane), min(c, lane))];
-            __syncwarp();
-        }
 #pragma unroll 1
-        for (int o = 0; o < (SYM && p.out2 != nullptr ? 2 : 1); ++o) {
-            const CUtensorMap *map = o == 0 ? &map_out : &map_out2;
-            if (o == 1) {
+    for (int o = 0; o < (p.out2 != nullptr ? 2 : 1); ++o) {
+        const CUtensorMap *map = o == 0 ? p.out : p.out2;
+        if (o == 1) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col + c == row + lane ? p.diag : 0.0f);
-            }
-            planes_to_stage(stage, v, lane);
-            stage_store(map, s32, col, row, b, lane);
-            if (SYM && col != row) {
-                // the mirror image: 8 x 8 blocks turned on their way through registers
-                uint32_t r[2][4][4];
-                const int j = lane >> 3, k = lane & 7;
+            for (int c = 0; c < 32; ++c) v[c] = p.alpha2 * v[c] + (col + c == row + lane ? p.diag : 0.0f);
+        }
+        planes_to_stage(stage, v, lane);
+        stage_store(map, s32, col, row, b, lane);
+        if (p.symmetric && col != row) {
+            // the mirror image: 8 x 8 blocks turned on their way through registers
+            uint32_t r[2][4][4];
+            const int j = lane >> 3, k = lane & 7;
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                                     : "=r"(r[q][i][0]), "=r"(r[q][i][1]), "=r"(r[q][i][2]), "=r"(r[q][i][3])
-                                     : "r"(s32 + 2048 * q + piece_at(8 * i + k, j)) : "memory");
-                stage_free(lane);
-#pragma unroll
-                for (int q = 0; q < 2; ++q)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
-                                         s32 + 2048 * q + piece_at(8 * j + k, i)),
-                                     "r"(r[q][i][0]), "r"(r[q][i][1]), "r"(r[q][i][2]), "r"(r[q][i][3]) : "memory");
-                stage_store(map, s32, row, col, b, lane);
-            }
+                for (int i = 0; i < 4; ++i)
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(r[q][i][0]), "=r"(r[q][i][1]), "=r"(r[q][i][2]), "=r"(r[q][i][3])
+                                 : "r"(s32 + 2048 * q + piece_at(8 * i + k, j)) : "memory");
             stage_free(lane);
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                                     s32 + 2048 * q + piece_at(8 * j + k, i)),
+                                 "r"(r[q][i][0]), "r"(r[q][i][1]), "r"(r[q][i][2]), "r"(r[q][i][3]) : "memory");
+            stage_store(map, s32, row, col, b, lane);
+        }
+        stage_free(lane);
+    }
+}
+
+// ---- what a kernel works through: tiles in one order for all its roles ----------
+struct Job {
+    const CUtensorMap *a, *b;
+    int a_mn, b_mn;
+    int row, col, width;   // the pair's tile: 256 rows, `width` columns (a multiple of 32)
+    int m, n;              // bounds of the output
+    int batch_a, batch_b, batch_out;
+    int kb0, kb1;          // contraction, in blocks of kBK
+    int phase;
+};
+struct Cursor {
+    int phase, base;       // of the tile looked at last
+    int seen;              // the dependency known to be met: phase * batch + matrix, or -1
+};
+
+// One product.
+template <typename Epi>
+struct SingleWork {
+    CUtensorMap map_a, map_b;
+    int m, n, kblocks, splits;  // splits > 1: the contraction in parts, one output each
+    int a_mn, b_mn;
+    TileGrid grid;
+    uint32_t types;             // of the instruction descriptor
+    Epi epi;
+
+    __device__ __forceinline__ int total() const { return grid.total; }
+    template <int BN>
+    __device__ __forceinline__ Job job(int t, Cursor &) const {
+        Job j;
+        int b, ti, tj;
+        tile_of<BN>(grid, t, b, ti, tj);
+        const int mat = b / splits, part = b - mat * splits, per = (kblocks + splits - 1) / splits;
+        j.a = &map_a;
+        j.b = &map_b;
+        j.a_mn = a_mn;
+        j.b_mn = b_mn;
+        j.row = ti * 2 * kBM;
+        j.col = tj * BN;
+        j.width = min(BN, (n - j.col + 31) & ~31);
+        j.m = m;
+        j.n = n;
+        j.batch_a = j.batch_b = mat;
+        j.batch_out = b;
+        j.kb0 = part * per;
+        j.kb1 = min(kblocks, j.kb0 + per);
+        j.phase = 0;
+        return j;
+    }
+    __device__ __forceinline__ bool wait(const Job &, Cursor &, volatile int *) const { return true; }
+    __device__ __forceinline__ void prepare(const Job &, EpiWarp &, int64_t, int64_t) const {}
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int64_t row0, int64_t col0, bool) const {
+        epi(v, w, j.batch_out, row0, col0, j.m, j.n);
+    }
+    __device__ __forceinline__ void done(const Job &, EpiWarp &) const {}
+};
+
+// All products of a Newton-Schulz run.  A phase is one product (or two that do
+// not depend on each other) of every matrix of the batch; a matrix' tiles of a
+// phase start once its tiles of the phase before are complete, whatever the
+// other matrices do, so that the next phase's tiles fill the SMs that the last
+// tiles of this one leave idle.  The tiles are dealt out in phase order and all
+// blocks are resident (a cooperative launch), so the tile that a wait is for is
+// always being worked on or done.
+struct NsWork {
+    CUtensorMap ka[kNsBuffers], kb[kNsBuffers], pl[kNsBuffers], mn[2];
+    NsProgram p;
+    TileGrid sym, full;
+    int *done_count;            // [phases, batch], zero at the start
+    int phases, first;
+    uint32_t types;
+
+    __device__ __forceinline__ int last() const { return p.steps - 1; }
+    // Gram form, phase 1 + 3 k + j: j = 0 B_k; j = 1 Q_k and T_k; j = 2 A_{k+1}, or the result
+    __device__ __forceinline__ int parts(int phase) const {
+        if (!p.gram || phase == 0 || (phase - 1) % 3 != 1) return 1;
+        const int k = (phase - 1) / 3;
+        return (k > 0 ? 1 : 0) + (k < last() ? 1 : 0);
+    }
+    __device__ __forceinline__ bool is_full(int phase) const {
+        return phase == phases - 1 || (!p.gram && phase % 3 == 2);
+    }
+    __device__ __forceinline__ int tiles(int phase) const {  // of one matrix
+        return is_full(phase) ? full.per_batch : sym.per_batch * parts(phase);
+    }
+    __device__ __forceinline__ int total() const {
+        int t = 0;
+        for (int q = first; q < phases; ++q) t += tiles(q) * p.batch;
+        return t;
+    }
+    // which product of the phase a tile of it belongs to: its position in its matrix' tiles
+    __device__ __forceinline__ int part_of(int phase, int r) const {
+        const int one = sym.per_batch;
+        const int which = parts(phase) == 2 ? r / one : 0;
+        return parts(phase) == 1 && p.gram && phase > 0 && (phase - 1) % 3 == 1 && (phase - 1) / 3 == 0 ? 1 : which;
+    }
+    struct Product {
+        int a, b, b_mn, k, n, c, out, out2;  // buffers (-1: none)
+        float alpha, beta, alpha2, diag;
+    };
+    __device__ __forceinline__ Product product(int phase, int part) const {
+        Product q;
+        q.b_mn = 0;
+        q.k = p.lo;
+        q.n = p.lo;
+        q.out2 = -1;
+        q.alpha2 = q.diag = 0.0f;
+        int kind, k;  // 0: A = X X^T, 1: B, 2: X' (direct) or the result, 3: Q, 4: T, 5: A' = P A P
+        if (!p.gram) {
+            k = phase / 3;
+            kind = phase % 3;
+        } else if (phase == 0) {
+            k = 0;
+            kind = 0;
+        } else if (phase == phases - 1) {
+            k = last();
+            kind = 2;
+        } else {
+            k = (phase - 1) / 3;
+            const int j = (phase - 1) % 3;
+            kind = j == 0 ? 1 : j == 2 ? 5 : part == 0 ? 3 : 4;
+        }
+        const int x = p.gram ? 0 : k & 1;
+        if (kind == 0) {
+            q.a = q.b = x;
+            q.k = p.hi;
+            q.c = -1;
+            q.alpha = p.scale_a / (p.scale_x * p.scale_x);
+            q.beta = 0.0f;
+            q.out = kNsA;
+        } else if (kind == 1) {
+            q.a = q.b = q.c = kNsA;
+            q.alpha = p.c / p.scale_a;
+            q.beta = p.b;
+            q.out = kNsB;
+            if (p.gram && k == 0) {
+                q.out2 = kNsQ;
+                q.alpha2 = p.scale_q / p.scale_a;
+                q.diag = p.a * p.scale_q;
+            }
+        } else if (kind == 2) {
+            q.n = p.hi;
+            q.b = x;
+            q.b_mn = 1;
+            q.out = phase == phases - 1 ? -1 : x ^ 1;
+            if (p.gram) {
+                q.a = kNsQ + (last() & 1);
+                q.c = -1;
+                q.alpha = p.factor / (p.scale_q * p.scale_x);
+                q.beta = 0.0f;
+            } else {
+                const float f = q.out < 0 ? p.factor / p.scale_x : 1.0f;
+                q.a = kNsB;
+                q.c = x;
+                q.alpha = f / p.scale_a;
+                q.beta = f * p.a;
+            }
+        } else {
+            // Q <- a Q + B Q;  T = a A + B A;  A <- a T + T B
+            q.a = kind == 5 ? kNsT : kNsB;
+            q.b = kind == 3 ? kNsQ + ((k - 1) & 1) : kind == 4 ? kNsA : kNsB;
+            q.c = kind == 5 ? kNsT : q.b;
+            q.out = kind == 3 ? kNsQ + (k & 1) : kind == 4 ? kNsT : kNsA;
+            q.alpha = 1.0f / p.scale_a;
+            q.beta = p.a;
+        }
+        return q;
+    }
+    // phase and matrix of tile t, and its position r among the matrix' tiles
+    __device__ __forceinline__ void locate(int t, Cursor &cur, int &b, int &r) const {
+        for (;;) {
+            const int per = tiles(cur.phase), count = per * p.batch;
+            if (t - cur.base < count) {
+                b = (t - cur.base) / per;
+                r = t - cur.base - b * per;
+                return;
+            }
+            cur.base += count;
+            ++cur.phase;
         }
     }
+    template <int BN>
+    __device__ __forceinline__ Job job(int t, Cursor &cur) const {
+        Job j;
+        int b, r;
+        locate(t, cur, b, r);
+        const bool f = is_full(cur.phase);
+        const int part = f ? 0 : part_of(cur.phase, r);
+        const Product q = product(cur.phase, part);
+        const TileGrid &g = f ? full : sym;
+        int zero, ti, tj;
+        tile_of<BN>(g, f ? r : r % sym.per_batch, zero, ti, tj);
+        j.a = ka + q.a;
+        j.b = q.b_mn ? mn + q.b : kb + q.b;
+        j.a_mn = 0;
+        j.b_mn = q.b_mn;
+        j.row = ti * 2 * kBM;
+        j.col = tj * BN;
+        j.m = p.lo;
+        j.n = q.n;
+        j.width = min(BN, (q.n - j.col + 31) & ~31);
+        j.batch_a = j.batch_b = j.batch_out = b;
+        j.kb0 = 0;
+        j.kb1 = (q.k + kBK - 1) / kBK;
+        j.phase = cur.phase | (part << 16);
+        return j;
+    }
+    __device__ __forceinline__ PlanesJob planes(const Job &j) const {
+        const int phase = j.phase & 65535;
+        const Product q = product(phase, j.phase >> 16);
+        PlanesJob e;
+        e.alpha = q.alpha;
+        e.beta = q.beta;
+        e.c = q.c < 0 ? nullptr : pl + q.c;
+        e.out = q.out < 0 ? nullptr : pl + q.out;
+        e.out2 = q.out2 < 0 ? nullptr : pl + q.out2;
+        e.alpha2 = q.alpha2;
+        e.diag = q.diag;
+        e.symmetric = !is_full(phase);
+        return e;
+    }
+    // Until the matrix' tiles of the phase before are complete (every epilogue
+    // warp of both CTAs counts once per tile).  All lanes call it.
+    __device__ __forceinline__ bool wait(const Job &j, Cursor &cur, volatile int *failed) const {
+        const int phase = j.phase & 65535;
+        if (phase == first) return true;
+        const int at = (phase - 1) * p.batch + j.batch_out;
+        if (cur.seen == at) return true;
+        const int want = tiles(phase - 1) * 2 * kEpiWarps;
+        uint64_t start = 0, now = 0;
+        for (int i = 0;; ++i) {
+            int have;
+            asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(have) : "l"(done_count + at) : "memory");
+            if (__all_sync(kFull, have >= want)) break;
+            if ((i & 63) == 63) {
+                asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+                if (start == 0) start = now;
+                const bool over = now - start > kWaitLimitNs;
+                if (__any_sync(kFull, over)) {
+                    atomicExch(&g_gemm_fault, 1);
+                    *failed = 1;
+                }
+                if (__any_sync(kFull, *failed != 0)) return false;
+            }
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");  // the loads that follow go through the other proxy
+        cur.seen = at;
+        return true;
+    }
+    __device__ __forceinline__ void prepare(const Job &j, EpiWarp &w, int64_t row0, int64_t col0) const {
+        const PlanesJob e = planes(j);
+        if (e.c != nullptr && planes_wanted(e, row0, col0)) planes_load_c(e, w, j.batch_out, row0, col0);
+    }
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int64_t row0, int64_t col0,
+                                          bool loaded) const {
+        planes_chunk(planes(j), p.final, v, w, j.batch_out, row0, col0, j.m, j.n, loaded);
+    }
+    // The tile's part of this warp is in memory: count it.
+    __device__ __forceinline__ void done(const Job &j, EpiWarp &w) const {
+        const int phase = j.phase & 65535;
+        if (phase == phases - 1) return;
+        if (w.lane == 0) {
+            asm volatile("cp.async.bulk.wait_group 0;\n fence.proxy.async;" ::: "memory");
+            __threadfence();
+            asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(done_count + phase * p.batch + j.batch_out)
+                         : "memory");
+        }
+        __syncwarp();
+    }
 };
+
+template <typename W> __device__ __forceinline__ int work_first(const W &) { return 0; }
+__device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 
 template <int BN, int PLANES>
 struct Config {
@@ -561,10 +832,9 @@ struct Config {
     static constexpr int kSmem = kStages * kStage + kEpiWarps * 32 * 32 * 4 + 1024;
 };
 
-template <int BN, int PLANES, typename Epi>
+template <int BN, int PLANES, typename Work>
 __global__ __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
-void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, int64_t m,
-                 int64_t n, int64_t k, TileGrid grid, int a_mn, int b_mn, uint32_t idesc, const __grid_constant__ Epi epi) {
+void gemm_kernel(const __grid_constant__ Work work) {
     using C = Config<BN, PLANES>;
     extern __shared__ unsigned char raw[];
     // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
@@ -593,31 +863,32 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                      "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
-    if (warp == kLoadA && lane < 2)
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &map_a : &map_b)));
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
-    const int kblocks = static_cast<int>((k + kBK - 1) / kBK);
+    const int total = work.total();
+    Cursor cur{work_first(work), 0, -1};
 
     if (warp == kLoadA || warp == kLoadB) {
         // ---- loads ----
         const bool is_a = warp == kLoadA;
-        const CUtensorMap *map = is_a ? &map_a : &map_b;
-        const bool mn = is_a ? a_mn != 0 : b_mn != 0;
-        const int pieces = mn ? (is_a ? kBM / 64 : BN / 128) : 1;  // 64 lines of an MN-major operand per load
         const uint32_t offset = is_a ? 0 : PLANES * C::kA, plane = is_a ? C::kA : C::kB;
         const bool expects = is_a && cta == 0;
         int s = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = pair; ok && t < grid.total; t += pairs) {
-            int b, ti, tj;
-            tile_of<BN>(grid, t, b, ti, tj);
-            const int line = is_a ? ti * 2 * kBM + static_cast<int>(cta) * kBM : tj * BN + static_cast<int>(cta) * (BN / 2);
-            for (int kb = 0; kb < kblocks; ++kb) {
+        for (int t = pair; ok && t < total; t += pairs) {
+            const Job j = work.template job<BN>(t, cur);
+            ok = work.wait(j, cur, &failed);
+            if (!ok) break;
+            const CUtensorMap *map = is_a ? j.a : j.b;
+            const bool mn = is_a ? j.a_mn != 0 : j.b_mn != 0;
+            const int pieces = mn ? (is_a ? kBM / 64 : BN / 128) : 1;  // 64 lines of an MN-major operand per load
+            const int line = is_a ? j.row + static_cast<int>(cta) * kBM : j.col + static_cast<int>(cta) * (j.width >> 1);
+            const int b = is_a ? j.batch_a : j.batch_b;
+            for (int kb = j.kb0; kb < j.kb1; ++kb) {
                 ok = warp_wait(empty + 8 * s, phase ^ 1, &failed);
                 if (!ok) break;
                 const uint32_t dst = smem_u32(smem) + s * C::kStage + offset;
@@ -625,7 +896,6 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     // the other CTA's and the other warp's bytes may arrive before they are expected
                     if (expects) bar_expect(full + 8 * s, 2 * C::kStage);
                     if (mn) {
-#pragma unroll
                         for (int p = 0; p < PLANES; ++p)
                             for (int h = 0; h < pieces; ++h)
                                 tma_load(dst + p * plane + h * 8192, map, full + 8 * s, line + 64 * h, kb * kBK, p, b);
@@ -650,17 +920,20 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
     } else if (warp == kMmaWarp && cta == 0) {
         // ---- products (for the pair) ----
-        const uint32_t a_step = a_mn ? 128u : 2u, b_step = b_mn ? 128u : 2u;  // 16 of k, in 16-byte units
-        const uint32_t a_lbo = a_mn ? 8192u : 16u, b_lbo = b_mn ? 8192u : 16u;
         int s = 0, buf = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for (int t = pair; ok && t < grid.total; t += pairs) {
+        for (int t = pair; ok && t < total; t += pairs) {
+            const Job j = work.template job<BN>(t, cur);
+            const uint32_t a_step = j.a_mn ? 128u : 2u, b_step = j.b_mn ? 128u : 2u;  // 16 of k, in 16-byte units
+            const uint32_t a_lbo = j.a_mn ? 8192u : 16u, b_lbo = j.b_mn ? 8192u : 16u;
+            const uint32_t idesc = work.types | (static_cast<uint32_t>(j.a_mn) << 15) | (static_cast<uint32_t>(j.b_mn) << 16) |
+                                   (static_cast<uint32_t>(j.width >> 3) << 17);
             ok = warp_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t d = tmem + buf * BN;
-            for (int kb = 0; kb < kblocks; ++kb) {
+            for (int kb = j.kb0; kb < j.kb1; ++kb) {
                 ok = warp_wait(full + 8 * s, phase, &failed);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -673,11 +946,11 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         db[p] = smem_desc(sb + p * C::kB, b_lbo, 1024);
                     }
 #pragma unroll
-                    for (int j = 0; j < kBK / 16; ++j) {
-                        mma_f16(d, da[0] + j * a_step, db[0] + j * b_step, idesc, (kb | j) != 0);
+                    for (int i = 0; i < kBK / 16; ++i) {
+                        mma_f16(d, da[0] + i * a_step, db[0] + i * b_step, idesc, kb != j.kb0 || i != 0);
                         if (PLANES == 2) {
-                            mma_f16(d, da[0] + j * a_step, db[PLANES - 1] + j * b_step, idesc, 1);
-                            mma_f16(d, da[PLANES - 1] + j * a_step, db[0] + j * b_step, idesc, 1);
+                            mma_f16(d, da[0] + i * a_step, db[PLANES - 1] + i * b_step, idesc, 1);
+                            mma_f16(d, da[PLANES - 1] + i * a_step, db[0] + i * b_step, idesc, 1);
                         }
                     }
                     mma_commit(empty + 8 * s);
@@ -695,18 +968,21 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for (int t = pair; t < grid.total; t += pairs) {
-            int b, ti, tj;
-            tile_of<BN>(grid, t, b, ti, tj);
-            const int64_t row0 = static_cast<int64_t>(ti) * 2 * kBM + cta * kBM + (warp & 3) * 32;
-            const int64_t col0 = static_cast<int64_t>(tj) * BN;
+        for (int t = pair; t < total; t += pairs) {
+            const Job j = work.template job<BN>(t, cur);
+            const int64_t row0 = j.row + static_cast<int>(cta) * kBM + (warp & 3) * 32;
             const int half = (warp >> 2) * (BN / 2);
-            if (ok && row0 < m && col0 + half < n) epi.prepare(w, b, row0, col0 + half);
+            const bool any = row0 < j.m && j.col + half < j.n;
+            if (ok && any) {
+                ok = work.wait(j, cur, &failed);  // (long met: the loads waited for it; here for this warp's own loads)
+                if (ok) work.prepare(j, w, row0, j.col + half);
+            }
             if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>((warp & 3) * 32) << 16);
 #pragma unroll 1
             for (int c = half; c < half + BN / 2; c += 32) {
+                if (!any || j.col + c >= j.n) break;
                 float v[32];
                 if (ok) {
                     tmem_read32(v, src + c);
@@ -714,15 +990,17 @@ void gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
                 }
-                if (row0 < m && col0 + c < n) epi(v, w, b, row0, col0 + c, m, n, c == half);
+                work.chunk(j, v, w, row0, j.col + c, c == half);
                 __syncwarp();
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive_cta0(acc_empty + 8 * buf);
+            work.done(j, w);
             if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
-        epi.finish(w);
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        __syncwarp();
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -815,52 +1093,71 @@ int64_t tile_count(const GemmShape &s, int bn) {
     return per;
 }
 
-template <int BN, int PLANES, typename Epi>
-int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, cudaStream_t st) {
-    using C = Config<BN, PLANES>;
-    CUtensorMap ma, mb;
-    int rc = operand_map(&ma, a, s.m, s.k, s.batch, kBM, s.kind);
-    if (rc) return rc;
-    rc = operand_map(&mb, b, s.n, s.k, s.batch, BN / 2, s.kind);
-    if (rc) return rc;
+TileGrid tile_grid(const GemmShape &s, int bn, int64_t copies) {
     TileGrid g;
     g.tiles_m = static_cast<int>((s.m + 2 * kBM - 1) / (2 * kBM));
-    g.tiles_n = static_cast<int>((s.n + BN - 1) / BN);
+    g.tiles_n = static_cast<int>((s.n + bn - 1) / bn);
     g.symmetric = s.symmetric;
-    g.batch = static_cast<int>(s.batch);
+    g.batch = static_cast<int>(copies);
     g.n_fast = g.tiles_n <= g.tiles_m;  // the operand with fewer tiles is the one read again and again, from L2
-    const int64_t per = tile_count(s, BN);
-    FL_REQUIRE(per * s.batch < (1 << 30), "gemm: too many tiles");
-    g.per_batch = static_cast<int>(per);
-    g.total = static_cast<int>(per * s.batch);
+    g.per_batch = static_cast<int>(tile_count(s, bn));
+    g.total = static_cast<int>(g.per_batch * copies);
+    return g;
+}
+
+int sm_pairs() {
     const int sms = fl_device_sm_count();
-    int pairs = (sms > 1 ? sms : 148) / 2;
-    if (pairs > g.total) pairs = g.total;
-    // fp32 accumulator, operand type, majors, N, M = 256 (the pair's)
-    const uint32_t type = s.kind == kBF16 ? 1u : 0u;
-    const uint32_t idesc = (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(a.mn_major != 0) << 15) |
-                           (static_cast<uint32_t>(b.mn_major != 0) << 16) | (static_cast<uint32_t>(BN >> 3) << 17) |
-                           (static_cast<uint32_t>(256 >> 4) << 24);
-    auto kernel = gemm_kernel<BN, PLANES, Epi>;
+    return (sms > 1 ? sms : 148) / 2;
+}
+
+// fp32 accumulator, operand type, M = 256 (the pair's)
+uint32_t instruction_types(int kind) {
+    const uint32_t type = kind == kBF16 ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(256 >> 4) << 24);
+}
+
+template <int BN, int PLANES, typename Epi>
+int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, int splits, cudaStream_t st) {
+    using C = Config<BN, PLANES>;
+    using W = SingleWork<Epi>;
+    W w;
+    int rc = operand_map(&w.map_a, a, s.m, s.k, s.batch, kBM, s.kind);
+    if (rc) return rc;
+    rc = operand_map(&w.map_b, b, s.n, s.k, s.batch, BN / 2, s.kind);
+    if (rc) return rc;
+    FL_REQUIRE(tile_count(s, BN) * s.batch * splits < (1 << 30), "gemm: too many tiles");
+    w.m = static_cast<int>(s.m);
+    w.n = static_cast<int>(s.n);
+    w.kblocks = static_cast<int>((s.k + kBK - 1) / kBK);
+    w.splits = splits;
+    w.a_mn = a.mn_major;
+    w.b_mn = b.mn_major;
+    w.grid = tile_grid(s, BN, s.batch * splits);
+    w.types = instruction_types(s.kind);
+    w.epi = epi;
+    int pairs = sm_pairs();
+    if (pairs > w.grid.total) pairs = w.grid.total;
+    auto kernel = gemm_kernel<BN, PLANES, W>;
     FL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     note_launch();
-    kernel<<<2 * pairs, kThreads, C::kSmem, st>>>(ma, mb, s.m, s.n, s.k, g, a.mn_major, b.mn_major, idesc, epi);
+    kernel<<<2 * pairs, kThreads, C::kSmem, st>>>(w);
     return check_launch("gemm");
+}
+
+int check_shape(const GemmShape &s) {
+    FL_REQUIRE(s.m > 0 && s.n > 0 && s.k > 0 && s.batch > 0 && s.m < (1ll << 31) - 512 && s.n < (1ll << 31) - 512 &&
+                   s.k < (1ll << 31) - 512 && s.batch < (1ll << 31),
+               "gemm: bad shape");
+    return FL_OK;
 }
 
 // 256-wide or 128-wide tiles: whichever needs less time on the slowest pair of
 // SMs, 256 when equal (half the loads of A per product).
-template <int PLANES, typename Epi>
-int run_any(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, cudaStream_t st) {
-    FL_REQUIRE(s.m > 0 && s.n > 0 && s.k > 0 && s.batch > 0 && s.m < (1ll << 31) - 512 && s.n < (1ll << 31) - 512 &&
-                   s.k < (1ll << 31) - 512 && s.batch < (1ll << 31),
-               "gemm: bad shape");
-    const int sms = fl_device_sm_count();
-    const int64_t pairs = (sms > 1 ? sms : 148) / 2;
+bool wide_tiles(const GemmShape &s) {
+    const int64_t pairs = sm_pairs();
     const int64_t wide = (tile_count(s, 256) * s.batch + pairs - 1) / pairs;
     const int64_t narrow = (tile_count(s, 128) * s.batch + pairs - 1) / pairs;
-    if (2 * wide <= narrow) return run<256, PLANES, Epi>(s, a, b, epi, st);
-    return run<128, PLANES, Epi>(s, a, b, epi, st);
+    return 2 * wide <= narrow;
 }
 
 template <typename T>
@@ -873,19 +1170,116 @@ int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b,
     };
     epi.p.aligned = rows_ready(e.out, e.ld_out, per) && rows_ready(e.residual, e.ld_res, per) && rows_ready(e.bias, 0, 1) &&
                     rows_ready(e.z, e.ld_z, 4);
-    return run_any<sizeof(T) == 4 ? 2 : 1>(s, a, b, epi, st);
+    constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
+    return wide_tiles(s) ? run<256, kPlanes>(s, a, b, epi, 1, st) : run<128, kPlanes>(s, a, b, epi, 1, st);
 }
 
-template <bool SYM>
-int planes_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
-                 cudaStream_t st) {
-    EpiPlanes<SYM> epi{};
-    epi.p = e;
-    int rc = FL_OK;
-    if (e.c != nullptr) rc = planes_map(&epi.map_c, e.c, e.c_ld, e.c_plane, e.c_batch, s.m, s.n, s.batch);
-    if (!rc && e.out != nullptr) rc = planes_map(&epi.map_out, e.out, e.ld, e.plane, e.batch, s.m, s.n, s.batch);
-    if (!rc && e.out2 != nullptr) rc = planes_map(&epi.map_out2, e.out2, e.ld2, e.plane2, e.batch2, s.m, s.n, s.batch);
-    return rc ? rc : run_any<2>(s, a, b, epi, st);
+template <int BN>
+int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, int *done_count, cudaStream_t st) {
+    using C = Config<BN, 2>;
+    NsWork w{};
+    w.p = p;
+    w.phases = phases;
+    w.first = first;
+    w.done_count = done_count;
+    w.types = instruction_types(kF16);
+    GemmShape square{p.lo, p.lo, p.lo, p.batch, 1, kF16}, full{p.lo, p.hi, p.lo, p.batch, 0, kF16};
+    w.sym = tile_grid(square, BN, 1);
+    w.full = tile_grid(full, BN, 1);
+    FL_REQUIRE(static_cast<double>(w.full.per_batch) * p.batch * phases * 2 < 1e9, "newton-schulz: too many tiles");
+    for (int i = 0; i < kNsBuffers; ++i) {
+        if (buf[i].p == nullptr) continue;
+        const int cols = i < 2 ? p.hi : p.lo;
+        GemmOperand o{buf[i].p, buf[i].ld, buf[i].plane, 2 * buf[i].plane, 2, 0};
+        int rc = operand_map(&w.ka[i], o, p.lo, cols, p.batch, kBM, kF16);
+        if (!rc) rc = operand_map(&w.kb[i], o, p.lo, cols, p.batch, BN / 2, kF16);
+        if (!rc) rc = planes_map(&w.pl[i], buf[i].p, o.ld, o.plane, o.batch, p.lo, cols, p.batch);
+        o.mn_major = 1;
+        if (!rc && i < 2) rc = operand_map(&w.mn[i], o, p.hi, p.lo, p.batch, BN / 2, kF16);
+        if (rc) return rc;
+    }
+    auto kernel = gemm_kernel<BN, 2, NsWork>;
+    FL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;  // the blocks wait for one another: all resident, or no launch
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int64_t most = static_cast<int64_t>(w.full.per_batch > 2 * w.sym.per_batch ? w.full.per_batch : 2 * w.sym.per_batch) * p.batch;
+    int pairs = sm_pairs();
+    if (pairs > most) pairs = static_cast<int>(most);
+    cfg.gridDim = dim3(2 * pairs);
+    // pairs of SMs that can be resident at once, asked once per device
+    static thread_local int known_device = -1, known_pairs = 0;
+    int device = 0;
+    FL_CUDA(cudaGetDevice(&device));
+    if (known_device != device) {
+        cudaLaunchConfig_t q = cfg;
+        cudaLaunchAttribute qa[1];
+        qa[0].id = cudaLaunchAttributeClusterDimension;
+        qa[0].val.clusterDim.x = 2;
+        qa[0].val.clusterDim.y = qa[0].val.clusterDim.z = 1;
+        q.attrs = qa;
+        q.numAttrs = 1;
+        q.gridDim = dim3(2 * sm_pairs());
+        FL_CUDA(cudaOccupancyMaxActiveClusters(&known_pairs, kernel, &q));
+        known_device = device;
+    }
+    FL_REQUIRE(known_pairs > 0, "newton-schulz: no pair of SMs can hold the kernel");
+    if (pairs > known_pairs) cfg.gridDim = dim3(2 * known_pairs);
+    note_launch();
+    FL_CUDA(cudaLaunchKernelEx(&cfg, kernel, w));
+    return check_launch("newton-schulz products");
+}
+
+// Sums the parts of A = X X^T into planes, both halves from the lower one: 32 x 32
+// tiles, grid (tiles, tiles, batch).
+__global__ void __launch_bounds__(256) combine_kernel(const float *parts, int splits, int lo, int64_t ldp, float alpha,
+                                                      __half *out, int64_t ld, int64_t plane) {
+    __shared__ float tile[32][33];
+    if (blockIdx.x > blockIdx.y) return;
+    const int64_t b = blockIdx.z;
+    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
+    const int64_t size = static_cast<int64_t>(lo) * ldp;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int i = i0 + threadIdx.y + 8 * q, j = j0 + threadIdx.x;
+        float s = 0.0f;
+        if (i < lo && j < lo)
+            for (int k = 0; k < splits; ++k) s += parts[(b * splits + k) * size + i * ldp + j];
+        tile[threadIdx.y + 8 * q][threadIdx.x] = s * alpha;
+    }
+    __syncthreads();
+    __half *hi = out + b * 2 * plane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int r = threadIdx.y + 8 * q, c = threadIdx.x;
+        for (int turned = 0; turned < 2; ++turned) {
+            if (turned && blockIdx.x == blockIdx.y) continue;
+            const int i = (turned ? j0 : i0) + r, j = (turned ? i0 : j0) + c;
+            if (i >= lo || j >= lo) continue;
+            const float v = turned ? tile[c][r] : blockIdx.x == blockIdx.y && c > r ? tile[c][r] : tile[r][c];
+            const __half h = __float2half_rn(v);
+            hi[i * ld + j] = h;
+            hi[plane + i * ld + j] = __float2half_rn(v - __half2float(h));
+        }
+    }
+}
+
+// How A = X X^T is split along the long side: enough parts to fill the pairs of
+// SMs, each at least 8 blocks of k long; 1 when its tiles fill half of them.
+int outer_splits(int64_t lo, int64_t hi, int64_t batch) {
+    GemmShape s{lo, lo, hi, batch, 1, kF16};
+    const int64_t tiles = tile_count(s, 256) * batch, kblocks = (hi + kBK - 1) / kBK;
+    int64_t n = sm_pairs() / tiles;
+    if (n > kblocks / 8) n = kblocks / 8;
+    if (n < 2) return 1;
+    const int64_t per = (kblocks + n - 1) / n;
+    return static_cast<int>((kblocks + per - 1) / per);  // every part has blocks
 }
 
 }  // namespace
@@ -894,16 +1288,47 @@ int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, 
                 cudaStream_t st) {
     const int planes = e.dtype == kOutF32 ? 2 : 1;
     FL_REQUIRE(a.planes == planes && b.planes == planes && !s.symmetric, "gemm: planes");
+    const int rc = check_shape(s);
+    if (rc) return rc;
     if (e.dtype == kOutF32) return linear_typed<float>(s, a, b, e, st);
     if (e.dtype == kOutF16) return linear_typed<__half>(s, a, b, e, st);
     return linear_typed<__nv_bfloat16>(s, a, b, e, st);
 }
 
-int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
-                cudaStream_t st) {
-    FL_REQUIRE(a.planes == 2 && b.planes == 2 && (!s.symmetric || (s.m == s.n && e.fin.ptr == nullptr)), "gemm: planes");
-    FL_REQUIRE(e.out != nullptr || e.fin.ptr != nullptr, "gemm: no output");
-    return s.symmetric ? planes_typed<true>(s, a, b, e, st) : planes_typed<false>(s, a, b, e, st);
+int ns_phases(int steps, int gram) { return gram ? (steps == 1 ? 3 : 1 + 3 * steps) : 3 * steps; }
+
+size_t ns_parts_bytes(int64_t lo, int64_t hi, int64_t batch) {
+    const int64_t n = outer_splits(lo, hi, batch);
+    return n > 1 ? static_cast<size_t>(n * batch * lo * ((lo + 7) & ~int64_t(7))) * sizeof(float) : 0;
+}
+
+int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float *parts, cudaStream_t st) {
+    const int phases = ns_phases(p.steps, p.gram);
+    GemmShape outer{p.lo, p.lo, p.hi, p.batch, 1, kF16};
+    int rc = check_shape(outer);
+    if (rc) return rc;
+    FL_REQUIRE(phases < 65536, "newton-schulz: too many steps");
+    const int splits = p.gram ? outer_splits(p.lo, p.hi, p.batch) : 1;
+    if (splits > 1) {
+        const GemmOperand x{buf[kNsX].p, buf[kNsX].ld, buf[kNsX].plane, 2 * buf[kNsX].plane, 2, 0};
+        EpiLinear<float> e{};
+        e.p.out = parts;
+        e.p.ld_out = (p.lo + 7) & ~7;
+        e.p.out_batch = p.lo * e.p.ld_out;
+        e.p.dtype = kOutF32;
+        e.p.aligned = 1;
+        rc = run<256, 2>(outer, x, x, e, splits, st);
+        if (rc) return rc;
+        const unsigned tiles = static_cast<unsigned>((p.lo + 31) / 32);
+        launch(combine_kernel, dim3(tiles, tiles, static_cast<unsigned>(p.batch)), dim3(32, 8), 0, st, parts, splits, p.lo,
+               e.p.ld_out, p.scale_a / (p.scale_x * p.scale_x), buf[kNsA].p, buf[kNsA].ld, buf[kNsA].plane);
+        rc = check_launch("newton-schulz combine");
+        if (rc) return rc;
+    }
+    const int first = splits > 1 ? 1 : 0;
+    // 256-wide tiles once a phase of the squares fills the pairs of SMs with them
+    const bool wide = tile_count(outer, 256) * p.batch >= sm_pairs();
+    return wide ? launch_ns<256>(p, buf, phases, first, done_count, st) : launch_ns<128>(p, buf, phases, first, done_count, st);
 }
 
 // Reads and clears the device fault word (synchronizes the device).

@@ -42,6 +42,7 @@ struct LinearEpilogue {
     int64_t ld_z;
     int dtype, act;
     int aligned;             // set by gemm_linear: rows of all arrays start on 16 bytes
+    int64_t out_batch;       // elements between the outputs of a batch (0: one output)
 };
 
 // A batch of matrices in a caller's memory: element (b, i, j) lies at
@@ -52,23 +53,28 @@ struct Strided {
     __host__ __device__ int64_t at(int64_t b, int64_t nb2) const { return (b / nb2) * b1 + (b % nb2) * b2; }
 };
 
-// Epilogue of a Newton-Schulz product: v = alpha * acc + beta * C[i, j], where
-// C is a 2-plane array, written as planes (mirrored when symmetric), or as the
-// last product's result: fin = v + keep * base.  Pitches are multiples of 8.
-struct PlanesEpilogue {
-    float alpha, beta;       // on the accumulator and on the planes' sum
-    const __half *c;         // NULL: no C
-    int64_t c_ld, c_plane, c_batch;
-    __half *out;             // planes out, or NULL
-    int64_t ld, plane, batch;
-    __half *out2;            // second planes output v * alpha2 + diag on the diagonal, or NULL
-    float alpha2, diag;
-    int64_t ld2, plane2, batch2;
-    Strided fin;             // final output (dtype), or no pointer
-    Strided base;            // fin = v + keep * base (fp32 only), or no pointer
+// The last Newton-Schulz product's result: out = v + keep * base.
+struct FinalOutput {
+    Strided out;             // of `dtype`
+    Strided base;            // fp32, or no pointer
     float keep;
     int64_t nb2;
     int dtype;
+};
+
+// The products of a Newton-Schulz run on the two-plane buffers below, in one
+// kernel.  X [lo, hi] holds scale_x * X at the start; A, B, Q, T are [lo, lo],
+// at scale_a (Q: scale_q).  gram 0: X <- a X + (b A + c A^2) X with A = X X^T,
+// X and X2 in turn.  gram 1: see muon.cu.  The result is factor * O.
+enum { kNsX = 0, kNsX2 = 1, kNsA = 2, kNsB = 3, kNsQ = 4, kNsQ2 = 5, kNsT = 6, kNsBuffers = 7 };
+struct NsBuffer {
+    __half *p;               // NULL: not used
+    int64_t ld, plane;       // the planes of one matrix follow each other, the matrices too
+};
+struct NsProgram {
+    int lo, hi, batch, steps, gram;
+    float a, b, c, scale_x, scale_a, scale_q, factor;
+    FinalOutput final;
 };
 
 struct GemmShape {
@@ -79,8 +85,11 @@ struct GemmShape {
 
 int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
                 cudaStream_t st);
-int gemm_planes(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const PlanesEpilogue &e,
-                cudaStream_t st);
+int ns_phases(int steps, int gram);
+// Bytes of `parts` (fp32 parts of A = X X^T, where the gram form splits it).
+size_t ns_parts_bytes(int64_t lo, int64_t hi, int64_t batch);
+// done_count: ns_phases * batch zeros.
+int ns_products(const NsProgram &p, const NsBuffer *buffers, int *done_count, float *parts, cudaStream_t st);
 
 // ---- activations -------------------------------------------------------------
 enum { kActNone = 0, kActRelu = 1, kActTanh = 2, kActSilu = 3, kActGelu = 4 };

@@ -82,9 +82,11 @@ __device__ __forceinline__ double block_sum(double v, double *scratch) {
 // batch).  Four columns a thread are in flight; the sums run in 64 bits, where
 // no square of an fp32 value overflows.
 template <typename T, bool MUON>
-__global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double *partial) {
+__global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double *partial, int *counts, int n_counts) {
     __shared__ double scratch[8];
     const int64_t b = blockIdx.y;
+    if (blockIdx.x == 0 && b == 0)  // the products' counters of finished tiles
+        for (int i = threadIdx.x; i < n_counts; i += blockDim.x) counts[i] = 0;
     const int64_t ub = s.u.at(b, s.nb2), mb = s.mom.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
     for (int64_t i = blockIdx.x; i < s.m; i += gridDim.x) {
@@ -169,9 +171,10 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
 }
 
 template <typename T, bool MUON>
-int normalize(const Source &s, bool turned, double eps, double *partial, int parts, __half *x, int64_t ld,
-              int64_t plane, cudaStream_t st) {
-    launch(square_sum_kernel<T, MUON>, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial);
+int normalize(const Source &s, bool turned, double eps, double *partial, int parts, int *counts, int n_counts, __half *x,
+              int64_t ld, int64_t plane, cudaStream_t st) {
+    launch(square_sum_kernel<T, MUON>, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial, counts,
+           n_counts);
     const dim3 grid(static_cast<unsigned>((s.n + 63) / 64), static_cast<unsigned>((s.m + 63) / 64),
                     static_cast<unsigned>(s.batch));
     if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
@@ -317,51 +320,15 @@ Range polynomial_range(double ca, double cb, double cc, int steps) {
     return r;
 }
 
-struct Planes {
-    __half *p;
-    int64_t ld, plane;
-    GemmOperand operand(int mn_major) const { return GemmOperand{p, ld, plane, 2 * plane, 2, mn_major}; }
-};
-Planes take_planes(Carve &ws, int64_t batch, int64_t rows, int64_t cols) {
-    Planes p;
-    p.ld = round8(cols);
-    p.plane = rows * p.ld;
-    p.p = ws.take<__half>(batch * 2 * p.plane);
-    return p;
+NsBuffer take_planes(Carve &ws, int64_t batch, int64_t rows, int64_t cols) {
+    NsBuffer b;
+    b.ld = round8(cols);
+    b.plane = rows * b.ld;
+    b.p = ws.take<__half>(batch * 2 * b.plane);
+    return b;
 }
 size_t planes_bytes(int64_t batch, int64_t rows, int64_t cols) {
     return carve_bytes<__half>(batch * 2 * rows * round8(cols));
-}
-
-GemmShape shape(int64_t m, int64_t n, int64_t k, int64_t batch, bool symmetric) {
-    GemmShape s;
-    s.m = m;
-    s.n = n;
-    s.k = k;
-    s.batch = batch;
-    s.symmetric = symmetric;
-    s.kind = kF16;
-    return s;
-}
-
-PlanesEpilogue epilogue(float alpha, const Planes *c, float beta, const Planes *out) {
-    PlanesEpilogue e{};
-    e.alpha = alpha;
-    if (c != nullptr) {
-        e.beta = beta;
-        e.c = c->p;
-        e.c_ld = c->ld;
-        e.c_plane = c->plane;
-        e.c_batch = 2 * c->plane;
-    }
-    if (out != nullptr) {
-        e.out = out->p;
-        e.ld = out->ld;
-        e.plane = out->plane;
-        e.batch = 2 * out->plane;
-    }
-    e.nb2 = 1;
-    return e;
 }
 
 Strided turn(Strided s, bool turned) {
@@ -396,91 +363,51 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     FL_REQUIRE(s.batch <= 65535 && (s.m + 63) / 64 <= 65535, "newton-schulz: too large a batch or matrix");
     Carve ws(wsp, ws_bytes);
     const int parts = parts_of(s.batch, s.m);
-    double *partial = ws.take<double>(s.batch * parts);
     const bool gram = use_gram(lo, hi, steps);
-    Planes x = take_planes(ws, s.batch, lo, hi), a = take_planes(ws, s.batch, lo, lo), b = take_planes(ws, s.batch, lo, lo);
-    Planes x2{}, q{}, q2{}, t{};
-    if (gram) {
-        q = take_planes(ws, s.batch, lo, lo);
-        q2 = take_planes(ws, s.batch, lo, lo);
-        t = take_planes(ws, s.batch, lo, lo);
-    } else {
-        x2 = take_planes(ws, s.batch, lo, hi);
+    const int n_counts = ns_phases(steps, gram) * static_cast<int>(s.batch);
+    double *partial = ws.take<double>(s.batch * parts);
+    int *counts = ws.take<int>(n_counts);
+    NsBuffer buf[kNsBuffers] = {};
+    bool fits = partial != nullptr && counts != nullptr;
+    for (int i = 0; i < kNsBuffers; ++i) {
+        if (gram ? i == kNsX2 : i >= kNsQ) continue;
+        buf[i] = take_planes(ws, s.batch, lo, i <= kNsX2 ? hi : lo);
+        fits = fits && buf[i].p != nullptr;
     }
-    FL_REQUIRE(partial && x.p && a.p && b.p && (gram ? t.p != nullptr : x2.p != nullptr), "newton-schulz: workspace too small");
-
+    const size_t part_bytes = gram ? ns_parts_bytes(lo, hi, s.batch) : 0;
+    float *outer_parts = part_bytes ? ws.take<float>(part_bytes / sizeof(float)) : nullptr;
+    FL_REQUIRE(fits && (part_bytes == 0 || outer_parts != nullptr), "newton-schulz: workspace too small");
+    const NsBuffer &x = buf[kNsX];
     int rc;
-    if (s.mom_out.ptr != nullptr) rc = normalize<float, true>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
-    else if (s.dtype == FL_F32) rc = normalize<float, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
-    else if (s.dtype == FL_F16) rc = normalize<__half, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
-    else rc = normalize<__nv_bfloat16, false>(s, turned, eps, partial, parts, x.p, x.ld, x.plane, st);
+    if (s.mom_out.ptr != nullptr)
+        rc = normalize<float, true>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+    else if (s.dtype == FL_F32)
+        rc = normalize<float, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+    else if (s.dtype == FL_F16)
+        rc = normalize<__half, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+    else
+        rc = normalize<__nv_bfloat16, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
     if (rc) return rc;
-
-    PlanesEpilogue last = epilogue(0.0f, nullptr, 0.0f, nullptr);
-    last.fin = turn(f.out, turned);
-    last.base = turn(f.base, turned);
-    last.keep = f.keep;
-    last.dtype = f.dtype;
-    last.nb2 = s.nb2;
-    const GemmShape square = shape(lo, lo, lo, s.batch, true);
-    // A = X X^T
-    const PlanesEpilogue to_a = epilogue(kScaleA / (kScaleX * kScaleX), nullptr, 0.0f, &a);
-    const GemmShape outer = shape(lo, lo, hi, s.batch, true);
-    if (!gram) {
-        for (int k = 0; k < steps && !rc; ++k) {
-            rc = gemm_planes(outer, x.operand(0), x.operand(0), to_a, st);
-            // B = b A + c A^2
-            if (!rc) rc = gemm_planes(square, a.operand(0), a.operand(0), epilogue(fc / kScaleA, &a, fb, &b), st);
-            if (rc) break;
-            // X <- a X + B X
-            if (k + 1 < steps) {
-                rc = gemm_planes(shape(lo, hi, lo, s.batch, false), b.operand(0), x.operand(1),
-                                 epilogue(1.0f / kScaleA, &x, fa, &x2), st);
-                const Planes u = x;
-                x = x2;
-                x2 = u;
-            } else {
-                PlanesEpilogue e = last;
-                const PlanesEpilogue c = epilogue(0.0f, &x, f.factor * fa / kScaleX, nullptr);
-                e.alpha = f.factor / (kScaleA * kScaleX);
-                e.beta = c.beta;
-                e.c = c.c;
-                e.c_ld = c.c_ld;
-                e.c_plane = c.c_plane;
-                e.c_batch = c.c_batch;
-                rc = gemm_planes(shape(lo, hi, lo, s.batch, false), b.operand(0), x.operand(1), e, st);
-            }
-        }
-        return rc;
-    }
-    // Gram form.  Q's scale leaves room for its largest factor (a^steps in the null space).
-    const float scale_q = exp2f(floorf(log2f(32768.0f / static_cast<float>(r.q))));
-    rc = gemm_planes(outer, x.operand(0), x.operand(0), to_a, st);
-    for (int k = 0; k < steps && !rc; ++k) {
-        PlanesEpilogue e = epilogue(fc / kScaleA, &a, fb, &b);  // B = b A + c A^2
-        if (k == 0) {                                           // and Q = a I + B
-            e.out2 = q.p;
-            e.ld2 = q.ld;
-            e.plane2 = q.plane;
-            e.batch2 = 2 * q.plane;
-            e.alpha2 = scale_q / kScaleA;
-            e.diag = fa * scale_q;
-        }
-        rc = gemm_planes(square, a.operand(0), a.operand(0), e, st);
-        if (!rc && k > 0) {  // Q <- a Q + B Q
-            rc = gemm_planes(square, b.operand(0), q.operand(0), epilogue(1.0f / kScaleA, &q, fa, &q2), st);
-            const Planes u = q;
-            q = q2;
-            q2 = u;
-        }
-        if (!rc && k + 1 < steps) {  // A <- P A P: T = a A + B A, A = a T + T B
-            rc = gemm_planes(square, b.operand(0), a.operand(0), epilogue(1.0f / kScaleA, &a, fa, &t), st);
-            if (!rc) rc = gemm_planes(square, t.operand(0), b.operand(0), epilogue(1.0f / kScaleA, &t, fa, &a), st);
-        }
-    }
-    if (rc) return rc;
-    last.alpha = f.factor / (scale_q * kScaleX);
-    return gemm_planes(shape(lo, hi, lo, s.batch, false), q.operand(0), x.operand(1), last, st);
+    NsProgram p{};
+    p.lo = static_cast<int>(lo);
+    p.hi = static_cast<int>(hi);
+    p.batch = static_cast<int>(s.batch);
+    p.steps = steps;
+    p.gram = gram;
+    p.a = fa;
+    p.b = fb;
+    p.c = fc;
+    p.scale_x = kScaleX;
+    p.scale_a = kScaleA;
+    // Q's scale leaves room for its largest factor (a^steps in the null space)
+    p.scale_q = exp2f(floorf(log2f(32768.0f / static_cast<float>(r.q))));
+    p.factor = f.factor;
+    p.final.out = turn(f.out, turned);
+    p.final.base = turn(f.base, turned);
+    p.final.keep = f.keep;
+    p.final.nb2 = s.nb2;
+    p.final.dtype = f.dtype;
+    return ns_products(p, buf, counts, outer_parts, st);
 }
 
 Strided strided(const fl_matrices *t) {
@@ -505,8 +432,10 @@ size_t fl_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n, int steps
     if (batch <= 0 || m <= 0 || n <= 0) return 0;
     const int64_t lo = m < n ? m : n, hi = m < n ? n : m;
     if (is_small(lo, hi, steps)) return 0;
-    size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + planes_bytes(batch, lo, hi) + 2 * planes_bytes(batch, lo, lo);
-    return b + (use_gram(lo, hi, steps) ? 3 * planes_bytes(batch, lo, lo) : planes_bytes(batch, lo, hi));
+    const bool gram = use_gram(lo, hi, steps);
+    size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + carve_bytes<int>(ns_phases(steps, gram) * batch);
+    b += (gram ? 1 : 2) * planes_bytes(batch, lo, hi) + (gram ? 5 : 2) * planes_bytes(batch, lo, lo);
+    return b + (gram ? ns_parts_bytes(lo, hi, batch) + 512 : 0);
 }
 
 int fl_orthogonalize(const fl_matrices *in, const fl_matrices *out, int64_t b1, int64_t b2, int64_t m, int64_t n,
