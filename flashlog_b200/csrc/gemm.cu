@@ -359,8 +359,8 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
 
 // What an epilogue warp keeps from chunk to chunk.
 struct EpiWarp {
-    float *stage;          // its staging tile (4 KB)
-    uint32_t bar, phase;   // its barrier for loads into the tile
+    float *stage;          // its staging tiles (4 KB each)
+    uint32_t bar, phase;   // their barriers for loads, 8 bytes apart, and a phase bit of each
     volatile int *failed;
     int lane;
 };
@@ -459,27 +459,26 @@ struct PlanesJob {
 __device__ __forceinline__ bool planes_wanted(const PlanesJob &p, int64_t row0, int64_t col0) {
     return !p.symmetric || col0 <= row0;
 }
-__device__ __forceinline__ void planes_load_c(const PlanesJob &p, EpiWarp &w, int b, int64_t row0, int64_t col0) {
+__device__ __forceinline__ void planes_load_c(const PlanesJob &p, EpiWarp &w, int tile, int b, int64_t row0, int64_t col0) {
     if (w.lane == 0) {
-        bar_expect(w.bar, 4096);
+        bar_expect(w.bar + 8 * tile, 4096);
         asm volatile(
             "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-            " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(w.stage)),
-            "l"(reinterpret_cast<uint64_t>(p.c)), "r"(w.bar), "r"(static_cast<int>(col0)),
+            " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(w.stage + 1024 * tile)),
+            "l"(reinterpret_cast<uint64_t>(p.c)), "r"(w.bar + 8 * tile), "r"(static_cast<int>(col0)),
             "r"(static_cast<int>(row0)), "r"(0), "r"(b) : "memory");
     }
 }
-// loaded: whether C of this chunk is on its way already
-__device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutput &f, float (&v)[32], EpiWarp &w, int b,
-                                             int64_t row0, int64_t col0, int64_t m, int64_t n, bool loaded) {
-    if (!planes_wanted(p, row0, col0)) return;
+// tile: the staging tile, into which C of this chunk has been asked for
+__device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutput &f, float (&v)[32], EpiWarp &w, int tile,
+                                             int b, int64_t row0, int64_t col0, int64_t m, int64_t n) {
     const int lane = w.lane;
-    unsigned char *stage = reinterpret_cast<unsigned char *>(w.stage);
+    float *tile_f = w.stage + 1024 * tile;
+    unsigned char *stage = reinterpret_cast<unsigned char *>(tile_f);
     const uint32_t s32 = smem_u32(stage);
     if (p.c != nullptr) {
-        if (!loaded) planes_load_c(p, w, b, row0, col0);
-        const bool ok = warp_wait(w.bar, w.phase, w.failed);
-        w.phase ^= 1;
+        const bool ok = warp_wait(w.bar + 8 * tile, (w.phase >> tile) & 1u, w.failed);
+        w.phase ^= 1u << tile;
         if (!ok) return;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -499,9 +498,9 @@ __device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutp
         for (int c = 0; c < 32; ++c) v[c] *= p.alpha;
     }
     if (p.out == nullptr) {
-        if (f.dtype == kOutF32) final_store<float>(f, v, w.stage, b, row0, col0, m, n, lane);
-        else if (f.dtype == kOutF16) final_store<__half>(f, v, w.stage, b, row0, col0, m, n, lane);
-        else final_store<__nv_bfloat16>(f, v, w.stage, b, row0, col0, m, n, lane);
+        if (f.dtype == kOutF32) final_store<float>(f, v, tile_f, b, row0, col0, m, n, lane);
+        else if (f.dtype == kOutF16) final_store<__half>(f, v, tile_f, b, row0, col0, m, n, lane);
+        else final_store<__nv_bfloat16>(f, v, tile_f, b, row0, col0, m, n, lane);
         // the staging tile is next written by a TMA load: order it behind these accesses
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -510,10 +509,10 @@ __device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutp
     const int row = static_cast<int>(row0), col = static_cast<int>(col0);
     if (p.symmetric && col == row) {
         // the tile on the diagonal: its upper half from the lower
-        stage_rows(w.stage, v, lane);
+        stage_rows(tile_f, v, lane);
         __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = w.stage[stage_at(max(c, lane), min(c, lane))];
+        for (int c = 0; c < 32; ++c) v[c] = tile_f[stage_at(max(c, lane), min(c, lane))];
         __syncwarp();
     }
 #pragma unroll 1
@@ -599,8 +598,9 @@ struct SingleWork {
         return j;
     }
     __device__ __forceinline__ bool wait(const Job &, Cursor &, volatile int *) const { return true; }
-    __device__ __forceinline__ void prepare(const Job &, EpiWarp &, int64_t, int64_t) const {}
-    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int64_t row0, int64_t col0, bool) const {
+    static constexpr int kTiles = 1;  // staging tiles per epilogue warp
+    __device__ __forceinline__ void ask(const Job &, EpiWarp &, int, int64_t, int64_t) const {}
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0) const {
         epi(v, w, j.batch_out, row0, col0, j.m, j.n);
     }
     __device__ __forceinline__ void done(const Job &, EpiWarp &) const {}
@@ -614,6 +614,7 @@ struct SingleWork {
 // blocks are resident (a cooperative launch), so the tile that a wait is for is
 // always being worked on or done.
 struct NsWork {
+    static constexpr int kTiles = 2;
     CUtensorMap ka[kNsBuffers], kb[kNsBuffers], pl[kNsBuffers], mn[2];
     NsProgram p;
     TileGrid sym, full;
@@ -770,14 +771,14 @@ struct NsWork {
         e.symmetric = !is_full(phase);
         return e;
     }
-    // Until the matrix' tiles of the phase before are complete (every epilogue
-    // warp of both CTAs counts once per tile).  All lanes call it.
+    // Until the matrix' tiles of the phase before are complete (both CTAs count
+    // each).  All lanes call it.
     __device__ __forceinline__ bool wait(const Job &j, Cursor &cur, volatile int *failed) const {
         const int phase = j.phase & 65535;
         if (phase == first) return true;
         const int at = (phase - 1) * p.batch + j.batch_out;
         if (cur.seen == at) return true;
-        const int want = tiles(phase - 1) * 2 * kEpiWarps;
+        const int want = tiles(phase - 1) * 2;
         uint64_t start = 0, now = 0;
         for (int i = 0;; ++i) {
             int have;
@@ -794,53 +795,58 @@ struct NsWork {
                 if (__any_sync(kFull, *failed != 0)) return false;
             }
         }
-        asm volatile("fence.proxy.async;" ::: "memory");  // the loads that follow go through the other proxy
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // the loads that follow go through the other proxy
         cur.seen = at;
         return true;
     }
-    __device__ __forceinline__ void prepare(const Job &j, EpiWarp &w, int64_t row0, int64_t col0) const {
+    // C of a chunk into a staging tile that is free
+    __device__ __forceinline__ void ask(const Job &j, EpiWarp &w, int tile, int64_t row0, int64_t col0) const {
         const PlanesJob e = planes(j);
-        if (e.c != nullptr && planes_wanted(e, row0, col0)) planes_load_c(e, w, j.batch_out, row0, col0);
+        if (e.c != nullptr && planes_wanted(e, row0, col0)) planes_load_c(e, w, tile, j.batch_out, row0, col0);
     }
-    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int64_t row0, int64_t col0,
-                                          bool loaded) const {
-        planes_chunk(planes(j), p.final, v, w, j.batch_out, row0, col0, j.m, j.n, loaded);
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int tile, int64_t row0,
+                                          int64_t col0) const {
+        const PlanesJob e = planes(j);
+        if (planes_wanted(e, row0, col0))
+            planes_chunk(e, p.final, v, w, tile, j.batch_out, row0, col0, j.m, j.n);
     }
-    // The tile's part of this warp is in memory: count it.
+    // The tile's part of this CTA is in memory: one count for all its epilogue warps.
     __device__ __forceinline__ void done(const Job &j, EpiWarp &w) const {
         const int phase = j.phase & 65535;
         if (phase == phases - 1) return;
-        if (w.lane == 0) {
-            asm volatile("cp.async.bulk.wait_group 0;\n fence.proxy.async;" ::: "memory");
-            __threadfence();
+        // a complete copy is visible to the thread that waited for it; the barrier and the release hand that on
+        if (w.lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+        if (threadIdx.x == 0)
             asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(done_count + phase * p.batch + j.batch_out)
                          : "memory");
-        }
-        __syncwarp();
     }
 };
 
 template <typename W> __device__ __forceinline__ int work_first(const W &) { return 0; }
 __device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 
-template <int BN, int PLANES>
+template <int BN, int PLANES, int TILES>
 struct Config {
     static constexpr int kA = kBM * kBK * 2;              // bytes of one plane of A per stage
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
     static constexpr int kStage = PLANES * (kA + kB);
-    static constexpr int kStages = kStageBudget / kStage > 8 ? 8 : kStageBudget / kStage;
-    static constexpr int kSmem = kStages * kStage + kEpiWarps * 32 * 32 * 4 + 1024;
+    // a second staging tile per epilogue warp, where three stages still fit next to it
+    static constexpr int kTiles = (kStageBudget - (TILES - 1) * kEpiWarps * 4096) / kStage >= 3 ? TILES : 1;
+    static constexpr int kFit = (kStageBudget - (kTiles - 1) * kEpiWarps * 4096) / kStage;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmem = kStages * kStage + kTiles * kEpiWarps * 4096 + 1024;
 };
 
 template <int BN, int PLANES, typename Work>
 __global__ __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 void gemm_kernel(const __grid_constant__ Work work) {
-    using C = Config<BN, PLANES>;
+    using C = Config<BN, PLANES, Work::kTiles>;
     extern __shared__ unsigned char raw[];
     // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
     unsigned char *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float *stage_epi = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
-    __shared__ uint64_t bars[2 * C::kStages + 4 + kEpiWarps];
+    __shared__ uint64_t bars[2 * C::kStages + 4 + C::kTiles * kEpiWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
@@ -851,7 +857,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::kStages, acc_full = empty + 8 * C::kStages,
                    acc_empty = acc_full + 16;
 
-    if (threadIdx.x < 2 * C::kStages + 4 + kEpiWarps) {
+    if (threadIdx.x < 2 * C::kStages + 4 + C::kTiles * kEpiWarps) {
         const int i = threadIdx.x, k = i - (2 * C::kStages + 2);
         // accumulator buffers free: every epilogue warp of both CTAs arrives
         bar_init(full + 8 * i, k == 0 || k == 1 ? 2 * kEpiWarps : 1);
@@ -964,7 +970,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        EpiWarp w{stage_epi + warp * 32 * 32, acc_empty + 16 + 8 * warp, 0, &failed, lane};
+        EpiWarp w{stage_epi + warp * C::kTiles * 1024, acc_empty + 16 + 8 * warp * C::kTiles, 0, &failed, lane};
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -975,7 +981,9 @@ void gemm_kernel(const __grid_constant__ Work work) {
             const bool any = row0 < j.m && j.col + half < j.n;
             if (ok && any) {
                 ok = work.wait(j, cur, &failed);  // (long met: the loads waited for it; here for this warp's own loads)
-                if (ok) work.prepare(j, w, row0, j.col + half);
+#pragma unroll
+                for (int q = 0; q < C::kTiles; ++q)
+                    if (ok && j.col + half + 32 * q < j.n) work.ask(j, w, q, row0, j.col + half + 32 * q);
             }
             if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -990,8 +998,10 @@ void gemm_kernel(const __grid_constant__ Work work) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
                 }
-                work.chunk(j, v, w, row0, j.col + c, c == half);
+                const int tile = ((c - half) >> 5) % C::kTiles, next = c + 32 * C::kTiles;
+                work.chunk(j, v, w, tile, row0, j.col + c);
                 __syncwarp();
+                if (ok && next < half + BN / 2 && j.col + next < j.n) work.ask(j, w, tile, row0, j.col + next);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -1118,8 +1128,8 @@ uint32_t instruction_types(int kind) {
 
 template <int BN, int PLANES, typename Epi>
 int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Epi &epi, int splits, cudaStream_t st) {
-    using C = Config<BN, PLANES>;
     using W = SingleWork<Epi>;
+    using C = Config<BN, PLANES, W::kTiles>;
     W w;
     int rc = operand_map(&w.map_a, a, s.m, s.k, s.batch, kBM, s.kind);
     if (rc) return rc;
@@ -1176,7 +1186,7 @@ int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b,
 
 template <int BN>
 int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, int *done_count, cudaStream_t st) {
-    using C = Config<BN, 2>;
+    using C = Config<BN, 2, NsWork::kTiles>;
     NsWork w{};
     w.p = p;
     w.phases = phases;
