@@ -119,6 +119,43 @@ __global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double 
     if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = total;
 }
 
+// Pass 1 of a plain update whose rows are contiguous and start on 16 bytes: a
+// warp per row, four 16-byte loads in flight per lane.
+template <typename T>
+__global__ void __launch_bounds__(256) square_sum_rows_kernel(const Source s, double *partial, int *counts, int n_counts) {
+    constexpr int kPer = 16 / sizeof(T);
+    __shared__ double scratch[8];
+    const int64_t b = blockIdx.y;
+    if (blockIdx.x == 0 && b == 0)
+        for (int i = threadIdx.x; i < n_counts; i += blockDim.x) counts[i] = 0;
+    const int lane = threadIdx.x & 31;
+    const T *base = static_cast<const T *>(s.u.ptr) + s.u.at(b, s.nb2);
+    const int pieces = static_cast<int>(s.n / kPer);
+    double sum[2] = {0.0, 0.0};
+    for (int64_t i = blockIdx.x * int64_t(8) + (threadIdx.x >> 5); i < s.m; i += gridDim.x * int64_t(8)) {
+        const T *row = base + i * s.u.i;
+        for (int q0 = lane; q0 < pieces; q0 += 128) {
+            union { uint4 u; T t[kPer]; } x[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                x[q].u = q0 + 32 * q < pieces ? reinterpret_cast<const uint4 *>(row)[q0 + 32 * q] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    const double v = to_f32(x[q].t[e]);
+                    sum[e & 1] = fma(v, v, sum[e & 1]);
+                }
+        }
+        for (int64_t j = pieces * kPer + lane; j < s.n; j += 32) {
+            const double v = to_f32(row[j]);
+            sum[0] = fma(v, v, sum[0]);
+        }
+    }
+    const double total = block_sum(sum[0] + sum[1], scratch);
+    if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = total;
+}
+
 // Pass 2: planes of X * 2^13, turned to [short, long]: 64 x 64 tiles, grid
 // (tiles of j, tiles of i, batch); a lane holds two neighbours, so rows are
 // written in whole cache lines.
@@ -126,19 +163,38 @@ template <typename T, bool MUON, bool TURNED>
 __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const double *partial, int parts, double eps,
                                                         __half *out, int64_t ld, int64_t plane) {
     __shared__ double scratch[8];
-    __shared__ float tile[TURNED ? 64 : 1][65];
+    // rows of 66 words, pairs of columns exchanged in every other 16 rows: pairs are written in one
+    // access, and a column is read with at most two rows to a bank
+    __shared__ __align__(8) float tile[TURNED ? 64 * 66 : 1];
+    auto at = [](int r, int c) { return r * 66 + (c ^ (((r >> 4) & 1) << 1)); };
     const int64_t b = blockIdx.z;
     const int64_t ub = s.u.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
     const int64_t i0 = blockIdx.y * int64_t(64), j0 = blockIdx.x * int64_t(64);
+    constexpr bool kApart = TURNED && sizeof(T) == 4;
     float v[8][2];
+    if (sizeof(T) == 2 && s.u.j == 1 && ((reinterpret_cast<uintptr_t>(s.u.ptr) | s.u.i * 2 | ub * 2) & 3) == 0) {
+        // 16-bit pairs
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + 2 * threadIdx.x;
+            union { unsigned u; T t[4 / sizeof(T)]; } x;
+            x.u = 0u;
+            const T *p = static_cast<const T *>(s.u.ptr) + ub + i * s.u.i + j;
+            if (i < s.m && j + 1 < s.n) x.u = *reinterpret_cast<const unsigned *>(p);
+            else if (i < s.m && j < s.n) x.t[0] = p[0];
+            v[k][0] = to_f32(x.t[0]);
+            v[k][1] = to_f32(x.t[sizeof(T) == 2 ? 1 : 0]);
+        }
+    } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            // turned tiles are read a lane per element (they turn in shared memory), others two neighbours a lane
-            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (TURNED ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
+            // two neighbours a lane; turned 32-bit tiles a lane per element (they turn in shared memory)
+            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (kApart ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
             v[k][w] = i < s.m && j < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i, j) : 0.0f;
         }
+    }
     double sum = 0.0;
     for (int p = threadIdx.y * 32 + threadIdx.x; p < parts; p += 256) sum += partial[b * parts + p];
     sum = warp_sum(sum);
@@ -150,9 +206,16 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     __half *hi = out + b * 2 * plane;
     if (TURNED) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) tile[threadIdx.y + 8 * k][threadIdx.x + 32 * w] = static_cast<float>(v[k][w] * scale);
+        for (int k = 0; k < 8; ++k) {
+            const int r = threadIdx.y + 8 * k;
+            const float x = static_cast<float>(v[k][0] * scale), y = static_cast<float>(v[k][1] * scale);
+            if (kApart) {
+                tile[at(r, threadIdx.x)] = x;
+                tile[at(r, threadIdx.x + 32)] = y;
+            } else {
+                *reinterpret_cast<float2 *>(&tile[at(r, 2 * threadIdx.x)]) = make_float2(x, y);
+            }
+        }
         __syncthreads();
     }
     const int64_t rows = TURNED ? s.n : s.m, cols = TURNED ? s.m : s.n, r0 = TURNED ? j0 : i0, c0 = TURNED ? i0 : j0;
@@ -160,8 +223,8 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     for (int k = 0; k < 8; ++k) {
         const int64_t r = r0 + threadIdx.y + 8 * k, c = c0 + 2 * threadIdx.x;
         if (r >= rows || c >= cols) continue;
-        const float a = TURNED ? tile[2 * threadIdx.x][threadIdx.y + 8 * k] : static_cast<float>(v[k][0] * scale);
-        const float z = TURNED ? tile[2 * threadIdx.x + 1][threadIdx.y + 8 * k] : static_cast<float>(v[k][1] * scale);
+        const float a = TURNED ? tile[at(2 * threadIdx.x, threadIdx.y + 8 * k)] : static_cast<float>(v[k][0] * scale);
+        const float z = TURNED ? tile[at(2 * threadIdx.x + 1, threadIdx.y + 8 * k)] : static_cast<float>(v[k][1] * scale);
         __half2 h, l;
         split_pair(a, z, h, l);
         // the pitch is a multiple of 8 and at least cols: the pair fits in the row
@@ -173,8 +236,12 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
 template <typename T, bool MUON>
 int normalize(const Source &s, bool turned, double eps, double *partial, int parts, int *counts, int n_counts, __half *x,
               int64_t ld, int64_t plane, cudaStream_t st) {
-    launch(square_sum_kernel<T, MUON>, dim3(parts, static_cast<unsigned>(s.batch)), 256, 0, st, s, partial, counts,
-           n_counts);
+    const int64_t size = sizeof(T);
+    const bool rows = !MUON && s.u.j == 1 && reinterpret_cast<uintptr_t>(s.u.ptr) % 16 == 0 && s.u.i * size % 16 == 0 &&
+                      s.u.b1 * size % 16 == 0 && s.u.b2 * size % 16 == 0;
+    const dim3 parts_grid(parts, static_cast<unsigned>(s.batch));
+    if (rows) launch(square_sum_rows_kernel<T>, parts_grid, 256, 0, st, s, partial, counts, n_counts);
+    else launch(square_sum_kernel<T, MUON>, parts_grid, 256, 0, st, s, partial, counts, n_counts);
     const dim3 grid(static_cast<unsigned>((s.n + 63) / 64), static_cast<unsigned>((s.m + 63) / 64),
                     static_cast<unsigned>(s.batch));
     if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
@@ -204,6 +271,7 @@ __device__ __forceinline__ void small_product(const float *A, int lda, const flo
         const int i0 = t / ch, j0 = t - i0 * ch, i1 = i0 + rh, j1 = j0 + ch;
         const int i1c = i1 < rows ? i1 : i0, j1c = j1 < cols ? j1 : j0;
         float s00 = 0.0f, s01 = 0.0f, s10 = 0.0f, s11 = 0.0f;
+#pragma unroll 8
         for (int k = 0; k < depth; ++k) {
             const float a0 = A[i0 * lda + k], a1 = A[i1c * lda + k];
             const float b0 = B_T ? B[j0 * ldb + k] : B[k * ldb + j0], b1 = B_T ? B[j1c * ldb + k] : B[k * ldb + j1c];
