@@ -5,6 +5,7 @@ The names exported here are those of the reference package
 kernels behind the C ABI of include/flashlog_b200.h.
 """
 from . import dropout, filters, readout  # noqa: F401  (value dropout; filter keys; channel readouts)
+from . import attention, muon  # noqa: F401  (relation head and weights; orthogonalised updates)
 from .flashlog_kernel import (  # noqa: F401
     FlashLogDenseMaxFunction,
     FlashLogDenseSumFunction,

@@ -196,7 +196,7 @@ SIGNATURES = {
     "fl_orthogonalize": (ctypes.c_int, [_MATRICES, _MATRICES, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int,
                                         _D, _D, _D, _D, _P, _SZ, _P]),
     "fl_muon_update": (ctypes.c_int, [_MATRICES, _MATRICES, _MATRICES, _MATRICES, _MATRICES, _I64, _I64, _I64, _I64,
-                                      _D, _D, ctypes.c_int, _D, _D, ctypes.c_int, _D, _D, _D, _D, _P, _SZ, _P]),
+                                      _D, _D, ctypes.c_int, _D, _D, ctypes.c_int, _D, _D, _D, _D, _P, _P, _SZ, _P]),
     "fl_gemm_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
 }
 

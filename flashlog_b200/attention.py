@@ -15,6 +15,8 @@ backward, and can be captured in a CUDA graph.
 """
 from __future__ import annotations
 
+import dataclasses
+
 import torch
 from torch import autograd
 from torch.autograd.function import once_differentiable
@@ -165,3 +167,58 @@ def relation_weights(logits, *, tau: float = 1.0, mask=None, states=None, bias=N
     else:
         w = ops.relation_weights(z, bias, mask, states, history, tau, repetition, frequency, presence)
     return w if logits.dim() == 2 else w.view(logits.shape)
+
+
+@dataclasses.dataclass
+class OperatorRules:
+    """What the attention of T hops may take, for engine.drum_propagate and
+    step.DrumTrainStep (relation_weights applied to every query's channels):
+
+    mask    bool or uint8 [S, n] with states int64 [T, Q]: the operators
+            allowed in each state, and each query's state at each hop
+    history int64 [Q, H]: operators that count as used (such as the query's
+            own relation, to keep it out of its own rule)
+    bias    [n], added to every query's logits
+    repetition, frequency, presence: the penalties of used operators
+
+    The step reads these tensors on every run: a captured step follows
+    changes made to them in place."""
+
+    mask: torch.Tensor | None = None
+    states: torch.Tensor | None = None
+    history: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+    repetition: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+
+    def check(self, T: int, Q: int, n: int):
+        """Raise unless the tensors fit T hops of Q queries and n operators."""
+        if (self.mask is None) != (self.states is None):
+            raise ValueError("operator rules: mask and states come together")
+        if self.mask is not None:
+            if self.mask.dim() != 2 or self.mask.shape[1] != n or self.mask.dtype not in (torch.bool, torch.uint8):
+                raise ValueError(f"operator rules: mask must be bool or uint8 [states, {n}]")
+            if tuple(self.states.shape) != (T, Q) or self.states.dtype != torch.int64:
+                raise ValueError(f"operator rules: states must be int64 [{T}, {Q}]")
+        if self.history is not None and (self.history.dim() != 2 or self.history.shape[0] != Q or
+                                         self.history.dtype != torch.int64):
+            raise ValueError(f"operator rules: history must be int64 [{Q}, H]")
+        if self.history is not None and self.history.shape[1] > ops.MAX_HISTORY:
+            raise ValueError(f"operator rules: at most {ops.MAX_HISTORY} history entries")
+        if self.bias is not None and (tuple(self.bias.shape) != (n,) or self.bias.dtype != torch.float32):
+            raise ValueError(f"operator rules: bias must be float32 [{n}]")
+        if not (1e-30 < self.repetition < 1e30 and abs(self.frequency) < 1e30 and abs(self.presence) < 1e30):
+            raise ValueError("operator rules: repetition must be positive and the penalties finite")
+
+    def rows(self, t: int, N: int):
+        """Keyword arguments of relation_weights for hop t's rows r = q * N + channel."""
+        kw = dict(repetition=self.repetition, frequency=self.frequency, presence=self.presence)
+        if self.mask is not None:
+            kw["mask"] = ops._lines(self.mask)
+            kw["states"] = self.states[t][:, None].expand(-1, N).reshape(-1)
+        if self.history is not None and self.history.shape[1] > 0:
+            kw["history"] = self.history[:, None, :].expand(-1, N, -1).reshape(-1, self.history.shape[1])
+        if self.bias is not None:
+            kw["bias"] = self.bias.contiguous()
+        return kw

@@ -412,6 +412,7 @@ __device__ __forceinline__ void final_store(const FinalOutput &e, const float (&
                                             int64_t row0, int64_t col0, int64_t m, int64_t n, int lane) {
     T *out = static_cast<T *>(e.out.ptr) + e.out.at(b, e.nb2);
     const float *base = e.base.ptr != nullptr ? static_cast<const float *>(e.base.ptr) + e.base.at(b, e.nb2) : nullptr;
+    const bool closed = e.gate != nullptr && *e.gate == 0.0f;
     const bool by_row = e.out.i == 1;  // lane = row is the contiguous direction
     if (!by_row) {
         stage_rows(stage, v, lane);
@@ -435,7 +436,7 @@ __device__ __forceinline__ void final_store(const FinalOutput &e, const float (&
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             x[k] = by_row ? v[l0 + k] : stage[stage_at(l0 + k, lane)];
-            if (base != nullptr) x[k] = fmaf(e.keep, b0[k], x[k]);
+            if (base != nullptr) x[k] = closed ? b0[k] : fmaf(e.keep, b0[k], x[k]);
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)

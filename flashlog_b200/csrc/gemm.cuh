@@ -57,6 +57,7 @@ struct Strided {
 struct FinalOutput {
     Strided out;             // of `dtype`
     Strided base;            // fp32, or no pointer
+    const float *gate;       // where it holds 0, out = base; or NULL
     float keep;
     int64_t nb2;
     int dtype;

@@ -45,6 +45,7 @@ struct Source {
     Strided u;          // the update itself (dtype), or the gradient of a Muon step (fp32)
     Strided mom;        // momentum in (no pointer: a plain update)
     Strided mom_out;
+    const float *gate;  // where it holds 0, momentum and parameter stay as they are; or NULL
     float beta;
     int nesterov, dtype;
     int64_t batch, nb2, m, n;
@@ -59,7 +60,8 @@ __device__ __forceinline__ float update_at(const Source &s, int64_t ub, int64_t 
     float *out = static_cast<float *>(s.mom_out.ptr) + ob + i * s.mom_out.i + j * s.mom_out.j;
     float v;
     if (FIRST) {
-        v = fmaf(s.beta, static_cast<const float *>(s.mom.ptr)[mb + i * s.mom.i + j * s.mom.j], g);
+        const float old = static_cast<const float *>(s.mom.ptr)[mb + i * s.mom.i + j * s.mom.j];
+        v = s.gate != nullptr && *s.gate == 0.0f ? old : fmaf(s.beta, old, g);
         *out = v;
     } else {
         v = *out;
@@ -87,6 +89,7 @@ __global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double 
     const int64_t b = blockIdx.y;
     if (blockIdx.x == 0 && b == 0)  // the products' counters of finished tiles
         for (int i = threadIdx.x; i < n_counts; i += blockDim.x) counts[i] = 0;
+    const bool closed = s.gate != nullptr && *s.gate == 0.0f;
     const int64_t ub = s.u.at(b, s.nb2), mb = s.mom.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
     double sum[4] = {0.0, 0.0, 0.0, 0.0};
     for (int64_t i = blockIdx.x; i < s.m; i += gridDim.x) {
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(256) square_sum_kernel(const Source s, double 
                 const int64_t j = j0 + 256 * q;
                 float u = g[q];
                 if (MUON) {
-                    v[q] = fmaf(s.beta, v[q], g[q]);
+                    if (!closed) v[q] = fmaf(s.beta, v[q], g[q]);
                     if (j < s.n) po[j * s.mom_out.j] = v[q];
                     u = s.nesterov ? fmaf(s.beta, v[q], g[q]) : v[q];
                 }
@@ -250,7 +253,8 @@ int normalize(const Source &s, bool turned, double eps, double *partial, int par
 }
 
 struct Finish {
-    Strided out, base;  // out = factor * O + keep * base
+    Strided out, base;  // out = factor * O + keep * base, or base where the gate is closed
+    const float *gate;
     float factor, keep;
     int dtype;
 };
@@ -329,8 +333,10 @@ __global__ void __launch_bounds__(512) small_kernel(const Source s, const Finish
     for (int t = threadIdx.x; t < m * n; t += blockDim.x) {
         const int i = t / n, j = t - i * n;
         float v = f.factor * X[turned ? j * ldx + i : i * ldx + j];
-        if (f.base.ptr != nullptr)
-            v = fmaf(f.keep, static_cast<const float *>(f.base.ptr)[bb + i * f.base.i + j * f.base.j], v);
+        if (f.base.ptr != nullptr) {
+            const float old = static_cast<const float *>(f.base.ptr)[bb + i * f.base.i + j * f.base.j];
+            v = f.gate != nullptr && *f.gate == 0.0f ? old : fmaf(f.keep, old, v);
+        }
         store_any(f.out.ptr, fb + i * f.out.i + j * f.out.j, v, f.dtype);
     }
 }
@@ -472,6 +478,7 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     p.factor = f.factor;
     p.final.out = turn(f.out, turned);
     p.final.base = turn(f.base, turned);
+    p.final.gate = f.gate;
     p.final.keep = f.keep;
     p.final.nb2 = s.nb2;
     p.final.dtype = f.dtype;
@@ -531,7 +538,8 @@ int fl_orthogonalize(const fl_matrices *in, const fl_matrices *out, int64_t b1, 
 int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_matrices *momentum,
                    const fl_matrices *param_out, const fl_matrices *momentum_out, int64_t b1, int64_t b2, int64_t m,
                    int64_t n, double lr, double beta, int nesterov, double weight_decay, double scale, int steps,
-                   double a, double b, double c, double eps, void *ws, size_t ws_bytes, fl_stream_t stream) {
+                   double a, double b, double c, double eps, const float *gate, void *ws, size_t ws_bytes,
+                   fl_stream_t stream) {
     int rc = check_batch(b1, b2, m, n, steps);
     if (rc) return rc;
     if (b1 * b2 == 0) return FL_OK;
@@ -542,6 +550,7 @@ int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_m
     s.u = strided(grad);
     s.mom = strided(momentum);
     s.mom_out = strided(momentum_out);
+    s.gate = gate;
     s.beta = static_cast<float>(beta);
     s.nesterov = nesterov;
     s.dtype = FL_F32;
@@ -552,6 +561,7 @@ int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_m
     Finish f{};
     f.out = strided(param_out);
     f.base = strided(param);
+    f.gate = gate;
     f.factor = static_cast<float>(-lr * scale);
     f.keep = static_cast<float>(1.0 - lr * weight_decay);
     f.dtype = FL_F32;

@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from . import ops
+from . import attention, ops
 from .ops import Graph
 
 
@@ -112,8 +112,14 @@ def check_status(status):
 
 
 def drum_propagate(heads, w_all, graph: Graph, r_size: int, *, c1=None, c2=0, mask_triple=None, tau_1=1.0,
-                   eps=1e-7, stats=None, status=None, dropout=0.0, dropout_seed=None, dropout_counter=0):
+                   eps=1e-7, stats=None, status=None, dropout=0.0, dropout_seed=None, dropout_counter=0, head=None,
+                   rules=None):
     """T hops of the sparse DRUM operator; w_all is [Q, T, N, n] logits.
+
+    head (weight [n, H], bias [n] or None): w_all is [Q, T, N, H] hidden
+    states, and the logits are attention.linear of them.  rules
+    (attention.OperatorRules): what the hops' weights may take; a query whose
+    rules leave nothing propagates nothing.
 
     dropout > 0: the training dropout of each hop's values
     (src/model_DRUM_kernel_sp.py:189-192), hop t drawing its keep bits from
@@ -123,7 +129,11 @@ def drum_propagate(heads, w_all, graph: Graph, r_size: int, *, c1=None, c2=0, ma
     Returns the final state (row_ptr, ent, val) with capacity-sized ent/val
     (live count row_ptr[-1]).
     """
+    if head is not None:
+        w_all = attention.linear(w_all, head[0], head[1])
     Q, T, N, n = w_all.shape
+    if rules is not None:
+        rules.check(T, Q, n)
     row_ptr, ent, val = initial_state(heads, N)
     topk = c2 // 2 if c2 and c2 > 0 else L.NO_BUDGET
     flags = L.FL_SKIP_NONPOS_W | L.FL_DROP_MASKED
@@ -138,7 +148,10 @@ def drum_propagate(heads, w_all, graph: Graph, r_size: int, *, c1=None, c2=0, ma
         drop = (float(dropout), draw_seed() if dropout_seed is None else int(dropout_seed),
                 device_counter(dropout_counter, heads.device))
     for t in range(T):
-        w_t = torch.softmax(w_all[:, t] / tau_1, dim=-1)
+        if rules is None:
+            w_t = torch.softmax(w_all[:, t] / tau_1, dim=-1)
+        else:
+            w_t = attention.relation_weights(w_all[:, t].reshape(Q * N, n), tau=tau_1, **rules.rows(t, N)).view(Q, N, n)
         val, row_ptr, ent = HopNorm.apply(val, w_t, row_ptr, ent, graph, r_size, topk, c1, flags, mask_triple, eps,
                                           stats, status, vis, drop is not None)
         if drop is not None:

@@ -57,7 +57,7 @@ def union_rows(rels: torch.Tensor, n_rows: int, group=None) -> torch.Tensor:
 
 
 def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: float, comm_stream=None,
-                                        group=None, rows=None):
+                                        group=None, rows=None, update=None, extra_grads=()):
     """One training step given as parts (DrumTrainStep.parts(), or replays of
     their CUDA graphs): after part j < T has been issued, hop T-1-j's table
     gradient grad_hop[T-1-j] is complete and its all-reduce (sum) is issued
@@ -67,7 +67,10 @@ def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: 
     rows (union_rows of the step): only those rows of each hop's gradient are
     all-reduced, gathered into a compact buffer and written back, and only
     those rows of the table are updated; the other rows are zero on every
-    rank, so the result is the same."""
+    rank, so the result is the same.  update (a callable such as
+    DrumTrainStep.update): called in the place of that SGD step, once the
+    hops' gradients and extra_grads (DrumTrainStep.grad_head) hold their mean
+    over the ranks."""
     world = dist.get_world_size(group)
     T = len(grad_hop)
 
@@ -92,6 +95,15 @@ def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: 
     if world > 1:
         if comm_stream is not None:
             torch.cuda.current_stream().wait_stream(comm_stream)
+    if update is not None:
+        if world > 1:
+            for g in grad_hop:
+                g.div_(world)
+            for g in extra_grads:
+                if g is not None:
+                    allreduce_mean_(g, group)
+        update()
+    elif world > 1:
         if rows is None:
             table.sub_(table_grad, alpha=lr / world)
         else:

@@ -57,6 +57,11 @@ def orthogonalize(update, steps: int = 5, coefficients=COEFFICIENTS, eps: float 
     return ops.orthogonalize(update, steps, coefficients, eps)
 
 
+def _check_gate(gate):
+    if gate is not None and (gate.dtype != torch.float32 or gate.numel() != 1):
+        raise ValueError("muon_update: gate must be one float32")
+
+
 def _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps):
     _check_matrix("muon_update", param)
     for name, t in (("param", param), ("grad", grad), ("momentum", momentum)):
@@ -89,27 +94,32 @@ def _overlaps_itself(t):
 
 @torch.no_grad()
 def muon_update(param, grad, momentum, *, lr: float, beta: float = 0.95, nesterov: bool = True,
-                weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
+                weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
+                gate=None):
     """One Muon step of param [..., m, n] (a batch of matrices), all fp32:
 
         momentum' = beta * momentum + grad;  U = grad + beta * momentum' (nesterov) or momentum'
         param' = param * (1 - lr * weight_decay) - lr * scale * orthogonalize(U)
 
-    scale defaults to sqrt(max(1, m / n)).  Returns (param', momentum') as new tensors."""
+    scale defaults to sqrt(max(1, m / n)).  gate (a float32 on the device): where it holds 0 -- a step that
+    failed, found on the device -- both come out as they went in.  Returns (param', momentum') as new tensors."""
+    _check_gate(gate)
     args = _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps)
     p2, m2 = torch.empty_like(param), torch.empty_like(momentum)
-    ops.muon_update(param, grad, momentum, p2, m2, nesterov=bool(nesterov), **args)
+    ops.muon_update(param, grad, momentum, p2, m2, nesterov=bool(nesterov), gate=gate, **args)
     return p2, m2
 
 
 @torch.no_grad()
 def muon_update_(param, grad, momentum, *, lr: float, beta: float = 0.95, nesterov: bool = True,
-                 weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7):
+                 weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
+                 gate=None):
     """muon_update in place: param and momentum are overwritten; returns param."""
+    _check_gate(gate)
     args = _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps)
     if _overlaps_itself(param) or _overlaps_itself(momentum):
         raise ValueError("muon_update_: param and momentum must not overlap themselves")
-    ops.muon_update(param, grad, momentum, param, momentum, nesterov=bool(nesterov), **args)
+    ops.muon_update(param, grad, momentum, param, momentum, nesterov=bool(nesterov), gate=gate, **args)
     return param
 
 

@@ -720,18 +720,18 @@ def _linear_params(x, weight, bias, residual, act):
                        0 if residual is None else _ld(residual), x.shape[0], n, k, FL_DTYPE[x.dtype], act)
 
 
-def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE, want_z: bool = False):
+def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE, want_z: bool = False, out=None):
     """y = act(x W^T + bias) + residual of [rows, k] and [n, k] matrices of one
-    dtype; with want_z also the fp32 pre-activation (None without an
-    activation).  Returns (y, z)."""
-    dev = _one_device("linear", x, weight, bias, residual)
+    dtype (into out, when given: contiguous); with want_z also the fp32
+    pre-activation (None without an activation).  Returns (y, z)."""
+    dev = _one_device("linear", x, weight, bias, residual, out)
     x, weight = _lines(x), _lines(weight)
     if bias is not None:
         bias = bias.contiguous()
     if residual is not None:
         residual = _lines(residual)
     rows, n = x.shape[0], weight.shape[0]
-    y = x.new_empty((rows, n))
+    y = x.new_empty((rows, n)) if out is None else out
     z = x.new_empty((rows, n), dtype=torch.float32) if want_z and act != L.FL_ACT_NONE else None
     if rows == 0:
         return y, z
@@ -773,12 +773,13 @@ def _weights_params(logits, bias, mask, states, history, tau, repetition, freque
 
 
 def relation_weights(logits, bias=None, mask=None, states=None, history=None, tau=1.0, repetition=1.0, frequency=0.0,
-                     presence=0.0):
+                     presence=0.0, out=None):
     """fl_relation_weights on 2-D tensors: logits [rows, n] (unit inner
     stride), bias [n] or [rows, n], mask bool or uint8 [states, n], states
-    int64 [rows], history int64 [rows, H].  Returns f32 [rows, n]."""
-    dev = _one_device("relation weights", logits, bias, mask, states, history)
-    w = logits.new_empty(logits.shape, dtype=torch.float32)
+    int64 [rows], history int64 [rows, H].  Returns f32 [rows, n] (out, when
+    given: contiguous)."""
+    dev = _one_device("relation weights", logits, bias, mask, states, history, out)
+    w = logits.new_empty(logits.shape, dtype=torch.float32) if out is None else out
     if w.numel() == 0:
         return w
     p = _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence)
@@ -853,9 +854,9 @@ def orthogonalize(update, steps: int, coefficients, eps: float):
 
 
 def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nesterov, weight_decay, scale, steps,
-                coefficients, eps):
+                coefficients, eps, gate=None):
     """fl_muon_update of fp32 tensors [..., m, n] of one shape, into the two outputs."""
-    dev = _one_device("muon_update", param, grad, momentum, param_out, momentum_out)
+    dev = _one_device("muon_update", param, grad, momentum, param_out, momentum_out, gate)
     if param.numel() == 0:
         return
     got = _as_batch((param, grad, momentum, param_out, momentum_out))
@@ -863,7 +864,7 @@ def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nes
         p2, m2 = (t.new_empty(t.shape) for t in (param_out, momentum_out))
         muon_update(param.contiguous(), grad.contiguous(), momentum.contiguous(), p2, m2, lr=lr, beta=beta,
                     nesterov=nesterov, weight_decay=weight_decay, scale=scale, steps=steps,
-                    coefficients=coefficients, eps=eps)
+                    coefficients=coefficients, eps=eps, gate=gate)
         param_out.copy_(p2)
         momentum_out.copy_(m2)
         return
@@ -872,7 +873,7 @@ def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nes
     nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
     ws = _workspace(nbytes, param)
     _call(dev, "muon_update", lib().fl_muon_update, *(ctypes.byref(t) for t in ts), b1, b2, m, n, lr, beta,
-          int(nesterov), weight_decay, scale, steps, *coefficients, eps, _ptr(ws), nbytes)
+          int(nesterov), weight_decay, scale, steps, *coefficients, eps, _ptr(gate), _ptr(ws), nbytes)
 
 
 def gemm_fault() -> bool:

@@ -35,6 +35,7 @@ import math
 import torch
 
 from . import _lib as L
+from . import muon, ops
 from .ops import Graph, _p, _stream, check, lib
 
 
@@ -88,12 +89,22 @@ class DrumTrainStep:
     A step whose forward overflowed a buffer (status word nonzero) leaves
     the table and the gradient untouched (the gradient is scaled by 0 on the
     device); `check` then raises.
+
+    head (weight [n, H], bias [n] or None): the table is [2R, T, N, H] hidden
+    states, and a hop's logits are attention.linear of the queries' rows; the
+    head is trained too (its gradients in grad_head).  rules
+    (attention.OperatorRules): what the weights may take; its bias is not
+    trained.  optimizer "muon": the table's T N matrices [2R, n or H] and the
+    head's weight take muon.muon_update_ steps (muon_options: beta, nesterov,
+    weight_decay, scale, steps, coefficients, eps) with momentum kept here,
+    the whole table each step; a head's bias takes the SGD step.  `update`
+    is the last part by itself, for a caller that reduced the gradients.
     """
 
     def __init__(self, graph: Graph, r_size: int, Q: int, T: int, N: int, c1, c2: int, table: torch.Tensor,
                  n_hide: int, lr: float = 0.01, eps: float = 1e-7, thr: float = 1e-7, stats: bool = True,
                  apply_update: bool = True, dropout: float = 0.0, dropout_seed: int = 0, zero_slack=None,
-                 record_grad_w: bool = False):
+                 record_grad_w: bool = False, head=None, rules=None, optimizer: str = "sgd", muon_options=None):
         dev = table.device
         self.dev, self.graph, self.r_size, self.Q, self.T, self.N = dev, graph, r_size, Q, T, N
         self.n = 2 * r_size + 1
@@ -102,6 +113,21 @@ class DrumTrainStep:
         self.flags = L.FL_SKIP_NONPOS_W | L.FL_DROP_MASKED
         self.eps, self.thr, self.lr = eps, thr, lr
         self.apply_update = apply_update
+        if optimizer not in ("sgd", "muon"):
+            raise ValueError(f"optimizer must be sgd or muon, got {optimizer!r}")
+        width = self.n if head is None else head[0].shape[-1]
+        if tuple(table.shape[1:]) != (T, N, width):
+            raise ValueError(f"table must be [2R, {T}, {N}, {width}], got {tuple(table.shape)}")
+        if head is not None:
+            if tuple(head[0].shape) != (self.n, width) or (head[1] is not None and tuple(head[1].shape) != (self.n,)):
+                raise ValueError(f"head must be a weight [{self.n}, H] and a bias [{self.n}] or None")
+            if any(t is not None and (t.dtype != torch.float32 or t.device != dev or not t.is_contiguous())
+                   for t in head):
+                raise ValueError("head must be contiguous float32 tensors on the table's device")
+        if rules is not None:
+            rules.check(T, Q, self.n)
+        self.head, self.rules, self.optimizer, self.width = head, rules, optimizer, width
+        self.muon_options = dict(muon_options or {})
         if not 0.0 <= float(dropout) <= 1.0:
             raise ValueError(f"dropout probability must lie in [0, 1], got {dropout}")
         self.dropout, self.dropout_seed = float(dropout), int(dropout_seed) & 0xFFFFFFFFFFFFFFFF
@@ -110,9 +136,14 @@ class DrumTrainStep:
         self.table = table
         # without the update: the dense table gradient, one contiguous [2R, N, n]
         # block per hop (grad_hop[t]); grad views it as the table's [2R, T, N, n]
-        self.grad_hop = None if apply_update else torch.zeros((T,) + tuple(table.shape[:1]) + tuple(table.shape[2:]),
-                                                              dtype=table.dtype, device=dev)
-        self.grad = None if apply_update else self.grad_hop.permute(1, 0, 2, 3)
+        keep_grad = not apply_update or optimizer == "muon"
+        self.grad_hop = torch.zeros((T,) + tuple(table.shape[:1]) + tuple(table.shape[2:]), dtype=table.dtype,
+                                    device=dev) if keep_grad else None
+        self.grad = self.grad_hop.permute(1, 0, 2, 3) if keep_grad else None
+        self.grad_head = None if head is None else tuple(None if t is None else torch.zeros_like(t) for t in head)
+        # momentum of the table's matrices, hop by hop as grad_hop, and of the head's weight
+        self.momentum = torch.zeros_like(self.grad_hop) if optimizer == "muon" else None
+        self.momentum_head = torch.zeros_like(head[0]) if optimizer == "muon" and head is not None else None
         rows = Q * N
         self.rows = rows
         csr = graph.csr
@@ -178,7 +209,12 @@ class DrumTrainStep:
         self.ok = torch.ones(1, dtype=f32, device=dev)  # 1 while the status word is clear
         self.scores = _buf(Q, f32, dev)
         self.loss = torch.zeros((), dtype=f32, device=dev)
-        self.grad_logits = torch.empty((Q, T, N, self.n), dtype=f32, device=dev)
+        # gradient of the batch's table rows: of the logits, or with a head of the hidden states
+        self.grad_logits = torch.empty((Q, T, N, width), dtype=f32, device=dev)
+        # with a head or rules the backward wants the hops' hidden states and logits again
+        self.hidden = None if head is None else [torch.empty((rows, width), dtype=f32, device=dev) for _ in range(T)]
+        self.logits = None if rules is None else [torch.empty((rows, self.n), dtype=f32, device=dev)
+                                                  for _ in range(T)]
         ws = 0
         for t in range(T):
             ws = max(ws, lib().fl_topc_workspace(rows, self.C[t]), lib().fl_hop_workspace(rows, self.S[t]),
@@ -246,6 +282,10 @@ class DrumTrainStep:
         ws, wsn = _p(self.ws), self.ws.numel()
         if self.dropout > 0:
             self.drop_counter.add_(1)
+        if self.head is not None:
+            for g_head in self.grad_head:
+                if g_head is not None:
+                    g_head.zero_()
         # hide the batch's own triples (src/main.py:888), remembering what was there
         hid = [self.pos[k][self.hide] for k in range(2)]
         old = [self.vis[k][hid[k]] for k in range(2)]
@@ -258,9 +298,7 @@ class DrumTrainStep:
         self.ent0[:rows].view(Q, N).copy_(self.heads.view(Q, 1).expand(Q, N))
         rp_in, ent_in, val_in = self.rp0, self.ent0, self.val0
         for t in range(T):
-            # this hop's attention rows [Q, N, n], gathered contiguous, then softmax
-            self.w[t][:rows * self.n].view(Q, N, self.n).copy_(
-                torch.softmax(self.table[:, t].index_select(0, self.rels), dim=-1))
+            self._weights(t)
             # c1
             if self.c1 is not None:
                 check(lb.fl_topc_select(_p(rp_in), _p(ent_in), _p(val_in), rows, self.C[t], self.c1, None,
@@ -318,6 +356,47 @@ class DrumTrainStep:
         self.ok.copy_(self.status == 0)
         self._backward_hop(T - 1)
 
+    def _weights(self, t):
+        """Hop t's attention rows [Q, N, n] into w[t]: gathered contiguous, through the head, then softmax."""
+        Q, N, rows, n = self.Q, self.N, self.rows, self.n
+        w = self.w[t][:rows * n]
+        if self.head is None and self.rules is None:
+            w.view(Q, N, n).copy_(torch.softmax(self.table[:, t].index_select(0, self.rels), dim=-1))
+            return
+        kept = self.hidden[t] if self.head is not None else self.logits[t]
+        torch.index_select(self.table[:, t], 0, self.rels, out=kept.view(Q, N, self.width))
+        z = kept
+        if self.head is not None:
+            z, _ = ops.linear_forward(kept, self.head[0], self.head[1],
+                                      out=None if self.rules is None else self.logits[t])
+        if self.rules is None:
+            w.view(Q, N, n).copy_(torch.softmax(z.view(Q, N, n), dim=-1))
+        else:
+            ops.relation_weights(z, out=w.view(rows, n), **self.rules.rows(t, N))
+
+    def _weights_backward(self, t):
+        """From grad_w to the gradient of hop t's table rows (and of the head)."""
+        Q, N, rows, n = self.Q, self.N, self.rows, self.n
+        wt, gw = self.w[t][:rows * n].view(Q, N, n), self.grad_w_of(t)
+        if self.rules is None:
+            # softmax backward, d logits = w * (g - sum(g * w)): torch's own kernel
+            dz = torch._softmax_backward_data(gw, wt, -1, torch.float32)
+        else:
+            kw = self.rules.rows(t, N)
+            dz, _ = ops.relation_weights_backward(wt.view(rows, n), gw.view(rows, n), self.logits[t],
+                                                  history=kw.get("history"), repetition=self.rules.repetition)
+            dz = dz.view(Q, N, n)
+        if self.head is None:
+            torch.mul(dz, self.ok, out=self.grad_logits[:, t])
+            return
+        dz = dz.view(rows, n) * self.ok
+        dx, dw, db = ops.linear_backward(self.hidden[t], self.head[0], None, dz,
+                                         want=(True, True, self.head[1] is not None))
+        self.grad_logits[:, t].copy_(dx.view(Q, N, self.width))
+        self.grad_head[0].add_(dw)
+        if db is not None:
+            self.grad_head[1].add_(db)
+
     def _backward_hop(self, t):
         """Backward of hop t; g_y[t] arrived through hop t's dropout (the same
         keep bits and scale), applied where it is written."""
@@ -341,19 +420,37 @@ class DrumTrainStep:
                 self.g_y[t - 1][:self.S[t]].copy_(self.grad_sel[:self.S[t]])
                 if self.dropout > 0:
                     self._dropout(self.g_y[t - 1], t - 1, st)
-        # softmax backward, d logits = w * (g - sum(g * w)): torch's own kernel
-        wt = self.w[t][:rows * self.n].view(Q, N, self.n)
-        gw = self.grad_w_of(t)
-        torch.mul(torch._softmax_backward_data(gw, wt, -1, torch.float32), self.ok, out=self.grad_logits[:, t])
-        if not self.apply_update:
+        self._weights_backward(t)
+        if self.grad_hop is not None:
             # hop t's dense table gradient, complete once this part has run
             self.grad_hop[t].zero_()
             self.grad_hop[t].index_add_(0, self.rels, self.grad_logits[:, t])
 
     def _finish(self):
         if self.apply_update:
-            # SGD on the rows of the batch's relations only: no dense gradient
-            self.table.index_add_(0, self.rels, self.grad_logits, alpha=-self.lr)
+            self.update()
+
+    def update(self):
+        """The optimizer's step from this run's gradients (in place; what parts() ends with under apply_update)."""
+        if self.optimizer == "sgd":
+            if self.grad_hop is None:
+                # SGD on the rows of the batch's relations only: no dense gradient
+                self.table.index_add_(0, self.rels, self.grad_logits, alpha=-self.lr)
+            else:
+                self.table.sub_(self.grad, alpha=self.lr)
+        else:
+            # matrices [2R, n or H] of every hop and channel: strided views of the table
+            muon.muon_update_(self.table.permute(1, 2, 0, 3), self.grad_hop.permute(0, 2, 1, 3),
+                              self.momentum.permute(0, 2, 1, 3), lr=self.lr, gate=self.ok, **self.muon_options)
+        if self.head is not None:
+            weight, bias = self.head
+            if self.optimizer == "sgd":
+                weight.sub_(self.grad_head[0], alpha=self.lr)
+            else:
+                muon.muon_update_(weight, self.grad_head[0], self.momentum_head, lr=self.lr, gate=self.ok,
+                                  **self.muon_options)
+            if bias is not None:
+                bias.sub_(self.grad_head[1], alpha=self.lr)
 
     def _drop(self, t):
         """fl_dropout of hop t for the kernels that write its values or their gradient (None: no dropout)."""

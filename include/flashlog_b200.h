@@ -548,11 +548,13 @@ int fl_orthogonalize(const fl_matrices *in, const fl_matrices *out, int64_t b1, 
 /* One Muon step, all f32: momentum_out = beta * momentum + grad; U =
  * grad + beta * momentum_out (nesterov) or momentum_out; param_out = param *
  * (1 - lr * weight_decay) - lr * scale * orthogonalised(U).  The outputs may
- * be the inputs (element for element). */
+ * be the inputs (element for element).  gate (a device float, or NULL): where
+ * it holds 0, parameter and momentum come out as they went in. */
 int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_matrices *momentum,
                    const fl_matrices *param_out, const fl_matrices *momentum_out, int64_t b1, int64_t b2, int64_t m,
                    int64_t n, double lr, double beta, int nesterov, double weight_decay, double scale, int steps,
-                   double a, double b, double c, double eps, void *ws, size_t ws_bytes, fl_stream_t stream);
+                   double a, double b, double c, double eps, const float *gate, void *ws, size_t ws_bytes,
+                   fl_stream_t stream);
 
 /* 1 if a bounded wait of a matrix-product kernel ran out since the last call
  * (its outputs hold NaN), else 0, in *fault; clears it.  Synchronizes. */
