@@ -764,6 +764,13 @@ struct NsWork {
         PlanesJob e;
         e.alpha = q.alpha;
         e.beta = q.beta;
+        const int shift = p.shift[j.batch_out];
+        if (shift != 0 && (phase == 0 || (!p.gram && phase % 3 == 0))) {
+            e.alpha *= exp2f(-2.0f * static_cast<float>(shift));  // A = X X^T
+        } else if (shift != 0 && phase == phases - 1) {
+            e.alpha *= exp2f(-static_cast<float>(shift));
+            e.beta *= exp2f(-static_cast<float>(shift));
+        }
         e.c = q.c < 0 ? nullptr : pl + q.c;
         e.out = q.out < 0 ? nullptr : pl + q.out;
         e.out2 = q.out2 < 0 ? nullptr : pl + q.out2;
@@ -1249,11 +1256,12 @@ int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, in
 
 // Sums the parts of A = X X^T into planes, both halves from the lower one: 32 x 32
 // tiles, grid (tiles, tiles, batch).
-__global__ void __launch_bounds__(256) combine_kernel(const float *parts, int splits, int lo, int64_t ldp, float alpha,
-                                                      __half *out, int64_t ld, int64_t plane) {
+__global__ void __launch_bounds__(256) combine_kernel(const float *parts, int splits, int lo, int64_t ldp, float scale,
+                                                      const int *shift, __half *out, int64_t ld, int64_t plane) {
     __shared__ float tile[32][33];
     if (blockIdx.x > blockIdx.y) return;
     const int64_t b = blockIdx.z;
+    const float alpha = scale * exp2f(-2.0f * static_cast<float>(shift[b]));
     const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
     const int64_t size = static_cast<int64_t>(lo) * ldp;
 #pragma unroll
@@ -1332,7 +1340,7 @@ int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float 
         if (rc) return rc;
         const unsigned tiles = static_cast<unsigned>((p.lo + 31) / 32);
         launch(combine_kernel, dim3(tiles, tiles, static_cast<unsigned>(p.batch)), dim3(32, 8), 0, st, parts, splits, p.lo,
-               e.p.ld_out, p.scale_a / (p.scale_x * p.scale_x), buf[kNsA].p, buf[kNsA].ld, buf[kNsA].plane);
+               e.p.ld_out, p.scale_a / (p.scale_x * p.scale_x), p.shift, buf[kNsA].p, buf[kNsA].ld, buf[kNsA].plane);
         rc = check_launch("newton-schulz combine");
         if (rc) return rc;
     }

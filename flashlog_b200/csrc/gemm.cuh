@@ -74,6 +74,7 @@ struct NsBuffer {
 };
 struct NsProgram {
     int lo, hi, batch, steps, gram;
+    const int *shift;        // [batch]: X holds scale_x * 2^shift * X (more than 0 for a matrix far below eps only)
     float a, b, c, scale_x, scale_a, scale_q, factor;
     FinalOutput final;
 };

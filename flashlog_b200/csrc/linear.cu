@@ -481,7 +481,7 @@ int check_linear(const fl_linear *p) {
     FL_REQUIRE(p->act >= FL_ACT_NONE && p->act <= FL_ACT_GELU, "linear: bad activation %d", p->act);
     FL_REQUIRE(p->rows >= 0 && p->n > 0 && p->k > 0 && p->rows < (1ll << 30) && p->n < (1ll << 30) && p->k < (1ll << 30),
                "linear: bad shape");
-    FL_REQUIRE(p->x != nullptr && p->w != nullptr && p->ld_x >= p->k && p->ld_w >= p->k &&
+    FL_REQUIRE((p->x != nullptr || p->rows == 0) && p->w != nullptr && p->ld_x >= p->k && p->ld_w >= p->k &&
                    (p->residual == nullptr || p->ld_res >= p->n),
                "linear: bad operand");
     return FL_OK;
@@ -615,15 +615,15 @@ int small_backward(const fl_linear *p, const float *z, const void *gy, int64_t l
 }  // namespace
 
 size_t linear_workspace(int64_t rows, int64_t n, int64_t k, int dtype) {
-    if (is_small(rows, n, k, dtype) || is_few_rows(rows, dtype)) return 0;
+    if (rows <= 0 || n <= 0 || k <= 0 || is_few_rows(rows, dtype) || is_small(rows, n, k, dtype)) return 0;
     return operand_bytes(rows, k, rows, dtype) + operand_bytes(n, k, n, dtype);
 }
 
 int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *wsp, size_t ws_bytes, cudaStream_t st) {
     int rc = check_linear(p);
     if (rc) return rc;
-    FL_REQUIRE(y != nullptr && ld_y >= p->n, "linear: bad output");
     if (p->rows == 0) return FL_OK;
+    FL_REQUIRE(y != nullptr && ld_y >= p->n, "linear: bad output");
     if (is_small(p->rows, p->n, p->k, p->dtype) || is_few_rows(p->rows, p->dtype)) {
         if (p->dtype == FL_F32) return small_forward<float>(p, y, ld_y, z, st);
         if (p->dtype == FL_F16) return small_forward<__half>(p, y, ld_y, z, st);
@@ -646,6 +646,7 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
 }
 
 size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act) {
+    if (rows <= 0 || n <= 0 || k <= 0) return 0;
     if (is_small_backward(rows, n, k, dtype)) return split_bytes(rows, k, n) + split_bytes(n, k, rows) + 256;
     size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
     if (act != FL_ACT_NONE) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
@@ -657,14 +658,14 @@ int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t 
                     void *wsp, size_t ws_bytes, cudaStream_t st) {
     int rc = check_linear(p);
     if (rc) return rc;
-    FL_REQUIRE(gy != nullptr && ld_gy >= p->n, "linear backward: bad gradient");
-    FL_REQUIRE(p->act == FL_ACT_NONE || z != nullptr, "linear backward: an activation needs the pre-activation");
     const int es = elem_size(p->dtype);
     if (p->rows == 0) {
         if (dw != nullptr) FL_CUDA(cudaMemsetAsync(dw, 0, p->n * p->k * es, st));
         if (dbias != nullptr) FL_CUDA(cudaMemsetAsync(dbias, 0, p->n * es, st));
         return FL_OK;
     }
+    FL_REQUIRE(gy != nullptr && ld_gy >= p->n, "linear backward: bad gradient");
+    FL_REQUIRE(p->act == FL_ACT_NONE || z != nullptr, "linear backward: an activation needs the pre-activation");
     Carve ws(wsp, ws_bytes);
     if (is_small_backward(p->rows, p->n, p->k, p->dtype)) {
         if (p->dtype == FL_F32) return small_backward<float>(p, z, gy, ld_gy, dx, dw, dbias, ws, st);

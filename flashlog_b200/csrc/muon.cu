@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256) square_sum_rows_kernel(const Source s, do
 // written in whole cache lines.
 template <typename T, bool MUON, bool TURNED>
 __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const double *partial, int parts, double eps,
-                                                        __half *out, int64_t ld, int64_t plane) {
+                                                        double growth, int *shift, __half *out, int64_t ld, int64_t plane) {
     __shared__ double scratch[8];
     // rows of 66 words, pairs of columns exchanged in every other 16 rows: pairs are written in one
     // access, and a column is read with at most two rows to a bank
@@ -205,7 +205,18 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     __syncthreads();
     sum = 0.0;
     for (int i = 0; i < 8; ++i) sum += scratch[i];
-    const double scale = static_cast<double>(kScaleX) / (sqrt(sum) + eps);
+    const double norm = sqrt(sum);
+    double scale = static_cast<double>(kScaleX) / (norm + eps);
+    // |X| is below 1 where eps counts; as long as the steps cannot bring it there (growth is the most they do),
+    // a power of two keeps its values away from the planes' smallest
+    int e = 0;
+    const double room = (norm + eps) / (norm * growth);
+    if (norm > 0.0 && room >= 2.0) {
+        e = static_cast<int>(floor(log2(room)));
+        e = e > 60 ? 60 : e;
+        scale = ldexp(scale, e);
+    }
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && threadIdx.y == 0) shift[b] = e;
     __half *hi = out + b * 2 * plane;
     if (TURNED) {
 #pragma unroll
@@ -237,8 +248,8 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
 }
 
 template <typename T, bool MUON>
-int normalize(const Source &s, bool turned, double eps, double *partial, int parts, int *counts, int n_counts, __half *x,
-              int64_t ld, int64_t plane, cudaStream_t st) {
+int normalize(const Source &s, bool turned, double eps, double growth, double *partial, int parts, int *counts,
+              int n_counts, int *shift, __half *x, int64_t ld, int64_t plane, cudaStream_t st) {
     const int64_t size = sizeof(T);
     const bool rows = !MUON && s.u.j == 1 && reinterpret_cast<uintptr_t>(s.u.ptr) % 16 == 0 && s.u.i * size % 16 == 0 &&
                       s.u.b1 * size % 16 == 0 && s.u.b2 * size % 16 == 0;
@@ -247,8 +258,8 @@ int normalize(const Source &s, bool turned, double eps, double *partial, int par
     else launch(square_sum_kernel<T, MUON>, parts_grid, 256, 0, st, s, partial, counts, n_counts);
     const dim3 grid(static_cast<unsigned>((s.n + 63) / 64), static_cast<unsigned>((s.m + 63) / 64),
                     static_cast<unsigned>(s.batch));
-    if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
-    else launch(normalize_kernel<T, MUON, false>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, x, ld, plane);
+    if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, growth, shift, x, ld, plane);
+    else launch(normalize_kernel<T, MUON, false>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, growth, shift, x, ld, plane);
     return check_launch("newton-schulz normalize");
 }
 
@@ -440,9 +451,9 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     const bool gram = use_gram(lo, hi, steps);
     const int n_counts = ns_phases(steps, gram) * static_cast<int>(s.batch);
     double *partial = ws.take<double>(s.batch * parts);
-    int *counts = ws.take<int>(n_counts);
+    int *counts = ws.take<int>(n_counts), *shift = ws.take<int>(s.batch);
     NsBuffer buf[kNsBuffers] = {};
-    bool fits = partial != nullptr && counts != nullptr;
+    bool fits = partial != nullptr && counts != nullptr && shift != nullptr;
     for (int i = 0; i < kNsBuffers; ++i) {
         if (gram ? i == kNsX2 : i >= kNsQ) continue;
         buf[i] = take_planes(ws, s.batch, lo, i <= kNsX2 ? hi : lo);
@@ -454,13 +465,13 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     const NsBuffer &x = buf[kNsX];
     int rc;
     if (s.mom_out.ptr != nullptr)
-        rc = normalize<float, true>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+        rc = normalize<float, true>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else if (s.dtype == FL_F32)
-        rc = normalize<float, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+        rc = normalize<float, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else if (s.dtype == FL_F16)
-        rc = normalize<__half, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+        rc = normalize<__half, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else
-        rc = normalize<__nv_bfloat16, false>(s, turned, eps, partial, parts, counts, n_counts, x.p, x.ld, x.plane, st);
+        rc = normalize<__nv_bfloat16, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     if (rc) return rc;
     NsProgram p{};
     p.lo = static_cast<int>(lo);
@@ -468,6 +479,7 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     p.batch = static_cast<int>(s.batch);
     p.steps = steps;
     p.gram = gram;
+    p.shift = shift;
     p.a = fa;
     p.b = fb;
     p.c = fc;
@@ -508,7 +520,8 @@ size_t fl_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n, int steps
     const int64_t lo = m < n ? m : n, hi = m < n ? n : m;
     if (is_small(lo, hi, steps)) return 0;
     const bool gram = use_gram(lo, hi, steps);
-    size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + carve_bytes<int>(ns_phases(steps, gram) * batch);
+    size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + carve_bytes<int>(ns_phases(steps, gram) * batch) +
+               carve_bytes<int>(batch);
     b += (gram ? 1 : 2) * planes_bytes(batch, lo, hi) + (gram ? 5 : 2) * planes_bytes(batch, lo, lo);
     return b + (gram ? ns_parts_bytes(lo, hi, batch) + 512 : 0);
 }

@@ -141,3 +141,140 @@ def test_backward(shape, dt, act):
         assert got.dtype == DT[dt] and got.shape == want.shape
         assert bool((err <= tol).all()), float((err / tol).max())
     assert torch.equal(dr, gy)
+
+
+# ---- what a caller may hand in ------------------------------------------------------------------
+def test_strides_and_leading_dimensions():
+    from flashlog_b200 import attention
+    g = torch.Generator().manual_seed(21)
+    r = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    for rows, k, n, dt in ((70, 48, 90, torch.float32), (300, 264, 520, torch.float32), (300, 264, 520, torch.bfloat16),
+                           (5, 33, 70, torch.float16)):
+        wide, tall = r(rows, k + 13).to(dt), r(k, n).to(dt)
+        x, w = wide[:, 5:5 + k], tall.T  # a slice of wider rows (odd offset); a transposed weight
+        res = r(n, rows).to(dt).T
+        bias = r(2 * n).to(dt)[::2]
+        y = attention.linear(x, w, bias, residual=res, activation="tanh")
+        assert_forward(y, x, w, bias, res, "tanh")
+        y3 = attention.linear(x.reshape(5, rows // 5, k), w, bias, residual=res.reshape(5, rows // 5, n), activation="tanh")
+        assert torch.equal(y3.reshape(rows, n), y)
+        one = attention.linear(x[0], w, bias)
+        assert one.shape == (n,)
+        assert_forward(one[None], x[:1], w, bias, None, "none")
+        expanded = x[:1].expand(rows, k)
+        assert_forward(attention.linear(expanded, w), expanded, w, None, None, "none")
+
+
+def test_empty_rows():
+    from flashlog_b200 import attention
+    x, w, b, _ = make(4, 8, 16, torch.float32)
+    e = x[:0].clone().requires_grad_()
+    w.requires_grad_()
+    b.requires_grad_()
+    y = attention.linear(e, w, b)
+    assert y.shape == (0, 16)
+    gx, gw, gb = torch.autograd.grad(y.sum(), [e, w, b])
+    assert gx.shape == (0, 8) and not gw.any() and not gb.any()
+
+
+@pytest.mark.parametrize("rows", [7, 60, 700])
+def test_lines_of_very_different_sizes(rows):
+    """fp32 lines keep their own accuracy: rows and weight rows scaled by powers of two from 2^-90 to 2^90."""
+    from flashlog_b200 import attention
+    x, w, b, _ = make(rows, 300, 401, torch.float32, seed=8, bias=False)
+    ex = torch.randint(-45, 46, (rows, 1), generator=torch.Generator().manual_seed(1)).cuda()
+    ew = torch.randint(-45, 46, (401, 1), generator=torch.Generator().manual_seed(2)).cuda()
+    xs, ws = torch.ldexp(x, 2 * ex), torch.ldexp(w, -2 * ew)
+    y = attention.linear(xs, ws)
+    want = xs.double() @ ws.double().T
+    S = xs.double().abs() @ ws.double().abs().T
+    tol = sum_tol(300) * S + half(torch.float32) * want.abs()
+    # results that fp32 holds: partial sums are at most S, so a sum with S beyond fp32 may overflow on its way
+    fits = (S < 3e38) & (S > 1e-30)
+    assert bool(((y.double() - want).abs() <= tol)[fits].all())
+
+
+def test_nonfinite_inputs_stay_in_their_rows():
+    from flashlog_b200 import attention
+    for rows, k, n in ((6, 40, 50), (300, 512, 700)):
+        x, w, b, _ = make(rows, k, n, torch.float32, seed=12)
+        clean = attention.linear(x, w, b)
+        x[2, 3], x[4, 1] = float("nan"), float("inf")
+        y = attention.linear(x, w, b)
+        keep = [i for i in range(rows) if i not in (2, 4)]
+        assert torch.equal(y[keep], clean[keep])
+        assert bool(y[2].isnan().all()) and not bool(y[4].isfinite().any())
+
+
+def test_other_stream_and_capture():
+    """On a stream of the caller's, and captured with its gradients: the same bits."""
+    from flashlog_b200 import attention
+    for rows, k, n in ((9, 128, 475), (300, 256, 475)):
+        x, w, b, _ = make(rows, k, n, torch.float32, seed=31)
+        gy = torch.randn(rows, n, generator=torch.Generator().manual_seed(5)).cuda()
+
+        def run(leaves):
+            y = attention.linear(*leaves, activation="silu")
+            return (y.detach(), *torch.autograd.grad(y, leaves, gy))
+
+        first = run([t.clone().requires_grad_() for t in (x, w, b)])
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+            second = run(leaves)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                captured = run(leaves)
+        torch.cuda.current_stream().wait_stream(s)
+        for _ in range(2):
+            g.replay()
+        torch.cuda.synchronize()
+        for a, c, d in zip(first, second, captured):
+            assert torch.equal(a, c) and torch.equal(a, d)
+
+
+def test_two_captured_graphs_do_not_share_memory():
+    from flashlog_b200 import attention
+    sets = [make(300, 200 + 8 * i, 333, torch.float32, seed=40 + i) for i in range(2)]
+    want = [attention.linear(x, w, b) for x, w, b, _ in sets]
+    graphs, outs = [], []
+    s = torch.cuda.Stream()
+    for x, w, b, _ in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(attention.linear(x, w, b))
+        graphs.append(g)
+    for order in ((0, 1), (1, 0)):
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_gradient_against_differences():
+    from flashlog_b200 import attention
+    x, w, b, _ = make(6, 20, 15, torch.float32, seed=50)
+    x.requires_grad_()
+    gy = torch.randn(6, 15, generator=torch.Generator().manual_seed(3)).cuda()
+    g, = torch.autograd.grad(attention.linear(x, w, b, activation="gelu"), [x], gy)
+    d = torch.zeros_like(x)
+    d[1, 2] = 2.0 ** -6
+    with torch.no_grad():
+        f = [(attention.linear(x + s * d, w, b, activation="gelu").double() * gy.double()).sum() for s in (1, -1)]
+    # cubic term: h^2 / 6 of a third derivative below 2 per weight (sum |gy w^3| < 30 here); roundings 15 * 2^-24 / h
+    assert abs(float((f[0] - f[1]) / 2.0 ** -5) - float(g[1, 2])) <= 30 * 2 * 2.0 ** -12 / 6 + 100 * 2.0 ** -24 * 2.0 ** 6
+
+
+def test_only_wanted_gradients():
+    from flashlog_b200 import attention
+    for rows in (40, 700):
+        x, w, b, res = make(rows, 300, 420, torch.float32, seed=60, res=True)
+        gy = torch.randn(rows, 420, generator=torch.Generator().manual_seed(6)).cuda()
+        full = [t.clone().requires_grad_() for t in (x, w, b, res)]
+        all4 = torch.autograd.grad(attention.linear(*full, activation="relu"), full, gy)
+        for k in range(4):
+            leaves = [x, w, b, res]
+            leaves[k] = leaves[k].clone().requires_grad_()
+            got, = torch.autograd.grad(attention.linear(*leaves, activation="relu"), [leaves[k]], gy)
+            assert torch.equal(got, all4[k])

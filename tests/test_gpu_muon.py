@@ -88,3 +88,145 @@ def test_orthogonalize_shapes(shape, dt):
     # near the rounding of the result itself: each element's is at most half a step (eps / 2) of it, so their
     # Frobenius norm is at most eps / 2 of the result's (2^-8 for bf16, 2^-11 for fp16)
     assert rel <= 2e-5 + (torch.finfo(DT[dt]).eps / 2 if dt != "fp32" else 0.0)
+
+
+def test_decaying_spectrum():
+    """A strong low-rank part over noise, the case that single 16-bit planes lose (see the kernel's comment)."""
+    from flashlog_b200 import muon
+    g = torch.Generator().manual_seed(4)
+    for m, n in ((200, 210), (128, 640)):
+        u = torch.randn(m, 3, generator=g) @ torch.randn(3, n, generator=g) + 1e-3 * torch.randn(m, n, generator=g)
+        u = u.cuda()
+        got, (want, _, _) = muon.orthogonalize(u), exact(u)
+        # what plain fp32 steps give is off by 5e-5 here; within ten times that
+        assert float((got.double() - want).norm() / want.norm()) <= 5e-4
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (300, 310), (100, 900)], ids=str)
+def test_zero_tiny_huge_and_nonfinite(shape):
+    from flashlog_b200 import muon
+    u = matrices(5, *shape, seed=9)
+    u[0] = 0
+    u[1] *= 1e25
+    u[2] *= 1e-20
+    u[3, 2, 3] = float("nan")
+    o = muon.orthogonalize(u)
+    assert not bool(o[0].any())
+    assert bool(o[3].isnan().any()) and bool(o[[1, 2, 4]].isfinite().all())
+    for k in (1, 2, 4):
+        assert_close(o[k:k + 1], u[k:k + 1])
+
+
+@pytest.mark.parametrize("steps,c", [(1, C), (2, C), (3, (1.5, -0.5, 0.0)), (8, C), (5, (2.0, -1.5, 0.5))])
+@pytest.mark.parametrize("shape", [(30, 40), (200, 208), (100, 700)], ids=str)
+def test_steps_and_coefficients(shape, steps, c):
+    from flashlog_b200 import muon
+    u = matrices(1, *shape, seed=steps)
+    assert_close(muon.orthogonalize(u, steps=steps, coefficients=c), u, steps, c)
+
+
+@pytest.mark.parametrize("shape", [(24, 25), (130, 140), (140, 900)], ids=str)
+def test_strided_batches(shape):
+    """Views of a table [m, T, N, n], transposed matrices, more batch dimensions than the kernels know."""
+    from flashlog_b200 import muon
+    m, n = shape
+    table = matrices(m, 2, 3, n, seed=2)
+    view = table.permute(1, 2, 0, 3)
+    want = muon.orthogonalize(view.contiguous())
+    assert torch.equal(muon.orthogonalize(view), want)
+    torch.testing.assert_close(muon.orthogonalize(view.mT), want.mT, rtol=1e-4, atol=1e-4)
+    odd = view[None].expand(2, -1, -1, -1, -1)
+    assert torch.equal(muon.orthogonalize(odd), want[None].expand(2, -1, -1, -1, -1))
+    assert muon.orthogonalize(view[:0]).shape == (0, 3, m, n)
+
+
+def muon64(p, g, mo, lr, beta, nesterov, wd, scale):
+    p, g, mo = p.double(), g.double(), mo.double()
+    m2 = beta * mo + g
+    o, _, _ = exact(g + beta * m2 if nesterov else m2)
+    return p * (1 - lr * wd) - lr * scale * o, m2
+
+
+@pytest.mark.parametrize("shape", [(24, 25), (300, 140), (200, 230), (90, 800)], ids=str)
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_update(shape, nesterov):
+    from flashlog_b200 import muon
+    m, n = shape
+    p, g, mo = (matrices(2, m, n, seed=s) for s in (1, 2, 3))
+    kw = dict(lr=0.1, beta=0.9, nesterov=nesterov, weight_decay=0.05)
+    want_p, want_m = muon64(p, g, mo, 0.1, 0.9, nesterov, 0.05, max(1.0, m / n) ** 0.5)
+    p0, m0 = p.clone(), mo.clone()
+    p2, m2 = muon.muon_update(p, g, mo, **kw)
+    assert torch.equal(p, p0) and torch.equal(mo, m0)
+    # momentum: one rounding of each operation; parameter: three, and lr * scale of the orthogonalised update's 2e-5
+    assert bool(((m2.double() - want_m).abs() <= 2 * 2.0 ** -24 * (0.9 * mo.double().abs() + g.double().abs())).all())
+    tol = 4 * 2.0 ** -24 * p.double().abs().max() * math.sqrt(m * n) + 0.1 * max(1.0, m / n) ** 0.5 * 2e-5 * math.sqrt(min(m, n)) * 1.3
+    assert float((p2.double() - want_p).flatten(1).norm(dim=1).max()) <= tol
+    assert muon.muon_update_(p, g, mo, **kw) is p
+    assert torch.equal(p, p2) and torch.equal(mo, m2)
+    # strided tensors of different layouts, in place
+    strided = [t.permute(1, 0, 2).contiguous().permute(1, 0, 2) for t in (p0, m0)]
+    muon.muon_update_(strided[0], g.mT.contiguous().mT, strided[1], **kw)
+    assert torch.equal(strided[0], p2) and torch.equal(strided[1], m2)
+
+
+@pytest.mark.parametrize("shape", [(24, 25), (200, 230), (90, 800)], ids=str)
+def test_closed_gate_changes_nothing(shape):
+    from flashlog_b200 import muon
+    p, g, mo = (matrices(2, *shape, seed=s) for s in (1, 2, 3))
+    g[:] = float("nan")
+    gate = torch.zeros(1, device="cuda")
+    p2, m2 = muon.muon_update(p, g, mo, lr=0.1, weight_decay=0.1, gate=gate)
+    assert torch.equal(p2, p) and torch.equal(m2, mo)
+    gate.fill_(1.0)
+    g = matrices(2, *shape, seed=7)
+    a = muon.muon_update(p, g, mo, lr=0.1, weight_decay=0.1, gate=gate)
+    b = muon.muon_update(p, g, mo, lr=0.1, weight_decay=0.1)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("shape", [(24, 25), (200, 230), (90, 800), (64, 4000)], ids=str)
+def test_same_bits_on_other_streams_and_in_graphs(shape):
+    """Repeated, on two streams at once, and replayed from two graphs: one result."""
+    from flashlog_b200 import muon
+    u = matrices(3, *shape, seed=5)
+    want = muon.orthogonalize(u)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(muon.orthogonalize(u))
+    graphs = []
+    for s in streams:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(muon.orthogonalize(u))
+        graphs.append(g)
+    for s, g in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_optimizer():
+    from flashlog_b200 import attention, muon
+    g = torch.Generator().manual_seed(6)
+    w = torch.randn(70, 50, generator=g).cuda().requires_grad_()
+    b = torch.randn(3, 20, 30, generator=g).cuda().requires_grad_()
+    idle = torch.randn(5, 6, generator=g).cuda().requires_grad_()
+    opt = muon.Muon([{"params": [w, idle]}, {"params": [b], "lr": 0.1}], lr=0.05, weight_decay=0.01)
+    x = torch.randn(8, 50, generator=g).cuda()
+    want = [w.detach().clone(), b.detach().clone()]
+    mom = [torch.zeros_like(t) for t in want]
+    for _ in range(3):
+        opt.zero_grad()
+        (attention.linear(x, w).square().sum() + (b ** 3).sum()).backward()
+        for i, (t, lr) in enumerate(((w, 0.05), (b, 0.1))):
+            muon.muon_update_(want[i], t.grad, mom[i], lr=lr, weight_decay=0.01)
+        opt.step()
+    assert torch.equal(w.detach(), want[0]) and torch.equal(b.detach(), want[1])
+    assert idle not in opt.state or not opt.state[idle]

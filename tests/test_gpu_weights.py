@@ -136,3 +136,146 @@ def test_parts_alone(n):
     check(z, kw, RULES)
     m = torch.rand(11, n, generator=torch.Generator().manual_seed(1)).cuda() < 0.2
     check(z, {"mask": m}, {})
+
+
+# ---- masks, infinities, odd inputs ----------------------------------------------------------------
+@pytest.mark.parametrize("n", [25, 1645, 8193])
+@pytest.mark.parametrize("rows", [6, 300])
+def test_empty_rows_and_hidden_garbage(n, rows):
+    """Rows whose mask leaves nothing are 0 with gradient 0; masked logits may hold NaN or infinities."""
+    from flashlog_b200 import attention
+    g = torch.Generator().manual_seed(n)
+    z = torch.randn(rows, n, generator=g).cuda()
+    mask = torch.rand(rows, n, generator=g).cuda() < 0.5
+    mask[0] = False
+    mask[1] = False
+    mask[1, n // 2] = True  # one left: weight 1
+    clean = attention.relation_weights(z, mask=mask)
+    dirty = z.clone()
+    dirty[~mask] = torch.tensor([float("nan"), float("inf"), -float("inf"), 3e38]).cuda()[
+        torch.randint(0, 4, (int((~mask).sum()),), generator=g).cuda()]
+    dirty.requires_grad_()
+    w = attention.relation_weights(dirty, mask=mask)
+    assert torch.equal(w, clean)
+    assert not bool(w[0].any()) and float(w[1, n // 2]) == 1.0
+    gw = torch.randn(rows, n, generator=g).cuda()
+    d, = torch.autograd.grad(w, [dirty], gw)
+    assert bool(d.isfinite().all()) and not bool(d[~mask].any()) and not bool(d[0].any())
+
+
+@pytest.mark.parametrize("n", [25, 475, 4097])
+def test_lowest_values_and_infinities(n):
+    from flashlog_b200 import attention
+    low = torch.finfo(torch.float32).min
+    z = torch.randn(5, n, generator=torch.Generator().manual_seed(2)).cuda()
+    z[0] = low                      # all at the type's lowest: equal weights
+    z[1] = -float("inf")            # nothing left
+    z[2, 1:] = low                  # one above
+    z[3, 0] = float("nan")
+    z[4, 0] = float("inf")
+    w = attention.relation_weights(z, tau=0.5)
+    torch.testing.assert_close(w[0], torch.full((n,), 1.0 / n, device="cuda"), rtol=1e-5, atol=0)
+    assert not bool(w[1].any())
+    assert float(w[2, 0]) == 1.0 and not bool(w[2, 1:].any())
+    assert bool(w[3].isnan().all()) and bool(w[4].isnan().any())
+    # the additive form of a mask: the lowest value as a bias
+    z = torch.randn(5, n, generator=torch.Generator().manual_seed(3)).cuda()
+    bias = torch.where(torch.rand(n, generator=torch.Generator().manual_seed(4)).cuda() < 0.5, low, 0.0)
+    bias[0] = 0.0
+    a, b = attention.relation_weights(z, bias=bias), attention.relation_weights(z, mask=bias == 0)
+    torch.testing.assert_close(a, b, rtol=1e-6, atol=0)
+    for dt in (torch.float16, torch.bfloat16):
+        zz = torch.full((2, n), torch.finfo(dt).min, dtype=dt, device="cuda")
+        torch.testing.assert_close(attention.relation_weights(zz), torch.full((2, n), 1.0 / n, device="cuda"), rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("n", [475, 29649])
+def test_long_histories(n):
+    """More entries than threads and than operators, every column used, the same one many times."""
+    for rows in (3, 90):
+        z, kw = inputs(rows, n, torch.float32, seed=6, states=0, hist=0, bias=None)
+        g = torch.Generator().manual_seed(8)
+        for hist in (700, 5000):
+            h = torch.randint(-3, n + 3, (rows, hist), generator=g)
+            h[0] = n - 1
+            check(z, {"history": h.cuda()}, dict(repetition=1.1, frequency=0.001, presence=0.1))
+    from flashlog_b200 import attention
+    z = torch.zeros(2, n, device="cuda")
+    h = torch.zeros(2, 65535, dtype=torch.int64, device="cuda")
+    w = attention.relation_weights(z, history=h, frequency=2.0 ** -16)
+    u = torch.zeros(n, dtype=torch.float64)
+    u[0] = -65535 * 2.0 ** -16
+    torch.testing.assert_close(w[1].double().cpu(), torch.softmax(u, 0), rtol=1e-5, atol=0)
+
+
+def test_strides_leading_dimensions_and_shared_gradients():
+    from flashlog_b200 import attention
+    z, kw = inputs(24, 130, torch.float32, seed=9)
+    plain = attention.relation_weights(z, **kw, **RULES)
+    wide = torch.zeros(24, 200, device="cuda")
+    wide[:, 7:137] = z
+    table = torch.zeros(7, 131, dtype=torch.bool, device="cuda")
+    table[:, 1:] = kw["mask"]
+    hist = torch.zeros(24, 11, dtype=torch.int64, device="cuda")
+    hist[:, ::2][:, :5] = kw["history"]
+    odd = attention.relation_weights(wide[:, 7:137], mask=table[:, 1:], states=kw["states"], history=hist[:, ::2][:, :5],
+                                     bias=kw["bias"], **RULES)
+    assert torch.equal(odd, plain)
+    lead = attention.relation_weights(z.view(2, 3, 4, 130), mask=kw["mask"], states=kw["states"].view(2, 3, 4),
+                                      history=kw["history"].view(2, 3, 4, 5), bias=kw["bias"], **RULES)
+    assert torch.equal(lead.view(24, 130), plain)
+    lz = z.clone().requires_grad_()
+    a, = torch.autograd.grad((attention.relation_weights(lz, **kw, **RULES) ** 2).sum(), [lz])
+    w = attention.relation_weights(lz, **kw, **RULES)
+    b, = torch.autograd.grad(w, [lz], 2 * w.detach())
+    assert torch.equal(a, b)
+    row = torch.randn(130, device="cuda")  # one gradient row for all rows, as a broadcast gives it
+    c, = torch.autograd.grad(attention.relation_weights(lz, **kw, **RULES), [lz], row.expand(24, 130))
+    d, = torch.autograd.grad(attention.relation_weights(lz, **kw, **RULES), [lz], row.expand(24, 130).contiguous())
+    assert torch.equal(c, d)
+    empty = attention.relation_weights(z[:0], bias=kw["bias"])
+    assert empty.shape == (0, 130)
+
+
+@pytest.mark.parametrize("rows,n", [(1, 29649), (40, 29649), (500, 1645), (60, 25)])
+def test_same_bits_on_another_stream_and_in_a_graph(rows, n):
+    from flashlog_b200 import attention
+    z, kw = inputs(rows, n, torch.float32, seed=13)
+    g = torch.randn(rows, n, generator=torch.Generator().manual_seed(1)).cuda()
+
+    def run(lz, lb):
+        w = attention.relation_weights(lz, **{**kw, "bias": lb}, **RULES)
+        return (w.detach(), *torch.autograd.grad(w, [lz, lb], g))
+
+    first = run(z.clone().requires_grad_(), kw["bias"].clone().requires_grad_())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        lz, lb = z.clone().requires_grad_(), kw["bias"].clone().requires_grad_()
+        second = run(lz, lb)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            third = run(lz, lb)
+    torch.cuda.current_stream().wait_stream(s)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_gradient_against_differences():
+    from flashlog_b200 import attention
+    z, kw = inputs(4, 60, torch.float32, seed=14)
+    kw["states"][:] = 1
+    g = torch.randn(4, 60, generator=torch.Generator().manual_seed(2)).cuda().double()
+    lz = z.clone().requires_grad_()
+    d, = torch.autograd.grad(attention.relation_weights(lz, **kw, **RULES), [lz], g.float())
+    k = int(d[2].abs().argmax())
+    h = 2.0 ** -7
+    e = torch.zeros_like(z)
+    e[2, k] = h
+    with torch.no_grad():
+        f = [(attention.relation_weights(z + s * e, **kw, **RULES).double() * g).sum() for s in (1, -1)]
+    # the third derivative of a softmax is below 1 / tau^3 times the slope, penalties scale by at most 1.3
+    assert abs(float((f[0] - f[1]) / (2 * h)) - float(d[2, k])) <= (1.3 / 0.8) ** 3 * 4 * h * h / 6 + 60 * 2.0 ** -23 * 4 / h
