@@ -834,8 +834,17 @@ struct NsWork {
 template <typename W> __device__ __forceinline__ int work_first(const W &) { return 0; }
 __device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 
+// The tensor cores truncate where they add to an accumulator: with two planes
+// (fp32 results) 12 additions per block of k lost 2e-8 of the sum each, 4e-6 at
+// k = 1024.  So a product on planes is cut into chunks of two blocks of k, each
+// into an accumulator of its own, and the epilogue warps add the chunks in
+// registers, rounding to nearest (0.5e-6, whatever k): 128-wide tiles, 64 sums a
+// thread, four accumulators in turn.  16-bit results keep one accumulator.
 template <int BN, int PLANES, int TILES>
 struct Config {
+    static constexpr int kChunk = PLANES == 2 ? 2 : 1 << 28;  // blocks of k per accumulator
+    static constexpr int kAccs = PLANES == 2 ? 512 / BN : 2;
+    static_assert(PLANES == 1 || BN == 128, "the chunks' sums have to fit the epilogue's registers");
     static constexpr int kA = kBM * kBK * 2;              // bytes of one plane of A per stage
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
     static constexpr int kStage = PLANES * (kA + kB);
@@ -854,7 +863,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
     // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
     unsigned char *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float *stage_epi = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
-    __shared__ uint64_t bars[2 * C::kStages + 4 + C::kTiles * kEpiWarps];
+    __shared__ uint64_t bars[2 * C::kStages + 2 * C::kAccs + C::kTiles * kEpiWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
@@ -863,18 +872,18 @@ void gemm_kernel(const __grid_constant__ Work work) {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::kStages, acc_full = empty + 8 * C::kStages,
-                   acc_empty = acc_full + 16;
+                   acc_empty = acc_full + 8 * C::kAccs;
 
-    if (threadIdx.x < 2 * C::kStages + 4 + C::kTiles * kEpiWarps) {
-        const int i = threadIdx.x, k = i - (2 * C::kStages + 2);
-        // accumulator buffers free: every epilogue warp of both CTAs arrives
-        bar_init(full + 8 * i, k == 0 || k == 1 ? 2 * kEpiWarps : 1);
+    if (threadIdx.x < 2 * C::kStages + 2 * C::kAccs + C::kTiles * kEpiWarps) {
+        const int i = threadIdx.x, k = i - (2 * C::kStages + C::kAccs);
+        // accumulators free: every epilogue warp of both CTAs arrives
+        bar_init(full + 8 * i, k >= 0 && k < C::kAccs ? 2 * kEpiWarps : 1);
         if (i == 0) failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                     "r"(2 * BN) : "memory");
+                     "r"(C::kAccs * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -943,42 +952,45 @@ void gemm_kernel(const __grid_constant__ Work work) {
             const uint32_t a_lbo = j.a_mn ? 8192u : 16u, b_lbo = j.b_mn ? 8192u : 16u;
             const uint32_t idesc = work.types | (static_cast<uint32_t>(j.a_mn) << 15) | (static_cast<uint32_t>(j.b_mn) << 16) |
                                    (static_cast<uint32_t>(j.width >> 3) << 17);
-            ok = warp_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t d = tmem + buf * BN;
-            for (int kb = j.kb0; kb < j.kb1; ++kb) {
-                ok = warp_wait(full + 8 * s, phase, &failed);
+            for (int k0 = j.kb0; ok && k0 < j.kb1; k0 = k0 + C::kChunk < j.kb1 ? k0 + C::kChunk : j.kb1) {
+                const int k1 = min(j.kb1, k0 + C::kChunk);
+                ok = warp_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t sa = smem_u32(smem) + s * C::kStage, sb = sa + PLANES * C::kA;
-                if (elect_one()) {
-                    uint64_t da[PLANES], db[PLANES];
+                const uint32_t d = tmem + buf * BN;
+                for (int kb = k0; kb < k1; ++kb) {
+                    ok = warp_wait(full + 8 * s, phase, &failed);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sa = smem_u32(smem) + s * C::kStage, sb = sa + PLANES * C::kA;
+                    if (elect_one()) {
+                        uint64_t da[PLANES], db[PLANES];
 #pragma unroll
-                    for (int p = 0; p < PLANES; ++p) {
-                        da[p] = smem_desc(sa + p * C::kA, a_lbo, 1024);
-                        db[p] = smem_desc(sb + p * C::kB, b_lbo, 1024);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kBK / 16; ++i) {
-                        mma_f16(d, da[0] + i * a_step, db[0] + i * b_step, idesc, kb != j.kb0 || i != 0);
-                        if (PLANES == 2) {
-                            mma_f16(d, da[0] + i * a_step, db[PLANES - 1] + i * b_step, idesc, 1);
-                            mma_f16(d, da[PLANES - 1] + i * a_step, db[0] + i * b_step, idesc, 1);
+                        for (int p = 0; p < PLANES; ++p) {
+                            da[p] = smem_desc(sa + p * C::kA, a_lbo, 1024);
+                            db[p] = smem_desc(sb + p * C::kB, b_lbo, 1024);
                         }
+#pragma unroll
+                        for (int i = 0; i < kBK / 16; ++i) {
+                            mma_f16(d, da[0] + i * a_step, db[0] + i * b_step, idesc, kb != k0 || i != 0);
+                            if (PLANES == 2) {
+                                mma_f16(d, da[0] + i * a_step, db[PLANES - 1] + i * b_step, idesc, 1);
+                                mma_f16(d, da[PLANES - 1] + i * a_step, db[0] + i * b_step, idesc, 1);
+                            }
+                        }
+                        mma_commit(empty + 8 * s);
                     }
-                    mma_commit(empty + 8 * s);
+                    __syncwarp();
+                    if (++s == C::kStages) { s = 0; phase ^= 1; }
                 }
+                if (elect_one()) mma_commit(acc_full + 8 * buf);
                 __syncwarp();
-                if (++s == C::kStages) { s = 0; phase ^= 1; }
+                if (++buf == C::kAccs) { buf = 0; acc_phase ^= 1; }
             }
-            if (elect_one()) mma_commit(acc_full + 8 * buf);
-            __syncwarp();
-            if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        EpiWarp w{stage_epi + warp * C::kTiles * 1024, acc_empty + 16 + 8 * warp * C::kTiles, 0, &failed, lane};
+        EpiWarp w{stage_epi + warp * C::kTiles * 1024, acc_empty + 8 * C::kAccs + 8 * warp * C::kTiles, 0, &failed, lane};
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -993,29 +1005,67 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 for (int q = 0; q < C::kTiles; ++q)
                     if (ok && j.col + half + 32 * q < j.n) work.ask(j, w, q, row0, j.col + half + 32 * q);
             }
-            if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * BN + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-#pragma unroll 1
-            for (int c = half; c < half + BN / 2; c += 32) {
-                if (!any || j.col + c >= j.n) break;
-                float v[32];
-                if (ok) {
-                    tmem_read32(v, src + c);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
-                }
+            const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+            auto next_acc = [&] {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive_cta0(acc_empty + 8 * buf);
+                if (++buf == C::kAccs) { buf = 0; acc_phase ^= 1; }
+            };
+            auto finish = [&](float (&v)[32], int c) {
                 const int tile = ((c - half) >> 5) % C::kTiles, next = c + 32 * C::kTiles;
                 work.chunk(j, v, w, tile, row0, j.col + c);
                 __syncwarp();
                 if (ok && next < half + BN / 2 && j.col + next < j.n) work.ask(j, w, tile, row0, j.col + next);
+            };
+            if constexpr (PLANES == 2) {
+                float sum[2][32];
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[q][i] = 0.0f;
+                for (int k0 = j.kb0; k0 < j.kb1; k0 += C::kChunk) {
+                    if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (ok && any) {
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            float v[32];
+                            tmem_read32(v, tmem + buf * BN + lanes + half + 32 * q);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sum[q][i] += v[i];
+                        }
+                    }
+                    next_acc();
+                }
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int c = half + 32 * q;
+                    if (!any || j.col + c >= j.n) continue;
+                    if (!ok) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[q][i] = __int_as_float(0x7fc00000);
+                    }
+                    finish(sum[q], c);
+                }
+            } else {
+                if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for (int c = half; c < half + BN / 2; c += 32) {
+                    if (!any || j.col + c >= j.n) break;
+                    float v[32];
+                    if (ok) {
+                        tmem_read32(v, tmem + buf * BN + lanes + c);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
+                    }
+                    finish(v, c);
+                }
+                next_acc();
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive_cta0(acc_empty + 8 * buf);
             work.done(j, w);
-            if (++buf == 2) { buf = 0; acc_phase ^= 1; }
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
@@ -1026,7 +1076,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
     cluster_sync();
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kAccs * BN));
     }
 }
 
@@ -1189,11 +1239,13 @@ int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b,
     epi.p.aligned = rows_ready(e.out, e.ld_out, per) && rows_ready(e.residual, e.ld_res, per) && rows_ready(e.bias, 0, 1) &&
                     rows_ready(e.z, e.ld_z, 4);
     constexpr int kPlanes = sizeof(T) == 4 ? 2 : 1;
-    return wide_tiles(s) ? run<256, kPlanes>(s, a, b, epi, 1, st) : run<128, kPlanes>(s, a, b, epi, 1, st);
+    if constexpr (kPlanes == 1)
+        if (wide_tiles(s)) return run<256, 1>(s, a, b, epi, 1, st);
+    return run<128, kPlanes>(s, a, b, epi, 1, st);
 }
 
-template <int BN>
 int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, int *done_count, cudaStream_t st) {
+    constexpr int BN = 128;
     using C = Config<BN, 2, NsWork::kTiles>;
     NsWork w{};
     w.p = p;
@@ -1293,7 +1345,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const float *parts, int sp
 // SMs, each at least 8 blocks of k long; 1 when its tiles fill half of them.
 int outer_splits(int64_t lo, int64_t hi, int64_t batch) {
     GemmShape s{lo, lo, hi, batch, 1, kF16};
-    const int64_t tiles = tile_count(s, 256) * batch, kblocks = (hi + kBK - 1) / kBK;
+    const int64_t tiles = tile_count(s, 128) * batch, kblocks = (hi + kBK - 1) / kBK;
     int64_t n = sm_pairs() / tiles;
     if (n > kblocks / 8) n = kblocks / 8;
     if (n < 2) return 1;
@@ -1336,7 +1388,7 @@ int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float 
         e.p.out_batch = p.lo * e.p.ld_out;
         e.p.dtype = kOutF32;
         e.p.aligned = 1;
-        rc = run<256, 2>(outer, x, x, e, splits, st);
+        rc = run<128, 2>(outer, x, x, e, splits, st);
         if (rc) return rc;
         const unsigned tiles = static_cast<unsigned>((p.lo + 31) / 32);
         launch(combine_kernel, dim3(tiles, tiles, static_cast<unsigned>(p.batch)), dim3(32, 8), 0, st, parts, splits, p.lo,
@@ -1345,9 +1397,7 @@ int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float 
         if (rc) return rc;
     }
     const int first = splits > 1 ? 1 : 0;
-    // 256-wide tiles once a phase of the squares fills the pairs of SMs with them
-    const bool wide = tile_count(outer, 256) * p.batch >= sm_pairs();
-    return wide ? launch_ns<256>(p, buf, phases, first, done_count, st) : launch_ns<128>(p, buf, phases, first, done_count, st);
+    return launch_ns(p, buf, phases, first, done_count, st);
 }
 
 // Reads and clears the device fault word (synchronizes the device).
