@@ -558,6 +558,7 @@ struct Job {
     int m, n;              // bounds of the output
     int batch_a, batch_b, batch_out;
     int kb0, kb1;          // contraction, in blocks of kBK
+    int per_acc;           // blocks per accumulator (planes; 1 << 28: all)
     int phase;
 };
 struct Cursor {
@@ -570,7 +571,7 @@ template <typename Epi>
 struct SingleWork {
     CUtensorMap map_a, map_b;
     int m, n, kblocks, splits;  // splits > 1: the contraction in parts, one output each
-    int a_mn, b_mn;
+    int a_mn, b_mn, per_acc;
     TileGrid grid;
     uint32_t types;             // of the instruction descriptor
     Epi epi;
@@ -595,6 +596,7 @@ struct SingleWork {
         j.batch_out = b;
         j.kb0 = part * per;
         j.kb1 = min(kblocks, j.kb0 + per);
+        j.per_acc = per_acc;
         j.phase = 0;
         return j;
     }
@@ -755,6 +757,7 @@ struct NsWork {
         j.batch_a = j.batch_b = j.batch_out = b;
         j.kb0 = 0;
         j.kb1 = (q.k + kBK - 1) / kBK;
+        j.per_acc = p.gram ? 3 : 6;
         j.phase = cur.phase | (part << 16);
         return j;
     }
@@ -834,16 +837,20 @@ struct NsWork {
 template <typename W> __device__ __forceinline__ int work_first(const W &) { return 0; }
 __device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 
-// The tensor cores truncate where they add to an accumulator: with two planes
-// (fp32 results) 12 additions per block of k lost 2e-8 of the sum each, 4e-6 at
-// k = 1024.  So a product on planes is cut into chunks of two blocks of k, each
-// into an accumulator of its own, and the epilogue warps add the chunks in
-// registers, rounding to nearest (0.5e-6, whatever k): 128-wide tiles, 64 sums a
-// thread, four accumulators in turn.  16-bit results keep one accumulator.
+// The tensor cores truncate where they add to an accumulator, which loses 2e-8
+// of the sum per addition: 4e-6 at k = 1024 with the 12 additions that two
+// planes take per block of k.  So the two cross products (hi lo, lo hi), 2^-11
+// of the whole, have an accumulator of their own, and hi hi is cut into chunks of
+// six blocks of k (24 additions, 0.5e-6 whatever k; three blocks where the Gram
+// form squares singular values), each into the next of three accumulators; the epilogue warps add the chunks in registers, rounding to
+// nearest.  64 sums a thread: 128-wide tiles.  (Chunks of two blocks with the
+// cross products inside reached the same accuracy 25% slower: three times the
+// accumulator reads.)  16-bit results keep one accumulator per tile.
 template <int BN, int PLANES, int TILES>
 struct Config {
-    static constexpr int kChunk = PLANES == 2 ? 2 : 1 << 28;  // blocks of k per accumulator
-    static constexpr int kAccs = PLANES == 2 ? 512 / BN : 2;
+    static constexpr int kAccs = PLANES == 2 ? 3 : 2;
+    static constexpr int kCross = kAccs * BN;                 // the cross products' columns of TMEM
+    static constexpr int kColumns = PLANES == 2 ? 4 * BN : 2 * BN;
     static_assert(PLANES == 1 || BN == 128, "the chunks' sums have to fit the epilogue's registers");
     static constexpr int kA = kBM * kBK * 2;              // bytes of one plane of A per stage
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
@@ -863,7 +870,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
     // (an offset, not a rounded pointer: the compiler keeps knowing that this is shared memory)
     unsigned char *smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float *stage_epi = reinterpret_cast<float *>(smem + C::kStages * C::kStage);
-    __shared__ uint64_t bars[2 * C::kStages + 2 * C::kAccs + C::kTiles * kEpiWarps];
+    __shared__ uint64_t bars[2 * C::kStages + 2 * C::kAccs + 1 + C::kTiles * kEpiWarps];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int failed;
 
@@ -872,18 +879,18 @@ void gemm_kernel(const __grid_constant__ Work work) {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(cta));
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const uint32_t full = smem_u32(bars), empty = full + 8 * C::kStages, acc_full = empty + 8 * C::kStages,
-                   acc_empty = acc_full + 8 * C::kAccs;
+                   acc_empty = acc_full + 8 * C::kAccs, cross_empty = acc_empty + 8 * C::kAccs;
 
-    if (threadIdx.x < 2 * C::kStages + 2 * C::kAccs + C::kTiles * kEpiWarps) {
+    if (threadIdx.x < 2 * C::kStages + 2 * C::kAccs + 1 + C::kTiles * kEpiWarps) {
         const int i = threadIdx.x, k = i - (2 * C::kStages + C::kAccs);
         // accumulators free: every epilogue warp of both CTAs arrives
-        bar_init(full + 8 * i, k >= 0 && k < C::kAccs ? 2 * kEpiWarps : 1);
+        bar_init(full + 8 * i, k >= 0 && k <= C::kAccs ? 2 * kEpiWarps : 1);
         if (i == 0) failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)),
-                     "r"(C::kAccs * BN) : "memory");
+                     "r"(C::kColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -944,16 +951,21 @@ void gemm_kernel(const __grid_constant__ Work work) {
     } else if (warp == kMmaWarp && cta == 0) {
         // ---- products (for the pair) ----
         int s = 0, buf = 0;
-        uint32_t phase = 0, acc_phase = 0;
+        uint32_t phase = 0, acc_phase = 0, cross_phase = 0;
         bool ok = true;
         for (int t = pair; ok && t < total; t += pairs) {
             const Job j = work.template job<BN>(t, cur);
+            if (PLANES == 2) {
+                ok = warp_wait(cross_empty, cross_phase ^ 1, &failed);
+                cross_phase ^= 1;
+                if (!ok) break;
+            }
             const uint32_t a_step = j.a_mn ? 128u : 2u, b_step = j.b_mn ? 128u : 2u;  // 16 of k, in 16-byte units
             const uint32_t a_lbo = j.a_mn ? 8192u : 16u, b_lbo = j.b_mn ? 8192u : 16u;
             const uint32_t idesc = work.types | (static_cast<uint32_t>(j.a_mn) << 15) | (static_cast<uint32_t>(j.b_mn) << 16) |
                                    (static_cast<uint32_t>(j.width >> 3) << 17);
-            for (int k0 = j.kb0; ok && k0 < j.kb1; k0 = k0 + C::kChunk < j.kb1 ? k0 + C::kChunk : j.kb1) {
-                const int k1 = min(j.kb1, k0 + C::kChunk);
+            for (int k0 = j.kb0; ok && k0 < j.kb1; k0 = k0 + j.per_acc < j.kb1 ? k0 + j.per_acc : j.kb1) {
+                const int k1 = min(j.kb1, k0 + j.per_acc);
                 ok = warp_wait(acc_empty + 8 * buf, acc_phase ^ 1, &failed);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -974,8 +986,9 @@ void gemm_kernel(const __grid_constant__ Work work) {
                         for (int i = 0; i < kBK / 16; ++i) {
                             mma_f16(d, da[0] + i * a_step, db[0] + i * b_step, idesc, kb != k0 || i != 0);
                             if (PLANES == 2) {
-                                mma_f16(d, da[0] + i * a_step, db[PLANES - 1] + i * b_step, idesc, 1);
-                                mma_f16(d, da[PLANES - 1] + i * a_step, db[0] + i * b_step, idesc, 1);
+                                mma_f16(tmem + C::kCross, da[0] + i * a_step, db[PLANES - 1] + i * b_step, idesc,
+                                        kb != j.kb0 || i != 0);
+                                mma_f16(tmem + C::kCross, da[PLANES - 1] + i * a_step, db[0] + i * b_step, idesc, 1);
                             }
                         }
                         mma_commit(empty + 8 * s);
@@ -990,7 +1003,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        EpiWarp w{stage_epi + warp * C::kTiles * 1024, acc_empty + 8 * C::kAccs + 8 * warp * C::kTiles, 0, &failed, lane};
+        EpiWarp w{stage_epi + warp * C::kTiles * 1024, cross_empty + 8 + 8 * warp * C::kTiles, 0, &failed, lane};
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -1024,20 +1037,26 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[q][i] = 0.0f;
-                for (int k0 = j.kb0; k0 < j.kb1; k0 += C::kChunk) {
+                auto add = [&](uint32_t columns) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        float v[32];
+                        tmem_read32(v, tmem + columns + lanes + half + 32 * q);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) sum[q][i] += v[i];
+                    }
+                };
+                for (int k0 = j.kb0; k0 < j.kb1; k0 += j.per_acc) {
                     if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok && any) {
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            float v[32];
-                            tmem_read32(v, tmem + buf * BN + lanes + half + 32 * q);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) sum[q][i] += v[i];
-                        }
-                    }
+                    if (ok && any) add(buf * BN);
                     next_acc();
                 }
+                // the last chunk's barrier covers the cross products too
+                if (ok && any) add(C::kCross);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive_cta0(cross_empty);
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     const int c = half + 32 * q;
@@ -1076,7 +1095,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
     cluster_sync();
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kAccs * BN));
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kColumns));
     }
 }
 
@@ -1200,6 +1219,7 @@ int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Ep
     w.splits = splits;
     w.a_mn = a.mn_major;
     w.b_mn = b.mn_major;
+    w.per_acc = PLANES == 1 ? 1 << 28 : splits > 1 ? 3 : 6;  // (split: the Gram form's first product)
     w.grid = tile_grid(s, BN, s.batch * splits);
     w.types = instruction_types(s.kind);
     w.epi = epi;
