@@ -1240,12 +1240,15 @@ int check_shape(const GemmShape &s) {
 }
 
 // 256-wide or 128-wide tiles: whichever needs less time on the slowest pair of
-// SMs, 256 when equal (half the loads of A per product).
+// SMs.  A 256-wide tile takes 1.6 times a 128-wide one, whose loads (62 bytes per
+// clock and SM instead of 43) the L2 does not deliver at the full matrix rate:
+// 29649 x 1024 x 4608 took 360 us in 128-wide tiles, 13 rounds of them, and
+// 200 us in 256-wide ones, 7 rounds.
 bool wide_tiles(const GemmShape &s) {
     const int64_t pairs = sm_pairs();
     const int64_t wide = (tile_count(s, 256) * s.batch + pairs - 1) / pairs;
     const int64_t narrow = (tile_count(s, 128) * s.batch + pairs - 1) / pairs;
-    return 2 * wide <= narrow;
+    return 8 * wide <= 5 * narrow;
 }
 
 template <typename T>

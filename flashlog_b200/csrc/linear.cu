@@ -41,12 +41,23 @@ __device__ __forceinline__ float block_max(float v, float *scratch) {
     return r;
 }
 
-// One block per row: the row's exponent, then its planes (second read from L1/L2).
-__global__ void pack_rows_kernel(const float *src, int64_t ld, int64_t cols, __half *out, int64_t ldp, int64_t plane,
-                                 int *exps) {
+// One block per row: the row's exponent, then its planes (second read from
+// L1/L2).  One or two matrices per launch.
+struct PackRows {
+    const float *src;
+    int64_t ld, rows;
+    __half *out;
+    int64_t plane;
+    int *exps;
+};
+__global__ void pack_rows_kernel(const PackRows a, const PackRows b, int64_t cols, int64_t ldp) {
     __shared__ float scratch[32];
-    const int64_t r = blockIdx.x;
-    const float *row = src + r * ld;
+    const bool second = static_cast<int64_t>(blockIdx.x) >= a.rows;
+    const PackRows &p = second ? b : a;
+    const int64_t r = second ? blockIdx.x - a.rows : blockIdx.x, ld = p.ld, plane = p.plane;
+    const float *src = p.src, *row = src + r * ld;
+    __half *out = p.out;
+    int *exps = p.exps;
     const bool vec = ((reinterpret_cast<uintptr_t>(src) & 15) == 0) && (ld & 3) == 0;
     const int64_t quads = vec ? cols >> 2 : 0;
     float mx = 0.0f;
@@ -95,17 +106,18 @@ __global__ void col_absmax_kernel(const float *src, int64_t ld, int64_t rows, in
     }
 }
 
-__global__ void col_exponent_kernel(const unsigned *bits, int *exps, int64_t n) {
-    const int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
-    if (i < n) exps[i] = line_exponent(__uint_as_float(bits[i]));
-}
-
-// Planes of a matrix scaled per column; 64 columns x 32 rows per block.
-__global__ void pack_cols_kernel(const float *src, int64_t ld, int64_t rows, int64_t cols, const int *exps,
+// Planes of a matrix scaled per column; 64 columns x 32 rows per block.  The
+// first rows' blocks also write the exponents.
+__global__ void pack_cols_kernel(const float *src, int64_t ld, int64_t rows, int64_t cols, const unsigned *bits, int *exps,
                                  __half *out, int64_t ldp, int64_t plane) {
     const int64_t c = blockIdx.x * int64_t(64) + 2 * threadIdx.x;
     if (c >= cols) return;
-    const int e0 = exps[c], e1 = c + 1 < cols ? exps[c + 1] : 0;
+    const int e0 = line_exponent(__uint_as_float(bits[c]));
+    const int e1 = c + 1 < cols ? line_exponent(__uint_as_float(bits[c + 1])) : 0;
+    if (exps != nullptr && blockIdx.y == 0 && threadIdx.y == 0) {
+        exps[c] = e0;
+        if (c + 1 < cols) exps[c + 1] = e1;
+    }
     const bool vec = ((reinterpret_cast<uintptr_t>(src) & 7) == 0) && (ld & 1) == 0 && c + 1 < cols;
     const int64_t r1 = min(rows, (blockIdx.y + int64_t(1)) * 32);
     for (int64_t r = blockIdx.y * int64_t(32) + threadIdx.y; r < r1; r += 8) {
@@ -133,27 +145,58 @@ __global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uin
 }
 
 // dz = gy * act'(z), written as T with pitch ldo (or not at all), and its
-// column sums over kSumRows rows at a time, taken before the rounding.
+// column sums over kSumRows rows at a time, taken before the rounding.  A block
+// takes 64 columns, eight loads per thread in flight.
 template <typename T>
 __global__ void dz_kernel(const T *gy, int64_t ld_gy, const float *z, int64_t rows, int64_t n, int act, T *out,
                           int64_t ldo, float *partial) {
-    __shared__ float part[8][33];
-    const int64_t c = blockIdx.x * int64_t(32) + threadIdx.x;
+    __shared__ float part[8][65];
+    const int64_t c0 = blockIdx.x * int64_t(64) + threadIdx.x;
     const int64_t r0 = blockIdx.y * int64_t(kSumRows), r1 = min(rows, r0 + kSumRows);
-    float sum = 0.0f;
-    if (c < n)
-        for (int64_t r = r0 + threadIdx.y; r < r1; r += 8) {
-            float d = to_f32<T>(gy[r * ld_gy + c]);
-            if (act != kActNone) d *= act_slope(z[r * n + c], act);
-            if (out != nullptr) out[r * ldo + c] = from_f32<T>(d);
-            sum += d;
-        }
-    part[threadIdx.y][threadIdx.x] = sum;
-    __syncthreads();
-    if (partial != nullptr && threadIdx.y == 0 && c < n) {
+    float sum[2] = {0.0f, 0.0f};
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += 32) {
+        float d[4][2];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) sum += part[i][threadIdx.x];
-        partial[blockIdx.y * n + c] = sum;
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const int64_t row = r + 8 * k, c = c0 + 32 * w;
+                d[k][w] = row < r1 && c < n ? to_f32<T>(gy[row * ld_gy + c]) : 0.0f;
+            }
+        if (act != kActNone) {
+            float s[4][2];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const int64_t row = r + 8 * k, c = c0 + 32 * w;
+                    s[k][w] = row < r1 && c < n ? z[row * n + c] : 0.0f;
+                }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    if (r + 8 * k < r1) d[k][w] *= act_slope(s[k][w], act);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const int64_t row = r + 8 * k, c = c0 + 32 * w;
+                if (out != nullptr && row < r1 && c < n) out[row * ldo + c] = from_f32<T>(d[k][w]);
+                sum[w] += d[k][w];
+            }
+    }
+    if (partial == nullptr) return;
+    part[threadIdx.y][threadIdx.x] = sum[0];
+    part[threadIdx.y][threadIdx.x + 32] = sum[1];
+    __syncthreads();
+    const int c = threadIdx.y * 32 + threadIdx.x;
+    if (c < 64 && blockIdx.x * int64_t(64) + c < n) {
+        float s = part[0][c];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += part[i][c];
+        partial[blockIdx.y * n + blockIdx.x * int64_t(64) + c] = s;
     }
 }
 
@@ -257,13 +300,14 @@ struct SmallArgs {
     int act;
 };
 
+constexpr int kT = 32, kPitch = 36;
+
 template <typename T, int MODE>
-__global__ void __launch_bounds__(128) small_gemm_kernel(const SmallArgs p) {
-    constexpr int kT = 32, kPitch = 36;
-    __shared__ __align__(16) float As[kT][kPitch], Bs[kT][kPitch];
+__device__ __forceinline__ void small_tile(const SmallArgs &p, int bx, int by, int bz, float (&As)[kT][kPitch],
+                                           float (&Bs)[kT][kPitch]) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t i0 = blockIdx.y * int64_t(kT), j0 = blockIdx.x * int64_t(kT);
-    const int64_t k0 = blockIdx.z * p.chunk, k1 = min(p.k, k0 + p.chunk);
+    const int64_t i0 = by * int64_t(kT), j0 = bx * int64_t(kT);
+    const int64_t k0 = bz * p.chunk, k1 = min(p.k, k0 + p.chunk);
     constexpr bool kAT = MODE == kGradW, kBT = MODE != kForward;  // the output index is contiguous
     constexpr bool kDz = MODE != kForward;
     // line e of the thread's eight is 4 e lines on; a tile further in k is one step
@@ -326,9 +370,9 @@ __global__ void __launch_bounds__(128) small_gemm_kernel(const SmallArgs p) {
     for (int u = 0; u < 2; ++u) {
         const int64_t i = i0 + ti + u;
         if (i >= p.m) continue;
-        const bool owns_sum = MODE == kGradW && blockIdx.x == 0 && tj == 0;
+        const bool owns_sum = MODE == kGradW && bx == 0 && tj == 0;
         if (p.partial != nullptr) {
-            float *q = p.partial + (blockIdx.z * p.m + i) * (p.n + 1);
+            float *q = p.partial + (bz * p.m + i) * (p.n + 1);
 #pragma unroll
             for (int v = 0; v < 4; ++v)
                 if (j0 + tj + v < p.n) q[j0 + tj + v] = acc[u][v];
@@ -354,17 +398,46 @@ __global__ void __launch_bounds__(128) small_gemm_kernel(const SmallArgs p) {
 }
 
 template <typename T>
-__global__ void reduce_kernel(const float *partial, int64_t splits, int64_t m, int64_t n, T *out, T *sum_out) {
-    const int64_t t = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
-    if (t >= m * (n + 1)) return;
-    const int64_t i = t / (n + 1), j = t - i * (n + 1);
-    float s = 0.0f;
-    for (int64_t q = 0; q < splits; ++q) s += partial[q * m * (n + 1) + t];
-    if (j < n) {
-        if (out != nullptr) out[i * n + j] = from_f32<T>(s);
-    } else if (sum_out != nullptr) {
-        sum_out[i] = from_f32<T>(s);
+__global__ void __launch_bounds__(128) small_forward_kernel(const SmallArgs p) {
+    __shared__ __align__(16) float As[kT][kPitch], Bs[kT][kPitch];
+    small_tile<T, kForward>(p, blockIdx.x, blockIdx.y, 0, As, Bs);
+}
+
+// Both gradients in one launch: the blocks below `split` are dx's tiles.
+struct GradGrid {
+    int tiles_x, tiles_w, per_x, per_w, split;  // tiles along the output's columns, tiles per part of k
+};
+template <typename T>
+__global__ void __launch_bounds__(128) small_backward_kernel(const SmallArgs x, const SmallArgs w, const GradGrid g) {
+    __shared__ __align__(16) float As[kT][kPitch], Bs[kT][kPitch];
+    const int b = blockIdx.x;
+    if (b < g.split) {
+        const int r = b % g.per_x;
+        small_tile<T, kGradX>(x, r % g.tiles_x, r / g.tiles_x, b / g.per_x, As, Bs);
+    } else {
+        const int c = b - g.split, r = c % g.per_w;
+        small_tile<T, kGradW>(w, r % g.tiles_w, r / g.tiles_w, c / g.per_w, As, Bs);
     }
+}
+
+// The parts of both gradients, added in order: elements below `count_x` are dx's.
+template <typename T>
+__device__ __forceinline__ void reduce_one(const SmallArgs &p, int64_t splits, int64_t t) {
+    const int64_t i = t / (p.n + 1), j = t - i * (p.n + 1);
+    float s = 0.0f;
+    for (int64_t q = 0; q < splits; ++q) s += p.partial[q * p.m * (p.n + 1) + t];
+    if (j < p.n) {
+        if (p.out != nullptr) static_cast<T *>(p.out)[i * p.n + j] = from_f32<T>(s);
+    } else if (p.sum_out != nullptr) {
+        static_cast<T *>(p.sum_out)[i] = from_f32<T>(s);
+    }
+}
+template <typename T>
+__global__ void reduce_kernel(const SmallArgs x, int64_t splits_x, int64_t count_x, const SmallArgs w, int64_t splits_w,
+                              int64_t count_w) {
+    const int64_t t = blockIdx.x * int64_t(blockDim.x) + threadIdx.x;
+    if (t < count_x) reduce_one<T>(x, splits_x, t);
+    else if (t - count_x < count_w) reduce_one<T>(w, splits_w, t - count_x);
 }
 
 // ---- host side -------------------------------------------------------------
@@ -389,10 +462,10 @@ size_t split_bytes(int64_t m, int64_t n, int64_t k) {
 }
 
 // Which path: microseconds as measured.  A small product takes 2.5 and, for
-// every 32 of k, 0.8, or its operations at 12 TFLOP/s where there are many; the
-// tensor path 11.5 in fp32 (two packs and the product), 5.5 in 16 bits when TMA
-// takes the operands as they are and 9 when it does not, and for the gradients
-// 55 and 22 in all.
+// every 32 of k, 0.8, or its operations at 12 TFLOP/s where there are many.  The
+// tensor path takes 12 in fp32 (the packing and the product) on the device and
+// 19 to launch; 5.5 in 16 bits when TMA takes the operands as they are and 9 when
+// it does not; for the gradients 55 and 22 in all.
 bool is_few_rows(int64_t rows, int dtype) { return rows <= (dtype == FL_F32 ? 16 : 8); }
 double small_us(int64_t m, int64_t n, int64_t k, int64_t chunk, bool reduced) {
     const double steps = 0.8 * static_cast<double>((chunk + 31) / 32);
@@ -400,7 +473,7 @@ double small_us(int64_t m, int64_t n, int64_t k, int64_t chunk, bool reduced) {
     return 2.5 + (steps > ops ? steps : ops) + (reduced ? 3.0 : 0.0);
 }
 bool is_small(int64_t rows, int64_t n, int64_t k, int dtype) {
-    return small_us(rows, n, k, k, false) <= (dtype == FL_F32 ? 11.5 : k % 8 == 0 ? 5.5 : 9.0);
+    return small_us(rows, n, k, k, false) <= (dtype == FL_F32 ? 16.0 : k % 8 == 0 ? 5.5 : 9.0);
 }
 bool is_small_backward(int64_t rows, int64_t n, int64_t k, int dtype) {
     const Split x = split_of(rows, k, n), w = split_of(n, k, rows);
@@ -418,7 +491,7 @@ size_t operand_bytes(int64_t lines, int64_t inner, int64_t exps, int dtype) {
 // Readies the matrix src [lines, inner] as a product operand.  by_line: the
 // uncontracted index is the line (K-major), else the inner index (MN-major).
 int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool by_line, int dtype, Carve &ws,
-                 GemmOperand *op, const int **exps, cudaStream_t st) {
+                 GemmOperand *op, const int **exps, cudaStream_t st, PackRows *pending = nullptr) {
     op->batch = 0;
     op->mn_major = by_line ? 0 : 1;
     *exps = nullptr;
@@ -449,8 +522,9 @@ int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool
     FL_REQUIRE(out != nullptr && ex != nullptr, "linear: workspace too small");
     const float *x = static_cast<const float *>(src);
     if (by_line) {
-        launch(pack_rows_kernel, static_cast<unsigned>(lines), inner > 2048 ? 512 : 128, 0, st, x, ld, inner, out, ldp,
-               plane, ex);
+        const PackRows a{x, ld, lines, out, plane, ex};
+        if (pending != nullptr) *pending = a;  // the caller packs it together with another
+        else launch(pack_rows_kernel, static_cast<unsigned>(lines), inner > 2048 ? 512 : 128, 0, st, a, a, inner, ldp);
     } else {
         unsigned *bits = ws.take<unsigned>(inner);
         FL_REQUIRE(bits != nullptr, "linear: workspace too small");
@@ -460,11 +534,10 @@ int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool
         launch(col_absmax_kernel, dim3(static_cast<unsigned>((inner + 31) / 32),
                                        static_cast<unsigned>((lines + chunk - 1) / chunk)),
                dim3(32, 8), 0, st, x, ld, lines, inner, chunk, bits);
-        launch(col_exponent_kernel, static_cast<unsigned>((inner + 255) / 256), 256, 0, st, bits, ex, inner);
         for (int64_t r = 0; r < lines; r += 65535 * 32) {
             const int64_t cnt = lines - r < 65535 * 32 ? lines - r : 65535 * 32;
             launch(pack_cols_kernel, dim3(static_cast<unsigned>((inner + 63) / 64), static_cast<unsigned>((cnt + 31) / 32)),
-                   dim3(32, 8), 0, st, x + r * ld, ld, cnt, inner, ex, out + r * ldp, ldp, plane);
+                   dim3(32, 8), 0, st, x + r * ld, ld, cnt, inner, bits, r == 0 ? ex : nullptr, out + r * ldp, ldp, plane);
         }
     }
     op->ptr = out;
@@ -515,7 +588,7 @@ int linear_dz(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy,
     // grid.y (row groups) is limited to 65535: 8 million rows
     const int64_t parts = (p->rows + kSumRows - 1) / kSumRows;
     FL_REQUIRE(parts <= 65535, "linear: more than %d rows in a backward pass", 65535 * kSumRows);
-    launch(dz_kernel<T>, dim3(static_cast<unsigned>((p->n + 31) / 32), static_cast<unsigned>(parts)), dim3(32, 8), 0, st,
+    launch(dz_kernel<T>, dim3(static_cast<unsigned>((p->n + 63) / 64), static_cast<unsigned>(parts)), dim3(32, 8), 0, st,
            static_cast<const T *>(gy), ld_gy, z, p->rows, p->n, p->act, out, ldo, partial);
     return check_launch("linear dz");
 }
@@ -556,26 +629,9 @@ int small_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, cudaStrea
     a.z_out = z;
     a.act = p->act;
     FL_REQUIRE((a.m + 31) / 32 <= 65535, "linear: too many rows");
-    launch(small_gemm_kernel<T, kForward>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32)),
+    launch(small_forward_kernel<T>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32)),
            128, 0, st, a);
     return check_launch("linear");
-}
-
-template <typename T, int MODE>
-int small_grad(SmallArgs a, Carve &ws, cudaStream_t st) {
-    const Split s = split_of(a.m, a.n, a.k);
-    a.chunk = s.chunk;
-    if (s.splits > 1) {
-        a.partial = ws.take<float>(s.splits * a.m * (a.n + 1));
-        FL_REQUIRE(a.partial != nullptr, "linear backward: workspace too small");
-    }
-    FL_REQUIRE((a.m + 31) / 32 <= 65535, "linear backward: too many rows");
-    launch(small_gemm_kernel<T, MODE>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32),
-                                            static_cast<unsigned>(s.splits)), 128, 0, st, a);
-    if (s.splits > 1)
-        launch(reduce_kernel<T>, static_cast<unsigned>((a.m * (a.n + 1) + 255) / 256), 256, 0, st, a.partial, s.splits, a.m,
-               a.n, static_cast<T *>(a.out), static_cast<T *>(MODE == kGradW ? a.sum_out : nullptr));
-    return check_launch("linear backward");
 }
 
 template <typename T>
@@ -587,29 +643,58 @@ int small_backward(const fl_linear *p, const float *z, const void *gy, int64_t l
     a.z = z;
     a.ld_z = p->n;
     a.act = p->act;
+    SmallArgs x = a, w = a;
+    GradGrid g{1, 1, 1, 1, 0};
+    Split sx{1, 0}, sw{1, 0};
+    int64_t blocks_w = 0;
+    const bool want_w = dw != nullptr || dbias != nullptr;
+    auto plan = [&](SmallArgs &q, Split &s, int &tiles, int &per) -> int {
+        s = split_of(q.m, q.n, q.k);
+        q.chunk = s.chunk;
+        tiles = static_cast<int>((q.n + kT - 1) / kT);
+        const int64_t all = tiles * ((q.m + kT - 1) / kT);
+        FL_REQUIRE(all * s.splits < (1ll << 30), "linear backward: too many tiles");
+        per = static_cast<int>(all);
+        if (s.splits > 1) {
+            q.partial = ws.take<float>(s.splits * q.m * (q.n + 1));
+            FL_REQUIRE(q.partial != nullptr, "linear backward: workspace too small");
+        }
+        return FL_OK;
+    };
     int rc = FL_OK;
     if (dx != nullptr) {
-        a.b = p->w;
-        a.ld_b = p->ld_w;
-        a.m = p->rows;
-        a.n = p->k;
-        a.k = p->n;
-        a.out = dx;
-        a.ld_out = p->k;
-        rc = small_grad<T, kGradX>(a, ws, st);
+        x.b = p->w;
+        x.ld_b = p->ld_w;
+        x.m = p->rows;
+        x.n = p->k;
+        x.k = p->n;
+        x.out = dx;
+        x.ld_out = p->k;
+        rc = plan(x, sx, g.tiles_x, g.per_x);
+        if (rc) return rc;
+        g.split = static_cast<int>(g.per_x * sx.splits);
     }
-    if (!rc && (dw != nullptr || dbias != nullptr)) {
-        a.b = p->x;
-        a.ld_b = p->ld_x;
-        a.m = p->n;
-        a.n = p->k;
-        a.k = p->rows;
-        a.out = dw;
-        a.ld_out = p->k;
-        a.sum_out = dbias;
-        rc = small_grad<T, kGradW>(a, ws, st);
+    if (want_w) {
+        w.b = p->x;
+        w.ld_b = p->ld_x;
+        w.m = p->n;
+        w.n = p->k;
+        w.k = p->rows;
+        w.out = dw;
+        w.ld_out = p->k;
+        w.sum_out = dbias;
+        rc = plan(w, sw, g.tiles_w, g.per_w);
+        if (rc) return rc;
+        blocks_w = g.per_w * sw.splits;
     }
-    return rc;
+    if (g.split + blocks_w == 0) return FL_OK;
+    launch(small_backward_kernel<T>, static_cast<unsigned>(g.split + blocks_w), 128, 0, st, x, w, g);
+    const int64_t count_x = dx != nullptr && sx.splits > 1 ? x.m * (x.n + 1) : 0;
+    const int64_t count_w = want_w && sw.splits > 1 ? w.m * (w.n + 1) : 0;
+    if (count_x + count_w > 0)
+        launch(reduce_kernel<T>, static_cast<unsigned>((count_x + count_w + 255) / 256), 256, 0, st, x, sx.splits, count_x, w,
+               sw.splits, count_w);
+    return check_launch("linear backward");
 }
 
 }  // namespace
@@ -632,9 +717,15 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
     Carve ws(wsp, ws_bytes);
     GemmOperand a, b;
     const int *ea, *eb;
-    rc = make_operand(p->x, p->ld_x, p->rows, p->k, true, p->dtype, ws, &a, &ea, st);
-    if (!rc) rc = make_operand(p->w, p->ld_w, p->n, p->k, true, p->dtype, ws, &b, &eb, st);
+    PackRows px{}, pw{};
+    rc = make_operand(p->x, p->ld_x, p->rows, p->k, true, p->dtype, ws, &a, &ea, st, &px);
+    if (!rc) rc = make_operand(p->w, p->ld_w, p->n, p->k, true, p->dtype, ws, &b, &eb, st, &pw);
     if (rc) return rc;
+    if (p->dtype == FL_F32) {
+        FL_REQUIRE(p->rows + p->n < (1ll << 31), "linear: bad shape");
+        launch(pack_rows_kernel, static_cast<unsigned>(p->rows + p->n), p->k > 2048 ? 512 : 128, 0, st, px, pw, p->k,
+               round8(p->k));
+    }
     LinearEpilogue e = plain_epilogue(y, ld_y, p->dtype, ea, eb);
     e.bias = p->bias;
     e.residual = p->residual;
@@ -649,7 +740,7 @@ size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, 
     if (rows <= 0 || n <= 0 || k <= 0) return 0;
     if (is_small_backward(rows, n, k, dtype)) return split_bytes(rows, k, n) + split_bytes(n, k, rows) + 256;
     size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
-    if (act != FL_ACT_NONE) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
+    if (act != FL_ACT_NONE || dtype != FL_F32) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
     const size_t ops = operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
     return dz + ops + carve_bytes<float>(((rows + kSumRows - 1) / kSumRows) * n);
 }
@@ -674,10 +765,12 @@ int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t 
     }
     const void *dz = gy;
     int64_t ld_dz = ld_gy;
-    if (p->act != FL_ACT_NONE || dbias != nullptr) {
+    // 16-bit gradients whose rows TMA cannot take are copied to an aligned pitch in the same pass
+    const bool copies = p->dtype != FL_F32 && !tma_ready(gy, ld_gy) && (dx != nullptr || dw != nullptr);
+    if (p->act != FL_ACT_NONE || dbias != nullptr || copies) {
         void *out = nullptr;
         const int64_t ldo = round8(p->n);
-        if (p->act != FL_ACT_NONE) {
+        if (p->act != FL_ACT_NONE || copies) {
             out = ws.take<char>(p->rows * ldo * es);
             FL_REQUIRE(out != nullptr, "linear backward: workspace too small");
             dz = out;
