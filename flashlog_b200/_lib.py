@@ -11,6 +11,7 @@ import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libflashlog_b200.so")
+BIND_PATH = os.path.join(HERE, "_bind.so")  # csrc/bind.cpp: torch tensors and autograd around the C ABI
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["api.cu", "scan.cu", "topc.cu", "hop.cu", "rules.cu", "csr.cu", "readout.cu", "masks.cu",
            "gemm.cu", "linear.cu", "weights.cu", "muon.cu"]
@@ -63,6 +64,36 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+def build_bind(force: bool = False, verbose: bool = False) -> str:
+    """Compile csrc/bind.cpp against torch's headers into flashlog_b200/_bind.so (needs the library: build first)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "bind.cpp")
+    deps = [src, os.path.join(os.path.dirname(HERE), "include", "flashlog_b200.h")]
+    stamp = BIND_PATH + ".torch"  # the torch it was compiled against
+    if not force and os.path.exists(BIND_PATH) and os.path.exists(stamp):
+        t = os.path.getmtime(BIND_PATH)
+        if all(os.path.getmtime(d) <= t for d in deps) and open(stamp).read() == torch.__version__:
+            return BIND_PATH
+    tmp = BIND_PATH + f".tmp{os.getpid()}"
+    torch_libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    # the system's compiler, as for the library: libstdc++ has to be the process' own
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_bind",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *("-isystem" + p for p in cpp_extension.include_paths("cuda")), "-I" + sysconfig.get_paths()["include"], src,
+           "-o", tmp, "-L" + HERE, "-l:" + os.path.basename(LIB_PATH), "-L" + torch_libs, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True, cwd=CSRC)
+    os.replace(tmp, BIND_PATH)
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
+    return BIND_PATH
+
+
 class fl_csr_side(ctypes.Structure):
     _fields_ = [("row_ptr", ctypes.c_void_p), ("col", ctypes.c_void_p), ("order", ctypes.c_void_p),
                 ("group_ptr", ctypes.c_void_p), ("group_start", ctypes.c_void_p),
@@ -94,34 +125,7 @@ class fl_dropout(ctypes.Structure):
 
 _DROP = ctypes.POINTER(fl_dropout)
 
-
-class fl_linear(ctypes.Structure):
-    """Mirror of fl_linear (include/flashlog_b200.h): the operands of the relation head."""
-    _fields_ = [("x", _P), ("w", _P), ("bias", _P), ("residual", _P), ("ld_x", _I64), ("ld_w", _I64),
-                ("ld_res", _I64), ("rows", _I64), ("n", _I64), ("k", _I64), ("dtype", ctypes.c_int),
-                ("act", ctypes.c_int)]
-
-
-_LINEAR = ctypes.POINTER(fl_linear)
-
-
-class fl_weights(ctypes.Structure):
-    """Mirror of fl_weights (include/flashlog_b200.h): logits and the rules applied to them."""
-    _fields_ = [("logits", _P), ("bias", _P), ("mask", _P), ("states", _P), ("history", _P), ("ld", _I64),
-                ("bias_ld", _I64), ("mask_ld", _I64), ("n_states", _I64), ("hist_ld", _I64), ("hist", _I64),
-                ("rows", _I64), ("n", _I64), ("tau", ctypes.c_double), ("repetition", ctypes.c_double),
-                ("frequency", ctypes.c_double), ("presence", ctypes.c_double), ("dtype", ctypes.c_int)]
-
-
-_WEIGHTS = ctypes.POINTER(fl_weights)
-
-
-class fl_matrices(ctypes.Structure):
-    """Mirror of fl_matrices (include/flashlog_b200.h): a strided batch of matrices."""
-    _fields_ = [("ptr", _P), ("stride_b1", _I64), ("stride_b2", _I64), ("stride_i", _I64), ("stride_j", _I64)]
-
-
-_MATRICES = ctypes.POINTER(fl_matrices)
+# The attention operators' structures are built by csrc/bind.cpp; from Python they pass as plain pointers.
 _D = ctypes.c_double
 
 # name -> (restype, argtypes)
@@ -186,16 +190,16 @@ SIGNATURES = {
                                          _P]),
     "fl_filtered_ranks_noalloc": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _I64, _I64, _I64, ctypes.c_int, _P, _P]),
     "fl_linear_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int]),
-    "fl_linear_forward": (ctypes.c_int, [_LINEAR, _P, _I64, _P, _P, _SZ, _P]),
+    "fl_linear_forward": (ctypes.c_int, [_P, _P, _I64, _P, _P, _SZ, _P]),
     "fl_linear_backward_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int, ctypes.c_int]),
-    "fl_linear_backward": (ctypes.c_int, [_LINEAR, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
-    "fl_relation_weights": (ctypes.c_int, [_WEIGHTS, _P, _P]),
+    "fl_linear_backward": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "fl_relation_weights": (ctypes.c_int, [_P, _P, _P]),
     "fl_relation_weights_workspace": (_SZ, [_I64, _I64]),
-    "fl_relation_weights_backward": (ctypes.c_int, [_WEIGHTS, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
+    "fl_relation_weights_backward": (ctypes.c_int, [_P, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
     "fl_newton_schulz_workspace": (_SZ, [_I64, _I64, _I64, ctypes.c_int]),
-    "fl_orthogonalize": (ctypes.c_int, [_MATRICES, _MATRICES, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int,
+    "fl_orthogonalize": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, _I64, ctypes.c_int, ctypes.c_int,
                                         _D, _D, _D, _D, _P, _SZ, _P]),
-    "fl_muon_update": (ctypes.c_int, [_MATRICES, _MATRICES, _MATRICES, _MATRICES, _MATRICES, _I64, _I64, _I64, _I64,
+    "fl_muon_update": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                       _D, _D, ctypes.c_int, _D, _D, ctypes.c_int, _D, _D, _D, _D, _P, _P, _SZ, _P]),
     "fl_gemm_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
 }
@@ -217,6 +221,24 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_bind = None
+
+
+def bind():
+    """The torch binding of the attention operators (raises if it was not built)."""
+    global _bind
+    if _bind is None:
+        if not os.path.exists(BIND_PATH):
+            raise RuntimeError(f"{BIND_PATH} is missing: build it with flashlog_b200._lib.build_bind() "
+                               "(there is no fallback)")
+        lib()  # _bind.so is linked against it
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("flashlog_b200._bind", BIND_PATH)
+        _bind = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_bind)
+    return _bind
 
 
 class FlashLogError(RuntimeError):

@@ -21,6 +21,7 @@ import math
 import torch
 
 from . import ops
+from ._lib import bind
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -54,7 +55,7 @@ def orthogonalize(update, steps: int = 5, coefficients=COEFFICIENTS, eps: float 
         raise ValueError(f"orthogonalize takes float32, float16 or bfloat16 matrices, got {update.dtype}")
     _check_matrix("orthogonalize", update)
     steps, coefficients, eps = _check("orthogonalize", steps, coefficients, eps)
-    return ops.orthogonalize(update, steps, coefficients, eps)
+    return bind().orthogonalize(update, steps, coefficients, eps)
 
 
 def _check_gate(gate):
@@ -62,7 +63,7 @@ def _check_gate(gate):
         raise ValueError("muon_update: gate must be one float32")
 
 
-def _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps):
+def _muon_args(param, grad, momentum, lr, beta, nesterov, weight_decay, scale, steps, coefficients, eps):
     _check_matrix("muon_update", param)
     for name, t in (("param", param), ("grad", grad), ("momentum", momentum)):
         if t.dtype != torch.float32 or t.shape != param.shape:
@@ -77,8 +78,7 @@ def _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coef
     scale = math.sqrt(max(1.0, m / n)) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"muon_update: scale must be finite, got {scale}")
-    return dict(lr=lr, beta=beta, weight_decay=weight_decay, scale=scale, steps=steps, coefficients=coefficients,
-                eps=eps)
+    return lr, beta, bool(nesterov), weight_decay, scale, steps, coefficients, eps
 
 
 def _overlaps_itself(t):
@@ -104,9 +104,9 @@ def muon_update(param, grad, momentum, *, lr: float, beta: float = 0.95, nestero
     scale defaults to sqrt(max(1, m / n)).  gate (a float32 on the device): where it holds 0 -- a step that
     failed, found on the device -- both come out as they went in.  Returns (param', momentum') as new tensors."""
     _check_gate(gate)
-    args = _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps)
+    args = _muon_args(param, grad, momentum, lr, beta, nesterov, weight_decay, scale, steps, coefficients, eps)
     p2, m2 = torch.empty_like(param), torch.empty_like(momentum)
-    ops.muon_update(param, grad, momentum, p2, m2, nesterov=bool(nesterov), gate=gate, **args)
+    bind().muon_update(param, grad, momentum, p2, m2, *args, gate)
     return p2, m2
 
 
@@ -116,10 +116,10 @@ def muon_update_(param, grad, momentum, *, lr: float, beta: float = 0.95, nester
                  gate=None):
     """muon_update in place: param and momentum are overwritten; returns param."""
     _check_gate(gate)
-    args = _muon_args(param, grad, momentum, lr, beta, weight_decay, scale, steps, coefficients, eps)
+    args = _muon_args(param, grad, momentum, lr, beta, nesterov, weight_decay, scale, steps, coefficients, eps)
     if _overlaps_itself(param) or _overlaps_itself(momentum):
         raise ValueError("muon_update_: param and momentum must not overlap themselves")
-    ops.muon_update(param, grad, momentum, param, momentum, nesterov=bool(nesterov), gate=gate, **args)
+    bind().muon_update(param, grad, momentum, param, momentum, *args, gate)
     return param
 
 

@@ -12,7 +12,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib as L
-from ._lib import check, lib
+from ._lib import bind, check, lib
 
 EPS = 1e-7
 
@@ -665,111 +665,30 @@ def readout_backward(row_ptr, ent, N: int, targets, g_scores, n_val: int, val_li
 # --------------------------------------------------------------------------
 # relation attention: head, weights, update
 # --------------------------------------------------------------------------
+# torch tensors in and out of csrc/bind.cpp, which allocates, checks devices and calls the C ABI
 FL_DTYPE = {torch.float32: L.FL_F32, torch.float16: L.FL_F16, torch.bfloat16: L.FL_BF16}
-
-
-def _one_device(what, first, *others):
-    """The index of the tensors' common CUDA device; raises unless there is exactly one (None: no tensor)."""
-    dev = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            if not t.is_cuda or dev < 0:
-                raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
-            raise ValueError(f"{what}: tensors on cuda:{dev} and {t.device}")
-    if dev < 0:
-        raise ValueError("flashlog_b200 runs on CUDA tensors only (no CPU fallback)")
-    return dev
-
-
-def _call(dev, what, fn, *args):
-    """fn(*args, the current stream of device `dev`), with that device current."""
-    now = torch._C._cuda_getDevice()
-    if now == dev:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc != 0:
-        check(rc, what)
-
-
-def _workspace(nbytes, like):
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+MAX_WEIGHT_COLUMNS = 65536
+MAX_HISTORY = 65535
 
 
 def _lines(t):
     """t as [rows, cols] lines the library can address: unit inner stride, rows at least a row apart."""
-    if t.is_contiguous():
-        return t
-    if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1):
+    if t.is_contiguous() or (t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1)):
         return t
     return t.contiguous()
-
-
-def _ld(t):
-    return max(t.stride(0), t.shape[1])
-
-
-def _linear_params(x, weight, bias, residual, act):
-    n, k = weight.shape
-    return L.fl_linear(x.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(residual), _ld(x), _ld(weight),
-                       0 if residual is None else _ld(residual), x.shape[0], n, k, FL_DTYPE[x.dtype], act)
 
 
 def linear_forward(x, weight, bias=None, residual=None, act: int = L.FL_ACT_NONE, want_z: bool = False, out=None):
     """y = act(x W^T + bias) + residual of [rows, k] and [n, k] matrices of one
     dtype (into out, when given: contiguous); with want_z also the fp32
     pre-activation (None without an activation).  Returns (y, z)."""
-    dev = _one_device("linear", x, weight, bias, residual, out)
-    x, weight = _lines(x), _lines(weight)
-    if bias is not None:
-        bias = bias.contiguous()
-    if residual is not None:
-        residual = _lines(residual)
-    rows, n = x.shape[0], weight.shape[0]
-    y = x.new_empty((rows, n)) if out is None else out
-    z = x.new_empty((rows, n), dtype=torch.float32) if want_z and act != L.FL_ACT_NONE else None
-    if rows == 0:
-        return y, z
-    p = _linear_params(x, weight, bias, residual, act)
-    nbytes = lib().fl_linear_workspace(rows, n, p.k, p.dtype)
-    ws = _workspace(nbytes, x)
-    _call(dev, "linear", lib().fl_linear_forward, ctypes.byref(p), y.data_ptr(), n, _ptr(z), _ptr(ws), nbytes)
-    return y, z
+    return bind().linear_forward(x, weight, bias, residual, act, want_z, out)
 
 
 def linear_backward(x, weight, z, gy, act: int = L.FL_ACT_NONE, want=(True, True, True)):
     """(dx, dweight, dbias) of linear_forward for the gradient gy [rows, n];
     want says which (None in the place of the others)."""
-    dev = _one_device("linear backward", x, weight, z, gy)
-    x, weight, gy = _lines(x), _lines(weight), _lines(gy)
-    rows, (n, k) = x.shape[0], weight.shape
-    dx = x.new_empty((rows, k)) if want[0] else None
-    dw = x.new_empty((n, k)) if want[1] else None
-    db = x.new_empty(n) if want[2] else None
-    p = _linear_params(x, weight, None, None, act)
-    nbytes = lib().fl_linear_backward_workspace(rows, n, k, p.dtype, act)
-    ws = _workspace(nbytes, x)
-    _call(dev, "linear backward", lib().fl_linear_backward, ctypes.byref(p), _ptr(z), gy.data_ptr(), _ld(gy), _ptr(dx),
-          _ptr(dw), _ptr(db), _ptr(ws), nbytes)
-    return dx, dw, db
-
-
-MAX_WEIGHT_COLUMNS = 65536
-MAX_HISTORY = 65535
-
-
-def _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence):
-    rows, n = logits.shape
-    return L.fl_weights(logits.data_ptr(), _ptr(bias), _ptr(mask), _ptr(states), _ptr(history), _ld(logits),
-                        0 if bias is None or bias.dim() == 1 else n, 0 if mask is None else _ld(mask),
-                        0 if mask is None else mask.shape[0], 0 if history is None else _ld(history),
-                        0 if history is None else history.shape[1], rows, n, tau, repetition, frequency, presence,
-                        FL_DTYPE[logits.dtype])
+    return bind().linear_backward(x, weight, z, gy, act, *want)
 
 
 def relation_weights(logits, bias=None, mask=None, states=None, history=None, tau=1.0, repetition=1.0, frequency=0.0,
@@ -778,102 +697,14 @@ def relation_weights(logits, bias=None, mask=None, states=None, history=None, ta
     stride), bias [n] or [rows, n], mask bool or uint8 [states, n], states
     int64 [rows], history int64 [rows, H].  Returns f32 [rows, n] (out, when
     given: contiguous)."""
-    dev = _one_device("relation weights", logits, bias, mask, states, history, out)
-    w = logits.new_empty(logits.shape, dtype=torch.float32) if out is None else out
-    if w.numel() == 0:
-        return w
-    p = _weights_params(logits, bias, mask, states, history, tau, repetition, frequency, presence)
-    _call(dev, "relation weights", lib().fl_relation_weights, ctypes.byref(p), w.data_ptr())
-    return w
+    return bind().weights_forward(logits, bias, mask, states, history, tau, repetition, frequency, presence, out)
 
 
 def relation_weights_backward(w, g, logits, bias=None, history=None, tau=1.0, repetition=1.0, want_logits=True,
                               want_bias=False):
     """(dlogits, dbias) of relation_weights for the gradient g f32 [rows, n]
     (rows may share one line: stride 0)."""
-    dev = _one_device("relation weights backward", w, g, logits, bias, history)
-    rows, n = w.shape
-    dz = logits.new_empty((rows, n)) if want_logits else None
-    db = torch.empty_like(bias) if want_bias else None
-    if g.stride(1) != 1:
-        g = g.contiguous()
-    p = _weights_params(logits, bias, None, None, history, tau, repetition, 0.0, 0.0)
-    nbytes = lib().fl_relation_weights_workspace(rows, n) if want_bias and bias.dim() == 1 else 0
-    ws = _workspace(nbytes, w)
-    _call(dev, "relation weights backward", lib().fl_relation_weights_backward, ctypes.byref(p), w.data_ptr(),
-          g.data_ptr(), g.stride(0), _ptr(dz), _ptr(db), _ptr(ws), nbytes)
-    return dz, db
-
-
-def _as_batch(ts):
-    """A common (b1, b2) of tensors [..., m, n] of one shape, with each one's fl_matrices; None when the leading
-    dimensions of some need more than two strides."""
-    merged, split = [], 1  # split: b2, the innermost batch dimensions that every tensor holds at one stride
-    total = 1
-    for n in ts[0].shape[:-2]:
-        total *= n
-    for t in ts:
-        dims = []
-        for n, s in zip(t.shape[:-2], t.stride()):
-            if n == 1:
-                continue
-            if dims and dims[-1][1] == n * s:
-                dims[-1] = (dims[-1][0] * n, s)
-            else:
-                dims.append((n, s))
-        if len(dims) > 2 or (len(dims) == 2 and split not in (1, dims[1][0])):
-            return None
-        if len(dims) == 2:
-            split = dims[1][0]
-        merged.append(dims)
-    out = []
-    for t, dims in zip(ts, merged):
-        s2 = dims[-1][1] if dims else 0
-        s1 = dims[0][1] if len(dims) == 2 else s2 * split
-        out.append(L.fl_matrices(t.data_ptr(), s1, s2, t.stride(-2), t.stride(-1)))
-    return total // split, split, out
-
-
-def orthogonalize(update, steps: int, coefficients, eps: float):
-    """fl_orthogonalize of update [..., m, n]: a new contiguous tensor of its dtype."""
-    dev = _one_device("orthogonalize", update)
-    out = update.new_empty(update.shape)
-    if out.numel() == 0:
-        return out
-    got = _as_batch((update, out))
-    if got is None:  # strides that two batch dimensions cannot express
-        update = update.contiguous()
-        got = _as_batch((update, out))
-    b1, b2, (src, dst) = got
-    m, n = update.shape[-2:]
-    nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
-    ws = _workspace(nbytes, update)
-    _call(dev, "orthogonalize", lib().fl_orthogonalize, ctypes.byref(src), ctypes.byref(dst), b1, b2, m, n,
-          FL_DTYPE[update.dtype], steps, *coefficients, eps, _ptr(ws), nbytes)
-    return out
-
-
-def muon_update(param, grad, momentum, param_out, momentum_out, *, lr, beta, nesterov, weight_decay, scale, steps,
-                coefficients, eps, gate=None):
-    """fl_muon_update of fp32 tensors [..., m, n] of one shape, into the two outputs."""
-    dev = _one_device("muon_update", param, grad, momentum, param_out, momentum_out, gate)
-    if param.numel() == 0:
-        return
-    got = _as_batch((param, grad, momentum, param_out, momentum_out))
-    if got is None:  # strides that two batch dimensions cannot express: through plain copies
-        p2, m2 = (t.new_empty(t.shape) for t in (param_out, momentum_out))
-        muon_update(param.contiguous(), grad.contiguous(), momentum.contiguous(), p2, m2, lr=lr, beta=beta,
-                    nesterov=nesterov, weight_decay=weight_decay, scale=scale, steps=steps,
-                    coefficients=coefficients, eps=eps, gate=gate)
-        param_out.copy_(p2)
-        momentum_out.copy_(m2)
-        return
-    b1, b2, ts = got
-    m, n = param.shape[-2:]
-    nbytes = lib().fl_newton_schulz_workspace(b1 * b2, m, n, steps)
-    ws = _workspace(nbytes, param)
-    _call(dev, "muon_update", lib().fl_muon_update, *(ctypes.byref(t) for t in ts), b1, b2, m, n, lr, beta,
-          int(nesterov), weight_decay, scale, steps, *coefficients, eps, _ptr(gate), _ptr(ws), nbytes)
+    return bind().weights_backward(w, g, logits, bias, history, tau, repetition, want_logits, want_bias)
 
 
 def gemm_fault() -> bool:

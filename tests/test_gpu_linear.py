@@ -278,3 +278,18 @@ def test_only_wanted_gradients():
             leaves[k] = leaves[k].clone().requires_grad_()
             got, = torch.autograd.grad(attention.linear(*leaves, activation="relu"), [leaves[k]], gy)
             assert torch.equal(got, all4[k])
+
+
+def test_second_derivative_is_an_error():
+    """Asking for a differentiable gradient is fine; differentiating it says so instead of giving zeros."""
+    from flashlog_b200 import attention
+    x, w, b, _ = make(5, 6, 7, torch.float32)
+    x.requires_grad_()
+    g, = torch.autograd.grad(attention.linear(x, w, b, activation="tanh").square().sum(), [x], create_graph=True)
+    assert g.requires_grad
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(g.sum(), [x])
+    z = torch.randn(4, 9, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(attention.relation_weights(z).square().sum(), [z], create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(g.sum(), [z])
