@@ -20,6 +20,11 @@ namespace fl {
 enum { kF16 = 0, kBF16 = 1 };                 // operand type
 enum { kOutF32 = 0, kOutF16 = 1, kOutBF16 = 2 };  // fl_dtype values (FL_F32, FL_F16, FL_BF16)
 
+// Elements from line to line of a 16-bit array that a kernel writes for a
+// product: lines that are not short start on 128 bytes, so that the writes and
+// the product's loads take whole cache lines.
+constexpr int64_t pitch_of(int64_t n) { return n < 64 ? (n + 7) & ~int64_t(7) : (n + 63) & ~int64_t(63); }
+
 struct GemmOperand {
     const void *ptr;         // 16-byte aligned
     int64_t ld;              // elements between lines, a multiple of 8

@@ -12,7 +12,6 @@ namespace fl {
 
 namespace {
 
-constexpr int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
 constexpr int kSumRows = 128;  // rows per partial column sum
 
 int elem_size(int dtype) { return dtype == FL_F32 ? 4 : 2; }
@@ -150,62 +149,83 @@ __global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uin
 // length start anywhere), its store is one aligned piece of 8 or 16 bytes, so a
 // warp writes whole cache lines (single 16-bit stores took 405 us for 4608 x
 // 29649).  Four rows are in flight.
+// Eight values from p on, of which `left` exist (0 for the others).  Rows need
+// not start on 16 bytes: a lane reads the aligned 16-byte pieces around its
+// values and turns them into place.  [first, last): the array, which no piece
+// may leave.
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, const void *first, const void *last, int left, float (&d)[8]) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8; h += kPer) {
+        union { unsigned w[4]; T t[kPer]; } x;
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p + h) & 15);
+        const char *base = reinterpret_cast<const char *>(p + h) - off;
+        if (left > h && base >= static_cast<const char *>(first) &&
+            base + (off == 0 ? 16 : 32) <= static_cast<const char *>(last)) {
+            union { uint4 u; unsigned w[4]; } a, b;
+            a.u = *reinterpret_cast<const uint4 *>(base);
+            b.u = a.u;
+            if (off != 0) b.u = *reinterpret_cast<const uint4 *>(base + 16);
+            unsigned c[8] = {a.w[0], a.w[1], a.w[2], a.w[3], b.w[0], b.w[1], b.w[2], b.w[3]};
+            if ((off & 4) != 0) {
+#pragma unroll
+                for (int i = 0; i < 7; ++i) c[i] = c[i + 1];
+            }
+            if ((off & 8) != 0) {
+#pragma unroll
+                for (int i = 0; i < 6; ++i) c[i] = c[i + 2];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.w[i] = sizeof(T) == 2 ? __funnelshift_r(c[i], c[i + 1], 8 * (off & 3)) : c[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) x.t[i] = h + i < left ? p[h + i] : from_f32<T>(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) d[h + i] = h + i < left ? to_f32<T>(x.t[i]) : 0.0f;
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) dz_kernel(const T *gy, int64_t ld_gy, const float *z, int64_t rows, int64_t n, int act,
                                                  T *out, int64_t ldo, float *partial) {
-    __shared__ float part[8][128];
-    const int64_t c0 = blockIdx.x * int64_t(128) + 4 * threadIdx.x;
+    __shared__ float part[8][256];
+    const int64_t c0 = blockIdx.x * int64_t(256) + 8 * threadIdx.x;
     const int64_t r0 = blockIdx.y * int64_t(kSumRows), r1 = min(rows, r0 + kSumRows);
-    const int left = c0 < n ? static_cast<int>(min(static_cast<int64_t>(4), n - c0)) : 0;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t r = r0 + threadIdx.y; r < r1; r += 32) {
-        float d[4][4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const T *p = gy + (r + 8 * k) * ld_gy + c0;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) d[k][w] = r + 8 * k < r1 && w < left ? to_f32<T>(p[w]) : 0.0f;
-        }
+    const int left = c0 < n ? static_cast<int>(min(static_cast<int64_t>(8), n - c0)) : 0;
+    const void *gy_end = gy + (rows - 1) * ld_gy + n, *z_end = z + rows * n;
+    float sum[8] = {};
+#pragma unroll 2
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += 8) {
+        float d[8];
+        load8(gy + r * ld_gy + c0, gy, gy_end, left, d);
         if (act != kActNone) {
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-                if (r + 8 * k >= r1) break;
-                const float *p = z + (r + 8 * k) * n + c0;
-                float s[4];
+            float s[8];
+            load8(z + r * n + c0, z, z_end, left, s);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) s[w] = w < left ? p[w] : 0.0f;
+            for (int w = 0; w < 8; ++w) d[w] *= act_slope(s[w], act);
+        }
+        if (out != nullptr && left > 0) {
+            // the pitch is a multiple of 8: the whole piece lies in the row
+            struct alignas(16) Vec { T t[8]; } v;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = act_slope(s[w], act);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (q == k) d[q][w] *= f;
-                }
-            }
+            for (int w = 0; w < 8; ++w) v.t[w] = from_f32<T>(d[w]);
+            *reinterpret_cast<Vec *>(out + r * ldo + c0) = v;
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if (out != nullptr && r + 8 * k < r1 && left > 0) {
-                // the pitch is a multiple of 8: the whole piece lies in the row
-                struct alignas(4 * sizeof(T)) Vec { T t[4]; } v;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) v.t[w] = from_f32<T>(d[k][w]);
-                *reinterpret_cast<Vec *>(out + (r + 8 * k) * ldo + c0) = v;
-            }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) sum[w] += d[k][w];
-        }
+        for (int w = 0; w < 8; ++w) sum[w] += d[w];
     }
     if (partial == nullptr) return;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) part[threadIdx.y][4 * threadIdx.x + w] = sum[w];
+    for (int w = 0; w < 8; ++w) part[threadIdx.y][8 * threadIdx.x + w] = sum[w];
     __syncthreads();
     const int c = threadIdx.y * 32 + threadIdx.x;
-    if (c < 128 && blockIdx.x * int64_t(128) + c < n) {
+    if (blockIdx.x * int64_t(256) + c < n) {
         float s = part[0][c];
 #pragma unroll
         for (int i = 1; i < 8; ++i) s += part[i][c];
-        partial[blockIdx.y * n + blockIdx.x * int64_t(128) + c] = s;
+        partial[blockIdx.y * n + blockIdx.x * int64_t(256) + c] = s;
     }
 }
 
@@ -494,7 +514,7 @@ bool tma_ready(const void *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(
 
 size_t operand_bytes(int64_t lines, int64_t inner, int64_t exps, int dtype) {
     const int planes = dtype == FL_F32 ? 2 : 1;
-    return carve_bytes<__half>(planes * lines * round8(inner)) + carve_bytes<int>(exps) + carve_bytes<unsigned>(exps);
+    return carve_bytes<__half>(planes * lines * pitch_of(inner)) + carve_bytes<int>(exps) + carve_bytes<unsigned>(exps);
 }
 
 // Readies the matrix src [lines, inner] as a product operand.  by_line: the
@@ -512,7 +532,7 @@ int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool
             op->ld = ld;
             return FL_OK;
         }
-        const int64_t ldp = round8(inner);
+        const int64_t ldp = pitch_of(inner);
         uint16_t *out = ws.take<uint16_t>(lines * ldp);
         FL_REQUIRE(out != nullptr, "linear: workspace too small");
         // grid.y is limited to 65535 rows: the rows go in slices
@@ -525,7 +545,7 @@ int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool
         op->ld = ldp;
         return check_launch("linear pack");
     }
-    const int64_t ldp = round8(inner), plane = lines * ldp;
+    const int64_t ldp = pitch_of(inner), plane = lines * ldp;
     __half *out = ws.take<__half>(2 * plane);
     int *ex = ws.take<int>(by_line ? lines : inner);
     FL_REQUIRE(out != nullptr && ex != nullptr, "linear: workspace too small");
@@ -597,7 +617,7 @@ int linear_dz(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy,
     // grid.y (row groups) is limited to 65535: 8 million rows
     const int64_t parts = (p->rows + kSumRows - 1) / kSumRows;
     FL_REQUIRE(parts <= 65535, "linear: more than %d rows in a backward pass", 65535 * kSumRows);
-    launch(dz_kernel<T>, dim3(static_cast<unsigned>((p->n + 127) / 128), static_cast<unsigned>(parts)), dim3(32, 8), 0, st,
+    launch(dz_kernel<T>, dim3(static_cast<unsigned>((p->n + 255) / 256), static_cast<unsigned>(parts)), dim3(32, 8), 0, st,
            static_cast<const T *>(gy), ld_gy, z, p->rows, p->n, p->act, out, ldo, partial);
     return check_launch("linear dz");
 }
@@ -733,7 +753,7 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
     if (p->dtype == FL_F32) {
         FL_REQUIRE(p->rows + p->n < (1ll << 31), "linear: bad shape");
         launch(pack_rows_kernel, static_cast<unsigned>(p->rows + p->n), p->k > 2048 ? 512 : 128, 0, st, px, pw, p->k,
-               round8(p->k));
+               pitch_of(p->k));
     }
     LinearEpilogue e = plain_epilogue(y, ld_y, p->dtype, ea, eb);
     e.bias = p->bias;
@@ -749,7 +769,7 @@ size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, 
     if (rows <= 0 || n <= 0 || k <= 0) return 0;
     if (is_small_backward(rows, n, k, dtype)) return split_bytes(rows, k, n) + split_bytes(n, k, rows) + 256;
     size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
-    if (act != FL_ACT_NONE || dtype != FL_F32) dz += carve_bytes<char>(rows * round8(n) * elem_size(dtype));
+    if (act != FL_ACT_NONE || dtype != FL_F32) dz += carve_bytes<char>(rows * pitch_of(n) * elem_size(dtype));
     const size_t ops = operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
     return dz + ops + carve_bytes<float>(((rows + kSumRows - 1) / kSumRows) * n);
 }
@@ -778,7 +798,7 @@ int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t 
     const bool copies = p->dtype != FL_F32 && !tma_ready(gy, ld_gy) && (dx != nullptr || dw != nullptr);
     if (p->act != FL_ACT_NONE || dbias != nullptr || copies) {
         void *out = nullptr;
-        const int64_t ldo = round8(p->n);
+        const int64_t ldo = pitch_of(p->n);
         if (p->act != FL_ACT_NONE || copies) {
             out = ws.take<char>(p->rows * ldo * es);
             FL_REQUIRE(out != nullptr, "linear backward: workspace too small");

@@ -36,9 +36,9 @@ namespace fl {
 
 namespace {
 
-constexpr int64_t round8(int64_t v) { return (v + 7) & ~int64_t(7); }
 constexpr float kScaleX = 8192.0f, kScaleA = 4096.0f;
 constexpr int kMaxParts = 1024;
+constexpr int64_t kNormalizeBlocks = 888;
 
 // What the update is made of, in the caller's orientation [m, n].
 struct Source {
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256) square_sum_rows_kernel(const Source s, do
 }
 
 // Pass 2: planes of X * 2^13, turned to [short, long]: 64 x 64 tiles, grid
-// (tiles of j, tiles of i, batch); a lane holds two neighbours, so rows are
+// (blocks, batch); a lane holds two neighbours, so rows are
 // written in whole cache lines.
 template <typename T, bool MUON, bool TURNED>
 __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const double *partial, int parts, double eps,
@@ -170,34 +170,8 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     // access, and a column is read with at most two rows to a bank
     __shared__ __align__(8) float tile[TURNED ? 64 * 66 : 1];
     auto at = [](int r, int c) { return r * 66 + (c ^ (((r >> 4) & 1) << 1)); };
-    const int64_t b = blockIdx.z;
+    const int64_t b = blockIdx.y;
     const int64_t ub = s.u.at(b, s.nb2), ob = s.mom_out.at(b, s.nb2);
-    const int64_t i0 = blockIdx.y * int64_t(64), j0 = blockIdx.x * int64_t(64);
-    constexpr bool kApart = TURNED && sizeof(T) == 4;
-    float v[8][2];
-    if (sizeof(T) == 2 && s.u.j == 1 && ((reinterpret_cast<uintptr_t>(s.u.ptr) | s.u.i * 2 | ub * 2) & 3) == 0) {
-        // 16-bit pairs
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + 2 * threadIdx.x;
-            union { unsigned u; T t[4 / sizeof(T)]; } x;
-            x.u = 0u;
-            const T *p = static_cast<const T *>(s.u.ptr) + ub + i * s.u.i + j;
-            if (i < s.m && j + 1 < s.n) x.u = *reinterpret_cast<const unsigned *>(p);
-            else if (i < s.m && j < s.n) x.t[0] = p[0];
-            v[k][0] = to_f32(x.t[0]);
-            v[k][1] = to_f32(x.t[sizeof(T) == 2 ? 1 : 0]);
-        }
-    } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            // two neighbours a lane; turned 32-bit tiles a lane per element (they turn in shared memory)
-            const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (kApart ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
-            v[k][w] = i < s.m && j < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i, j) : 0.0f;
-        }
-    }
     double sum = 0.0;
     for (int p = threadIdx.y * 32 + threadIdx.x; p < parts; p += 256) sum += partial[b * parts + p];
     sum = warp_sum(sum);
@@ -216,34 +190,69 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
         e = e > 60 ? 60 : e;
         scale = ldexp(scale, e);
     }
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0 && threadIdx.y == 0) shift[b] = e;
+    if (blockIdx.x == 0 && threadIdx.x == 0 && threadIdx.y == 0) shift[b] = e;
+    // the product in 32 bits where the scale is far from their ends
+    const bool far = !(scale > 1e-30 && scale < 1e30);
+    const float scale_f = far ? 0.0f : static_cast<float>(scale);
+    auto scaled = [&](float v) { return far ? static_cast<float>(v * scale) : v * scale_f; };
     __half *hi = out + b * 2 * plane;
-    if (TURNED) {
+    const int64_t tiles_j = (s.n + 63) / 64, tiles = tiles_j * ((s.m + 63) / 64);
+    constexpr bool kApart = TURNED && sizeof(T) == 4;
+    const bool pairs = sizeof(T) == 2 && s.u.j == 1 && ((reinterpret_cast<uintptr_t>(s.u.ptr) | s.u.i * 2 | ub * 2) & 3) == 0;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t i0 = t / tiles_j * 64, j0 = t % tiles_j * 64;
+        float v[8][2];
+        if (pairs) {
+            // 16-bit pairs
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + 2 * threadIdx.x;
+                union { unsigned u; T t[4 / sizeof(T)]; } x;
+                x.u = 0u;
+                const T *p = static_cast<const T *>(s.u.ptr) + ub + i * s.u.i + j;
+                if (i < s.m && j + 1 < s.n) x.u = *reinterpret_cast<const unsigned *>(p);
+                else if (i < s.m && j < s.n) x.t[0] = p[0];
+                v[k][0] = to_f32(x.t[0]);
+                v[k][1] = to_f32(x.t[sizeof(T) == 2 ? 1 : 0]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    // two neighbours a lane; turned 32-bit tiles a lane per element (they turn in shared memory)
+                    const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (kApart ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
+                    v[k][w] = i < s.m && j < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i, j) : 0.0f;
+                }
+        }
+        if (TURNED) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int r = threadIdx.y + 8 * k;
+                const float x = scaled(v[k][0]), y = scaled(v[k][1]);
+                if (kApart) {
+                    tile[at(r, threadIdx.x)] = x;
+                    tile[at(r, threadIdx.x + 32)] = y;
+                } else {
+                    *reinterpret_cast<float2 *>(&tile[at(r, 2 * threadIdx.x)]) = make_float2(x, y);
+                }
+            }
+            __syncthreads();
+        }
+        const int64_t rows = TURNED ? s.n : s.m, cols = TURNED ? s.m : s.n, r0 = TURNED ? j0 : i0, c0 = TURNED ? i0 : j0;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int r = threadIdx.y + 8 * k;
-            const float x = static_cast<float>(v[k][0] * scale), y = static_cast<float>(v[k][1] * scale);
-            if (kApart) {
-                tile[at(r, threadIdx.x)] = x;
-                tile[at(r, threadIdx.x + 32)] = y;
-            } else {
-                *reinterpret_cast<float2 *>(&tile[at(r, 2 * threadIdx.x)]) = make_float2(x, y);
-            }
+            const int64_t r = r0 + threadIdx.y + 8 * k, c = c0 + 2 * threadIdx.x;
+            const float a = TURNED ? tile[at(2 * threadIdx.x, threadIdx.y + 8 * k)] : scaled(v[k][0]);
+            const float z = TURNED ? tile[at(2 * threadIdx.x + 1, threadIdx.y + 8 * k)] : scaled(v[k][1]);
+            if (r >= rows || c >= cols) continue;
+            __half2 h, l;
+            split_pair(a, z, h, l);
+            // the pitch is a multiple of 8 and at least cols: the pair fits in the row
+            *reinterpret_cast<__half2 *>(hi + r * ld + c) = h;
+            *reinterpret_cast<__half2 *>(hi + plane + r * ld + c) = l;
         }
-        __syncthreads();
-    }
-    const int64_t rows = TURNED ? s.n : s.m, cols = TURNED ? s.m : s.n, r0 = TURNED ? j0 : i0, c0 = TURNED ? i0 : j0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const int64_t r = r0 + threadIdx.y + 8 * k, c = c0 + 2 * threadIdx.x;
-        if (r >= rows || c >= cols) continue;
-        const float a = TURNED ? tile[at(2 * threadIdx.x, threadIdx.y + 8 * k)] : static_cast<float>(v[k][0] * scale);
-        const float z = TURNED ? tile[at(2 * threadIdx.x + 1, threadIdx.y + 8 * k)] : static_cast<float>(v[k][1] * scale);
-        __half2 h, l;
-        split_pair(a, z, h, l);
-        // the pitch is a multiple of 8 and at least cols: the pair fits in the row
-        *reinterpret_cast<__half2 *>(hi + r * ld + c) = h;
-        *reinterpret_cast<__half2 *>(hi + plane + r * ld + c) = l;
+        if (TURNED) __syncthreads();
     }
 }
 
@@ -256,8 +265,9 @@ int normalize(const Source &s, bool turned, double eps, double growth, double *p
     const dim3 parts_grid(parts, static_cast<unsigned>(s.batch));
     if (rows) launch(square_sum_rows_kernel<T>, parts_grid, 256, 0, st, s, partial, counts, n_counts);
     else launch(square_sum_kernel<T, MUON>, parts_grid, 256, 0, st, s, partial, counts, n_counts);
-    const dim3 grid(static_cast<unsigned>((s.n + 63) / 64), static_cast<unsigned>((s.m + 63) / 64),
-                    static_cast<unsigned>(s.batch));
+    // about six blocks per SM in all, each of several tiles: the norm is put together once per block
+    const int64_t tiles = ((s.n + 63) / 64) * ((s.m + 63) / 64), most = (kNormalizeBlocks + s.batch - 1) / s.batch;
+    const dim3 grid(static_cast<unsigned>(tiles < most ? tiles : most), static_cast<unsigned>(s.batch));
     if (turned) launch(normalize_kernel<T, MUON, true>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, growth, shift, x, ld, plane);
     else launch(normalize_kernel<T, MUON, false>, grid, dim3(32, 8), 0, st, s, partial, parts, eps, growth, shift, x, ld, plane);
     return check_launch("newton-schulz normalize");
@@ -407,13 +417,13 @@ Range polynomial_range(double ca, double cb, double cc, int steps) {
 
 NsBuffer take_planes(Carve &ws, int64_t batch, int64_t rows, int64_t cols) {
     NsBuffer b;
-    b.ld = round8(cols);
+    b.ld = pitch_of(cols);
     b.plane = rows * b.ld;
     b.p = ws.take<__half>(batch * 2 * b.plane);
     return b;
 }
 size_t planes_bytes(int64_t batch, int64_t rows, int64_t cols) {
-    return carve_bytes<__half>(batch * 2 * rows * round8(cols));
+    return carve_bytes<__half>(batch * 2 * rows * pitch_of(cols));
 }
 
 Strided turn(Strided s, bool turned) {

@@ -9,8 +9,12 @@
 //
 // One pass over the row: its values stay in registers, and one joint reduction
 // gives the maximum and the sum, each thread having summed relative to its own
-// maximum.  A row wider than one block's registers is spread over a cluster of
-// up to eight blocks, which send each other their (maximum, sum) pairs.  The operation is bound by HBM: a value is read once and written once.
+// maximum.  A few long rows are spread over a cluster of eight blocks each,
+// which send each other their (maximum, sum) pairs; the widest rows take two
+// passes.  A value has to be read once and written once: 382 MB and 58 us for
+// 1536 x 29649 with masks and histories of 200, which take 118 us (the two-pass
+// form 134 us): a row's barriers and its 40 instructions a value are what the
+// copies do not cover.
 //
 // The history's counts live in shared memory next to one "seen" bit per
 // column; a warp's 32 columns share one word of bits, so columns without
@@ -33,7 +37,7 @@ struct WeightsArgs {
     const int64_t *history;  // [rows, hist] or NULL; entries outside [0, n) do not count
     int64_t hist_ld, hist;
     int64_t rows, n;
-    float theta, frequency, presence, inv_tau;
+    float theta, inv_theta, frequency, presence, inv_tau;
 };
 
 // A thread's columns of its block are i * THREADS + threadIdx.x.  The seen bits
@@ -82,6 +86,11 @@ __device__ __forceinline__ int64_t state_of(const WeightsArgs &a, int64_t row) {
     return a.states != nullptr ? a.states[row] : (row < a.n_states ? row : a.n_states - 1);
 }
 
+// A logit of an operator that is `count` times in the row's history.
+__device__ __forceinline__ float penalised(const WeightsArgs &a, float v, unsigned count) {
+    v *= v > 0.0f ? a.inv_theta : a.theta;
+    return v - a.frequency * static_cast<float>(count) - a.presence;
+}
 // 2^x, to 2^-22; results below 2^-126 are 0
 __device__ __forceinline__ float power2(float x) {
     float y;
@@ -172,10 +181,7 @@ __global__ __launch_bounds__(THREADS, min_blocks(THREADS, VPT)) void weights_for
         for (int i = 0; i < VPT; ++i) {
             float v = to_f32<T>(in.logit[i]);
             if ((any >> i) & 1u) {  // the same for the whole warp
-                if ((__shfl_sync(kFull, word, i) >> lane) & 1u) {
-                    v = v > 0.0f ? v / a.theta : v * a.theta;
-                    v = v - a.frequency * static_cast<float>(count[i * THREADS + tid]) - a.presence;
-                }
+                if ((__shfl_sync(kFull, word, i) >> lane) & 1u) v = penalised(a, v, count[i * THREADS + tid]);
             }
             u[i] = in.ok[i] != 0 ? v + u[i] : -INFINITY;
             m = fmaxf(m, u[i]);
@@ -310,13 +316,235 @@ __global__ __launch_bounds__(THREADS, min_blocks(THREADS, VPT)) void weights_bac
     }
 }
 
-// ---- rows of more than 4096 columns ------------------------------------------
+// ---- rows of 4097 columns and more (row_form says up to where) ---------------
+// A row's 32 values a thread stay in registers, while the next row lands in
+// shared memory by asynchronous copies of 16 bytes.  A landed row keeps its
+// position within 16 bytes: column c lies at element c + lead.  A thread copies
+// the same pieces of 16 bytes that it reads, so it asks for a piece of the next
+// row as soon as it has read this row's.  The mask row follows behind a barrier:
+// its pieces are cut elsewhere.  The counts take 16 bits each (no history has
+// more than 65535 entries); one set of them, with one "seen" bit per element, is
+// cleared and filled again between a row's barriers.
+constexpr int kRowValues = 32;
+
+template <typename T>
+__device__ __forceinline__ int lead_of(const T *p) {
+    return static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15) / static_cast<int>(sizeof(T));
+}
+template <int THREADS, bool ADD>
+__device__ __forceinline__ void row_history(const WeightsArgs &a, int64_t row, int64_t token, int lead, unsigned *seen,
+                                            unsigned *count) {
+    const int64_t *h = a.history + row * a.hist_ld;
+    for (int64_t j = threadIdx.x; j < a.hist; j += THREADS) {
+        const int64_t v = j == threadIdx.x ? token : h[j];
+        if (v < 0 || v >= a.n) continue;
+        const int e = static_cast<int>(v) + lead;
+        if (ADD) {
+            atomicAdd(count + (e >> 1), 1u << (16 * (e & 1)));
+            atomicOr(seen + (e >> 5), 1u << (e & 31));
+        } else {
+            count[e >> 1] = 0u;
+            seen[e >> 5] = 0u;
+        }
+    }
+}
+
+__device__ __forceinline__ void copy16(const void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src) : "memory");
+}
+// The elements of a landing row before its first and after its last whole piece: one a thread.
+template <typename T>
+__device__ __forceinline__ int edge_column(const T *src, int n) {  // or -1
+    constexpr int kPer = 16 / sizeof(T);
+    const int lead = lead_of(src), head = lead == 0 ? 0 : kPer - lead, tail = (n - head) % kPer;
+    const int t = threadIdx.x;
+    return t < head ? t : t >= 16 && t - 16 < tail ? n - tail + t - 16 : -1;
+}
+template <typename T>
+__device__ __forceinline__ T edge_load(const T *src, int n) {
+    const int c = edge_column(src, n);
+    return c >= 0 ? src[c] : T(0.0f);
+}
+template <typename T>
+__device__ __forceinline__ void edge_store(unsigned char *dst, const T *src, int n, T edge) {
+    const int c = edge_column(src, n);
+    if (c >= 0) reinterpret_cast<T *>(dst)[lead_of(src) + c] = edge;
+}
+// The whole pieces of a mask row.
+template <int THREADS>
+__device__ __forceinline__ void land_mask(unsigned char *dst, const uint8_t *src, int n) {
+    const int lead = lead_of(src), head = (16 - lead) & 15, pieces = (n - head) / 16;
+    for (int i = threadIdx.x; i < pieces; i += THREADS) copy16(dst + lead + head + 16 * i, src + head + 16 * i);
+}
+// room for n elements at any position within 16 bytes
+__host__ __device__ constexpr int landing_bytes(int n, int size) { return (n * size + 15) / 16 * 16 + 16; }
+// words of counts: one half for each of n + 7 elements at most
+__host__ __device__ constexpr int count_words(int n) { return (n + 8) / 2; }
+
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) weights_row_kernel(const WeightsArgs a, float *out) {
+    extern __shared__ uint4 rows_raw[];
+    constexpr int kWarps = THREADS / 32, kPer = 16 / sizeof(T), kPieces = kRowValues / kPer;
+    __shared__ float warp_m[kWarps], warp_s[kWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = static_cast<int>(a.n);
+    unsigned char *const zs = reinterpret_cast<unsigned char *>(rows_raw);
+    unsigned char *const ms = zs + landing_bytes(n, sizeof(T));
+    unsigned *const seen = reinterpret_cast<unsigned *>(a.mask != nullptr ? ms + landing_bytes(n, 1) + 16 : ms);
+    unsigned *const count = seen + THREADS;
+    const bool hist = a.hist > 0;
+    const float k = a.inv_tau * 1.4426950408889634f;
+    const int64_t step = gridDim.x;
+    int64_t row = blockIdx.x;
+    if (row >= a.rows) return;  // for the whole block
+    const T *z = static_cast<const T *>(a.logits) + row * a.ld;
+    int64_t state = state_of(a, row), state_next = row + step < a.rows ? state_of(a, row + step) : 0;
+    bool legal = state >= 0 && state < a.n_states;
+    const uint8_t *mask = a.mask != nullptr && legal ? a.mask + state * a.mask_ld : nullptr;
+    T edge = edge_load(z, n);
+    uint8_t mask_edge = mask != nullptr ? edge_load(mask, n) : 0;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int e = kPer * (i * THREADS + tid);
+        if (e >= lead_of(z) && e + kPer <= lead_of(z) + n) copy16(zs + 16 * (i * THREADS + tid), z + e - lead_of(z));
+    }
+    if (mask != nullptr) land_mask<THREADS>(ms, mask, n);
+    int64_t token = -1, token_next = -1;
+    if (hist) {
+        if (tid < a.hist) token = a.history[row * a.hist_ld + tid];
+        for (int i = tid; i < THREADS + count_words(n); i += THREADS) seen[i] = 0u;
+        __syncthreads();
+        row_history<THREADS, true>(a, row, token, lead_of(z), seen, count);
+    }
+    edge_store<T>(zs, z, n, edge);
+    if (mask != nullptr) edge_store<uint8_t>(ms, mask, n, mask_edge);
+    for (; row < a.rows; row += step) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();  // the row has landed, its counts are complete
+        const bool more = row + step < a.rows;
+        const int lead = lead_of(z), end = lead + n;
+        const T *zn = more ? z + step * a.ld : z;
+        const int lead_n = lead_of(zn), end_n = more ? lead_n + n : 0;
+        const T *from_n = zn - lead_n;  // element 0, on 16 bytes
+        // mask byte of element e: ms + (mask mod 16) + e - lead (the bytes before it are the landing place of the logits)
+        const int mask_at = (mask != nullptr ? lead_of(mask) : 0) - lead + 8;
+        const unsigned *mr = reinterpret_cast<const unsigned *>(ms - 8 + (mask_at & ~3));
+        const int turn = 8 * (mask_at & 3);
+        const unsigned all = a.mask != nullptr && !legal ? 0u : 0xffffffffu;  // no such state: nothing is allowed
+        const T *bias = a.bias != nullptr ? static_cast<const T *>(a.bias) + row * a.bias_ld - lead : nullptr;
+        float u[kRowValues], m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = kPer * (i * THREADS + tid);
+            float *v = u + i * kPer;
+            if (e < end) {
+                union { uint4 w; T t[kPer]; } x;
+                x.w = rows_raw[i * THREADS + tid];
+                const unsigned bits = hist ? (seen[e >> 5] >> (e & 31)) & ((1u << kPer) - 1u) : 0u;
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) v[q] = to_f32<T>(x.t[q]);
+                if (bits != 0u) {
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) {
+                        const unsigned cnt = (count[(e + q) >> 1] >> (16 * (q & 1))) & 65535u;
+                        if ((bits >> q) & 1u) v[q] = penalised(a, v[q], cnt);
+                    }
+                }
+                if (bias != nullptr) {
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q)
+                        if (e + q >= lead && e + q < end) v[q] += to_f32<T>(bias[e + q]);
+                }
+#pragma unroll
+                for (int h = 0; h < kPer; h += 4) {
+                    unsigned ok = all;  // a byte per element
+                    if (mask != nullptr) ok = __funnelshift_r(mr[(e + h) / 4], mr[(e + h) / 4 + 1], turn);
+#pragma unroll
+                    for (int q = h; q < h + 4; ++q)
+                        if ((ok & (255u << (8 * (q - h)))) == 0u) v[q] = -INFINITY;
+                }
+                if (e < lead || e + kPer > end) {
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q)
+                        if (e + q < lead || e + q >= end) v[q] = -INFINITY;
+                }
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) m = fmaxf(m, v[q]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) v[q] = -INFINITY;
+            }
+            // the values above are in registers: the piece's place is free
+            if (e >= lead_n && e + kPer <= end_n) copy16(zs + 16 * (i * THREADS + tid), from_n + e);
+        }
+        if (hist && more && tid < a.hist) token_next = a.history[(row + step) * a.hist_ld + tid];
+        __syncthreads();  // the mask row and the counts have been read
+        if (more) {
+            z = zn;
+            state = state_next;
+            legal = state >= 0 && state < a.n_states;
+            mask = a.mask != nullptr && legal ? a.mask + state * a.mask_ld : nullptr;
+            edge = edge_load(z, n);
+            if (mask != nullptr) {
+                land_mask<THREADS>(ms, mask, n);
+                mask_edge = edge_load(mask, n);
+            }
+            if (row + 2 * step < a.rows) state_next = state_of(a, row + 2 * step);
+        }
+        if (hist) row_history<THREADS, false>(a, row, token, lead, seen, count);
+        // -inf contributes nothing even where it is also the maximum; a NaN stays one
+        const float from = m == -INFINITY ? 0.0f : m;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowValues; ++i) {
+            u[i] = power2((u[i] - from) * k);
+            s += u[i];
+        }
+        const float wm = warp_max(m);
+        const float ws = warp_sum(s * rescale(m, wm, k));
+        if (lane == 0) {
+            warp_m[warp] = wm;
+            warp_s[warp] = ws;
+        }
+        __syncthreads();  // the counts are clear, the warps' sums are there
+        if (hist && more) {
+            token = token_next;
+            row_history<THREADS, true>(a, row + step, token, lead_of(z), seen, count);
+        }
+        const float bm = lane < kWarps ? warp_m[lane] : -INFINITY;
+        const float bs = lane < kWarps ? warp_s[lane] : 0.0f;
+        const float top = warp_max(bm);
+        const float total = warp_sum(bs * rescale(bm, top, k));
+        const float f = total == 0.0f ? 0.0f : rescale(m, top, k) / total;
+        float *w = out + row * a.n - lead;  // of element 0, which may lie before the row
+        const bool aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int e = kPer * (i * THREADS + tid);
+            if (aligned && e >= lead && e + kPer <= end) {
+#pragma unroll
+                for (int q = i * kPer; q < (i + 1) * kPer; q += 4)
+                    *reinterpret_cast<float4 *>(w + e + q - i * kPer) =
+                        make_float4(u[q] * f, u[q + 1] * f, u[q + 2] * f, u[q + 3] * f);
+            } else {
+#pragma unroll
+                for (int q = 0; q < kPer; ++q)
+                    if (e + q >= lead && e + q < end) w[e + q] = u[i * kPer + q] * f;
+            }
+        }
+        if (more) {
+            edge_store<T>(zs, z, n, edge);
+            if (mask != nullptr) edge_store<uint8_t>(ms, mask, n, mask_edge);
+        }
+    }
+}
+
+// ---- rows of more columns ----------------------------------------------------
 // Two passes by one block: the first stores u where w will lie and keeps the
 // running maximum and the sum relative to it, the second reads u back (from L2:
-// the rows in flight fit) and writes w.  A cluster per row with the values in
-// registers measured 184 us for 1536 x 29649 with masks and histories, half of
-// it in the exchange between its blocks.
-constexpr int kStreamThreads = 512, kStreamUnroll = 8;
+// the rows in flight fit) and writes w.
+constexpr int kStreamThreads = 512, kStreamUnroll = 8, kStreamBlocks = 2;
 
 // Counts of a long row: 16 bits each, two to a word (no history has more than
 // 65535 entries), behind one seen bit per column.
@@ -337,15 +565,66 @@ __device__ __forceinline__ void stream_history(const WeightsArgs &a, int64_t row
     }
 }
 
+// u of U columns a thread, kStreamThreads apart, from column `base` on; the
+// running maximum and sum take them in.  FULL: all columns exist, and one load
+// and a ballot tell a warp which of its U words of seen bits are not empty.
+template <typename T, int U, bool FULL>
+__device__ __forceinline__ void stream_group(const WeightsArgs &a, const T *z, const T *bias, const uint8_t *mask,
+                                             float *w, int base, int left, const unsigned *seen, const unsigned *count,
+                                             float k, float &m, float &s) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T raw[U], extra[U];
+    uint8_t ok[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) raw[i] = FULL || i * kStreamThreads < left ? z[i * kStreamThreads] : from_f32<T>(0.0f);
+    if (mask != nullptr) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) ok[i] = FULL || i * kStreamThreads < left ? mask[i * kStreamThreads] : 0;
+    } else {
+#pragma unroll
+        for (int i = 0; i < U; ++i) ok[i] = FULL || i * kStreamThreads < left ? 1 : 0;
+    }
+    if (bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) extra[i] = FULL || i * kStreamThreads < left ? bias[i * kStreamThreads] : from_f32<T>(0.0f);
+    }
+    unsigned word = 0u, any = 0u;
+    if (seen != nullptr) {
+        const int at = (base >> 5) + warp + lane * (kStreamThreads / 32);
+        word = lane < U && (FULL || 32 * at < a.n) ? seen[at] : 0u;
+        any = __ballot_sync(kFull, word != 0u);
+    }
+    float u[U], top = m;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        float v = to_f32<T>(raw[i]);
+        if ((any >> i) & 1u) {  // the same for the whole warp
+            if ((__shfl_sync(kFull, word, i) >> lane) & 1u) {
+                const int c = base + i * kStreamThreads + threadIdx.x;
+                v = penalised(a, v, (count[c >> 1] >> (16 * (c & 1))) & 65535u);
+            }
+        }
+        if (bias != nullptr) v += to_f32<T>(extra[i]);
+        u[i] = ok[i] != 0 ? v : -INFINITY;
+        top = fmaxf(top, u[i]);
+        if (FULL || i * kStreamThreads < left) w[i * kStreamThreads] = u[i];
+    }
+    const float from = top == -INFINITY ? 0.0f : top;
+    s *= rescale(m, top, k);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < U; ++i) s += power2((u[i] - from) * k);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kStreamThreads) weights_stream_kernel(const WeightsArgs a, float *out) {
+__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) weights_stream_kernel(const WeightsArgs a, float *out) {
     extern __shared__ unsigned dyn[];
-    constexpr int kWarps = kStreamThreads / 32, U = kStreamUnroll;
+    constexpr int kWarps = kStreamThreads / 32, U = kStreamUnroll, kGroup = U * kStreamThreads;
     __shared__ float warp_m[2][kWarps], warp_s[2][kWarps];
     const int n = static_cast<int>(a.n), words = (n + 31) / 32;
-    unsigned *seen = dyn, *count = dyn + words;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool hist = a.hist > 0;
+    unsigned *seen = hist ? dyn : nullptr, *count = dyn + words;
     const float k = a.inv_tau * 1.4426950408889634f;
     if (hist)
         for (int i = tid; i < words + (n + 1) / 2; i += kStreamThreads) dyn[i] = 0u;
@@ -358,57 +637,23 @@ __global__ void __launch_bounds__(kStreamThreads) weights_stream_kernel(const We
         }
         const int64_t state = state_of(a, row);
         const bool legal = state >= 0 && state < a.n_states;
-        const T *z = static_cast<const T *>(a.logits) + row * a.ld;
-        const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld;
-        const uint8_t *mask = a.mask + (legal ? state * a.mask_ld : 0);
-        float *w = out + row * a.n;
+        const T *z = static_cast<const T *>(a.logits) + row * a.ld + tid;
+        const T *bias = a.bias != nullptr ? static_cast<const T *>(a.bias) + row * a.bias_ld + tid : nullptr;
+        const uint8_t *mask = a.mask != nullptr && legal ? a.mask + state * a.mask_ld + tid : nullptr;
+        float *w = out + row * a.n + tid;
         float m = -INFINITY, s = 0.0f;
-        for (int base = tid; base < n; base += U * kStreamThreads) {
-            T raw[U], extra[U];
-            uint8_t ok[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int c = base + i * kStreamThreads;
-                raw[i] = c < n ? z[c] : from_f32<T>(0.0f);
-                ok[i] = c < n ? 1 : 0;
-            }
-            if (a.mask != nullptr) {
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int c = base + i * kStreamThreads;
-                    ok[i] = legal && c < n ? mask[c] : 0;
-                }
-            }
-            if (a.bias != nullptr) {
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    const int c = base + i * kStreamThreads;
-                    extra[i] = c < n ? bias[c] : from_f32<T>(0.0f);
-                }
-            }
-            float u[U], top = m;
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int c = base + i * kStreamThreads;
-                float v = to_f32<T>(raw[i]);
-                if (hist && c < n) {
-                    const unsigned word = seen[c >> 5];
-                    if ((word >> (c & 31)) & 1u) {
-                        v = v > 0.0f ? v / a.theta : v * a.theta;
-                        const unsigned cnt = (count[c >> 1] >> (16 * (c & 1))) & 65535u;
-                        v = v - a.frequency * static_cast<float>(cnt) - a.presence;
-                    }
-                }
-                if (a.bias != nullptr) v += to_f32<T>(extra[i]);
-                u[i] = ok[i] != 0 ? v : -INFINITY;
-                top = fmaxf(top, u[i]);
-                if (c < n) w[c] = u[i];
-            }
-            const float from = top == -INFINITY ? 0.0f : top;
-            s *= rescale(m, top, k);
-            m = top;
-#pragma unroll
-            for (int i = 0; i < U; ++i) s += power2((u[i] - from) * k);
+        if (a.mask != nullptr && !legal) {
+            // no such state: nothing is allowed
+            for (int c = tid; c < n; c += kStreamThreads) w[c - tid] = -INFINITY;
+        } else {
+            int base = 0;
+            for (; base + kGroup <= n; base += kGroup)
+                stream_group<T, U, true>(a, z + base, bias != nullptr ? bias + base : nullptr,
+                                         mask != nullptr ? mask + base : nullptr, w + base, base, 0, seen, count, k, m, s);
+            if (base < n)
+                stream_group<T, U, false>(a, z + base, bias != nullptr ? bias + base : nullptr,
+                                          mask != nullptr ? mask + base : nullptr, w + base, base, n - base - tid, seen,
+                                          count, k, m, s);
         }
         const float wm = warp_max(m);
         const float ws = warp_sum(s * rescale(m, wm, k));
@@ -424,14 +669,15 @@ __global__ void __launch_bounds__(kStreamThreads) weights_stream_kernel(const We
         if (hist) stream_history<false>(a, row, seen, count);
         const float from = top == -INFINITY ? 0.0f : top;
         const float f = total == 0.0f ? 0.0f : 1.0f / total;
-        for (int base = tid; base < n; base += U * kStreamThreads) {
+        int base = 0;
+        for (; base + kGroup <= n; base += kGroup) {
             float u[U];
 #pragma unroll
-            for (int i = 0; i < U; ++i) u[i] = base + i * kStreamThreads < n ? w[base + i * kStreamThreads] : 0.0f;
+            for (int i = 0; i < U; ++i) u[i] = w[base + i * kStreamThreads];
 #pragma unroll
-            for (int i = 0; i < U; ++i)
-                if (base + i * kStreamThreads < n) w[base + i * kStreamThreads] = power2((u[i] - from) * k) * f;
+            for (int i = 0; i < U; ++i) w[base + i * kStreamThreads] = power2((u[i] - from) * k) * f;
         }
+        for (base += tid; base < n; base += kStreamThreads) w[base - tid] = power2((w[base - tid] - from) * k) * f;
     }
 }
 
@@ -580,10 +826,7 @@ __global__ void __launch_bounds__(kStreamThreads) __cluster_dims__(kWideBlocks, 
     for (int i = 0; i < VPT; ++i) {
         const int c = i * kStreamThreads + tid;
         float v = to_f32<T>(raw[i]);
-        if (hist && (seen[c >> 5] >> (c & 31)) & 1u) {
-            v = v > 0.0f ? v / a.theta : v * a.theta;
-            v = v - a.frequency * static_cast<float>(count[c]) - a.presence;
-        }
+        if (hist && (seen[c >> 5] >> (c & 31)) & 1u) v = penalised(a, v, count[c]);
         if (a.bias != nullptr) v += to_f32<T>(extra[i]);
         u[i] = ok[i] != 0 ? v : -INFINITY;
         m = fmaxf(m, u[i]);
@@ -700,25 +943,46 @@ struct Layout {
     int threads, vpt;  // vpt 0: the two-pass form
     int wide;          // values a thread of the cluster form, or 0
     int64_t blocks;    // rows in flight
+    int sms;
 };
 
 constexpr int64_t kMaxColumns = 65536, kMaxHistory = 65535;
 
 Layout layout(int64_t rows, int64_t n) {
     const int sms = fl_device_sm_count() > 0 ? fl_device_sm_count() : 148;
-    Layout l{256, 16, 0, 0};
+    Layout l{256, 16, 0, 0, sms};
     // Sixteen values a thread: what a row costs each thread besides (the
     // reductions, the history) is then spread far enough (12288 x 4096: 113 us
     // with eight, 80 us with sixteen).
-    if (n <= 128) l = {32, 4, 0, 0};
-    else if (n <= 512) l = {32, 16, 0, 0};
-    else if (n <= 1024) l = {64, 16, 0, 0};
-    else if (n <= 2048) l = {128, 16, 0, 0};
-    else if (n > 4096) l = {kStreamThreads, 0, 0, 0};
+    if (n <= 128) l = {32, 4, 0, 0, sms};
+    else if (n <= 512) l = {32, 16, 0, 0, sms};
+    else if (n <= 1024) l = {64, 16, 0, 0, sms};
+    else if (n <= 2048) l = {128, 16, 0, 0, sms};
+    else if (n > 4096) l = {kStreamThreads, 0, 0, 0, sms};
     if (l.vpt == 0 && rows * kWideBlocks <= 2 * sms) l.wide = n <= 8 * kWideBlocks * kStreamThreads ? 8 : 16;
     const int64_t fit = static_cast<int64_t>(sms) * (l.vpt ? min_blocks(l.threads, l.vpt) : 3);
     l.blocks = rows < fit ? rows : fit;
     return l;
+}
+
+// The form that holds a row in registers while the next one lands: its shared
+// memory, and its threads or 0.  Against the two-pass form, 40 million values
+// with masks and histories of 200: 90 us and 137 us at n = 8000, 90 and 115 at
+// 16000 (bf16: 94 and 138, 96 and 113).  A block of 1024 threads is alone on its
+// SM and nothing covers its barriers: it wins with most of its values in use
+// (92 us and 106 us at n = 32000, 115 and 109 at 20000) and in 32 bits (bf16:
+// 113 and 100 at 32000).
+size_t row_smem(int64_t n, size_t size, bool mask, bool hist, int threads) {
+    const int c = static_cast<int>(n);
+    return landing_bytes(c, static_cast<int>(size)) + (mask ? landing_bytes(c, 1) + 16 : 0) +
+           (hist ? (threads + count_words(c)) * sizeof(unsigned) : 0);
+}
+int row_form(int64_t n, size_t size, bool mask, bool hist) {
+    const int64_t elements = n + 7;  // a row that starts 7 elements after a 16-byte boundary
+    if (n <= 4096 || elements > 1024 * kRowValues) return 0;
+    const int threads = elements <= 256 * kRowValues ? 256 : elements <= 512 * kRowValues ? 512 : 1024;
+    if (threads == 1024 && (size != 4 || n < 24 * 1024)) return 0;
+    return row_smem(n, size, mask, hist, threads) <= 226 * 1024 ? threads : 0;
 }
 
 template <typename K, typename... Args>
@@ -751,6 +1015,17 @@ int forward_t(const WeightsArgs &a, float *w, cudaStream_t st) {
     const size_t smem = history_smem(l, a.n, a.hist > 0, true);
     if (l.wide == 8) return launch_rows(weights_wide_kernel<T, 8>, l, smem, st, a, w);
     if (l.wide == 16) return launch_rows(weights_wide_kernel<T, 16>, l, smem, st, a, w);
+    const int row_threads = row_form(a.n, sizeof(T), a.mask != nullptr, a.hist > 0);
+    if (row_threads != 0) {
+        l.threads = row_threads;
+        const size_t bytes = row_smem(a.n, sizeof(T), a.mask != nullptr, a.hist > 0, row_threads);
+        const int64_t room = static_cast<int64_t>(228 * 1024 / (bytes + 1280));  // blocks whose memory an SM has
+        const int64_t fit = l.sms * (room < 1024 / row_threads ? room : 1024 / row_threads);
+        l.blocks = a.rows < fit ? a.rows : fit;
+        if (row_threads == 256) return launch_rows(weights_row_kernel<T, 256>, l, bytes, st, a, w);
+        if (row_threads == 512) return launch_rows(weights_row_kernel<T, 512>, l, bytes, st, a, w);
+        if constexpr (sizeof(T) == 4) return launch_rows(weights_row_kernel<T, 1024>, l, bytes, st, a, w);
+    }
     if (l.vpt == 0 && a.rows < (1ll << 31)) l.blocks = a.rows;  // a block per row: the hardware balances them
     if (l.vpt == 0) return launch_rows(weights_stream_kernel<T>, l, smem, st, a, w);
     int rc = FL_OK;
@@ -802,7 +1077,8 @@ int weights_args(const fl_weights *p, WeightsArgs *a) {
                "relation weights: bad history (at most %lld entries)", static_cast<long long>(kMaxHistory));
     *a = WeightsArgs{p->logits, p->ld, p->bias, p->bias_ld, static_cast<const uint8_t *>(p->mask), p->mask_ld,
                      p->mask != nullptr ? p->n_states : 0, p->states, p->history, p->hist_ld, p->hist, p->rows, p->n,
-                     static_cast<float>(p->repetition), static_cast<float>(p->frequency),
+                     static_cast<float>(p->repetition),
+                     static_cast<float>(1.0 / p->repetition), static_cast<float>(p->frequency),
                      static_cast<float>(p->presence), static_cast<float>(1.0 / p->tau)};
     return FL_OK;
 }

@@ -279,3 +279,38 @@ def test_gradient_against_differences():
         f = [(attention.relation_weights(z + s * e, **kw, **RULES).double() * g).sum() for s in (1, -1)]
     # the third derivative of a softmax is below 1 / tau^3 times the slope, penalties scale by at most 1.3
     assert abs(float((f[0] - f[1]) / (2 * h)) - float(d[2, k])) <= (1.3 / 0.8) ** 3 * 4 * h * h / 6 + 60 * 2.0 ** -23 * 4 / h
+
+
+# ---- rows of thousands of columns, more of them than are in flight at once --------------------------
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,n", [(650, 4097), (600, 8186), (310, 16377), (310, 16378), (160, 24577), (150, 32761),
+                                    (150, 32762)])
+def test_long_rows(rows, n, dt):
+    """Odd row starts (every position within 16 bytes), longer histories than a block has threads, states without
+    a mask row, both kinds of bias."""
+    z, kw = inputs(rows, n, DT[dt], seed=n, hist=7, bias="shared" if n % 2 else "full")
+    check(z, kw, RULES, backward=False)
+    wide = torch.zeros(rows, n + 3, dtype=z.dtype, device="cuda")
+    wide[:, 1:n + 1] = z
+    again = check(wide[:, 1:n + 1], {k: kw[k] for k in ("mask", "states")}, {"tau": 1.5}, backward=False)
+    assert not bool(again[(kw["states"] < 0) | (kw["states"] >= 7)].any())
+    few = z[:5].repeat(40, 1)[:100]  # few rows, long histories with many repetitions
+    hist = torch.randint(-1, 40, (100, 1500), generator=torch.Generator().manual_seed(3)).cuda()
+    check(few, {"history": hist}, {"frequency": 0.01, "repetition": 1.1}, backward=False)
+
+
+def test_long_rows_in_a_graph_and_on_a_stream():
+    from flashlog_b200 import attention
+    z, kw = inputs(300, 29649, torch.float32, seed=8, bias=None)
+    want = attention.relation_weights(z, **kw, **RULES)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        assert torch.equal(attention.relation_weights(z, **kw, **RULES), want)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = attention.relation_weights(z, **kw, **RULES)
+    out.fill_(7.0)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
