@@ -149,41 +149,47 @@ __global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uin
 // length start anywhere), its store is one aligned piece of 8 or 16 bytes, so a
 // warp writes whole cache lines (single 16-bit stores took 405 us for 4608 x
 // 29649).  Four rows are in flight.
-// Eight values from p on, of which `left` exist (0 for the others).  Rows need
-// not start on 16 bytes: a lane reads the aligned 16-byte pieces around its
-// values and turns them into place.  [first, last): the array, which no piece
-// may leave.
+// Eight values from p on.  Rows need not start on 16 bytes: a lane reads the
+// aligned 16-byte pieces around its values (pieces_load) and turns them into
+// place (pieces_turn).
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, const void *first, const void *last, int left, float (&d)[8]) {
-    constexpr int kPer = 16 / sizeof(T);
+struct Pieces {
+    static constexpr int kCount = 8 * sizeof(T) / 16 + 1;
+    uint4 w[kCount];
+};
+template <typename T>
+__device__ __forceinline__ const char *pieces_at(const T *p) {
+    return reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+}
+template <typename T>
+__device__ __forceinline__ void pieces_load(const T *p, Pieces<T> &x) {
+    const uint4 *base = reinterpret_cast<const uint4 *>(pieces_at(p));
+    const bool aligned = (reinterpret_cast<uintptr_t>(p) & 15) == 0;  // then the last piece is not needed
 #pragma unroll
-    for (int h = 0; h < 8; h += kPer) {
-        union { unsigned w[4]; T t[kPer]; } x;
-        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p + h) & 15);
-        const char *base = reinterpret_cast<const char *>(p + h) - off;
-        if (left > h && base >= static_cast<const char *>(first) &&
-            base + (off == 0 ? 16 : 32) <= static_cast<const char *>(last)) {
-            union { uint4 u; unsigned w[4]; } a, b;
-            a.u = *reinterpret_cast<const uint4 *>(base);
-            b.u = a.u;
-            if (off != 0) b.u = *reinterpret_cast<const uint4 *>(base + 16);
-            unsigned c[8] = {a.w[0], a.w[1], a.w[2], a.w[3], b.w[0], b.w[1], b.w[2], b.w[3]};
-            if ((off & 4) != 0) {
+    for (int i = 0; i < Pieces<T>::kCount; ++i) x.w[i] = base[aligned && i == Pieces<T>::kCount - 1 ? i - 1 : i];
+}
+template <typename T>
+__device__ __forceinline__ void pieces_turn(const T *p, const Pieces<T> &x, float (&d)[8]) {
+    constexpr int kWords = 4 * Pieces<T>::kCount, kPer = 4 / sizeof(T);
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    unsigned c[kWords];
 #pragma unroll
-                for (int i = 0; i < 7; ++i) c[i] = c[i + 1];
-            }
-            if ((off & 8) != 0) {
+    for (int i = 0; i < Pieces<T>::kCount; ++i)
+        c[4 * i] = x.w[i].x, c[4 * i + 1] = x.w[i].y, c[4 * i + 2] = x.w[i].z, c[4 * i + 3] = x.w[i].w;
+    if ((off & 4) != 0) {
 #pragma unroll
-                for (int i = 0; i < 6; ++i) c[i] = c[i + 2];
-            }
+        for (int i = 0; i < kWords - 1; ++i) c[i] = c[i + 1];
+    }
+    if ((off & 8) != 0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x.w[i] = sizeof(T) == 2 ? __funnelshift_r(c[i], c[i + 1], 8 * (off & 3)) : c[i];
-        } else {
+        for (int i = 0; i < kWords - 2; ++i) c[i] = c[i + 2];
+    }
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) x.t[i] = h + i < left ? p[h + i] : from_f32<T>(0.0f);
-        }
+    for (int i = 0; i < 8 / kPer; ++i) {
+        union { unsigned u; T t[kPer]; } y;
+        y.u = sizeof(T) == 2 ? __funnelshift_r(c[i], c[i + 1], 8 * (off & 3)) : c[i];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) d[h + i] = h + i < left ? to_f32<T>(x.t[i]) : 0.0f;
+        for (int k = 0; k < kPer; ++k) d[i * kPer + k] = to_f32<T>(y.t[k]);
     }
 }
 
@@ -191,30 +197,49 @@ template <typename T>
 __global__ void __launch_bounds__(256) dz_kernel(const T *gy, int64_t ld_gy, const float *z, int64_t rows, int64_t n, int act,
                                                  T *out, int64_t ldo, float *partial) {
     __shared__ float part[8][256];
+    constexpr int U = 4;  // rows in flight
     const int64_t c0 = blockIdx.x * int64_t(256) + 8 * threadIdx.x;
     const int64_t r0 = blockIdx.y * int64_t(kSumRows), r1 = min(rows, r0 + kSumRows);
     const int left = c0 < n ? static_cast<int>(min(static_cast<int64_t>(8), n - c0)) : 0;
-    const void *gy_end = gy + (rows - 1) * ld_gy + n, *z_end = z + rows * n;
+    const char *const first = reinterpret_cast<const char *>(gy);
+    const char *const last = reinterpret_cast<const char *>(gy + (rows - 1) * ld_gy + n);
     float sum[8] = {};
-#pragma unroll 2
-    for (int64_t r = r0 + threadIdx.y; r < r1; r += 8) {
-        float d[8];
-        load8(gy + r * ld_gy + c0, gy, gy_end, left, d);
-        if (act != kActNone) {
-            float s[8];
-            load8(z + r * n + c0, z, z_end, left, s);
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += 8 * U) {
+        const T *p = gy + r * ld_gy + c0;
+        float d[U][8];
+        // eight columns of all rows exist, and no piece leaves the array
+        if (left == 8 && r + 8 * (U - 1) < r1 && pieces_at(p) >= first &&
+            pieces_at(p + 8 * (U - 1) * ld_gy) + 16 * Pieces<T>::kCount <= last) {
+            Pieces<T> x[U];
 #pragma unroll
-            for (int w = 0; w < 8; ++w) d[w] *= act_slope(s[w], act);
+            for (int k = 0; k < U; ++k) pieces_load(p + 8 * k * ld_gy, x[k]);
+#pragma unroll
+            for (int k = 0; k < U; ++k) pieces_turn(p + 8 * k * ld_gy, x[k], d[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+#pragma unroll
+                for (int w = 0; w < 8; ++w) d[k][w] = r + 8 * k < r1 && w < left ? to_f32<T>(p[8 * k * ld_gy + w]) : 0.0f;
         }
-        if (out != nullptr && left > 0) {
-            // the pitch is a multiple of 8: the whole piece lies in the row
-            struct alignas(16) Vec { T t[8]; } v;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) v.t[w] = from_f32<T>(d[w]);
-            *reinterpret_cast<Vec *>(out + r * ldo + c0) = v;
+        for (int k = 0; k < U; ++k) {
+            if (r + 8 * k >= r1 || left <= 0) continue;
+            if (act != kActNone) {
+                const float *pz = z + (r + 8 * k) * n + c0;
+#pragma unroll
+                for (int w = 0; w < 8; ++w)
+                    if (w < left) d[k][w] *= act_slope(pz[w], act);
+            }
+            if (out != nullptr) {
+                // the pitch is a multiple of 8: the whole piece lies in the row
+                struct alignas(16) Vec { T t[8]; } v;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) v.t[w] = from_f32<T>(d[k][w]);
+                *reinterpret_cast<Vec *>(out + (r + 8 * k) * ldo + c0) = v;
+            }
+#pragma unroll
+            for (int w = 0; w < 8; ++w) sum[w] += d[k][w];
         }
-#pragma unroll
-        for (int w = 0; w < 8; ++w) sum[w] += d[w];
     }
     if (partial == nullptr) return;
 #pragma unroll

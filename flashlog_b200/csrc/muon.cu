@@ -202,28 +202,36 @@ __global__ void __launch_bounds__(256) normalize_kernel(const Source s, const do
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
         const int64_t i0 = t / tiles_j * 64, j0 = t % tiles_j * 64;
         float v[8][2];
-        if (pairs) {
-            // 16-bit pairs
+        // a whole tile's loads have no conditions between them: all are in flight together
+        const bool whole = i0 + 64 <= s.m && j0 + 64 <= s.n;
+        if (pairs && whole) {
+            const T *p = static_cast<const T *>(s.u.ptr) + ub + (i0 + threadIdx.y) * s.u.i + j0 + 2 * threadIdx.x;
+            union { unsigned u; T t[4 / sizeof(T)]; } x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k].u = *reinterpret_cast<const unsigned *>(p + 8 * k * s.u.i);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + 2 * threadIdx.x;
-                union { unsigned u; T t[4 / sizeof(T)]; } x;
-                x.u = 0u;
-                const T *p = static_cast<const T *>(s.u.ptr) + ub + i * s.u.i + j;
-                if (i < s.m && j + 1 < s.n) x.u = *reinterpret_cast<const unsigned *>(p);
-                else if (i < s.m && j < s.n) x.t[0] = p[0];
-                v[k][0] = to_f32(x.t[0]);
-                v[k][1] = to_f32(x.t[sizeof(T) == 2 ? 1 : 0]);
+                v[k][0] = to_f32(x[k].t[0]);
+                v[k][1] = to_f32(x[k].t[sizeof(T) == 2 ? 1 : 0]);
             }
         } else {
+            // two neighbours a lane; turned 32-bit tiles a lane per element (they turn in shared memory)
+            const int64_t i = i0 + threadIdx.y, j = j0 + (kApart ? threadIdx.x : 2 * threadIdx.x);
+            if (whole) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    // two neighbours a lane; turned 32-bit tiles a lane per element (they turn in shared memory)
-                    const int64_t i = i0 + threadIdx.y + 8 * k, j = j0 + (kApart ? threadIdx.x + 32 * w : 2 * threadIdx.x + w);
-                    v[k][w] = i < s.m && j < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i, j) : 0.0f;
-                }
+                    for (int w = 0; w < 2; ++w)
+                        v[k][w] = update_at<T, MUON, false>(s, ub, 0, ob, i + 8 * k, j + (kApart ? 32 * w : w));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const int64_t c = j + (kApart ? 32 * w : w);
+                        v[k][w] = i + 8 * k < s.m && c < s.n ? update_at<T, MUON, false>(s, ub, 0, ob, i + 8 * k, c) : 0.0f;
+                    }
+            }
         }
         if (TURNED) {
 #pragma unroll
