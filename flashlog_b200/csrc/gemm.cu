@@ -239,6 +239,69 @@ __device__ __forceinline__ void stage_global(unsigned char *stage, T *p, int64_t
     }
 }
 
+// What an epilogue warp keeps from chunk to chunk.
+struct EpiWarp {
+    float *stage;          // its staging tiles (4 KB each)
+    uint32_t bar, phase;   // their barriers for loads, 8 bytes apart, and a phase bit of each
+    volatile int *failed;
+    int lane;
+    uint4 bias[4], res[4]; // of a linear head's next chunk in 16 bits: asked for a chunk ahead
+};
+
+// In 16 bits without z, a chunk's bias and residual are loaded while the chunk
+// before it (or the products) are under way.
+template <typename T>
+__device__ __forceinline__ bool chunk_ahead(const LinearEpilogue &e, int64_t col0, int64_t n) {
+    return sizeof(T) == 2 && e.aligned && e.z == nullptr && e.out_batch == 0 && col0 + 32 <= n;
+}
+template <typename T>
+__device__ __forceinline__ void ask_ahead(const LinearEpilogue &e, EpiWarp &w, int64_t row0, int64_t col0, int64_t m) {
+    if (e.bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w.bias[q] = reinterpret_cast<const uint4 *>(static_cast<const T *>(e.bias) + col0)[q];
+    }
+    if (e.residual != nullptr) {
+        const T *p = static_cast<const T *>(e.residual) + (row0 + w.lane / 4) * e.ld_res + col0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (row0 + w.lane / 4 + 8 * q < m) w.res[q] = reinterpret_cast<const uint4 *>(p + 8 * q * e.ld_res)[w.lane & 3];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void linear_ahead(const LinearEpilogue &e, float (&v)[32], EpiWarp &w, int64_t row0,
+                                             int64_t col0, int64_t next, int64_t m, int64_t n) {
+    const int lane = w.lane;
+    unsigned char *stage = reinterpret_cast<unsigned char *>(w.stage), *other = stage + 2048;
+    if (e.bias != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            union { uint4 u; T t[16 / sizeof(T)]; } x;
+            x.u = w.bias[q];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[8 * q + c] += to_f32<T>(x.t[c % (16 / sizeof(T))]);
+        }
+    }
+    if (e.residual != nullptr) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4 *>(other + piece_at(lane / 4 + 8 * q, lane & 3)) = w.res[q];
+    }
+    if (next >= 0 && chunk_ahead<T>(e, next, n)) ask_ahead<T>(e, w, row0, next, m);
+    apply_act(v, e.act);
+    __syncwarp();
+    if (e.residual != nullptr) {
+        float t[32];
+        rows_from_stage<T>(other, t, lane);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] += t[c];
+    }
+    rows_to_stage<T>(stage, v, lane);
+    __syncwarp();
+    stage_global<T, true>(stage, static_cast<T *>(e.out) + row0 * e.ld_out + col0, e.ld_out,
+                          static_cast<int>(min(static_cast<int64_t>(32), m - row0)), lane);
+    __syncwarp();
+}
+
 // Rows that start on 16 bytes: lane = row for the arithmetic.
 template <typename T>
 __device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[32], unsigned char *stage, int64_t row0,
@@ -357,20 +420,18 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
     __syncwarp();
 }
 
-// What an epilogue warp keeps from chunk to chunk.
-struct EpiWarp {
-    float *stage;          // its staging tiles (4 KB each)
-    uint32_t bar, phase;   // their barriers for loads, 8 bytes apart, and a phase bit of each
-    volatile int *failed;
-    int lane;
-};
-
 template <typename T>
 struct EpiLinear {
     LinearEpilogue p;
-    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int b, int64_t row0, int64_t col0, int64_t m,
-                                               int64_t n) const {
-        if (p.out_batch == 0) {
+    __device__ __forceinline__ void ask(EpiWarp &w, int64_t row0, int64_t col0, int64_t m, int64_t n) const {
+        if (chunk_ahead<T>(p, col0, n)) ask_ahead<T>(p, w, row0, col0, m);
+    }
+    // next: the warp's next chunk of the tile, or -1
+    __device__ __forceinline__ void operator()(float (&v)[32], EpiWarp &w, int b, int64_t row0, int64_t col0, int64_t next,
+                                               int64_t m, int64_t n) const {
+        if (chunk_ahead<T>(p, col0, n)) {
+            linear_ahead<T>(p, v, w, row0, col0, next, m, n);
+        } else if (p.out_batch == 0) {
             linear_store<T>(p, v, w.stage, row0, col0, m, n, w.lane);
         } else {
             LinearEpilogue q = p;
@@ -602,9 +663,13 @@ struct SingleWork {
     }
     __device__ __forceinline__ bool wait(const Job &, Cursor &, volatile int *) const { return true; }
     static constexpr int kTiles = 1;  // staging tiles per epilogue warp
-    __device__ __forceinline__ void ask(const Job &, EpiWarp &, int, int64_t, int64_t) const {}
-    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0) const {
-        epi(v, w, j.batch_out, row0, col0, j.m, j.n);
+    __device__ __forceinline__ void ask(const Job &j, EpiWarp &w, int, int64_t row0, int64_t col0) const {
+        epi.ask(w, row0, col0, j.m, j.n);
+    }
+    static constexpr bool kAskNext = false;  // the epilogue asks for its next chunk itself
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0,
+                                          int64_t next) const {
+        epi(v, w, j.batch_out, row0, col0, next, j.m, j.n);
     }
     __device__ __forceinline__ void done(const Job &, EpiWarp &) const {}
 };
@@ -815,8 +880,9 @@ struct NsWork {
         const PlanesJob e = planes(j);
         if (e.c != nullptr && planes_wanted(e, row0, col0)) planes_load_c(e, w, tile, j.batch_out, row0, col0);
     }
-    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int tile, int64_t row0,
-                                          int64_t col0) const {
+    static constexpr bool kAskNext = true;
+    __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int tile, int64_t row0, int64_t col0,
+                                          int64_t) const {
         const PlanesJob e = planes(j);
         if (planes_wanted(e, row0, col0))
             planes_chunk(e, p.final, v, w, tile, j.batch_out, row0, col0, j.m, j.n);
@@ -1003,7 +1069,12 @@ void gemm_kernel(const __grid_constant__ Work work) {
         }
     } else if (warp < kEpiWarps) {
         // ---- epilogue ----
-        EpiWarp w{stage_epi + warp * C::kTiles * 1024, cross_empty + 8 + 8 * warp * C::kTiles, 0, &failed, lane};
+        EpiWarp w;
+        w.stage = stage_epi + warp * C::kTiles * 1024;
+        w.bar = cross_empty + 8 + 8 * warp * C::kTiles;
+        w.phase = 0;
+        w.failed = &failed;
+        w.lane = lane;
         int buf = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
@@ -1027,9 +1098,10 @@ void gemm_kernel(const __grid_constant__ Work work) {
             };
             auto finish = [&](float (&v)[32], int c) {
                 const int tile = ((c - half) >> 5) % C::kTiles, next = c + 32 * C::kTiles;
-                work.chunk(j, v, w, tile, row0, j.col + c);
+                const bool more = next < half + BN / 2 && j.col + next < j.n;
+                work.chunk(j, v, w, tile, row0, j.col + c, more ? j.col + next : -1);
                 __syncwarp();
-                if (ok && next < half + BN / 2 && j.col + next < j.n) work.ask(j, w, tile, row0, j.col + next);
+                if (Work::kAskNext && ok && more) work.ask(j, w, tile, row0, j.col + next);
             };
             if constexpr (PLANES == 2) {
                 float sum[2][32];
