@@ -352,46 +352,68 @@ __device__ __forceinline__ void linear_rows(const LinearEpilogue &e, float (&v)[
 // Any alignment: lane = column, the rows one after another from the staging
 // tile, so that a warp's store is a whole 64- or 128-byte piece of a row.
 template <typename T>
-__device__ __forceinline__ void linear_columns(const LinearEpilogue &e, const float *stage, int64_t row0, int64_t col0,
-                                               int rows, int64_t n, int lane, bool exact_scale, int row_exp,
-                                               int col_exp) {
+__device__ __forceinline__ void columns_store(T *p, int64_t ld, const float *stage, int rows, bool in, int lane) {
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r)
+        if (in) p[r * ld] = from_f32<T>(stage[stage_at(r, lane)]);
+}
+template <typename T>
+__device__ __forceinline__ void linear_columns(const LinearEpilogue &e, float (&v)[32], float *stage, int64_t row0,
+                                               int64_t col0, int rows, int64_t n, int lane, bool exact_scale,
+                                               int row_exp, int col_exp) {
     const int64_t col = col0 + lane;
     const bool in = col < n;
     const float bias = in && e.bias != nullptr ? to_f32(static_cast<const T *>(e.bias)[col]) : 0.0f;
     const float factor = exact_scale ? 1.0f : __int_as_float((col_exp + 127) << 23);
+    const float row_factor = exact_scale ? 1.0f : __int_as_float((row_exp + 127) << 23);
     T *out = static_cast<T *>(e.out) + row0 * e.ld_out + col;
-    const T *res = static_cast<const T *>(e.residual) + row0 * e.ld_res + col;
-    float *pz = e.z + row0 * e.ld_z + col;
-    const bool plain = !exact_scale && e.z == nullptr && e.act == kActNone && e.residual == nullptr && rows == 32;
-    if (plain) {
+    if (!exact_scale) {
+        if (e.row_exp != nullptr) {
 #pragma unroll
-        for (int r = 0; r < 32; ++r) {
-            const T y = from_f32<T>(fmaf(stage[stage_at(r, lane)], factor, bias));
-            if (in) *out = y;
-            out += e.ld_out;
+            for (int c = 0; c < 32; ++c) v[c] *= row_factor;
         }
+        if (e.z == nullptr && e.act == kActNone && e.residual == nullptr && rows == 32) {
+            stage_rows(stage, v, lane);
+            __syncwarp();
+#pragma unroll
+            for (int r = 0; r < 32; ++r) {
+                const T y = from_f32<T>(fmaf(stage[stage_at(r, lane)], factor, bias));
+                if (in) *out = y;
+                out += e.ld_out;
+            }
+            return;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = fmaf(v[c], __shfl_sync(kFull, factor, c), __shfl_sync(kFull, bias, c));
+    } else {
+#pragma unroll 1
+        for (int c0 = 0; c0 < 32; c0 += 8) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+                if (c >= c0 && c < c0 + 8)
+                    v[c] = scale_pow2(v[c], row_exp + __shfl_sync(kFull, col_exp, c)) + __shfl_sync(kFull, bias, c);
+        }
+    }
+    if (e.z != nullptr) {
+        stage_rows(stage, v, lane);
+        __syncwarp();
+        columns_store<float>(e.z + row0 * e.ld_z + col, e.ld_z, stage, rows, in, lane);
+        __syncwarp();
+    }
+    apply_act(v, e.act);
+    stage_rows(stage, v, lane);
+    __syncwarp();
+    if (e.residual == nullptr) {
+        columns_store<T>(out, e.ld_out, stage, rows, in, lane);
         return;
     }
-#pragma unroll 1
-    for (int r0 = 0; r0 < rows; r0 += 8) {
-        float z[8], y[8];
+    const T *res = static_cast<const T *>(e.residual) + row0 * e.ld_res + col;
+    T y[32];  // in flight together
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const bool on = in && r0 + k < rows;
-            y[k] = e.residual != nullptr && on ? to_f32(res[k * e.ld_res]) : 0.0f;
-            z[k] = stage[stage_at(r0 + k, lane)];
-            if (exact_scale) z[k] = scale_pow2(z[k], __shfl_sync(kFull, row_exp, r0 + k) + col_exp);
-            z[k] = fmaf(z[k], factor, bias);
-            if (e.z != nullptr && on) pz[k * e.ld_z] = z[k];
-        }
-        apply_act(z, e.act);
+    for (int r = 0; r < 32; ++r) y[r] = in && r < rows ? res[r * e.ld_res] : from_f32<T>(0.0f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (in && r0 + k < rows) out[k * e.ld_out] = from_f32<T>(z[k] + y[k]);
-        out += 8 * e.ld_out;
-        res += 8 * e.ld_res;
-        pz += 8 * e.ld_z;
-    }
+    for (int r = 0; r < 32; ++r)
+        if (in && r < rows) out[r * e.ld_out] = from_f32<T>(stage[stage_at(r, lane)] + to_f32(y[r]));
 }
 
 template <typename T>
@@ -410,13 +432,7 @@ __device__ __forceinline__ void linear_store(const LinearEpilogue &e, float (&v)
         linear_rows<T>(e, v, reinterpret_cast<unsigned char *>(stage), row0, col0, rows, lane, rf);
         return;
     }
-    if (e.row_exp != nullptr) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] *= rf;
-    }
-    stage_rows(stage, v, lane);
-    __syncwarp();
-    linear_columns<T>(e, stage, row0, col0, rows, n, lane, exact_scale, re, ce);
+    linear_columns<T>(e, v, stage, row0, col0, rows, n, lane, exact_scale, re, ce);
     __syncwarp();
 }
 
