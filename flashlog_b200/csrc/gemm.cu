@@ -703,7 +703,7 @@ struct NsWork {
     NsProgram p;
     TileGrid sym, full;
     int *done_count;            // [phases, batch], zero at the start
-    int phases, first;
+    int phases, first, stop;    // all phases; this launch runs those from first to stop - 1
     uint32_t types;
 
     __device__ __forceinline__ int last() const { return p.steps - 1; }
@@ -721,7 +721,7 @@ struct NsWork {
     }
     __device__ __forceinline__ int total() const {
         int t = 0;
-        for (int q = first; q < phases; ++q) t += tiles(q) * p.batch;
+        for (int q = first; q < stop; ++q) t += tiles(q) * p.batch;
         return t;
     }
     // which product of the phase a tile of it belongs to: its position in its matrix' tiles
@@ -906,7 +906,7 @@ struct NsWork {
     // The tile's part of this CTA is in memory: one count for all its epilogue warps.
     __device__ __forceinline__ void done(const Job &j, EpiWarp &w) const {
         const int phase = j.phase & 65535;
-        if (phase == phases - 1) return;
+        if (phase == stop - 1) return;
         // a complete copy is visible to the thread that waited for it; the barrier and the release hand that on
         if (w.lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
@@ -933,12 +933,12 @@ struct Config {
     static constexpr int kAccs = PLANES == 2 ? 3 : 2;
     static constexpr int kCross = kAccs * BN;                 // the cross products' columns of TMEM
     static constexpr int kColumns = PLANES == 2 ? 4 * BN : 2 * BN;
-    static_assert(PLANES == 1 || BN == 128, "the chunks' sums have to fit the epilogue's registers");
+    static_assert(PLANES == 1 || BN <= 128, "the chunks' sums have to fit the epilogue's registers");
     static constexpr int kA = kBM * kBK * 2;              // bytes of one plane of A per stage
     static constexpr int kB = (BN / 2) * kBK * 2;         // of B (this CTA's half)
     static constexpr int kStage = PLANES * (kA + kB);
-    // a second staging tile per epilogue warp, where three stages still fit next to it
-    static constexpr int kTiles = (kStageBudget - (TILES - 1) * kEpiWarps * 4096) / kStage >= 3 ? TILES : 1;
+    // a second staging tile per epilogue warp, where it has two chunks of 32 columns
+    static constexpr int kTiles = TILES < BN / 64 ? TILES : BN / 64;
     static constexpr int kFit = (kStageBudget - (kTiles - 1) * kEpiWarps * 4096) / kStage;
     static constexpr int kStages = kFit > 8 ? 8 : kFit;
     static constexpr int kSmem = kStages * kStage + kTiles * kEpiWarps * 4096 + 1024;
@@ -1120,14 +1120,15 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 if (Work::kAskNext && ok && more) work.ask(j, w, tile, row0, j.col + next);
             };
             if constexpr (PLANES == 2) {
-                float sum[2][32];
+                constexpr int kChunks = BN / 64;
+                float sum[kChunks][32];
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                for (int q = 0; q < kChunks; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[q][i] = 0.0f;
                 auto add = [&](uint32_t columns) {
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
+                    for (int q = 0; q < kChunks; ++q) {
                         float v[32];
                         tmem_read32(v, tmem + columns + lanes + half + 32 * q);
 #pragma unroll
@@ -1146,7 +1147,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 __syncwarp();
                 if (lane == 0) bar_arrive_cta0(cross_empty);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
+                for (int q = 0; q < kChunks; ++q) {
                     const int c = half + 32 * q;
                     if (!any || j.col + c >= j.n) continue;
                     if (!ok) {
@@ -1355,13 +1356,14 @@ int linear_typed(const GemmShape &s, const GemmOperand &a, const GemmOperand &b,
     return run<128, kPlanes>(s, a, b, epi, 1, st);
 }
 
-int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, int *done_count, cudaStream_t st) {
-    constexpr int BN = 128;
+template <int BN>
+int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, int stop, int *done_count, cudaStream_t st) {
     using C = Config<BN, 2, NsWork::kTiles>;
     NsWork w{};
     w.p = p;
     w.phases = phases;
     w.first = first;
+    w.stop = stop;
     w.done_count = done_count;
     w.types = instruction_types(kF16);
     GemmShape square{p.lo, p.lo, p.lo, p.batch, 1, kF16}, full{p.lo, p.hi, p.lo, p.batch, 0, kF16};
@@ -1376,7 +1378,7 @@ int launch_ns(const NsProgram &p, const NsBuffer *buf, int phases, int first, in
         if (!rc) rc = operand_map(&w.kb[i], o, p.lo, cols, p.batch, BN / 2, kF16);
         if (!rc) rc = planes_map(&w.pl[i], buf[i].p, o.ld, o.plane, o.batch, p.lo, cols, p.batch);
         o.mn_major = 1;
-        if (!rc && i < 2) rc = operand_map(&w.mn[i], o, p.hi, p.lo, p.batch, BN / 2, kF16);
+        if (!rc && i < 2 && BN >= 128) rc = operand_map(&w.mn[i], o, p.hi, p.lo, p.batch, BN / 2, kF16);
         if (rc) return rc;
     }
     auto kernel = gemm_kernel<BN, 2, NsWork>;
@@ -1508,7 +1510,14 @@ int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float 
         if (rc) return rc;
     }
     const int first = splits > 1 ? 1 : 0;
-    return launch_ns(p, buf, phases, first, done_count, st);
+    // Few matrices: 64-wide tiles put the short products on twice the SMs and leave each half the products and
+    // half the epilogue, which is most of a phase's time; the last product, with X, has tiles enough.
+    const GemmShape square{p.lo, p.lo, p.lo, p.batch, 1, kF16};
+    if (p.gram && tile_count(square, 64) * p.batch <= sm_pairs()) {
+        rc = launch_ns<64>(p, buf, phases, first, phases - 1, done_count, st);
+        return rc ? rc : launch_ns<128>(p, buf, phases, phases - 1, phases, done_count, st);
+    }
+    return launch_ns<128>(p, buf, phases, first, phases, done_count, st);
 }
 
 // Reads and clears the device fault word (synchronizes the device).
