@@ -57,7 +57,7 @@ def union_rows(rels: torch.Tensor, n_rows: int, group=None) -> torch.Tensor:
 
 
 def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: float, comm_stream=None,
-                                        group=None, rows=None, update=None, extra_grads=()):
+                                        group=None, rows=None, update=None, extra_grads=(), gate=None):
     """One training step given as parts (DrumTrainStep.parts(), or replays of
     their CUDA graphs): after part j < T has been issued, hop T-1-j's table
     gradient grad_hop[T-1-j] is complete and its all-reduce (sum) is issued
@@ -70,7 +70,9 @@ def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: 
     rank, so the result is the same.  update (a callable such as
     DrumTrainStep.update): called in the place of that SGD step, once the
     hops' gradients and extra_grads (DrumTrainStep.grad_head) hold their mean
-    over the ranks."""
+    over the ranks.  gate (DrumTrainStep.ok, which a Muon update looks at): it
+    becomes the least of the ranks', so that after a step that failed on one
+    rank none of them updates and their parameters stay alike."""
     world = dist.get_world_size(group)
     T = len(grad_hop)
 
@@ -102,6 +104,8 @@ def run_parts_with_overlapped_allreduce(parts, grad_hop, table_grad, table, lr: 
             for g in extra_grads:
                 if g is not None:
                     allreduce_mean_(g, group)
+            if gate is not None:
+                dist.all_reduce(gate, op=dist.ReduceOp.MIN, group=group)
         update()
     elif world > 1:
         if rows is None:

@@ -92,6 +92,11 @@ def _overlaps_itself(t):
     return False
 
 
+def _range(t):
+    first = t.data_ptr()
+    return first, first + t.element_size() * (1 + sum(s * (n - 1) for n, s in zip(t.shape, t.stride())))
+
+
 @torch.no_grad()
 def muon_update(param, grad, momentum, *, lr: float, beta: float = 0.95, nesterov: bool = True,
                 weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
@@ -114,11 +119,15 @@ def muon_update(param, grad, momentum, *, lr: float, beta: float = 0.95, nestero
 def muon_update_(param, grad, momentum, *, lr: float, beta: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, scale=None, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
                  gate=None):
-    """muon_update in place: param and momentum are overwritten; returns param."""
+    """muon_update in place: param and momentum are overwritten; returns param.  param, grad and momentum must lie
+    apart in memory."""
     _check_gate(gate)
     args = _muon_args(param, grad, momentum, lr, beta, nesterov, weight_decay, scale, steps, coefficients, eps)
     if _overlaps_itself(param) or _overlaps_itself(momentum):
         raise ValueError("muon_update_: param and momentum must not overlap themselves")
+    spans = sorted(_range(t) for t in (param, grad, momentum)) if param.numel() else []
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("muon_update_: param, grad and momentum must lie apart in memory")
     bind().muon_update(param, grad, momentum, param, momentum, *args, gate)
     return param
 

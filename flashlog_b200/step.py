@@ -450,7 +450,7 @@ class DrumTrainStep:
                 muon.muon_update_(weight, self.grad_head[0], self.momentum_head, lr=self.lr, gate=self.ok,
                                   **self.muon_options)
             if bias is not None:
-                bias.sub_(self.grad_head[1], alpha=self.lr)
+                bias.addcmul_(self.grad_head[1], self.ok, value=-self.lr)
 
     def _drop(self, t):
         """fl_dropout of hop t for the kernels that write its values or their gradient (None: no dropout)."""

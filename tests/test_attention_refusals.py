@@ -102,6 +102,12 @@ def test_in_place_update_refuses_overlapping_views():
     with pytest.raises(ValueError, match="overlap"):
         muon.muon_update_(P.clone(), P, torch.zeros(9).as_strided((4, 6), (1, 1)), lr=0.1)
     assert not muon._overlaps_itself(torch.zeros(3, 4, 5, 6).permute(1, 2, 0, 3))
+    both = torch.zeros(2, 4, 6)
+    for args in ((P, P, P.clone()), (P.clone(), P, P), (P, P.clone(), P), (both[0], both.view(-1)[20:44].view(4, 6), P)):
+        with pytest.raises(ValueError, match="apart"):
+            muon.muon_update_(*args, lr=0.1)
+    with pytest.raises(ValueError, match="CUDA"):  # neighbours in one buffer are fine
+        muon.muon_update_(both[0], both[1], P.clone(), lr=0.1)
 
 
 def test_optimizer_refuses():

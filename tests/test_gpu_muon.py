@@ -230,3 +230,18 @@ def test_optimizer():
         opt.step()
     assert torch.equal(w.detach(), want[0]) and torch.equal(b.detach(), want[1])
     assert idle not in opt.state or not opt.state[idle]
+
+
+@pytest.mark.parametrize("shape", [(65, 129), (300, 520), (1025, 1600), (2, 700, 1100), (1200, 260), (1100, 4000)], ids=str)
+def test_short_products_in_narrow_tiles(shape):
+    """Few matrices of the Gram form: their short products and the last one are two launches."""
+    from flashlog_b200 import muon
+    u = matrices(*shape, seed=9)
+    assert_close(muon.orthogonalize(u), u)
+    assert_close(muon.orthogonalize(u, steps=1), u, steps=1)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = muon.orthogonalize(u)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, muon.orthogonalize(u))
