@@ -9,9 +9,15 @@
 // and one B, both planes of an operand at once (issuing a load takes about 130
 // cycles: one warp for both would hold up 128-wide tiles); one warp (of the
 // pair's first CTA) issues the matrix instructions; eight warps read the
-// accumulators back (two TMEM buffers, so a tile's epilogue runs under the next
-// tile's products).  Waits are bounded: one that runs out marks the device
+// accumulators back (two or three in TMEM take turns, so an epilogue runs under
+// the next products).  Waits are bounded: one that runs out marks the device
 // fault word, and the tiles left get NaN.
+//
+// Measured (1.66 PFLOP/s is what one large bf16 product reaches): 4608 x 1024 ->
+// 29649 in bf16 225 us (1.24 PFLOP/s: rows of odd length leave through the
+// staging tile); its two gradients 156 us and 171 us (1.8 and 1.64 PFLOP/s in
+// bursts); 4608 x 1024 -> 1645 on two planes 52 us (0.9 PFLOP/s of matrix
+// instructions): 128-wide tiles want 43 bytes per clock and SM from the L2.
 #include <cuda.h>
 
 #include "gemm.cuh"
@@ -198,16 +204,16 @@ __device__ __forceinline__ int piece_at(int r, int q) { return r * 64 + (((q ^ (
 // side (four or eight to a row), through the staging tile.
 template <typename T>
 __device__ __forceinline__ void rows_to_stage(unsigned char *stage, const float (&v)[32], int lane) {
-    if (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4) {
         stage_rows(reinterpret_cast<float *>(stage), v, lane);
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        union { uint4 u; unsigned w[4]; } x;
+        for (int q = 0; q < 4; ++q) {
+            union { uint4 u; unsigned w[4]; } x;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x.w[c] = pack_pair<T>(v[q * 8 + 2 * c], v[q * 8 + 2 * c + 1]);
-        *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = x.u;
+            for (int c = 0; c < 4; ++c) x.w[c] = pack_pair<T>(v[q * 8 + 2 * c], v[q * 8 + 2 * c + 1]);
+            *reinterpret_cast<uint4 *>(stage + piece_at(lane, q)) = x.u;
+        }
     }
 }
 template <typename T>
@@ -696,7 +702,11 @@ struct SingleWork {
 // other matrices do, so that the next phase's tiles fill the SMs that the last
 // tiles of this one leave idle.  The tiles are dealt out in phase order and all
 // blocks are resident (a cooperative launch), so the tile that a wait is for is
-// always being worked on or done.
+// always being worked on or done.  Against a launch per product: 9 matrices of
+// 1644 x 1645 2371 -> 2189 us, one of 29649 x 1024 750 -> 599 us.  Nine matrices
+// of 474 x 475 take 210 us, 14 us for each of 15 phases: the matrix instructions
+// of a tile are 3 us of it, the rest is its way through loads, epilogue, stores
+// and the next phase's wait.
 struct NsWork {
     static constexpr int kTiles = 2;
     CUtensorMap ka[kNsBuffers], kb[kNsBuffers], pl[kNsBuffers], mn[2];
@@ -924,8 +934,9 @@ __device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 // planes take per block of k.  So the two cross products (hi lo, lo hi), 2^-11
 // of the whole, have an accumulator of their own, and hi hi is cut into chunks of
 // six blocks of k (24 additions, 0.5e-6 whatever k; three blocks where the Gram
-// form squares singular values), each into the next of three accumulators; the epilogue warps add the chunks in registers, rounding to
-// nearest.  64 sums a thread: 128-wide tiles.  (Chunks of two blocks with the
+// form squares singular values), each into the next of three accumulators; the
+// epilogue warps add the chunks in registers, rounding to nearest.  64 sums a
+// thread: 128-wide tiles.  (Chunks of two blocks with the
 // cross products inside reached the same accuracy 25% slower: three times the
 // accumulator reads.)  16-bit results keep one accumulator per tile.
 template <int BN, int PLANES, int TILES>

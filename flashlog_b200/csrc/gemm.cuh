@@ -3,7 +3,7 @@
 //
 // Operands are 16-bit arrays in global memory, each as 1 or 2 planes.  Two
 // fp16 planes hold one fp32 matrix as hi + lo (22 bits); the product is then
-// hi*hi + hi*lo + lo*hi into one fp32 accumulator (the dropped lo*lo is below
+// hi*hi + hi*lo + lo*hi in fp32 accumulators (the dropped lo*lo is below
 // 2^-22 of each term), three matrix instructions per step on operands that
 // were loaded once.  An operand is K-major (its contraction index is
 // contiguous) or MN-major (its output index is), so products with a transposed
@@ -132,7 +132,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 // two values at a time: one conversion instruction packs both
 template <typename T> __device__ __forceinline__ unsigned pack_pair(float a, float b);
-template <> __device__ __forceinline__ unsigned pack_pair<float>(float, float) { return 0; }  // not a 16-bit type
 template <> __device__ __forceinline__ unsigned pack_pair<__half>(float a, float b) {
     union { __half2 h; unsigned u; } x;
     x.h = __floats2half2_rn(a, b);

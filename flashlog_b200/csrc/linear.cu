@@ -143,12 +143,6 @@ __global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uin
     *reinterpret_cast<unsigned *>(out + r * ldp + c) = a | (b << 16);
 }
 
-// dz = gy * act'(z), written as T with pitch ldo (or not at all), and its
-// column sums over kSumRows rows at a time, taken before the rounding.  A lane
-// takes four neighbouring columns: its loads are single values (rows of odd
-// length start anywhere), its store is one aligned piece of 8 or 16 bytes, so a
-// warp writes whole cache lines (single 16-bit stores took 405 us for 4608 x
-// 29649).  Four rows are in flight.
 // Eight values from p on.  Rows need not start on 16 bytes: a lane reads the
 // aligned 16-byte pieces around its values (pieces_load) and turns them into
 // place (pieces_turn).
@@ -193,6 +187,12 @@ __device__ __forceinline__ void pieces_turn(const T *p, const Pieces<T> &x, floa
     }
 }
 
+// dz = gy * act'(z), written as T with pitch ldo (or not at all), and its
+// column sums over kSumRows rows at a time, taken before the rounding.  A lane
+// takes eight neighbouring columns of four rows, all in flight, and stores whole
+// pieces: 4608 x 29649 in bf16, copied to an aligned pitch, 120 us (546 MB, 4.6
+// TB/s), where single 16-bit loads and stores took 405 us and single loads alone
+// 167 us.
 template <typename T>
 __global__ void __launch_bounds__(256) dz_kernel(const T *gy, int64_t ld_gy, const float *z, int64_t rows, int64_t n, int act,
                                                  T *out, int64_t ldo, float *partial) {
