@@ -16,8 +16,9 @@
 // Measured (1.66 PFLOP/s is what one large bf16 product reaches): 4608 x 1024 ->
 // 29649 in bf16 225 us (1.24 PFLOP/s: rows of odd length leave through the
 // staging tile); its two gradients 156 us and 171 us (1.8 and 1.64 PFLOP/s in
-// bursts); 4608 x 1024 -> 1645 on two planes 52 us (0.9 PFLOP/s of matrix
-// instructions): 128-wide tiles want 43 bytes per clock and SM from the L2.
+// bursts); 4608 x 1024 -> 1645 on two planes 45 us (1.0 PFLOP/s of matrix
+// instructions; its 234 tiles take the place of 296), 4608 x 4096 -> 4736 with
+// its packing 453 us (1.19 PFLOP/s).
 #include <cuda.h>
 
 #include "gemm.cuh"
@@ -938,7 +939,9 @@ __device__ __forceinline__ int work_first(const NsWork &w) { return w.first; }
 // epilogue warps add the chunks in registers, rounding to nearest.  64 sums a
 // thread: 128-wide tiles.  (Chunks of two blocks with the
 // cross products inside reached the same accuracy 25% slower: three times the
-// accumulator reads.)  16-bit results keep one accumulator per tile.
+// accumulator reads.  256-wide tiles, 128 sums a thread and one accumulator whose
+// reads the cross products covered, took 2950 us instead of 2430 for 9 matrices
+// of 1644 x 1645 and 475 instead of 453 for 4608 x 4096 -> 4736.)  16-bit results keep one accumulator per tile.
 template <int BN, int PLANES, int TILES>
 struct Config {
     static constexpr int kAccs = PLANES == 2 ? 3 : 2;
