@@ -498,6 +498,25 @@ __device__ __forceinline__ void final_store(const FinalOutput &e, const float (&
     const float *base = e.base.ptr != nullptr ? static_cast<const float *>(e.base.ptr) + e.base.at(b, e.nb2) : nullptr;
     const bool closed = e.gate != nullptr && *e.gate == 0.0f;
     const bool by_row = e.out.i == 1;  // lane = row is the contiguous direction
+    if constexpr (sizeof(T) == 2) {
+        // whole tiles whose lines start on 16 bytes: side by side through the staging tile
+        const int64_t pitch = by_row ? e.out.j : e.out.i;
+        if (base == nullptr && row0 + 32 <= m && col0 + 32 <= n && (by_row || e.out.j == 1) && pitch % 8 == 0 &&
+            (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+            unsigned char *tile = reinterpret_cast<unsigned char *>(stage);
+            if (by_row) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    *reinterpret_cast<T *>(tile + piece_at(c, lane >> 3) + 2 * (lane & 7)) = from_f32<T>(v[c]);
+            } else {
+                rows_to_stage<T>(tile, v, lane);
+            }
+            __syncwarp();
+            stage_global<T, true>(tile, out + (by_row ? row0 + col0 * pitch : row0 * pitch + col0), pitch, 32, lane);
+            __syncwarp();
+            return;
+        }
+    }
     if (!by_row) {
         stage_rows(stage, v, lane);
         __syncwarp();
