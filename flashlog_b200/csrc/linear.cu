@@ -183,14 +183,28 @@ __global__ void pack_cols_kernel(const float *src, int64_t ld, int64_t rows, int
     }
 }
 
-// 16-bit rows copied to an aligned pitch (rows whose pitch or base TMA cannot take).
-__global__ void pack16_kernel(const uint16_t *src, int64_t ld, int64_t cols, uint16_t *out, int64_t ldp) {
-    const int64_t r = blockIdx.y;
-    const int64_t c = (blockIdx.x * int64_t(blockDim.x) + threadIdx.x) * 2;
-    if (c >= cols) return;
-    const uint16_t *p = src + r * ld + c;
-    const unsigned a = p[0], b = c + 1 < cols ? p[1] : 0;
-    *reinterpret_cast<unsigned *>(out + r * ldp + c) = a | (b << 16);
+// 16-bit rows copied to an aligned pitch (rows whose pitch or base TMA cannot
+// take): a warp per row, two values a lane, eight such pairs in flight (23734 x
+// 572: 12.6 us; a block per row took 28.7).
+__global__ void __launch_bounds__(256) pack16_kernel(const uint16_t *src, int64_t ld, int64_t rows, int64_t cols,
+                                                     uint16_t *out, int64_t ldp) {
+    constexpr int U = 8;
+    const int64_t r = blockIdx.x * int64_t(8) + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const uint16_t *p = src + r * ld;
+    uint16_t *o = out + r * ldp;
+    for (int64_t c0 = 2 * (threadIdx.x & 31); c0 < cols; c0 += 64 * U) {
+        unsigned a[U], b[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t c = c0 + 64 * i;
+            a[i] = c < cols ? p[c] : 0u;
+            b[i] = c + 1 < cols ? p[c + 1] : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (c0 + 64 * i < cols) *reinterpret_cast<unsigned *>(o + c0 + 64 * i) = a[i] | (b[i] << 16);
+    }
 }
 
 // Eight values from p on.  Rows need not start on 16 bytes: a lane reads the
@@ -610,12 +624,9 @@ int make_operand(const void *src, int64_t ld, int64_t lines, int64_t inner, bool
         const int64_t ldp = pitch_of(inner);
         uint16_t *out = ws.take<uint16_t>(lines * ldp);
         FL_REQUIRE(out != nullptr, "linear: workspace too small");
-        // grid.y is limited to 65535 rows: the rows go in slices
-        for (int64_t r = 0; r < lines; r += 65535) {
-            const int64_t cnt = lines - r < 65535 ? lines - r : 65535;
-            launch(pack16_kernel, dim3(static_cast<unsigned>((inner + 511) / 512), static_cast<unsigned>(cnt)), 256, 0, st,
-                   static_cast<const uint16_t *>(src) + r * ld, ld, inner, out + r * ldp, ldp);
-        }
+        FL_REQUIRE(lines < (1ll << 31), "linear: bad shape");
+        launch(pack16_kernel, static_cast<unsigned>((lines + 7) / 8), 256, 0, st, static_cast<const uint16_t *>(src), ld,
+               lines, inner, out, ldp);
         op->ptr = out;
         op->ld = ldp;
         return check_launch("linear pack");
