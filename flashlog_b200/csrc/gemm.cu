@@ -811,11 +811,11 @@ struct NsWork {
             q.n = p.hi;
             q.b = x;
             q.b_mn = 1;
-            q.out = phase == phases - 1 ? -1 : x ^ 1;
+            q.out = phase == phases - 1 && p.last ? -1 : x ^ 1;
             if (p.gram) {
                 q.a = kNsQ + (last() & 1);
                 q.c = -1;
-                q.alpha = p.factor / (p.scale_q * p.scale_x);
+                q.alpha = q.out < 0 ? p.factor / (p.scale_q * p.scale_x) : 1.0f / p.scale_q;
                 q.beta = 0.0f;
             } else {
                 const float f = q.out < 0 ? p.factor / p.scale_x : 1.0f;
@@ -884,7 +884,7 @@ struct NsWork {
         const int shift = p.shift[j.batch_out];
         if (shift != 0 && (phase == 0 || (!p.gram && phase % 3 == 0))) {
             e.alpha *= exp2f(-2.0f * static_cast<float>(shift));  // A = X X^T
-        } else if (shift != 0 && phase == phases - 1) {
+        } else if (shift != 0 && phase == phases - 1 && p.last) {
             e.alpha *= exp2f(-static_cast<float>(shift));
             e.beta *= exp2f(-static_cast<float>(shift));
         }
@@ -1515,15 +1515,28 @@ int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, 
     return linear_typed<__nv_bfloat16>(s, a, b, e, st);
 }
 
-int ns_phases(int steps, int gram) { return gram ? (steps == 1 ? 3 : 1 + 3 * steps) : 3 * steps; }
+// At most three steps on squared singular values, then X is formed and squared
+// again (see muon.cu).
+int ns_segments(int steps, int gram) { return gram ? (steps + 2) / 3 : 1; }
+
+namespace {
+int segment_phases(int steps, int gram) { return gram ? (steps == 1 ? 3 : 1 + 3 * steps) : 3 * steps; }
+}  // namespace
+
+int ns_phases(int steps, int gram) {
+    const int segments = ns_segments(steps, gram);
+    int phases = 0;
+    for (int i = 0; i < segments; ++i) phases += segment_phases(ns_segment_steps(steps, segments, i), gram);
+    return phases;
+}
 
 size_t ns_parts_bytes(int64_t lo, int64_t hi, int64_t batch) {
     const int64_t n = outer_splits(lo, hi, batch);
     return n > 1 ? static_cast<size_t>(n * batch * lo * ((lo + 7) & ~int64_t(7))) * sizeof(float) : 0;
 }
 
-int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float *parts, cudaStream_t st) {
-    const int phases = ns_phases(p.steps, p.gram);
+static int ns_segment(const NsProgram &p, const NsBuffer *buf, int *done_count, float *parts, cudaStream_t st) {
+    const int phases = segment_phases(p.steps, p.gram);
     GemmShape outer{p.lo, p.lo, p.hi, p.batch, 1, kF16};
     int rc = check_shape(outer);
     if (rc) return rc;
@@ -1554,6 +1567,24 @@ int ns_products(const NsProgram &p, const NsBuffer *buf, int *done_count, float 
         return rc ? rc : launch_ns<128>(p, buf, phases, phases - 1, phases, done_count, st);
     }
     return launch_ns<128>(p, buf, phases, first, phases, done_count, st);
+}
+
+int ns_products(const NsProgram &program, const NsBuffer *buffers, int *done_count, float *parts, cudaStream_t st) {
+    const int segments = ns_segments(program.steps, program.gram);
+    NsBuffer buf[kNsBuffers];
+    for (int i = 0; i < kNsBuffers; ++i) buf[i] = buffers[i];
+    for (int i = 0; i < segments; ++i) {
+        NsProgram p = program;
+        p.steps = ns_segment_steps(program.steps, segments, i);
+        p.last = i == segments - 1;
+        const int rc = ns_segment(p, buf, done_count, parts, st);
+        if (rc) return rc;
+        done_count += segment_phases(p.steps, p.gram) * p.batch;
+        const NsBuffer x = buf[kNsX];  // the next segment starts from what this one has written
+        buf[kNsX] = buf[kNsX2];
+        buf[kNsX2] = x;
+    }
+    return FL_OK;
 }
 
 // Reads and clears the device fault word (synchronizes the device).

@@ -71,7 +71,8 @@ struct FinalOutput {
 // The products of a Newton-Schulz run on the two-plane buffers below, in one
 // kernel.  X [lo, hi] holds scale_x * X at the start; A, B, Q, T are [lo, lo],
 // at scale_a (Q: scale_q).  gram 0: X <- a X + (b A + c A^2) X with A = X X^T,
-// X and X2 in turn.  gram 1: see muon.cu.  The result is factor * O.
+// X and X2 in turn.  gram 1: see muon.cu; X and X2 in turn from segment to
+// segment.  The result is factor * O.
 enum { kNsX = 0, kNsX2 = 1, kNsA = 2, kNsB = 3, kNsQ = 4, kNsQ2 = 5, kNsT = 6, kNsBuffers = 7 };
 struct NsBuffer {
     __half *p;               // NULL: not used
@@ -79,6 +80,7 @@ struct NsBuffer {
 };
 struct NsProgram {
     int lo, hi, batch, steps, gram;
+    int last;                // this segment's product is the result (set by ns_products)
     const int *shift;        // [batch]: X holds scale_x * 2^shift * X (more than 0 for a matrix far below eps only)
     float a, b, c, scale_x, scale_a, scale_q, factor;
     FinalOutput final;
@@ -92,7 +94,11 @@ struct GemmShape {
 
 int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
                 cudaStream_t st);
+// Phases of the whole run, and how many segments of the Gram form it takes.
 int ns_phases(int steps, int gram);
+int ns_segments(int steps, int gram);
+// Steps of segment i: as many in each, the first ones one more.
+inline int ns_segment_steps(int steps, int segments, int i) { return steps / segments + (i < steps % segments ? 1 : 0); }
 // Bytes of `parts` (fp32 parts of A = X X^T, where the gram form splits it).
 size_t ns_parts_bytes(int64_t lo, int64_t hi, int64_t batch);
 // done_count: ns_phases * batch zeros.

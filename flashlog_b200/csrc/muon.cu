@@ -16,15 +16,21 @@
 // Two forms, by the sides' ratio r = long / short, in units of 2 short^3
 // operations with symmetric products at half:
 //   direct: X is multiplied in every step:    steps (1.5 r + 0.5)
-//   Gram:   everything but the first and last product is short x short: with
-//           P = a I + b A + c A^2, A <- P A P and Q <- P Q, at the end O = Q X:
-//           1.5 r + 2 steps - 1.5
+//   Gram:   everything but the first and last product of a segment of steps is
+//           short x short: with P = a I + b A + c A^2, A <- P A P and Q <- P Q,
+//           at the end X <- Q X:  1.5 r + 2 steps - 1.5 for each segment
 // All the short matrices are polynomials of the first A: symmetric, so only
-// their lower triangles are computed.  For five steps the Gram form does less
-// from r = 1.02 on; it is taken from r = 1.5: it works with squared singular
-// values, and nearly square matrices have ones so small that this costs it a
-// digit against the direct form (2e-5 instead of 1e-6 at 75 x 74; at 1.5 the
-// smallest singular value of noise is 0.1 of the largest, and both are alike).
+// their lower triangles are computed.
+//
+// The Gram form works with squared singular values: what A is rounded by grows
+// by up to a^2 a step in the directions of small ones, and Q holds factors of up
+// to a^steps beside factors of 1.  Where the singular values fall as 1 / i^2 (128
+// x 256), five steps in one segment are off by 2.7e-4 and seven by 2e-2; plain
+// fp32 steps by 1.0e-5 and 4.5e-5.  So a segment has at most three steps, then X
+// is formed and squared again: 7.7e-6 and 3.1e-5.  Five steps cost 3 r + 7.
+// Measured, Gram and direct form: 1024 x 1536 274 and 258 us, x 2048 287 and 284,
+// x 4096 356 and 429, x 29649 907 and 2188; 9 x 474 x 711 281 and 235, x 950 291
+// and 266, x 1422 323 and 316; 3 x 1645 x 3290 1343 and 1523.  Taken from r = 2.
 //
 // Matrices too small to fill a tile run whole in one block, in fp32
 // multiply-adds from shared memory: 9 matrices of 24 x 25 take 15 us.
@@ -397,7 +403,7 @@ bool is_small(int64_t lo, int64_t hi, int steps) {
 
 bool use_gram(int64_t lo, int64_t hi, int steps) {
     const double r = static_cast<double>(hi) / static_cast<double>(lo);
-    return r >= 1.5 && 1.5 * r + 2.0 * steps - 1.5 < steps * (1.5 * r + 0.5);
+    return r >= 2.0 && ns_segments(steps, 1) * (1.5 * r - 1.5) + 2.0 * steps < steps * (1.5 * r + 0.5);
 }
 
 int parts_of(int64_t batch, int64_t m) {
@@ -407,10 +413,11 @@ int parts_of(int64_t batch, int64_t m) {
     return static_cast<int>(p);
 }
 
-// Largest |x|, |A|, |b A + c A^2|, |A P| and |Q| (the factor O / X) over
-// singular values in [0, 1]: what the fp16 planes have to hold.
+// Largest |x|, |A|, |b A + c A^2|, |A P| and |Q| (the factor of a segment of the
+// Gram form) over singular values in [0, 1]: what the fp16 planes have to hold.
+// growth: the largest factor of all steps.
 struct Range {
-    double x, a, b, ap, q;
+    double x, a, b, ap, q, growth;
 };
 Range polynomial_range(double ca, double cb, double cc, int steps) {
     // a function of four numbers that a program hardly ever changes: the last answer is kept
@@ -421,10 +428,15 @@ Range polynomial_range(double ca, double cb, double cc, int steps) {
     key[1] = cb;
     key[2] = cc;
     key[3] = steps;
-    r = Range{0, 0, 0, 0, 0};
+    r = Range{0, 0, 0, 0, 0, 0};
+    const int segments = ns_segments(steps, 1);
     for (int i = 0; i <= 4096; ++i) {
-        double x = i / 4096.0, q = 1.0;
-        for (int k = 0; k < steps; ++k) {
+        double x = i / 4096.0, q = 1.0, growth = 1.0;
+        for (int k = 0, segment = 0, left = 0; k < steps; ++k, --left) {
+            if (left == 0) {
+                left = ns_segment_steps(steps, segments, segment++);
+                q = 1.0;
+            }
             const double t = x * x, bt = cb * t + cc * t * t, p = ca + bt;
             r.x = fmax(r.x, fabs(x));
             r.a = fmax(r.a, t);
@@ -432,7 +444,9 @@ Range polynomial_range(double ca, double cb, double cc, int steps) {
             r.ap = fmax(r.ap, fabs(t * p));
             x *= p;
             q *= p;
+            growth *= p;
             r.q = fmax(r.q, fabs(q));
+            r.growth = fmax(r.growth, fabs(growth));
             if (!(fabs(x) < 1e6)) { r.x = 1e6; return r; }
         }
         r.x = fmax(r.x, fabs(x));
@@ -490,7 +504,7 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     NsBuffer buf[kNsBuffers] = {};
     bool fits = partial != nullptr && counts != nullptr && shift != nullptr;
     for (int i = 0; i < kNsBuffers; ++i) {
-        if (gram ? i == kNsX2 : i >= kNsQ) continue;
+        if (gram ? i == kNsX2 && ns_segments(steps, 1) == 1 : i >= kNsQ) continue;
         buf[i] = take_planes(ws, s.batch, lo, i <= kNsX2 ? hi : lo);
         fits = fits && buf[i].p != nullptr;
     }
@@ -500,13 +514,13 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     const NsBuffer &x = buf[kNsX];
     int rc;
     if (s.mom_out.ptr != nullptr)
-        rc = normalize<float, true>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
+        rc = normalize<float, true>(s, turned, eps, r.growth, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else if (s.dtype == FL_F32)
-        rc = normalize<float, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
+        rc = normalize<float, false>(s, turned, eps, r.growth, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else if (s.dtype == FL_F16)
-        rc = normalize<__half, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
+        rc = normalize<__half, false>(s, turned, eps, r.growth, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     else
-        rc = normalize<__nv_bfloat16, false>(s, turned, eps, r.q, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
+        rc = normalize<__nv_bfloat16, false>(s, turned, eps, r.growth, partial, parts, counts, n_counts, shift, x.p, x.ld, x.plane, st);
     if (rc) return rc;
     NsProgram p{};
     p.lo = static_cast<int>(lo);
@@ -520,7 +534,7 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
     p.c = fc;
     p.scale_x = kScaleX;
     p.scale_a = kScaleA;
-    // Q's scale leaves room for its largest factor (a^steps in the null space)
+    // Q's scale leaves room for its largest factor (a^steps of a segment in the null space)
     p.scale_q = exp2f(floorf(log2f(32768.0f / static_cast<float>(r.q))));
     p.factor = f.factor;
     p.final.out = turn(f.out, turned);
@@ -557,7 +571,8 @@ size_t fl_newton_schulz_workspace(int64_t batch, int64_t m, int64_t n, int steps
     const bool gram = use_gram(lo, hi, steps);
     size_t b = carve_bytes<double>(batch * parts_of(batch, m)) + carve_bytes<int>(ns_phases(steps, gram) * batch) +
                carve_bytes<int>(batch);
-    b += (gram ? 1 : 2) * planes_bytes(batch, lo, hi) + (gram ? 5 : 2) * planes_bytes(batch, lo, lo);
+    b += (gram && ns_segments(steps, 1) == 1 ? 1 : 2) * planes_bytes(batch, lo, hi) +
+         (gram ? 5 : 2) * planes_bytes(batch, lo, lo);
     return b + (gram ? ns_parts_bytes(lo, hi, batch) + 512 : 0);
 }
 
