@@ -996,7 +996,8 @@ int row_form(int64_t n, size_t size, bool mask, bool hist) {
 
 template <typename K, typename... Args>
 int launch_rows(K kernel, const Layout &l, size_t smem, cudaStream_t st, Args... args) {
-    if (smem > 48 * 1024)
+    // 48 KB need no permission, for this and what a kernel holds anyway (256 bytes at most) together
+    if (smem > 40 * 1024)
         FL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     const int64_t grid = l.wide ? l.blocks * kWideBlocks : l.blocks;
     launch(kernel, static_cast<unsigned>(grid), l.threads, smem, st, args...);
