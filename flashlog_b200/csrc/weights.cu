@@ -388,8 +388,8 @@ __device__ __forceinline__ void land_mask(unsigned char *dst, const uint8_t *src
 }
 // room for n elements at any position within 16 bytes
 __host__ __device__ constexpr int landing_bytes(int n, int size) { return (n * size + 15) / 16 * 16 + 16; }
-// words of counts: one half for each of n + 7 elements at most
-__host__ __device__ constexpr int count_words(int n) { return (n + 8) / 2; }
+// words of counts: one half for each element of whole pieces, up to seven before the row and seven after it
+__host__ __device__ constexpr int count_words(int n) { return (n + 16) / 2; }
 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) weights_row_kernel(const WeightsArgs a, float *out) {
