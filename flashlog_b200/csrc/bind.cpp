@@ -94,15 +94,21 @@ bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor &t) { return given(t) && t->requires_grad(); }
 
 // Passes a gradient on; differentiating it again is an error, not a silent zero.
+// The tensors after it are what it was made of.
 struct Once : torch::autograd::Function<Once> {
-    static Tensor forward(AutogradContext *, const Tensor &grad, const Tensor &, const Tensor &) { return grad.view_as(grad); }
+    static Tensor forward(AutogradContext *, const Tensor &grad, const OptTensor &, const OptTensor &, const OptTensor &,
+                          const OptTensor &) {
+        return grad.view_as(grad);
+    }
     static variable_list backward(AutogradContext *, variable_list) {
         TORCH_CHECK(false, "flashlog_b200 attention operators are differentiable once");
     }
 };
-Tensor once(const Tensor &grad, const Tensor &a, const Tensor &b) {
-    if (!grad.defined() || !at::GradMode::is_enabled() || !(wants_grad(a) || wants_grad(b))) return grad;
-    return Once::apply(grad, a, b);
+Tensor once(const Tensor &grad, const OptTensor &gy, const OptTensor &a, const OptTensor &b = std::nullopt,
+            const OptTensor &c = std::nullopt) {
+    if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
+    if (!(wants_grad(gy) || wants_grad(a) || wants_grad(b) || wants_grad(c))) return grad;
+    return Once::apply(grad, gy, a, b, c);
 }
 
 // ---- the head --------------------------------------------------------------------
@@ -175,6 +181,8 @@ struct Linear : torch::autograd::Function<Linear> {
         ctx->saved_data["act"] = act;
         ctx->saved_data["bias"] = given(bias);
         ctx->saved_data["residual"] = given(residual);
+        // the gradients do not read the bias (it may change in place); with an activation they depend on it
+        if (act != FL_ACT_NONE && wants_grad(bias)) ctx->saved_data["through_bias"] = *bias;
         ctx->save_for_backward({x, w, z});
         return y;
     }
@@ -195,9 +203,18 @@ struct Linear : torch::autograd::Function<Linear> {
                 std::tie(dx, dw, db) = linear_backward(saved[0], saved[1], saved[2], gy, ctx->saved_data["act"].toInt(),
                                                        want_x, want_w, want_bias);
             }
-            out[0] = once(dx, gy, saved[1]);
-            out[1] = once(dw, gy, saved[0]);
-            out[2] = once(db, gy, saved[0]);
+            const Tensor &x = saved[0], &w = saved[1];
+            if (ctx->saved_data["act"].toInt() == FL_ACT_NONE) {
+                out[0] = once(dx, gy, w);
+                out[1] = once(dw, gy, x);
+                out[2] = once(db, gy, std::nullopt);
+            } else {  // act' at the pre-activation, which every input has a part in
+                const auto it = ctx->saved_data.find("through_bias");
+                const Tensor b = it == ctx->saved_data.end() ? Tensor() : it->second.toTensor();
+                out[0] = once(dx, gy, x, w, b);
+                out[1] = once(dw, gy, x, w, b);
+                out[2] = once(db, gy, x, w, b);
+            }
         }
         if (want_res) out[3] = gy;
         return out;
@@ -345,8 +362,9 @@ struct Weights : torch::autograd::Function<Weights> {
             std::tie(dz, db) = weights_backward(w, g, z, saved[2], saved[3], ctx->saved_data["tau"].toDouble(),
                                                 ctx->saved_data["repetition"].toDouble(), want_z, want_bias);
         }
-        out[0] = once(dz, g, z);
-        out[1] = once(db, g, z);
+        // both are made of the weights, which logits and bias have a part in
+        out[0] = once(dz, g, z, saved[2]);
+        out[1] = once(db, g, z, saved[2]);
         return out;
     }
 };
