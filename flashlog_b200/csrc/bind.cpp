@@ -93,6 +93,12 @@ Tensor workspace(size_t bytes, const Tensor &like) {
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor &t) { return given(t) && t->requires_grad(); }
 
+// Forward-mode derivatives are not there: an error, not a result without its tangent.
+void no_tangent(const char *what, std::initializer_list<OptTensor> tensors) {
+    for (const OptTensor &t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!given(t) || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // Passes a gradient on; differentiating it again is an error, not a silent zero.
 // The tensors after it are what it was made of.
 struct Once : torch::autograd::Function<Once> {
@@ -234,6 +240,7 @@ Tensor linear(const Tensor &x, const Tensor &w, const OptTensor &bias, const Opt
         FL_VALUE(bias->scalar_type() == x.scalar_type(), "linear: tensors of one dtype, got ", x.scalar_type(), " and ",
                  bias->scalar_type());
     }
+    no_tangent("linear", {x, w, bias, residual});
     const bool flat = x.dim() == 2;
     std::vector<int64_t> shape;
     if (!flat || given(residual)) {
@@ -404,6 +411,7 @@ Tensor relation_weights(const Tensor &logits, double tau, const OptTensor &mask0
         FL_VALUE(history0->size(-1) <= kMaxHistory, "relation_weights: at most ", kMaxHistory, " history entries, got ",
                  history0->size(-1));
     }
+    no_tangent("relation_weights", {logits, bias0});
     const bool flat = logits.dim() == 2;
     const Tensor z = lines(flat ? logits : logits.reshape({-1, n}));
     OptTensor bias, mask, states, history;
@@ -466,6 +474,7 @@ bool as_batch(at::ArrayRef<Tensor> ts, int64_t &b1, int64_t &b2, std::vector<fl_
 Tensor orthogonalize(const Tensor &update, int64_t steps, const Coefficients &c, double eps) {
     Devices d{"orthogonalize"};
     d.add(update);
+    no_tangent("orthogonalize", {update});
     Tensor out = at::empty(update.sizes(), update.options());
     if (out.numel() == 0) return out;
     int64_t b1, b2;
@@ -495,6 +504,7 @@ void muon_update(const Tensor &param, const Tensor &grad, const Tensor &momentum
     d.add(param_out);
     d.add(momentum_out);
     d.add(gate);
+    no_tangent("muon_update", {param, grad, momentum});
     if (param.numel() == 0) return;
     int64_t b1, b2;
     std::vector<fl_matrices> f;

@@ -1,4 +1,5 @@
-"""What autograd is told about the relation attention: a second derivative is an error whichever input it is of."""
+"""What autograd is told about the relation attention: a second derivative is an error whichever input it is of, and so
+are forward-mode derivatives."""
 import pytest
 import torch
 
@@ -56,3 +57,39 @@ def test_gradients_that_depend_on_nothing_need_no_graph():
     x.requires_grad_(), b.requires_grad_()
     gx, gb = torch.autograd.grad(attention.linear(x, w, b).sum(), (x, b), create_graph=True)
     assert not gx.requires_grad and not gb.requires_grad
+
+
+@pytest.mark.parametrize("which", range(4), ids=["x", "weight", "bias", "residual"])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_of_linear_is_an_error(which, leaf):
+    """Also for tensors that require no gradient."""
+    import torch.autograd.forward_ad as fwd
+    from flashlog_b200 import attention
+    ts = [*head(), torch.ones(20, 10).cuda()]
+    if leaf:
+        ts[0].requires_grad_()
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        ts[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
+        attention.linear(*ts)
+
+
+@pytest.mark.parametrize("which", [0, 1], ids=["logits", "bias"])
+def test_forward_mode_of_weights_is_an_error(which):
+    import torch.autograd.forward_ad as fwd
+    from flashlog_b200 import attention
+    ts = [torch.ones(6, 40).cuda(), torch.ones(40).cuda()]
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        ts[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
+        attention.relation_weights(ts[0], bias=ts[1])
+
+
+def test_forward_mode_of_updates_is_an_error():
+    import torch.autograd.forward_ad as fwd
+    from flashlog_b200 import muon
+    u = torch.randn(6, 40).cuda()
+    with fwd.dual_level():
+        dual = fwd.make_dual(u, torch.ones_like(u))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            muon.orthogonalize(dual)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            muon.muon_update(u, dual, torch.zeros_like(u), lr=0.1)
