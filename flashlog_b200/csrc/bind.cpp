@@ -93,6 +93,11 @@ Tensor workspace(size_t bytes, const Tensor &like) {
 bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const OptTensor &t) { return given(t) && t->requires_grad(); }
 
+// Autograd's note that a kernel wrote into a tensor that it may have saved.
+void written(const Tensor &t) {
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 // Forward-mode derivatives are not there: an error, not a result without its tangent.
 void no_tangent(const char *what, std::initializer_list<OptTensor> tensors) {
     for (const OptTensor &t : tensors)
@@ -156,6 +161,7 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor &x0, const Tensor &w0, co
     const size_t bytes = fl_linear_workspace(rows, n, p.k, p.dtype);
     const Tensor ws = workspace(bytes, x);
     check(fl_linear_forward(&p, ptr(y), n, ptr<float>(z), ptr(ws), bytes, on.stream), "linear");
+    if (given(out)) written(y);
     return {y, z};
 }
 
@@ -312,6 +318,7 @@ Tensor weights_forward(const Tensor &z, const OptTensor &bias, const OptTensor &
     const fl_weights p = weights_params(z, bias, mask, states, history, {tau, repetition, frequency, presence});
     OnDevice on(z);
     check(fl_relation_weights(&p, ptr<float>(w), on.stream), "relation weights");
+    if (given(out)) written(w);
     return w;
 }
 
@@ -525,6 +532,8 @@ void muon_update(const Tensor &param, const Tensor &grad, const Tensor &momentum
                          static_cast<int>(steps), std::get<0>(c), std::get<1>(c), std::get<2>(c), eps, ptr<float>(gate),
                          ptr(ws), bytes, on.stream),
           "muon_update");
+    written(param_out);
+    written(momentum_out);
 }
 
 }  // namespace

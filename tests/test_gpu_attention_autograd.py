@@ -93,3 +93,54 @@ def test_forward_mode_of_updates_is_an_error():
             muon.orthogonalize(dual)
         with pytest.raises(RuntimeError, match="forward-mode"):
             muon.muon_update(u, dual, torch.zeros_like(u), lr=0.1)
+
+
+def saved_by_a_graph(shape, strided):
+    """A leaf (a contiguous one, or a view of a wider table) and the loss of a graph that saved it."""
+    base = torch.randn(shape[0], 2, shape[1]).cuda()
+    w = base.permute(1, 0, 2) if strided else base.permute(1, 0, 2).contiguous()
+    w.requires_grad_()
+    return w, w.square().sum()
+
+
+@pytest.mark.parametrize("shape", [(20, 30), (300, 280)], ids=str)  # one block; the tensor path
+@pytest.mark.parametrize("strided", [False, True])
+def test_updates_in_place_are_seen_by_autograd(shape, strided):
+    """As after torch's own optimizers: a graph that saved the parameter before the step cannot run on the new one."""
+    from flashlog_b200 import muon
+    w, loss = saved_by_a_graph(shape, strided)
+    w.grad = torch.randn_like(w)
+    before = w._version
+    optimizer = muon.Muon([w], lr=0.1)
+    optimizer.step()
+    momentum = optimizer.state[w]["momentum"]
+    assert w._version > before and momentum._version > 0
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+
+
+def test_outputs_given_by_the_caller_are_seen_by_autograd():
+    from flashlog_b200 import ops
+    x, w, b = head()
+    out = torch.empty(20, 10).cuda().requires_grad_()
+    loss = out.square().sum()
+    with torch.no_grad():
+        ops.linear_forward(x, w, b, out=out)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    out = torch.empty(20, 10).cuda().requires_grad_()
+    loss = out.square().sum()
+    with torch.no_grad():
+        ops.relation_weights(x @ w.T, out=out)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+
+
+def test_updates_of_inference_tensors_run():
+    from flashlog_b200 import muon
+    with torch.inference_mode():
+        p, g, m = (torch.randn(20, 30).cuda() for _ in range(3))
+        q, n = muon.muon_update(p, g, m, lr=0.1)
+        muon.muon_update_(p, g, m, lr=0.1)
+    assert torch.equal(p, q) and torch.equal(m, n)
+    muon.muon_update_(p, g, m, lr=0.1)
