@@ -518,7 +518,8 @@ __device__ __forceinline__ void small_tile(const SmallArgs &p, int bx, int by, i
 template <typename T>
 __global__ void __launch_bounds__(128) small_forward_kernel(const SmallArgs p) {
     __shared__ __align__(16) float As[kT][kPitch], Bs[kT][kPitch];
-    small_tile<T, kForward>(p, blockIdx.x, blockIdx.y, 0, As, Bs);
+    const int tiles_n = static_cast<int>((p.n + kT - 1) / kT), by = blockIdx.x / tiles_n;
+    small_tile<T, kForward>(p, blockIdx.x - by * tiles_n, by, 0, As, Bs);
 }
 
 // Both gradients in one launch: the blocks below `split` are dx's tiles.
@@ -746,9 +747,9 @@ int small_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, cudaStrea
     a.ld_out = ld_y;
     a.z_out = z;
     a.act = p->act;
-    FL_REQUIRE((a.m + 31) / 32 <= 65535, "linear: too many rows");
-    launch(small_forward_kernel<T>, dim3(static_cast<unsigned>((a.n + 31) / 32), static_cast<unsigned>((a.m + 31) / 32)),
-           128, 0, st, a);
+    const int64_t tiles = ((a.m + kT - 1) / kT) * ((a.n + kT - 1) / kT);  // (a small product has few, whatever its sides)
+    FL_REQUIRE(tiles < (1ll << 31), "linear: too many tiles");
+    launch(small_forward_kernel<T>, static_cast<unsigned>(tiles), 128, 0, st, a);
     return check_launch("linear");
 }
 
