@@ -603,8 +603,8 @@ bool is_small_backward(int64_t rows, int64_t n, int64_t k, int dtype) {
 bool tma_ready(const void *p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
 size_t operand_bytes(int64_t lines, int64_t inner, int64_t exps, int dtype) {
-    const int planes = dtype == FL_F32 ? 2 : 1;
-    return carve_bytes<__half>(planes * lines * pitch_of(inner)) + carve_bytes<int>(exps) + carve_bytes<unsigned>(exps);
+    if (dtype != FL_F32) return carve_bytes<__half>(lines * pitch_of(inner));
+    return carve_bytes<__half>(2 * lines * pitch_of(inner)) + carve_bytes<int>(exps) + carve_bytes<unsigned>(exps);
 }
 
 // Readies the matrix src [lines, inner] as a product operand.  by_line: the
@@ -857,10 +857,11 @@ int linear_forward(const fl_linear *p, void *y, int64_t ld_y, float *z, void *ws
 size_t linear_backward_workspace(int64_t rows, int64_t n, int64_t k, int dtype, int act) {
     if (rows <= 0 || n <= 0 || k <= 0) return 0;
     if (is_small_backward(rows, n, k, dtype)) return split_bytes(rows, k, n) + split_bytes(n, k, rows) + 256;
-    size_t dz = 2 * operand_bytes(rows, n, rows > n ? rows : n, dtype);  // both scalings of dz
-    if (act != FL_ACT_NONE || dtype != FL_F32) dz += carve_bytes<char>(rows * pitch_of(n) * elem_size(dtype));
-    const size_t ops = operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
-    return dz + ops + carve_bytes<float>(((rows + kSumRows - 1) / kSumRows) * n);
+    size_t b = carve_bytes<float>(((rows + kSumRows - 1) / kSumRows) * n);  // column sums
+    // dz: of an activation, and of 16-bit gradients whose rows TMA cannot take
+    if (act != FL_ACT_NONE || dtype != FL_F32) b += carve_bytes<char>(rows * pitch_of(n) * elem_size(dtype));
+    if (dtype == FL_F32) b += operand_bytes(rows, n, rows, dtype) + operand_bytes(rows, n, n, dtype);  // its two scalings
+    return b + operand_bytes(n, k, k, dtype) + operand_bytes(rows, k, k, dtype);
 }
 
 int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t ld_gy, void *dx, void *dw, void *dbias,
