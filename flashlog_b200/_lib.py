@@ -202,6 +202,7 @@ SIGNATURES = {
     "fl_muon_update": (ctypes.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                       _D, _D, ctypes.c_int, _D, _D, ctypes.c_int, _D, _D, _D, _D, _P, _P, _SZ, _P]),
     "fl_gemm_fault": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
+    "fl_gemm_wait_limits": (ctypes.c_int, [_I64, _I64]),
 }
 
 _lib = None

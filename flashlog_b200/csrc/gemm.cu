@@ -11,7 +11,8 @@
 // pair's first CTA) issues the matrix instructions; eight warps read the
 // accumulators back (two or three in TMEM take turns, so an epilogue runs under
 // the next products).  Waits are bounded: one that runs out marks the device
-// fault word, and the tiles left get NaN.
+// fault word, and the tiles that the block has left get NaN, as does what is
+// computed from them.
 //
 // Measured (1.66 PFLOP/s is what one large bf16 product reaches): 4608 x 1024 ->
 // 29649 in bf16 225 us (1.24 PFLOP/s: rows of odd length leave through the
@@ -33,9 +34,11 @@ constexpr int kEpiWarps = 8;    // warp w reads TMEM lanes 32 (w % 4).., columns
 constexpr int kLoadA = kEpiWarps, kLoadB = kEpiWarps + 1, kMmaWarp = kEpiWarps + 2;
 constexpr int kThreads = 32 * (kEpiWarps + 3);
 constexpr int kStageBudget = 192 * 1024;
-constexpr uint64_t kWaitLimitNs = 4000000000ull;  // four seconds: far above any wait between healthy roles
 
 __device__ int g_gemm_fault;    // set when a bounded wait ran out
+// Limits in ns: of a role for another of its pair, and of a phase's tiles for the phase before.  Four seconds are
+// far above any wait between healthy roles.
+__device__ uint64_t g_wait_limit = 4000000000ull, g_phase_limit = 4000000000ull;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -68,8 +71,22 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
             if (bar_try(bar, parity)) return true;
         if (*failed) return false;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    } while (now - start < kWaitLimitNs);
+    } while (now - start < *const_cast<volatile uint64_t *>(&g_wait_limit));
     *failed = 1;
+    atomicExch(&g_gemm_fault, 1);
+    return false;
+}
+
+// A copy that was started lands, whatever happens to the roles: nobody writes to its place before.
+__device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity) {
+    uint64_t start, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+    for (;;) {
+        for (int i = 0; i < 64; ++i)
+            if (bar_try(bar, parity)) return true;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (now - start >= 4000000000ull) break;
+    }
     atomicExch(&g_gemm_fault, 1);
     return false;
 }
@@ -250,6 +267,7 @@ __device__ __forceinline__ void stage_global(unsigned char *stage, T *p, int64_t
 struct EpiWarp {
     float *stage;          // its staging tiles (4 KB each)
     uint32_t bar, phase;   // their barriers for loads, 8 bytes apart, and a phase bit of each
+    uint32_t asked;        // a bit of each into which a load is under way
     volatile int *failed;
     int lane;
     uint4 bias[4], res[4]; // of a linear head's next chunk in 16 bits: asked for a chunk ahead
@@ -567,6 +585,7 @@ __device__ __forceinline__ bool planes_wanted(const PlanesJob &p, int64_t row0, 
     return !p.symmetric || col0 <= row0;
 }
 __device__ __forceinline__ void planes_load_c(const PlanesJob &p, EpiWarp &w, int tile, int b, int64_t row0, int64_t col0) {
+    w.asked |= 1u << tile;
     if (w.lane == 0) {
         bar_expect(w.bar + 8 * tile, 4096);
         asm volatile(
@@ -576,17 +595,25 @@ __device__ __forceinline__ void planes_load_c(const PlanesJob &p, EpiWarp &w, in
             "r"(static_cast<int>(row0)), "r"(0), "r"(b) : "memory");
     }
 }
-// tile: the staging tile, into which C of this chunk has been asked for
+// tile: the staging tile, into which C of this chunk has been asked for.  ok: the
+// products are there; else the tile becomes NaN.
 __device__ __forceinline__ void planes_chunk(const PlanesJob &p, const FinalOutput &f, float (&v)[32], EpiWarp &w, int tile,
-                                             int b, int64_t row0, int64_t col0, int64_t m, int64_t n) {
+                                             int b, int64_t row0, int64_t col0, int64_t m, int64_t n, bool ok) {
     const int lane = w.lane;
     float *tile_f = w.stage + 1024 * tile;
     unsigned char *stage = reinterpret_cast<unsigned char *>(tile_f);
     const uint32_t s32 = smem_u32(stage);
-    if (p.c != nullptr) {
-        const bool ok = warp_wait(w.bar + 8 * tile, (w.phase >> tile) & 1u, w.failed);
+    if ((w.asked >> tile) & 1u) {
+        ok = __all_sync(kFull, landed(w.bar + 8 * tile, (w.phase >> tile) & 1u)) && ok;
         w.phase ^= 1u << tile;
-        if (!ok) return;
+        w.asked ^= 1u << tile;
+    } else if (p.c != nullptr) {
+        ok = false;
+    }
+    if (!ok) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = __int_as_float(0x7fc00000);
+    } else if (p.c != nullptr) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             union { uint4 u; __half2 h[4]; } a, z;
@@ -712,8 +739,9 @@ struct SingleWork {
         epi.ask(w, row0, col0, j.m, j.n);
     }
     static constexpr bool kAskNext = false;  // the epilogue asks for its next chunk itself
+    // (a tile that failed holds NaN)
     __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int, int64_t row0, int64_t col0,
-                                          int64_t next) const {
+                                          int64_t next, bool) const {
         epi(v, w, j.batch_out, row0, col0, next, j.m, j.n);
     }
     __device__ __forceinline__ void done(const Job &, EpiWarp &) const {}
@@ -909,10 +937,10 @@ struct NsWork {
             int have;
             asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(have) : "l"(done_count + at) : "memory");
             if (__all_sync(kFull, have >= want)) break;
-            if ((i & 63) == 63) {
+            if ((i & 63) == 0) {
                 asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
                 if (start == 0) start = now;
-                const bool over = now - start > kWaitLimitNs;
+                const bool over = now - start >= *const_cast<volatile uint64_t *>(&g_phase_limit);
                 if (__any_sync(kFull, over)) {
                     atomicExch(&g_gemm_fault, 1);
                     *failed = 1;
@@ -931,10 +959,10 @@ struct NsWork {
     }
     static constexpr bool kAskNext = true;
     __device__ __forceinline__ void chunk(const Job &j, float (&v)[32], EpiWarp &w, int tile, int64_t row0, int64_t col0,
-                                          int64_t) const {
+                                          int64_t, bool ok) const {
         const PlanesJob e = planes(j);
         if (planes_wanted(e, row0, col0))
-            planes_chunk(e, p.final, v, w, tile, j.batch_out, row0, col0, j.m, j.n);
+            planes_chunk(e, p.final, v, w, tile, j.batch_out, row0, col0, j.m, j.n, ok);
     }
     // The tile's part of this CTA is in memory: one count for all its epilogue warps.
     __device__ __forceinline__ void done(const Job &j, EpiWarp &w) const {
@@ -1124,7 +1152,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
         EpiWarp w;
         w.stage = stage_epi + warp * C::kTiles * 1024;
         w.bar = cross_empty + 8 + 8 * warp * C::kTiles;
-        w.phase = 0;
+        w.phase = w.asked = 0;
         w.failed = &failed;
         w.lane = lane;
         int buf = 0;
@@ -1151,7 +1179,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
             auto finish = [&](float (&v)[32], int c) {
                 const int tile = ((c - half) >> 5) % C::kTiles, next = c + 32 * C::kTiles;
                 const bool more = next < half + BN / 2 && j.col + next < j.n;
-                work.chunk(j, v, w, tile, row0, j.col + c, more ? j.col + next : -1);
+                work.chunk(j, v, w, tile, row0, j.col + c, more ? j.col + next : -1, ok);
                 __syncwarp();
                 if (Work::kAskNext && ok && more) work.ask(j, w, tile, row0, j.col + next);
             };
@@ -1590,8 +1618,19 @@ int ns_products(const NsProgram &program, const NsBuffer *buffers, int *done_cou
 // Reads and clears the device fault word (synchronizes the device).
 int gemm_fault(int *fault) {
     int zero = 0;
+    FL_REQUIRE(fault != nullptr, "gemm_fault: null result");
+    FL_CUDA(cudaDeviceSynchronize());  // (a copy waits for streams that block the legacy one only)
     FL_CUDA(cudaMemcpyFromSymbol(fault, g_gemm_fault, sizeof(int)));
     if (*fault) FL_CUDA(cudaMemcpyToSymbol(g_gemm_fault, &zero, sizeof(int)));
+    return FL_OK;
+}
+
+int gemm_wait_limits(int64_t wait_ns, int64_t phase_ns) {
+    FL_REQUIRE(wait_ns >= 0 && phase_ns >= 0, "gemm_wait_limits: limits must be at least 0");
+    const uint64_t wait = static_cast<uint64_t>(wait_ns), phase = static_cast<uint64_t>(phase_ns);
+    FL_CUDA(cudaDeviceSynchronize());
+    FL_CUDA(cudaMemcpyToSymbol(g_wait_limit, &wait, sizeof(wait)));
+    FL_CUDA(cudaMemcpyToSymbol(g_phase_limit, &phase, sizeof(phase)));
     return FL_OK;
 }
 

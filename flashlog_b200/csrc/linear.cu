@@ -941,6 +941,7 @@ int linear_backward(const fl_linear *p, const float *z, const void *gy, int64_t 
 }
 
 int gemm_fault(int *fault);
+int gemm_wait_limits(int64_t wait_ns, int64_t phase_ns);
 
 }  // namespace fl
 
@@ -965,5 +966,7 @@ int fl_linear_backward(const fl_linear *p, const float *z, const void *gy, int64
 }
 
 int fl_gemm_fault(int *fault) { return gemm_fault(fault); }
+
+int fl_gemm_wait_limits(int64_t wait_ns, int64_t phase_ns) { return gemm_wait_limits(wait_ns, phase_ns); }
 
 }  // extern "C"

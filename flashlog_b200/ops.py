@@ -708,7 +708,14 @@ def relation_weights_backward(w, g, logits, bias=None, history=None, tau=1.0, re
 
 
 def gemm_fault() -> bool:
-    """Whether a bounded wait of a matrix product ran out since the last call (synchronizes)."""
+    """Whether a bounded wait of a matrix product ran out on the current device since the last call (synchronizes it).
+    What the product had left then, and what was computed from it, holds NaN."""
     f = ctypes.c_int(0)
     check(lib().fl_gemm_fault(ctypes.byref(f)), "gemm_fault")
     return bool(f.value)
+
+
+def gemm_wait_limits(wait_s: float = 4.0, phase_s: float = 4.0):
+    """Limits of those waits on the current device, in seconds: of a kernel's parts for one another, and of a
+    Newton-Schulz product for the one before it.  Synchronizes the device."""
+    check(lib().fl_gemm_wait_limits(int(wait_s * 1e9), int(phase_s * 1e9)), "gemm_wait_limits")

@@ -464,6 +464,11 @@ class DrumTrainStep:
               "value_dropout")
 
     def check(self):
-        """Raise if any hop ran out of its buffers (one host read)."""
+        """Raise if any hop ran out of its buffers (one host read), or a wait of the head's or the update's products
+        ran out (the step's results hold NaN)."""
         if int(self.status.item()) & L.FL_STATUS_SLOT_OVERFLOW:
             raise RuntimeError("a hop exceeded its static capacity")
+        if self.head is not None or self.optimizer == "muon":
+            with torch.cuda.device(self.dev):
+                if ops.gemm_fault():
+                    raise RuntimeError("a wait of a matrix product ran out")

@@ -556,9 +556,18 @@ int fl_muon_update(const fl_matrices *param, const fl_matrices *grad, const fl_m
                    double a, double b, double c, double eps, const float *gate, void *ws, size_t ws_bytes,
                    fl_stream_t stream);
 
-/* 1 if a bounded wait of a matrix-product kernel ran out since the last call
- * (its outputs hold NaN), else 0, in *fault; clears it.  Synchronizes. */
+/* 1 if a bounded wait of a matrix-product kernel ran out on the current device
+ * since the last call, else 0, in *fault; clears it.  The parts of the result
+ * that were left then, and what was computed from them, hold NaN.  Synchronizes
+ * the device. */
 int fl_gemm_fault(int *fault);
+
+/* The limits of those waits on the current device, in ns (4 s each at the
+ * start): of the parts of a kernel for one another, and of a Newton-Schulz
+ * product's tiles for those of the product before (0: a product whose
+ * predecessor is not ready at the first look is given up).  For tests and
+ * tighter watchdogs.  Synchronizes the device. */
+int fl_gemm_wait_limits(int64_t wait_ns, int64_t phase_ns);
 
 #ifdef __cplusplus
 }
