@@ -100,13 +100,16 @@ class OperatorRules:
         if not (1e-30 < self.repetition < 1e30 and abs(self.frequency) < 1e30 and abs(self.presence) < 1e30):
             raise ValueError("operator rules: repetition must be positive and the penalties finite")
 
-    def rows(self, t: int, N: int):
-        """Keyword arguments of relation_weights for hop t's rows r = q * N + channel."""
+    def rows(self, t: int, N: int, history=None):
+        """Keyword arguments of relation_weights for hop t's rows r = q * N + channel.  history: the queries' histories
+        by row, where the caller has them (they are the same for every hop)."""
         kw = dict(repetition=self.repetition, frequency=self.frequency, presence=self.presence)
         if self.mask is not None:
             kw["mask"] = ops._lines(self.mask)
             kw["states"] = self.states[t][:, None].expand(-1, N).reshape(-1)
-        if self.history is not None and self.history.shape[1] > 0:
+        if history is not None:
+            kw["history"] = history
+        elif self.history is not None and self.history.shape[1] > 0:
             kw["history"] = self.history[:, None, :].expand(-1, N, -1).reshape(-1, self.history.shape[1])
         if self.bias is not None:
             kw["bias"] = self.bias.contiguous()

@@ -148,10 +148,11 @@ def drum_propagate(heads, w_all, graph: Graph, r_size: int, *, c1=None, c2=0, ma
         drop = (float(dropout), draw_seed() if dropout_seed is None else int(dropout_seed),
                 device_counter(dropout_counter, heads.device))
     for t in range(T):
-        if rules is None:
+        if rules is None and head is None:
             w_t = torch.softmax(w_all[:, t] / tau_1, dim=-1)
         else:
-            w_t = attention.relation_weights(w_all[:, t].reshape(Q * N, n), tau=tau_1, **rules.rows(t, N)).view(Q, N, n)
+            kw = {} if rules is None else rules.rows(t, N)
+            w_t = attention.relation_weights(w_all[:, t].reshape(Q * N, n), tau=tau_1, **kw).view(Q, N, n)
         val, row_ptr, ent = HopNorm.apply(val, w_t, row_ptr, ent, graph, r_size, topk, c1, flags, mask_triple, eps,
                                           stats, status, vis, drop is not None)
         if drop is not None:

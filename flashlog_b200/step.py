@@ -213,8 +213,12 @@ class DrumTrainStep:
         self.grad_logits = torch.empty((Q, T, N, width), dtype=f32, device=dev)
         # with a head or rules the backward wants the hops' hidden states and logits again
         self.hidden = None if head is None else [torch.empty((rows, width), dtype=f32, device=dev) for _ in range(T)]
-        self.logits = None if rules is None else [torch.empty((rows, self.n), dtype=f32, device=dev)
-                                                  for _ in range(T)]
+        self.logits = None if rules is None and head is None else [torch.empty((rows, self.n), dtype=f32, device=dev)
+                                                                   for _ in range(T)]
+        # the queries' histories by row, for all hops and the backward of a run
+        self.history = None
+        if rules is not None and rules.history is not None and rules.history.shape[1] > 0:
+            self.history = torch.empty((rows, rules.history.shape[1]), dtype=torch.int64, device=dev)
         ws = 0
         for t in range(T):
             ws = max(ws, lib().fl_topc_workspace(rows, self.C[t]), lib().fl_hop_workspace(rows, self.S[t]),
@@ -365,26 +369,24 @@ class DrumTrainStep:
             return
         kept = self.hidden[t] if self.head is not None else self.logits[t]
         torch.index_select(self.table[:, t], 0, self.rels, out=kept.view(Q, N, self.width))
-        z = kept
         if self.head is not None:
-            z, _ = ops.linear_forward(kept, self.head[0], self.head[1],
-                                      out=None if self.rules is None else self.logits[t])
-        if self.rules is None:
-            w.view(Q, N, n).copy_(torch.softmax(z.view(Q, N, n), dim=-1))
-        else:
-            ops.relation_weights(z, out=w.view(rows, n), **self.rules.rows(t, N))
+            ops.linear_forward(kept, self.head[0], self.head[1], out=self.logits[t])
+        if self.history is not None and t == 0:
+            self.history.view(Q, N, -1).copy_(self.rules.history[:, None, :].expand(-1, N, -1))
+        kw = {} if self.rules is None else self.rules.rows(t, N, self.history)
+        ops.relation_weights(self.logits[t], out=w.view(rows, n), **kw)
 
     def _weights_backward(self, t):
         """From grad_w to the gradient of hop t's table rows (and of the head)."""
         Q, N, rows, n = self.Q, self.N, self.rows, self.n
         wt, gw = self.w[t][:rows * n].view(Q, N, n), self.grad_w_of(t)
-        if self.rules is None:
+        if self.head is None and self.rules is None:
             # softmax backward, d logits = w * (g - sum(g * w)): torch's own kernel
             dz = torch._softmax_backward_data(gw, wt, -1, torch.float32)
         else:
-            kw = self.rules.rows(t, N)
             dz, _ = ops.relation_weights_backward(wt.view(rows, n), gw.view(rows, n), self.logits[t],
-                                                  history=kw.get("history"), repetition=self.rules.repetition)
+                                                  history=self.history,
+                                                  repetition=1.0 if self.rules is None else self.rules.repetition)
             dz = dz.view(Q, N, n)
         if self.head is None:
             torch.mul(dz, self.ok, out=self.grad_logits[:, t])
