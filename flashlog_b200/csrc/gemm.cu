@@ -691,6 +691,7 @@ struct Job {
     int m, n;              // bounds of the output
     int batch_a, batch_b, batch_out;
     int kb0, kb1;          // contraction, in blocks of kBK
+    int wrap;              // from this block on, A's second plane with B once more
     int per_acc;           // blocks per accumulator (planes; 1 << 28: all)
     int phase;
 };
@@ -704,6 +705,7 @@ template <typename Epi>
 struct SingleWork {
     CUtensorMap map_a, map_b;
     int m, n, kblocks, splits;  // splits > 1: the contraction in parts, one output each
+    int in_turn;                // A's two planes one after the other
     int a_mn, b_mn, per_acc;
     TileGrid grid;
     uint32_t types;             // of the instruction descriptor
@@ -728,7 +730,8 @@ struct SingleWork {
         j.batch_a = j.batch_b = mat;
         j.batch_out = b;
         j.kb0 = part * per;
-        j.kb1 = min(kblocks, j.kb0 + per);
+        j.kb1 = in_turn ? 2 * kblocks : min(kblocks, j.kb0 + per);
+        j.wrap = in_turn ? kblocks : 1 << 28;
         j.per_acc = per_acc;
         j.phase = 0;
         return j;
@@ -899,6 +902,7 @@ struct NsWork {
         j.batch_a = j.batch_b = j.batch_out = b;
         j.kb0 = 0;
         j.kb1 = (q.k + kBK - 1) / kBK;
+        j.wrap = 1 << 28;
         j.per_acc = p.gram ? 3 : 6;
         j.phase = cur.phase | (part << 16);
         return j;
@@ -1068,15 +1072,16 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 ok = warp_wait(empty + 8 * s, phase ^ 1, &failed);
                 if (!ok) break;
                 const uint32_t dst = smem_u32(smem) + s * C::kStage + offset;
+                const int k = (kb >= j.wrap ? kb - j.wrap : kb) * kBK, turn = is_a && kb >= j.wrap ? 1 : 0;
                 if (elect_one()) {
                     // the other CTA's and the other warp's bytes may arrive before they are expected
                     if (expects) bar_expect(full + 8 * s, 2 * C::kStage);
                     if (mn) {
                         for (int p = 0; p < PLANES; ++p)
                             for (int h = 0; h < pieces; ++h)
-                                tma_load(dst + p * plane + h * 8192, map, full + 8 * s, line + 64 * h, kb * kBK, p, b);
+                                tma_load(dst + p * plane + h * 8192, map, full + 8 * s, line + 64 * h, k, p + turn, b);
                     } else {
-                        tma_load(dst, map, full + 8 * s, kb * kBK, line, 0, b);  // all planes
+                        tma_load(dst, map, full + 8 * s, k, line, turn, b);  // all planes
                     }
                 }
                 __syncwarp();
@@ -1221,7 +1226,9 @@ void gemm_kernel(const __grid_constant__ Work work) {
                     finish(sum[q], c);
                 }
             } else {
+                const bool two = j.kb1 - j.kb0 > j.per_acc;  // A's planes in turn: both accumulators
                 if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
+                if (two && ok) ok = warp_wait(acc_full + 8 * (buf ^ 1), acc_phase ^ static_cast<uint32_t>(buf), &failed);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                 for (int c = half; c < half + BN / 2; c += 32) {
@@ -1229,6 +1236,13 @@ void gemm_kernel(const __grid_constant__ Work work) {
                     float v[32];
                     if (ok) {
                         tmem_read32(v, tmem + buf * BN + lanes + c);
+                        if (two) {
+                            float lo[32];
+                            tmem_read32(lo, tmem + (buf ^ 1) * BN + lanes + c);
+                            const float f0 = work.epi.p.first, f1 = work.epi.p.second;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = fmaf(f1, lo[i], f0 * v[i]);
+                        }
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7fc00000);
@@ -1236,6 +1250,7 @@ void gemm_kernel(const __grid_constant__ Work work) {
                     finish(v, c);
                 }
                 next_acc();
+                if (two) next_acc();
             }
             work.done(j, w);
         }
@@ -1287,7 +1302,7 @@ int operand_map(CUtensorMap *map, const GemmOperand &o, int64_t lines_mn, int64_
     cuuint64_t strides[3] = {ld, o.planes > 1 ? static_cast<cuuint64_t>(o.plane) * 2 : ld,
                              batch > 1 ? static_cast<cuuint64_t>(o.batch) * 2 : ld};
     cuuint32_t box[4] = {64, static_cast<cuuint32_t>(o.mn_major ? kBK : box_rows),
-                         static_cast<cuuint32_t>(o.mn_major ? 1 : o.planes), 1};
+                         static_cast<cuuint32_t>(o.mn_major || o.in_turn ? 1 : o.planes), 1};
     cuuint32_t unit[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, kind == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                           const_cast<void *>(o.ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -1372,7 +1387,8 @@ int run(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const Ep
     w.splits = splits;
     w.a_mn = a.mn_major;
     w.b_mn = b.mn_major;
-    w.per_acc = PLANES == 1 ? 1 << 28 : splits > 1 ? 3 : 6;  // (split: the Gram form's first product)
+    w.in_turn = a.in_turn;
+    w.per_acc = PLANES == 1 ? (a.in_turn ? w.kblocks : 1 << 28) : splits > 1 ? 3 : 6;  // (split: the Gram form's first product)
     w.grid = tile_grid(s, BN, s.batch * splits);
     w.types = instruction_types(s.kind);
     w.epi = epi;
@@ -1535,9 +1551,12 @@ int outer_splits(int64_t lo, int64_t hi, int64_t batch) {
 int gemm_linear(const GemmShape &s, const GemmOperand &a, const GemmOperand &b, const LinearEpilogue &e,
                 cudaStream_t st) {
     const int planes = e.dtype == kOutF32 ? 2 : 1;
-    FL_REQUIRE(a.planes == planes && b.planes == planes && !s.symmetric, "gemm: planes");
+    FL_REQUIRE(a.planes == (a.in_turn ? 2 : planes) && b.planes == planes && !b.in_turn && !s.symmetric &&
+                   (!a.in_turn || planes == 1),
+               "gemm: planes");
     const int rc = check_shape(s);
     if (rc) return rc;
+    FL_REQUIRE(!a.in_turn || s.k < (1ll << 30), "gemm: bad shape");
     if (e.dtype == kOutF32) return linear_typed<float>(s, a, b, e, st);
     if (e.dtype == kOutF16) return linear_typed<__half>(s, a, b, e, st);
     return linear_typed<__nv_bfloat16>(s, a, b, e, st);

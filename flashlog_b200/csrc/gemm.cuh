@@ -32,6 +32,8 @@ struct GemmOperand {
     int64_t batch;           // elements between the batch's matrices (multiple of 8)
     int planes;              // 1 or 2
     int mn_major;            // 0: lines are output indices, k contiguous; 1: lines are k
+    int in_turn;             // A of a product with one plane: its second plane follows the first along k, into a
+                             // second accumulator (D = first * (hi B) + second * (lo B))
 };
 
 // Epilogue of the linear head: z = acc * 2^(ea[i] + eb[j]) + bias[j],
@@ -48,6 +50,7 @@ struct LinearEpilogue {
     int dtype, act;
     int aligned;             // set by gemm_linear: rows of all arrays start on 16 bytes
     int64_t out_batch;       // elements between the outputs of a batch (0: one output)
+    float first, second;     // of the accumulators, where A's planes are taken in turn
 };
 
 // A batch of matrices in a caller's memory: element (b, i, j) lies at
