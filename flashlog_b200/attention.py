@@ -33,8 +33,11 @@ def linear(x, weight, bias=None, residual=None, activation: str = "none"):
     [..., n] has their dtype.  activation: none, relu, tanh, silu or gelu (the
     erf form).  Differentiable once in every tensor.
 
-    Sums run in fp32 whatever the dtype; fp32 keeps fp32 accuracy.  A fp32 row
-    (or weight row) that holds an infinity gives NaN."""
+    Sums run in fp32 whatever the dtype.  fp32 values keep 22 bits or more down
+    to 2^-29 of the largest of their row (of x or weight; in the backward also
+    of their column), and are off by at most 2^-50 of that below.  A fp32 row
+    (or weight row) that holds an infinity gives NaN.  A backward pass takes at
+    most 8,388,480 rows."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")

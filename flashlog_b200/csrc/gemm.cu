@@ -738,6 +738,7 @@ struct SingleWork {
     }
     __device__ __forceinline__ bool wait(const Job &, Cursor &, volatile int *) const { return true; }
     static constexpr int kTiles = 1;  // staging tiles per epilogue warp
+    __device__ __forceinline__ float cross() const { return epi.p.second; }
     __device__ __forceinline__ void ask(const Job &j, EpiWarp &w, int, int64_t row0, int64_t col0) const {
         epi.ask(w, row0, col0, j.m, j.n);
     }
@@ -763,6 +764,7 @@ struct SingleWork {
 // and the next phase's wait.
 struct NsWork {
     static constexpr int kTiles = 2;
+    __device__ __forceinline__ float cross() const { return 1.0f; }
     CUtensorMap ka[kNsBuffers], kb[kNsBuffers], pl[kNsBuffers], mn[2];
     NsProgram p;
     TileGrid sym, full;
@@ -1195,23 +1197,23 @@ void gemm_kernel(const __grid_constant__ Work work) {
                 for (int q = 0; q < kChunks; ++q)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[q][i] = 0.0f;
-                auto add = [&](uint32_t columns) {
+                auto add = [&](uint32_t columns, float factor) {
 #pragma unroll
                     for (int q = 0; q < kChunks; ++q) {
                         float v[32];
                         tmem_read32(v, tmem + columns + lanes + half + 32 * q);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sum[q][i] += v[i];
+                        for (int i = 0; i < 32; ++i) sum[q][i] = fmaf(v[i], factor, sum[q][i]);
                     }
                 };
                 for (int k0 = j.kb0; k0 < j.kb1; k0 += j.per_acc) {
                     if (ok) ok = warp_wait(acc_full + 8 * buf, acc_phase, &failed);
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    if (ok && any) add(buf * BN);
+                    if (ok && any) add(buf * BN, 1.0f);
                     next_acc();
                 }
                 // the last chunk's barrier covers the cross products too
-                if (ok && any) add(C::kCross);
+                if (ok && any) add(C::kCross, work.cross());
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) bar_arrive_cta0(cross_empty);
@@ -1595,6 +1597,7 @@ static int ns_segment(const NsProgram &p, const NsBuffer *buf, int *done_count, 
         e.p.out = parts;
         e.p.ld_out = (p.lo + 7) & ~7;
         e.p.out_batch = p.lo * e.p.ld_out;
+        e.p.second = 1.0f;
         e.p.dtype = kOutF32;
         e.p.aligned = 1;
         rc = run<128, 2>(outer, x, x, e, splits, st);

@@ -50,7 +50,8 @@ struct LinearEpilogue {
     int dtype, act;
     int aligned;             // set by gemm_linear: rows of all arrays start on 16 bytes
     int64_t out_batch;       // elements between the outputs of a batch (0: one output)
-    float first, second;     // of the accumulators, where A's planes are taken in turn
+    float first, second;     // of the accumulators, where A's planes are taken in turn; with two planes an operand,
+                             // second is that of the cross products (1 / the scale of the lo planes)
 };
 
 // A batch of matrices in a caller's memory: element (b, i, j) lies at

@@ -3,9 +3,11 @@
 //
 // fp32 operands are split into two fp16 planes, hi + lo, after scaling each
 // line of the uncontracted index by a power of two that brings its largest
-// value to [2^14, 2^15): a value keeps 22 bits down to 2^-18 of its line's
-// largest, and no line can lose bits to another line's size.  The exponents
-// are undone in the product's epilogue.
+// value to [2^14, 2^15): no line can lose bits to another line's size.  lo is
+// held 2048 times as large, where it reaches as far down as hi: a value keeps 22
+// bits down to 2^-29 of its line's largest, and is off by at most 2^-50 of that
+// below.  Scale and exponents are undone in the product's epilogue; the cross
+// products have an accumulator of their own anyway.
 #include "gemm.cuh"
 
 namespace fl {
@@ -13,6 +15,7 @@ namespace fl {
 namespace {
 
 constexpr int kSumRows = 128;  // rows per partial column sum
+constexpr float kLoScale = 2048.0f;
 
 int elem_size(int dtype) { return dtype == FL_F32 ? 4 : 2; }
 
@@ -27,7 +30,7 @@ __device__ __forceinline__ int line_exponent(float absmax) {
 __device__ __forceinline__ void split_scaled(float v, int e, __half &hi, __half &lo) {
     const float s = scale_pow2(v, -e);
     hi = __float2half_rn(s);
-    lo = __float2half_rn(s - __half2float(hi));
+    lo = __float2half_rn((s - __half2float(hi)) * kLoScale);
 }
 
 __device__ __forceinline__ float block_max(float v, float *scratch) {
@@ -723,6 +726,7 @@ LinearEpilogue plain_epilogue(void *out, int64_t ld, int dtype, const int *re, c
     e.ld_out = ld;
     e.dtype = dtype;
     e.act = kActNone;
+    e.second = 1.0f / kLoScale;
     return e;
 }
 

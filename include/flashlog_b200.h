@@ -470,9 +470,10 @@ enum { FL_ACT_NONE = 0, FL_ACT_RELU = 1, FL_ACT_TANH = 2, FL_ACT_SILU = 3, FL_AC
 
 /* y = act(x W^T + bias) + residual: x [rows, k], W [n, k], bias [n] or NULL,
  * residual [rows, n] or NULL, all of one dtype; ld_* are elements between
- * rows (at least the row's length).  fp32 is computed to fp32 accuracy
- * (operands as two fp16 planes scaled per line, or fp32 multiply-adds for few
- * rows), 16-bit types with fp32 sums and one rounding at the end. */
+ * rows (at least the row's length).  fp32 operands are two fp16 planes scaled
+ * per line: values keep 22 bits down to 2^-29 of their line's largest and are
+ * off by at most 2^-50 of it below (few rows and small products run in fp32
+ * multiply-adds).  16-bit types have fp32 sums and one rounding at the end. */
 typedef struct fl_linear {
     const void *x, *w, *bias, *residual;
     int64_t ld_x, ld_w, ld_res;
