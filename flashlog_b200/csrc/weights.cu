@@ -37,7 +37,10 @@ struct WeightsArgs {
     const int64_t *history;  // [rows, hist] or NULL; entries outside [0, n) do not count
     int64_t hist_ld, hist;
     int64_t rows, n;
-    float theta, inv_theta, frequency, presence, inv_tau;
+    float theta, frequency, presence, inv_tau;
+    float k;                 // log2 e / tau, rounded once: w is a power of 2 of (u - max) k.  (From 1 / tau and
+                             // log2 e, each rounded, the weights were off by 2.0e-7 at tau = 0.9, now by 0.8e-7;
+                             // a softmax by divisions and expf is off by 1.6e-7.)
 };
 
 // A thread's columns of its block are i * THREADS + threadIdx.x.  The seen bits
@@ -88,10 +91,11 @@ __device__ __forceinline__ int64_t state_of(const WeightsArgs &a, int64_t row) {
 
 // A logit of an operator that is `count` times in the row's history.
 __device__ __forceinline__ float penalised(const WeightsArgs &a, float v, unsigned count) {
-    v *= v > 0.0f ? a.inv_theta : a.theta;
+    v = v > 0.0f ? v / a.theta : v * a.theta;
     return v - a.frequency * static_cast<float>(count) - a.presence;
 }
-// 2^x, to 2^-22; results below 2^-126 are 0
+// 2^x, to 2^-22, a fourth of what the exponent's own rounding moves a weight of
+// e^-16; results below 2^-126 are 0
 __device__ __forceinline__ float power2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,7 +158,7 @@ __global__ __launch_bounds__(THREADS, min_blocks(THREADS, VPT)) void weights_for
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int left = static_cast<int>(a.n) - tid;  // the thread's column i exists iff i * THREADS < left
     const bool hist = a.hist > 0;
-    const float k = a.inv_tau * 1.4426950408889634f;
+    const float k = a.k;
     const int64_t step = gridDim.x;
     int64_t row = blockIdx.x;
     RowInputs<T, VPT> in;
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) weights_row_kernel(co
     unsigned *const seen = reinterpret_cast<unsigned *>(a.mask != nullptr ? ms + landing_bytes(n, 1) + 16 : ms);
     unsigned *const count = seen + THREADS;
     const bool hist = a.hist > 0;
-    const float k = a.inv_tau * 1.4426950408889634f;
+    const float k = a.k;
     const int64_t step = gridDim.x;
     int64_t row = blockIdx.x;
     if (row >= a.rows) return;  // for the whole block
@@ -634,7 +638,7 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) weights_stream_
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool hist = a.hist > 0;
     unsigned *seen = hist ? dyn : nullptr, *count = dyn + words;
-    const float k = a.inv_tau * 1.4426950408889634f;
+    const float k = a.k;
     if (hist)
         for (int i = tid; i < words + (n + 1) / 2; i += kStreamThreads) dyn[i] = 0u;
     int flip = 0;
@@ -811,7 +815,7 @@ __global__ void __launch_bounds__(kStreamThreads) __cluster_dims__(kWideBlocks, 
     const int c0 = static_cast<int>(cluster_rank()) * kChunk, left = static_cast<int>(a.n) - c0 - tid;
     const int64_t row = blockIdx.x / kWideBlocks;
     const bool hist = a.hist > 0;
-    const float k = a.inv_tau * 1.4426950408889634f;
+    const float k = a.k;
     const T *z = static_cast<const T *>(a.logits) + row * a.ld + c0 + tid;
     const T *bias = static_cast<const T *>(a.bias) + row * a.bias_ld + c0 + tid;
     T raw[VPT], extra[VPT];
@@ -1092,8 +1096,8 @@ int weights_args(const fl_weights *p, WeightsArgs *a) {
     *a = WeightsArgs{p->logits, p->ld, p->bias, p->bias_ld, static_cast<const uint8_t *>(p->mask), p->mask_ld,
                      p->mask != nullptr ? p->n_states : 0, p->states, p->history, p->hist_ld, p->hist, p->rows, p->n,
                      static_cast<float>(p->repetition),
-                     static_cast<float>(1.0 / p->repetition), static_cast<float>(p->frequency),
-                     static_cast<float>(p->presence), static_cast<float>(1.0 / p->tau)};
+                     static_cast<float>(p->frequency), static_cast<float>(p->presence), static_cast<float>(1.0 / p->tau),
+                     static_cast<float>(1.4426950408889634 / p->tau)};
     return FL_OK;
 }
 
