@@ -116,7 +116,10 @@ class DrumTrainStep:
         if optimizer not in ("sgd", "muon"):
             raise ValueError(f"optimizer must be sgd or muon, got {optimizer!r}")
         width = self.n if head is None else head[0].shape[-1]
-        if tuple(table.shape[1:]) != (T, N, width):
+        # a table of more hops serves a step that keeps only gradients
+        hops = table.shape[1] if table.dim() == 4 else -1
+        if table.dim() != 4 or tuple(table.shape[2:]) != (N, width) or hops < T or (
+                hops > T and (apply_update or optimizer != "sgd")):
             raise ValueError(f"table must be [2R, {T}, {N}, {width}], got {tuple(table.shape)}")
         if head is not None:
             if tuple(head[0].shape) != (self.n, width) or (head[1] is not None and tuple(head[1].shape) != (self.n,)):
