@@ -494,7 +494,7 @@ int newton_schulz(const Source &s, const Finish &f, int steps, double ca, double
         if (s.dtype == FL_F16) return run_small<__half, false>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
         return run_small<__nv_bfloat16, false>(s, f, turned, lo, hi, steps, fa, fb, fc, eps, st);
     }
-    FL_REQUIRE(s.batch <= 65535 && (s.m + 63) / 64 <= 65535, "newton-schulz: too large a batch or matrix");
+    FL_REQUIRE(s.batch <= 65535, "newton-schulz: at most 65535 matrices that one block cannot hold");
     Carve ws(wsp, ws_bytes);
     const int parts = parts_of(s.batch, s.m);
     const bool gram = use_gram(lo, hi, steps);

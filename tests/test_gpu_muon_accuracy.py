@@ -66,3 +66,15 @@ def test_many_steps(shape):
     # at 1 the polynomial's slope is 0: what is left are the last step's roundings, three products of matrices of
     # norm 1 in the spectral sense, each off by at most 4 * 2^-22 of its factors' Frobenius norms, sqrt(m) each
     assert float((got - w @ v).norm()) <= 3 * 4 * 2.0 ** -22 * shape[0]
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_very_long_matrices(turned):
+    """5 million rows of 8: near the steps in 64 bits, as other sizes are (white noise: nothing is amplified)."""
+    from flashlog_b200 import muon
+    g = torch.Generator(device="cuda").manual_seed(2)
+    u = torch.randn(8, 5_000_000, generator=g, device="cuda")
+    x = u.double() / (torch.linalg.matrix_norm(u.double()) + 1e-7)
+    want = steps_in(x, 5, torch.float64)
+    got = muon.orthogonalize(u.mT.contiguous()).mT if turned else muon.orthogonalize(u)
+    assert float(torch.linalg.matrix_norm(got.double() - want) / torch.linalg.matrix_norm(want)) <= 2e-5
