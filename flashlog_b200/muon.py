@@ -51,7 +51,7 @@ def orthogonalize(update, steps: int = 5, coefficients=COEFFICIENTS, eps: float 
     every product fp32 sums whatever the dtype, so the result is about as near
     as plain fp32 steps come, for decaying singular values too; it has the
     update's dtype and is rounded once.  Sides are below 2^24; of matrices too
-    large for one block (some 100 x 100) a batch has at most 65,535.  The
+    large for one block (from some 55 x 55 on) a batch has at most 65,535.  The
     coefficients must keep singular values of [0, 1] within 3.  A matrix that
     holds a NaN or an infinity gives NaN.  Not differentiable."""
     if update.dtype not in ops.FL_DTYPE:

@@ -216,8 +216,11 @@ class DrumTrainStep:
         self.grad_logits = torch.empty((Q, T, N, width), dtype=f32, device=dev)
         # with a head or rules the backward wants the hops' hidden states and logits again
         self.hidden = None if head is None else [torch.empty((rows, width), dtype=f32, device=dev) for _ in range(T)]
-        self.logits = None if rules is None and head is None else [torch.empty((rows, self.n), dtype=f32, device=dev)
-                                                                   for _ in range(T)]
+        # (the logits' signs, under a repetition penalty; without rules one buffer serves all hops)
+        self.logits = None
+        if rules is not None or head is not None:
+            each = [torch.empty((rows, self.n), dtype=f32, device=dev) for _ in range(1 if rules is None else T)]
+            self.logits = each * T if rules is None else each
         # the queries' histories by row, for all hops and the backward of a run
         self.history = None
         if rules is not None and rules.history is not None and rules.history.shape[1] > 0:
