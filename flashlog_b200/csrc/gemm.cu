@@ -16,10 +16,11 @@
 //
 // Measured (1.66 PFLOP/s is what one large bf16 product reaches): 4608 x 1024 ->
 // 29649 in bf16 225 us (1.24 PFLOP/s: rows of odd length leave through the
-// staging tile); its two gradients 156 us and 171 us (1.8 and 1.64 PFLOP/s in
-// bursts); 4608 x 1024 -> 1645 on two planes 45 us (1.0 PFLOP/s of matrix
-// instructions; its 234 tiles take the place of 296), 4608 x 4096 -> 4736 with
-// its packing 453 us (1.19 PFLOP/s).
+// staging tile), 357 us with SiLU, 670 us with GELU and a residual; its two
+// gradients 156 us and 171 us (1.8 and 1.64 PFLOP/s in bursts), of an activation
+// on two planes of dz 1295 us with the pass that makes them; 4608 x 1024 -> 1645
+// on two planes 45 us (1.0 PFLOP/s of matrix instructions; its 234 tiles take the
+// place of 296), 4608 x 4096 -> 4736 with its packing 453 us (1.19 PFLOP/s).
 #include <cuda.h>
 
 #include "gemm.cuh"
@@ -758,7 +759,8 @@ struct SingleWork {
 // tiles of this one leave idle.  The tiles are dealt out in phase order and all
 // blocks are resident (a cooperative launch), so the tile that a wait is for is
 // always being worked on or done.  Against a launch per product: 9 matrices of
-// 1644 x 1645 2371 -> 2189 us, one of 29649 x 1024 750 -> 599 us.  Nine matrices
+// 1644 x 1645 2371 -> 2189 us, one of 29649 x 1024 (five steps in one segment) 750
+// -> 599 us.  Nine matrices
 // of 474 x 475 take 210 us, 14 us for each of 15 phases: the matrix instructions
 // of a tile are 3 us of it, the rest is its way through loads, epilogue, stores
 // and the next phase's wait.

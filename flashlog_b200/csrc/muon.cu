@@ -35,10 +35,11 @@
 // Matrices too small to fill a tile run whole in one block, in fp32
 // multiply-adds from shared memory: 9 matrices of 24 x 25 take 15 us.
 //
-// Measured: 29649 x 1024 in bf16 550 us (norm 16, planes 49, A in parts 97, the
-// short products 218, the last product 180); a Muon step of 9 matrices of 1644 x
-// 1645 2.5 ms, 2.3 ms of it products at 1.06 PFLOP/s of matrix instructions; of
-// 9 matrices of 474 x 475 225 us, 15 dependent phases of 14 us.
+// Measured: 29649 x 1024 in bf16 845 us (norm 18, planes 51; two segments, each A
+// in parts 98 and its product with X 186; their short products 129 and 80); a
+// Muon step of 9 matrices of 1644 x 1645 2.5 ms, 2.3 ms of it products at 1.06
+// PFLOP/s of matrix instructions; of 9 matrices of 474 x 475 230 us, 15 dependent
+// phases of 14 us.
 #include <math.h>
 
 #include "gemm.cuh"
