@@ -80,6 +80,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 
 // A copy that was started lands, whatever happens to the roles: nobody writes to its place before.
 __device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity) {
+    if (bar_try(bar, parity)) return true;
     uint64_t start, now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
     for (;;) {
